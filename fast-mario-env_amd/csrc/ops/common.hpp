@@ -1,0 +1,63 @@
+// What the policy's operators share: element types, wave reductions, and the host's checks and errors.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+#include "../../../include/mario_ops.h"
+
+namespace mo {
+
+typedef __bf16 bf16;
+
+__device__ __forceinline__ float as_f32(float x) { return x; }
+__device__ __forceinline__ float as_f32(bf16 x) { return (float)x; }
+// The one rounding of a value to the type it is stored in (to nearest even).
+template <class T> __device__ __forceinline__ T as(float x) { return (T)x; }
+
+// N consecutive elements as they lie in memory, moved in accesses of up to 16 bytes.
+template <class T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack { T v[N]; };
+
+constexpr int kWave = 64;
+
+// ---- host side
+inline thread_local std::string g_err;
+
+inline int fail(const std::string& what) {
+    g_err = what;
+    return -1;
+}
+inline bool ok(hipError_t e, const char* what) {
+    if (e == hipSuccess) return true;
+    fail(std::string(what) + ": " + hipGetErrorString(e));
+    return false;
+}
+inline int launched(const char* what) { return ok(hipGetLastError(), what) ? 0 : -1; }
+
+// A buffer a kernel is about to touch: memory of the current GPU (device, pinned host or managed), aligned to its
+// elements. Anything else is refused before a kernel could fault on it.
+inline bool usable(const void* p, const char* name, size_t align) {
+    if (!p) { fail(std::string(name) + ": null"); return false; }
+    if ((uintptr_t)p % align) { fail(std::string(name) + ": not aligned to its elements"); return false; }
+    int dev = 0;
+    if (!ok(hipGetDevice(&dev), "hipGetDevice")) return false;
+    hipPointerAttribute_t at;
+    const hipError_t e = hipPointerGetAttributes(&at, p);
+    (void)hipGetLastError();   // a refused pointer must not surface as the error of a later launch
+    const bool good = e == hipSuccess && ((at.type == hipMemoryTypeDevice && at.device == dev) ||
+                                          at.type == hipMemoryTypeHost || at.type == hipMemoryTypeManaged);
+    if (!good) fail(std::string(name) + ": not memory of GPU " + std::to_string(dev));
+    return good;
+}
+
+inline int compute_units() {
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) return 256;
+    return cus;
+}
+
+}  // namespace mo

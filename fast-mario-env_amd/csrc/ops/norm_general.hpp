@@ -1,0 +1,327 @@
+// Group norm with an activation, channels last: any channel and group counts, any sample size.
+#pragma once
+#include "common.hpp"
+
+namespace mo {
+
+// With h = (x - mean) rstd and z = weight h + bias:  y = act(z). Going back, dz = dy act'(z), dbias = sum dz, dweight = sum dz h
+// and, with dh = weight dz,  dx = rstd (dh - mean(dh) - h mean(dh h)), the means over the group.
+template <int ACT> __device__ __forceinline__ float act(float z) {
+    if (ACT == MO_ACT_RELU) return z <= 0.f ? 0.f : z;   // (a NaN stays one)
+    if (ACT == MO_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    return z;
+}
+template <int ACT> __device__ __forceinline__ float act_grad(float z) {
+    if (ACT == MO_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (ACT == MO_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        return s * (1.f + z * (1.f - s));
+    }
+    return 1.f;
+}
+
+// n values of mean `mean` and squared deviations `m2`, joined by another set (Chan et al.): no difference of large sums.
+struct Moments {
+    float n, mean, m2;
+    __device__ __forceinline__ void join(const Moments& o) {
+        const float t = n + o.n;
+        if (t == 0.f) return;
+        const float d = o.mean - mean, w = o.n / t;
+        mean = fmaf(d, w, mean);
+        m2 = m2 + o.m2 + d * d * n * w;
+        n = t;
+    }
+};
+
+// A sample is cut into slabs of `px` pixels; a block takes a slab. Its threads are LN lanes along the channels (V each) by
+// pixel lanes, so a thread's channels stay its own.
+struct NormCut {
+    int64_t slabs, px;
+    int nv, LN, PL;   // packs of V channels a pixel; channel lanes; pixel lanes
+};
+
+struct NormArgs {
+    MoNorm a;
+    NormCut c;
+    float* part;      // per (sample, slab): [2][C], or the same summed
+    float* means;     // (B, groups, 2): mean and rstd; going back, mean(dh) and mean(dh h)
+};
+
+constexpr int NORM_THREADS = 256;
+
+// Each channel's mean and squared deviations over a slab, into part.
+template <class T, int V>
+__global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
+    __shared__ float sm[NORM_THREADS][V], s2[NORM_THREADS][V], sn[NORM_THREADS];
+    const MoNorm& a = k.a;
+    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int t = threadIdx.x, pl = t / k.c.LN;
+    float* part = k.part + (int64_t)blockIdx.x * 2 * a.C;
+    for (int c0 = 0; c0 < k.c.nv; c0 += k.c.LN) {
+        const int cv = c0 + t % k.c.LN;
+        const bool live = pl < k.c.PL && cv < k.c.nv;
+        float mean[V] = {}, m2[V] = {}, n = 0.f;
+        if (live)
+            for (int64_t p = p0 + pl; p < p1; p += k.c.PL) {
+                const Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + (b * a.S + p) * a.C + cv * V);
+                n += 1.f;
+                const float r = 1.f / n;
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float v = as_f32(x.v[i]), d = v - mean[i];
+                    mean[i] = fmaf(d, r, mean[i]);
+                    m2[i] = fmaf(d, v - mean[i], m2[i]);
+                }
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; i++) { sm[t][i] = mean[i]; s2[t][i] = m2[i]; }
+        sn[t] = n;
+        __syncthreads();
+        if (live && pl == 0) {                            // the pixel lanes in their order
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                Moments m{sn[t], sm[t][i], s2[t][i]};
+                for (int j = 1; j < k.c.PL; j++) m.join({sn[t + j * k.c.LN], sm[t + j * k.c.LN][i], s2[t + j * k.c.LN][i]});
+                part[cv * V + i] = m.mean;
+                part[a.C + cv * V + i] = m.m2;
+            }
+        }
+    }
+}
+
+// Mean and rstd of a sample's group, a wave each, from its channels' moments in every slab.
+__global__ void __launch_bounds__(kWave) k_norm_means(NormArgs k) {
+    const MoNorm& a = k.a;
+    const int64_t b = blockIdx.x / a.groups;
+    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups;
+    Moments m{0.f, 0.f, 0.f};
+    for (int64_t i = threadIdx.x; i < k.c.slabs * cg; i += kWave) {
+        const int64_t slab = i / cg;
+        const float* p = k.part + (b * k.c.slabs + slab) * 2 * a.C + g * cg + i % cg;
+        m.join({(float)(min((slab + 1) * k.c.px, a.S) - slab * k.c.px), p[0], p[a.C]});
+    }
+    for (int s = 1; s < kWave; s *= 2) {
+        const Moments o{__shfl_xor(m.n, s), __shfl_xor(m.mean, s), __shfl_xor(m.m2, s)};
+        Moments lo = (threadIdx.x & s) ? o : m;           // every lane joins the two in the same order
+        lo.join((threadIdx.x & s) ? m : o);
+        m = lo;
+    }
+    if (threadIdx.x == 0) {
+        k.means[2 * blockIdx.x] = m.mean;
+        k.means[2 * blockIdx.x + 1] = 1.f / sqrtf(m.m2 / m.n + a.eps);
+    }
+}
+
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(NormArgs k) {
+    const MoNorm& a = k.a;
+    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int t = threadIdx.x, pl = t / k.c.LN, cg = a.C / a.groups;
+    if (pl >= k.c.PL) return;
+    for (int cv = t % k.c.LN; cv < k.c.nv; cv += k.c.LN) {
+        float w[V], s[V], mean[V];                        // z = (x - mean) w + s
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int c = cv * V + i;
+            const float* m = k.means + 2 * (b * a.groups + c / cg);
+            mean[i] = m[0];
+            w[i] = m[1] * (a.weight ? a.weight[c] : 1.f);
+            s[i] = a.bias ? a.bias[c] : 0.f;
+        }
+        for (int64_t p = p0 + pl; p < p1; p += k.c.PL) {
+            const int64_t at = (b * a.S + p) * a.C + cv * V;
+            Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + at);
+#pragma unroll
+            for (int i = 0; i < V; i++) x.v[i] = as<T>(act<ACT>(fmaf(as_f32(x.v[i]) - mean[i], w[i], s[i])));
+            *(Pack<T, V>*)((T*)a.y + at) = x;
+        }
+    }
+}
+
+// Each channel's sums of dz h and of dz over a slab, into part.
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(NormArgs k) {
+    __shared__ float sw[NORM_THREADS][V], sb[NORM_THREADS][V];
+    const MoNorm& a = k.a;
+    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int t = threadIdx.x, pl = t / k.c.LN, cg = a.C / a.groups;
+    float* part = k.part + (int64_t)blockIdx.x * 2 * a.C;
+    for (int c0 = 0; c0 < k.c.nv; c0 += k.c.LN) {
+        const int cv = c0 + t % k.c.LN;
+        const bool live = pl < k.c.PL && cv < k.c.nv;
+        float dw[V] = {}, db[V] = {};
+        if (live) {
+            float w[V], s[V], mean[V], r[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int c = cv * V + i;
+                const float* m = a.stats + 2 * (b * a.groups + c / cg);
+                mean[i] = m[0];
+                r[i] = m[1];
+                w[i] = a.weight ? a.weight[c] : 1.f;
+                s[i] = a.bias ? a.bias[c] : 0.f;
+            }
+            for (int64_t p = p0 + pl; p < p1; p += k.c.PL) {
+                const int64_t at = (b * a.S + p) * a.C + cv * V;
+                const Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + at), dy = *(const Pack<T, V>*)((const T*)a.dy + at);
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float h = (as_f32(x.v[i]) - mean[i]) * r[i], dz = as_f32(dy.v[i]) * act_grad<ACT>(fmaf(h, w[i], s[i]));
+                    dw[i] = fmaf(dz, h, dw[i]);
+                    db[i] += dz;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; i++) { sw[t][i] = dw[i]; sb[t][i] = db[i]; }
+        __syncthreads();
+        if (live && pl == 0) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                for (int j = 1; j < k.c.PL; j++) { dw[i] += sw[t + j * k.c.LN][i]; db[i] += sb[t + j * k.c.LN][i]; }
+                part[cv * V + i] = dw[i];
+                part[a.C + cv * V + i] = db[i];
+            }
+        }
+    }
+}
+
+// mean(dh) and mean(dh h) of a sample's group, a wave each, from its channels' sums.
+__global__ void __launch_bounds__(kWave) k_norm_dmeans(NormArgs k) {
+    const MoNorm& a = k.a;
+    const int64_t b = blockIdx.x / a.groups;
+    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups;
+    float m1 = 0.f, m2 = 0.f;
+    for (int64_t i = threadIdx.x; i < k.c.slabs * cg; i += kWave) {
+        const int c = g * cg + (int)(i % cg);
+        const float* p = k.part + (b * k.c.slabs + i / cg) * 2 * a.C + c;
+        const float w = a.weight ? a.weight[c] : 1.f;
+        m2 = fmaf(w, p[0], m2);
+        m1 = fmaf(w, p[a.C], m1);
+    }
+    for (int s = 1; s < kWave; s *= 2) { m1 += __shfl_xor(m1, s); m2 += __shfl_xor(m2, s); }
+    if (threadIdx.x == 0) {
+        const float by = 1.f / ((float)a.S * (float)cg);
+        k.means[2 * blockIdx.x] = m1 * by;
+        k.means[2 * blockIdx.x + 1] = m2 * by;
+    }
+}
+
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(NORM_THREADS) k_norm_dx(NormArgs k) {
+    const MoNorm& a = k.a;
+    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int t = threadIdx.x, pl = t / k.c.LN, cg = a.C / a.groups;
+    if (pl >= k.c.PL) return;
+    for (int cv = t % k.c.LN; cv < k.c.nv; cv += k.c.LN) {
+        float w[V], s[V], mean[V], r[V], m1[V], m2[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int c = cv * V + i;
+            const int64_t g = 2 * (b * a.groups + c / cg);
+            mean[i] = a.stats[g];
+            r[i] = a.stats[g + 1];
+            m1[i] = k.means[g];
+            m2[i] = k.means[g + 1];
+            w[i] = a.weight ? a.weight[c] : 1.f;
+            s[i] = a.bias ? a.bias[c] : 0.f;
+        }
+        for (int64_t p = p0 + pl; p < p1; p += k.c.PL) {
+            const int64_t at = (b * a.S + p) * a.C + cv * V;
+            const Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + at);
+            Pack<T, V> dy = *(const Pack<T, V>*)((const T*)a.dy + at);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float h = (as_f32(x.v[i]) - mean[i]) * r[i], dz = as_f32(dy.v[i]) * act_grad<ACT>(fmaf(h, w[i], s[i]));
+                dy.v[i] = as<T>(r[i] * (w[i] * dz - m1[i] - h * m2[i]));
+            }
+            *(Pack<T, V>*)((T*)a.dx + at) = dy;
+        }
+    }
+}
+
+// Sums the rows of `in` (rows, cols) that belong to block row blockIdx.y: 64 columns by 4 row lanes, joined in order. The last
+// round (one block row) writes the first half of the columns to dweight and the rest to dbias.
+__global__ void __launch_bounds__(256) k_norm_colsum(const float* in, int64_t rows, int cols, float* out, float* dweight, float* dbias) {
+    __shared__ float s[4][64];
+    const int c = blockIdx.x * 64 + threadIdx.x % 64, r0 = threadIdx.x / 64;
+    float sum = 0.f;
+    if (c < cols)
+        for (int64_t r = (int64_t)blockIdx.y * 4 + r0; r < rows; r += 4 * (int64_t)gridDim.y) sum += in[r * cols + c];
+    s[r0][threadIdx.x % 64] = sum;
+    __syncthreads();
+    if (r0 || c >= cols) return;
+    sum = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
+    if (out) out[(int64_t)blockIdx.y * cols + c] = sum;
+    else if (c < cols / 2) dweight[c] = sum;
+    else dbias[c - cols / 2] = sum;
+}
+
+constexpr int NORM_SUM_ROWS = 256;   // rows that the first round of column sums leaves
+
+// rows of (2, C) sums -> dweight, dbias, in two rounds where there are many rows; `spare` holds NORM_SUM_ROWS rows.
+inline int norm_colsum(const MoNorm& a, const float* rows_of, int64_t rows, float* spare, hipStream_t s) {
+    const int cols = 2 * a.C;
+    const dim3 grid((unsigned)((cols + 63) / 64));
+    if (rows > NORM_SUM_ROWS) {
+        hipLaunchKernelGGL(k_norm_colsum, dim3(grid.x, NORM_SUM_ROWS), dim3(256), 0, s, rows_of, rows, cols, spare, nullptr, nullptr);
+        if (launched("k_norm_colsum")) return -1;
+        rows_of = spare;
+        rows = NORM_SUM_ROWS;
+    }
+    hipLaunchKernelGGL(k_norm_colsum, grid, dim3(256), 0, s, rows_of, rows, cols, nullptr, a.dweight, a.dbias);
+    return launched("k_norm_colsum");
+}
+
+// ---- host side
+inline bool norm_wide(const MoNorm& a) {   // 8 channels an access (of 16 bytes, or two of them)
+    uintptr_t p = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.dx;
+    return a.C % 8 == 0 && p % 16 == 0;
+}
+
+// Slabs: enough blocks for the chip where samples are few, and at least 16 KB of a sample in each.
+inline NormCut norm_cut(const MoNorm& a, int V) {
+    NormCut c;
+    const int64_t per_px = (int64_t)a.C * (a.dtype == MO_BF16 ? 2 : 4);
+    const int64_t most = std::max<int64_t>(1, a.S * per_px / (16 << 10)), want = std::max<int64_t>(1, 4096 / std::max<int64_t>(1, a.B));
+    c.px = (a.S + std::min(most, want) - 1) / std::min(most, want);
+    c.slabs = (a.S + c.px - 1) / c.px;
+    c.nv = a.C / V;
+    c.LN = std::min(c.nv, NORM_THREADS);
+    c.PL = NORM_THREADS / c.LN;
+    return c;
+}
+
+struct NormWork { int64_t part, means, spare, total; };   // in floats
+inline NormWork norm_general_work(const MoNorm& a, const NormCut& c, bool backward) {
+    NormWork w;
+    w.part = a.B * c.slabs * 2 * a.C;
+    w.means = a.B * a.groups * 2;
+    w.spare = backward ? (int64_t)NORM_SUM_ROWS * 2 * a.C : 0;
+    w.total = w.part + w.means + w.spare;
+    return w;
+}
+
+template <class T, int V, int ACT> int norm_general(const MoNorm& a, bool backward, hipStream_t s) {
+    NormArgs k{a, norm_cut(a, V), nullptr, nullptr};
+    const NormWork w = norm_general_work(a, k.c, backward);
+    k.part = (float*)a.work;
+    k.means = k.part + w.part;
+    const dim3 grid((unsigned)(a.B * k.c.slabs)), per_group((unsigned)(a.B * a.groups));
+    if (!backward) {
+        if (a.stats) k.means = a.stats;
+        hipLaunchKernelGGL((k_norm_moments<T, V>), grid, dim3(NORM_THREADS), 0, s, k);
+        hipLaunchKernelGGL(k_norm_means, per_group, dim3(kWave), 0, s, k);
+        hipLaunchKernelGGL((k_norm_apply<T, V, ACT>), grid, dim3(NORM_THREADS), 0, s, k);
+        return launched("k_norm_apply");
+    }
+    hipLaunchKernelGGL((k_norm_sums<T, V, ACT>), grid, dim3(NORM_THREADS), 0, s, k);
+    hipLaunchKernelGGL(k_norm_dmeans, per_group, dim3(kWave), 0, s, k);
+    hipLaunchKernelGGL((k_norm_dx<T, V, ACT>), grid, dim3(NORM_THREADS), 0, s, k);
+    if (launched("k_norm_dx")) return -1;
+    return a.dweight ? norm_colsum(a, k.part, a.B * k.c.slabs, k.part + w.part + w.means, s) : 0;
+}
+
+}  // namespace mo

@@ -13,10 +13,12 @@ import os
 LIB_ENV_VAR = "MARIO_HIP_LIB"
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libmario_hip.so"
+OPS_LIB_NAME = "libmario_ops.so"
 
 _P = ctypes.c_void_p
 _i64, _i32, _dbl = ctypes.c_int64, ctypes.c_int, ctypes.c_double
 _lib = None
+_ops = None
 
 
 def lib_path() -> str:
@@ -84,6 +86,55 @@ def lib() -> ctypes.CDLL:
     L.mh_timing_read.argtypes = [_P, _P, _P]
     _lib = L
     return L
+
+
+class MoRows(ctypes.Structure):
+    _fields_ = [("p", _P), ("st", _i64), ("sn", _i64), ("sh", _i64)]
+
+
+class MoAttend(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "H", "D", "E")] + [("T", _i64), ("N", _i64), ("scale", ctypes.c_float)]
+                + [(n, MoRows) for n in ("q", "k", "v", "out")]
+                + [(n, _P) for n in ("decay", "start", "state", "state_out", "saved", "work")]
+                + [(n, MoRows) for n in ("dout", "dq", "dk", "dv")] + [("dstate_out", _P), ("dstate", _P)])
+
+
+class MoNorm(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "act", "C", "groups")] + [("B", _i64), ("S", _i64), ("eps", ctypes.c_float)]
+                + [(n, _P) for n in ("x", "weight", "bias", "y", "stats", "work", "dy", "dx", "dweight", "dbias")])
+
+
+def ops_lib() -> ctypes.CDLL:
+    """libmario_ops.so: the operators of a policy with a memory (include/mario_ops.h)."""
+    global _ops
+    if _ops is not None:
+        return _ops
+    path = os.path.join(HERE, OPS_LIB_NAME)
+    if not os.path.isfile(path):
+        raise NativeLibraryError(
+            f"fast_mario_env_amd: {path} is missing. Build it with `python -c \"import __graft_entry__ as g; "
+            f"g.build()\"` from the repository root (needs hipcc with gfx950 support).")
+    L = ctypes.CDLL(path)
+    L.mo_last_error.restype = ctypes.c_char_p
+    attend, norm = ctypes.POINTER(MoAttend), ctypes.POINTER(MoNorm)
+    L.mo_attend_saved.restype = L.mo_attend_work.restype = L.mo_group_norm_work.restype = _i64
+    L.mo_attend_saved.argtypes = [attend]
+    L.mo_attend_work.argtypes = [attend, _i32]
+    for f in (L.mo_attend, L.mo_attend_backward):
+        f.argtypes = [attend, _P]
+    rows = ctypes.POINTER(MoRows)
+    L.mo_attend_step.argtypes = [_i32, _i64, _i32, _i32, _i32, ctypes.c_float, rows, rows, rows, _P, _P, _P, rows, _P]
+    L.mo_group_norm_work.argtypes = [norm, _i32]
+    for f in (L.mo_group_norm, L.mo_group_norm_backward):
+        f.argtypes = [norm, _P]
+    _ops = L
+    return L
+
+
+def ops_check(rc: int, what: str) -> int:
+    if rc < 0:
+        raise RuntimeError(f"{what} failed: {ops_lib().mo_last_error().decode(errors='replace')}")
+    return rc
 
 
 def check(rc: int, what: str) -> None:

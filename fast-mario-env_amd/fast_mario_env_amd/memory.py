@@ -1,0 +1,337 @@
+"""The operators of a policy that remembers its episode, on the GPU.
+
+The reference's policy sees four stacked frames and keeps nothing between steps (src/fast_mario_env/ppo/model.py:13-38). A
+memory of fixed size per env goes on where the stack ends:
+
+- `linear_attention`: over a stored rollout (T, N), each head's memory a matrix that decays by the head's factor each step and
+  is cleared where an episode starts; with the gradients of training.
+- `linear_attention_step`: one step of the same for every env, the memories updated in place: what acting needs.
+- `group_norm_act`: group norm and an activation over channels-last features: of the memory's output (a group a head; its size
+  grows with the episode) and of convolutions; with its gradients.
+
+Float32 or bf16 in and out, sums and states in float32. On the GPU they are HIP kernels (libmario_ops.so, include/mario_ops.h),
+queued on torch's current stream. CPU tensors, and what torch traces or transforms, take torch operations.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from .rollout import _torch, _transformed
+
+ACTS = {"none": 0, "relu": 1, "silu": 2}
+MAX_HEAD = 128
+
+
+def _kernel_takes(*ts):
+    """Whether a kernel called by address computes these: plain tensors on a GPU that nothing traces or transforms."""
+    torch = _torch()
+    return (all(type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and not t.is_neg() for t in ts)
+            and not _transformed(*ts))
+
+
+def _dtype(t):
+    return {_torch().float32: 0, _torch().bfloat16: 1}[t.dtype]
+
+
+def _rows(t):
+    """The tensor's head vectors (T, N, H, d) or (N, H, d) as the library takes them; the last dimension is contiguous."""
+    from ._native import MoRows
+    st = t.stride() if t.dim() == 4 else (0,) + t.stride()
+    return MoRows(t.data_ptr(), *st[:3])
+
+
+def _last_contiguous(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _work(nbytes, device):
+    torch = _torch()
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _stream(device):
+    return _torch().cuda.current_stream(device).cuda_stream
+
+
+def head_decays(heads: int, device="cuda"):
+    """Factors (heads,) whose memories last from about 22 steps (half-life) to about 1,400: 1 - 2^-5 .. 1 - 2^-11."""
+    torch = _torch()
+    return (1.0 - 2.0 ** -torch.linspace(5.0, 11.0, heads, dtype=torch.float64)).float().to(device)
+
+
+# ---------------------------------------------------------------- linear attention
+def _check_attend(name, lead, q, k, v, decay, start, state):
+    torch = _torch()
+    H, D, E = q.shape[-2], q.shape[-1], v.shape[-1]
+    if (q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype or tuple(k.shape) != tuple(q.shape)
+            or tuple(v.shape[:-1]) != tuple(q.shape[:-1]) or not (1 <= D <= MAX_HEAD and 1 <= E <= MAX_HEAD) or H < 1):
+        raise ValueError(f"{name}: q and k must be ({lead}, H, D), v ({lead}, H, E), all float32 or all bf16, head sizes 1 .. {MAX_HEAD}")
+    if decay.dtype != torch.float32 or tuple(decay.shape) != (H,):
+        raise ValueError(f"{name}: decay must be ({H},) float32")
+    if decay.requires_grad:
+        raise ValueError(f"{name}: decay is a constant of the heads: it has no gradient here")
+    if start is not None and (start.dtype != torch.bool or tuple(start.shape) != tuple(q.shape[:-2])):
+        raise ValueError(f"{name}: start must be ({lead}) bool")
+    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != (q.shape[-3], H, D, E)):
+        raise ValueError(f"{name}: state must be (N, H, D, E) = {(q.shape[-3], H, D, E)} float32")
+    if any(t is not None and t.device != q.device for t in (k, v, decay, start, state)):
+        raise ValueError(f"{name}: all tensors must be on the device of q ({q.device})")
+
+
+def _attend_args(q, k, v, decay, start, scale):
+    from ._native import MoAttend
+    T, N, H, D = q.shape
+    a = MoAttend(dtype=_dtype(q), H=H, D=D, E=v.shape[-1], T=T, N=N, scale=scale, q=_rows(q), k=_rows(k), v=_rows(v),
+                 decay=decay.data_ptr(), start=_ptr(start))
+    return a
+
+
+def _attend_forward(q, k, v, decay, start, state, scale, keep):
+    """out, state_out and what the gradient takes up (None unless `keep`)."""
+    torch = _torch()
+    from ._native import ops_check, ops_lib
+    L, dev = ops_lib(), q.device
+    with torch.cuda.device(dev):
+        a = _attend_args(q, k, v, decay, start, scale)
+        out = torch.empty(q.shape[:3] + v.shape[-1:], dtype=q.dtype, device=dev)
+        state_out = torch.empty(q.shape[1:] + v.shape[-1:], dtype=torch.float32, device=dev)
+        a.out, a.state, a.state_out = _rows(out), _ptr(state), state_out.data_ptr()
+        saved = _work(ops_check(L.mo_attend_saved(a), "mo_attend_saved"), dev) if keep else None
+        work = _work(ops_check(L.mo_attend_work(a, 0), "mo_attend_work"), dev)
+        a.saved, a.work = _ptr(saved), _ptr(work)
+        ops_check(L.mo_attend(a, _stream(dev)), "mo_attend")
+    return out, state_out, saved
+
+
+def _attend_backward(q, k, v, decay, start, state, saved, scale, dout, dstate_out, want_dstate):
+    torch = _torch()
+    from ._native import ops_check, ops_lib
+    L, dev = ops_lib(), q.device
+    with torch.cuda.device(dev):
+        a = _attend_args(q, k, v, decay, start, scale)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        dstate = torch.empty(q.shape[1:] + v.shape[-1:], dtype=torch.float32, device=dev) if want_dstate else None
+        a.state, a.saved, a.dstate_out, a.dstate = _ptr(state), _ptr(saved), _ptr(dstate_out), _ptr(dstate)
+        a.dout, a.dq, a.dk, a.dv = _rows(dout), _rows(dq), _rows(dk), _rows(dv)
+        work = _work(ops_check(L.mo_attend_work(a, 1), "mo_attend_work"), dev)
+        a.work = _ptr(work)
+        ops_check(L.mo_attend_backward(a, _stream(dev)), "mo_attend_backward")
+    return dq, dk, dv, dstate
+
+
+_functions = {}
+
+
+def _function(name):
+    """The autograd functions, made on first use (torch is imported late throughout this package)."""
+    if _functions:
+        return _functions[name]
+    torch = _torch()
+    once = torch.autograd.function.once_differentiable
+
+    class Attend(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, v, decay, start, state, scale):
+            out, state_out, saved = _attend_forward(q, k, v, decay, start, state, scale, True)
+            ctx.save_for_backward(q, k, v, decay, start, state, saved)
+            ctx.scale = scale
+            ctx.set_materialize_grads(False)
+            return out, state_out
+
+        @staticmethod
+        @once
+        def backward(ctx, dout, dstate_out):
+            q, k, v, decay, start, state, saved = ctx.saved_tensors
+            if dout is None:
+                dout = torch.zeros(1, dtype=q.dtype, device=q.device).expand(v.shape)
+            dout = _last_contiguous(dout)
+            if dstate_out is not None:
+                dstate_out = dstate_out.contiguous()
+            dq, dk, dv, dstate = _attend_backward(q, k, v, decay, start, state, saved, ctx.scale, dout, dstate_out,
+                                                  state is not None and ctx.needs_input_grad[5])
+            return dq, dk, dv, None, None, dstate, None
+
+    class Norm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, groups, weight, bias, eps, act):
+            y, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
+            ctx.save_for_backward(x, weight, bias, stats)
+            ctx.how = (groups, eps, act)
+            return y
+
+        @staticmethod
+        @once
+        def backward(ctx, dy):
+            x, weight, bias, stats = ctx.saved_tensors
+            dx, dw, db = _norm_backward(x, weight, bias, stats, dy.contiguous(), *ctx.how, any(ctx.needs_input_grad[2:4]))
+            return dx, None, dw, db, None, None
+
+    _functions.update(attend=Attend, norm=Norm)
+    return _functions[name]
+
+
+def _attend_plain(q, k, v, decay, start, state, scale):
+    """The recurrence step by step in torch operations, in float32."""
+    torch = _torch()
+    S = q.new_zeros(q.shape[1:] + v.shape[-1:], dtype=torch.float32) if state is None else state
+    g, out = decay[:, None, None], []
+    for t in range(q.shape[0]):
+        S = g * S
+        if start is not None:
+            S = torch.where(start[t][:, None, None, None], torch.zeros_like(S), S)
+        S = S + k[t].float()[..., :, None] * v[t].float()[..., None, :]
+        out.append((q[t].float()[..., :, None] * S).sum(-2) * scale)
+    out = torch.stack(out).to(q.dtype) if out else v.new_empty(v.shape)
+    return out, S.clone() if S is state else S
+
+
+def linear_attention(q, k, v, decay, start=None, state=None, scale=None):
+    """Linear attention with a decay for each head over T steps of N envs. With g = decay[h], of each env and head:
+
+        S_t = (0 where start[t], else g S_{t-1}) + k_t v_t^T,    out_t = scale S_t^T q_t,    S_{-1} = state
+
+    q, k (T, N, H, D) and v (T, N, H, E), all float32 or all bf16, head sizes up to 128, any strides (views of a fused
+    projection are taken as they lie); decay (H,) float32 in [0, 1], a constant without gradient (`head_decays`); start (T, N)
+    bool, the steps that start an episode, as `gae` takes them: nothing of an episode reaches the next one; state (N, H, D, E)
+    float32 or None for zeros; scale: 1/sqrt(D) if None. Returns out (T, N, H, E) in the type of q and the state after the last
+    step, float32. Differentiable once in q, k, v and state.
+
+    Sums and states are float32. With bf16 inputs the masked products of a chunk and the state that multiplies q are rounded to
+    bf16 where they enter a matrix product; the state itself is not."""
+    torch = _torch()
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("linear_attention: q, k and v must be (T, N, H, head size)")
+    _check_attend("linear_attention", "T, N", q, k, v, decay, start, state)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    every = [t for t in (q, k, v, decay, start, state) if t is not None]
+    if not _kernel_takes(*every):
+        return _attend_plain(q, k, v, decay, start, state, scale)
+    q, k, v = (_last_contiguous(t) for t in (q, k, v))
+    decay = decay.contiguous()
+    start = None if start is None else start.contiguous()
+    state = None if state is None else state.contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in every):
+        return _function("attend").apply(q, k, v, decay, start, state, scale)
+    return _attend_forward(q, k, v, decay, start, state, scale, False)[:2]
+
+
+def linear_attention_step(q, k, v, decay, state, start=None, scale=None):
+    """One step of `linear_attention` for every env: q, k (N, H, D), v (N, H, E), start (N,) bool or None; state (N, H, D, E)
+    float32, contiguous, is updated in place. Returns out (N, H, E) in the type of q. No gradient."""
+    torch = _torch()
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("linear_attention_step: q, k and v must be (N, H, head size)")
+    _check_attend("linear_attention_step", "N", q, k, v, decay, start, state)
+    if not state.is_contiguous():
+        raise ValueError("linear_attention_step: state is updated in place and must be contiguous")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+        raise ValueError("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention to train")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if not _kernel_takes(*(t for t in (q, k, v, decay, state, start) if t is not None)):
+        out, S = _attend_plain(q[None], k[None], v[None], decay, None if start is None else start[None], state, scale)
+        state.copy_(S)
+        return out[0]
+    from ._native import ops_check, ops_lib
+    q, k, v = (_last_contiguous(t) for t in (q, k, v))
+    decay = decay.contiguous()
+    start = None if start is None else start.contiguous()
+    N, H, D = q.shape
+    with torch.cuda.device(q.device):
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
+        ops_check(ops_lib().mo_attend_step(_dtype(q), N, H, D, v.shape[-1], scale, _rows(q), _rows(k), _rows(v), decay.data_ptr(),
+                                           _ptr(start), state.data_ptr(), _rows(out), _stream(q.device)), "mo_attend_step")
+    return out
+
+
+# ---------------------------------------------------------------- group norm and activation
+def _norm_args(x, groups, weight, bias, eps, act):
+    from ._native import MoNorm
+    B, C = x.shape[0], x.shape[-1]
+    return MoNorm(dtype=_dtype(x), act=ACTS[act], C=C, groups=groups, B=B, S=x.shape[1], eps=eps, x=x.data_ptr(),
+                  weight=_ptr(weight), bias=_ptr(bias))
+
+
+def _norm_forward(x, groups, weight, bias, eps, act, keep):
+    """y and, if `keep`, each group's mean and 1 / deviation, of x (B, S, C) contiguous."""
+    torch = _torch()
+    from ._native import ops_check, ops_lib
+    L, dev = ops_lib(), x.device
+    with torch.cuda.device(dev):
+        y = torch.empty_like(x)
+        stats = torch.empty(x.shape[0], groups, 2, dtype=torch.float32, device=dev) if keep else None
+        a = _norm_args(x, groups, weight, bias, eps, act)
+        a.y, a.stats = y.data_ptr(), _ptr(stats)
+        work = _work(ops_check(L.mo_group_norm_work(a, 0), "mo_group_norm_work"), dev)
+        a.work = _ptr(work)
+        ops_check(L.mo_group_norm(a, _stream(dev)), "mo_group_norm")
+    return y, stats
+
+
+def _norm_backward(x, weight, bias, stats, dy, groups, eps, act, want_params):
+    torch = _torch()
+    from ._native import ops_check, ops_lib
+    L, dev = ops_lib(), x.device
+    with torch.cuda.device(dev):
+        dx = torch.empty_like(x)
+        dw = db = None
+        if want_params and weight is not None:
+            dw, db = (torch.empty if x.shape[0] else torch.zeros)((2,) + weight.shape, dtype=torch.float32, device=dev)
+        a = _norm_args(x, groups, weight, bias, eps, act)
+        a.stats, a.dy, a.dx, a.dweight, a.dbias = stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db)
+        work = _work(ops_check(L.mo_group_norm_work(a, 1), "mo_group_norm_work"), dev)
+        a.work = _ptr(work)
+        ops_check(L.mo_group_norm_backward(a, _stream(dev)), "mo_group_norm_backward")
+    return dx, dw, db
+
+
+def _norm_plain(x, groups, weight, bias, eps, act):
+    """The same in torch operations, in float32."""
+    torch = _torch()
+    y = x.float().reshape(x.shape[0], groups, x.shape[1] // groups, -1)
+    d = y - y.mean((2, 3), keepdim=True)
+    z = (d * torch.rsqrt(d.square().mean((2, 3), keepdim=True) + eps)).reshape(x.shape)
+    if weight is not None:
+        one = (1, -1) + (1,) * (x.dim() - 2)
+        z = z * weight.float().view(one) + bias.float().view(one)
+    z = z.clamp(min=0.0) if act == "relu" else z * torch.sigmoid(z) if act == "silu" else z
+    return z.to(x.dtype)
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
+    """act(group_norm(x)): x (B, C, ...) float32 or bf16, its channels in `groups` groups of consecutive ones, each normalised
+    over the group's channels and all positions of a sample (biased variance), scaled and shifted per channel by weight and
+    bias (C,) (both or neither; float32, other float types are converted), then act: "none", "relu" or "silu". All in float32,
+    rounded once. The result has x's type and lies channels last, as x does (`memory_format=torch.channels_last`, or (B, C));
+    an x that lies otherwise is copied first. Differentiable once."""
+    torch = _torch()
+    if x.dim() < 2 or x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("group_norm_act: x must be (B, C, ...) float32 or bf16")
+    C = x.shape[1]
+    if not isinstance(groups, int) or groups < 1 or C < 1 or C % groups:
+        raise ValueError(f"group_norm_act: {C} channels do not fall into {groups} equal groups")
+    if act not in ACTS:
+        raise ValueError(f"group_norm_act: act must be one of {', '.join(ACTS)}")
+    if not eps >= 0:
+        raise ValueError("group_norm_act: eps must be >= 0")
+    if (weight is None) != (bias is None):
+        raise ValueError("group_norm_act: weight and bias go together")
+    if weight is not None and any(tuple(p.shape) != (C,) or not p.is_floating_point() or p.device != x.device for p in (weight, bias)):
+        raise ValueError(f"group_norm_act: weight and bias must be ({C},) on the device of x ({x.device})")
+    if x.dim() > 2 and x[0, 0].numel() == 0 if x.shape[0] else False:
+        raise ValueError("group_norm_act: a sample has no positions")
+    every = [t for t in (x, weight, bias) if t is not None]
+    if not _kernel_takes(*every):
+        return _norm_plain(x, groups, weight, bias, eps, act)
+    last = x.movedim(1, -1)
+    rows = last.contiguous().view(x.shape[0], -1, C) if x.shape[0] else last.reshape(0, 1, C)
+    if weight is not None:
+        weight, bias = weight.float().contiguous(), bias.float().contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in every):
+        y = _function("norm").apply(rows, groups, weight, bias, eps, act)
+    else:
+        y = _norm_forward(rows, groups, weight, bias, eps, act, False)[0]
+    return y.view(last.shape).movedim(-1, 1)
