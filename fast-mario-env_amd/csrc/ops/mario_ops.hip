@@ -2,6 +2,7 @@
 // is built for bit-exact float sums and scalar code, these for matrix instructions and memory.
 #include <algorithm>
 
+#include "attend_chunk_back.hpp"
 #include "attend_step.hpp"
 #include "attend_walk.hpp"
 #include "common.hpp"
@@ -43,6 +44,18 @@ bool norm_sizes(const MoNorm* a) {
 
 template <class F> int by_type(int dtype, F f) { return dtype == MO_BF16 ? f(bf16{}) : f(float{}); }
 
+// Heads in whole 16-byte pieces go by chunks on the matrix cores, the rest step by step.
+template <class T> int attend_forward(const MoAttend& a, hipStream_t s) {
+    if (!chunks_take(a, false)) return walk_forward<T>(a, s);
+    const int p = padded_head(a);
+    return p == 32 ? attend_chunks<T, 32>(a, s) : p == 64 ? attend_chunks<T, 64>(a, s) : attend_chunks<T, 128>(a, s);
+}
+template <class T> int attend_back(const MoAttend& a, hipStream_t s) {
+    if (!chunks_take(a, true) || (!a.saved && attend_cut(a, 1).chunks > 1)) return walk_backward<T>(a, s);
+    const int p = padded_head(a);
+    return p == 32 ? attend_back_chunks<T, 32>(a, s) : p == 64 ? attend_back_chunks<T, 64>(a, s) : attend_back_chunks<T, 128>(a, s);
+}
+
 // No C++ exception leaves a C entry point.
 template <class F> auto guarded(F f) noexcept -> decltype(f()) {
     try {
@@ -73,11 +86,17 @@ extern "C" {
 const char* mo_last_error(void) { return g_err.c_str(); }
 
 int64_t mo_attend_saved(const MoAttend* a) {
-    return guarded([&]() -> int64_t { return attend_sizes(a) ? 0 : -1; });
+    return guarded([&]() -> int64_t {
+        if (!attend_sizes(a)) return -1;
+        return chunks_take(*a, false) ? a->N * a->H * (attend_cut(*a, 1).chunks - 1) * a->D * a->E * (int64_t)size_of(a->dtype) : 0;
+    });
 }
 
-int64_t mo_attend_work(const MoAttend* a, int) {
-    return guarded([&]() -> int64_t { return attend_sizes(a) ? 0 : -1; });
+int64_t mo_attend_work(const MoAttend* a, int backward) {
+    return guarded([&]() -> int64_t {
+        if (!attend_sizes(a)) return -1;
+        return chunks_take(*a, backward) ? cut_bytes(*a, attend_cut(*a, backward ? BACKWARD_PER_CU : FORWARD_PER_CU)) : 0;
+    });
 }
 
 int mo_attend(const MoAttend* a, void* stream) {
@@ -90,7 +109,9 @@ int mo_attend(const MoAttend* a, void* stream) {
         if (!usable(a->decay, "decay", 4) || !usable(a->state_out, "state_out", 4) || (a->state && !usable(a->state, "state", 4)) ||
             (a->T && a->start && !usable(a->start, "start", 1)))
             return -1;
-        return by_type(a->dtype, [&](auto t) { return walk_forward<decltype(t)>(*a, (hipStream_t)stream); });
+        if (mo_attend_work(a, 0) > 0 && !usable(a->work, "work", 16)) return -1;
+        if (a->saved && mo_attend_saved(a) > 0 && !usable(a->saved, "saved", 16)) return -1;
+        return by_type(a->dtype, [&](auto t) { return attend_forward<decltype(t)>(*a, (hipStream_t)stream); });
     });
 }
 
@@ -105,7 +126,9 @@ int mo_attend_backward(const MoAttend* a, void* stream) {
         if (!usable(a->decay, "decay", 4) || (a->state && !usable(a->state, "state", 4)) || (a->T && a->start && !usable(a->start, "start", 1)) ||
             (a->dstate_out && !usable(a->dstate_out, "dstate_out", 4)) || (a->dstate && !usable(a->dstate, "dstate", 4)))
             return -1;
-        return by_type(a->dtype, [&](auto t) { return walk_backward<decltype(t)>(*a, (hipStream_t)stream); });
+        if (mo_attend_work(a, 1) > 0 && !usable(a->work, "work", 16)) return -1;
+        if (a->saved && mo_attend_saved(a) > 0 && !usable(a->saved, "saved", 16)) return -1;
+        return by_type(a->dtype, [&](auto t) { return attend_back<decltype(t)>(*a, (hipStream_t)stream); });
     });
 }
 

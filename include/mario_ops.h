@@ -57,7 +57,9 @@ typedef struct MoAttend {
     float* dstate;
 } MoAttend;
 
-/* Bytes of `saved`, and of `work` for the forward (backward = 0) or backward call; sizes and strides have to be set. */
+/* Bytes of `saved`, and of `work` for the forward (backward = 0) or backward call; sizes and the rows of q, k, v (and dout)
+ * have to be set. Heads of whole 16-byte pieces whose rows lie on 16 bytes go by chunks of steps on the matrix cores; others
+ * go step by step and need neither. */
 int64_t mo_attend_saved(const MoAttend* a);
 int64_t mo_attend_work(const MoAttend* a, int backward);
 int mo_attend(const MoAttend* a, void* stream);
