@@ -6,7 +6,7 @@
 #include "attend_step.hpp"
 #include "attend_walk.hpp"
 #include "common.hpp"
-#include "norm_general.hpp"
+#include "norm_small.hpp"
 
 using namespace mo;
 
@@ -66,17 +66,28 @@ template <class F> auto guarded(F f) noexcept -> decltype(f()) {
     }
 }
 
-template <class T, int V> int norm_by_act(const MoNorm& a, bool backward, hipStream_t s) {
-    if (a.act == MO_ACT_RELU) return norm_general<T, V, MO_ACT_RELU>(a, backward, s);
-    if (a.act == MO_ACT_SILU) return norm_general<T, V, MO_ACT_SILU>(a, backward, s);
-    return norm_general<T, V, MO_ACT_NONE>(a, backward, s);
+template <class F> int by_act(int act, F f) {
+    if (act == MO_ACT_RELU) return f(std::integral_constant<int, MO_ACT_RELU>{});
+    if (act == MO_ACT_SILU) return f(std::integral_constant<int, MO_ACT_SILU>{});
+    return f(std::integral_constant<int, MO_ACT_NONE>{});
 }
 
 int norm_run(const MoNorm& a, bool backward, hipStream_t s) {
     return by_type(a.dtype, [&](auto t) {
         typedef decltype(t) T;
-        return norm_wide(a) ? norm_by_act<T, 8>(a, backward, s) : norm_by_act<T, 1>(a, backward, s);
+        return by_act(a.act, [&](auto act) {
+            constexpr int A = decltype(act)::value;
+            SmallCut c;
+            if (norm_small_takes(a, backward, c)) return norm_small<T, A>(a, c, backward, s);
+            return norm_wide(a) ? norm_general<T, 8, A>(a, backward, s) : norm_general<T, 1, A>(a, backward, s);
+        });
     });
+}
+
+int64_t norm_work(const MoNorm& a, bool backward) {
+    SmallCut c;
+    if (norm_small_takes(a, backward, c)) return 4 * norm_small_work(a, c, backward);
+    return 4 * norm_general_work(a, norm_cut(a, norm_wide(a) ? 8 : 1), backward).total;
 }
 
 }  // namespace
@@ -151,7 +162,7 @@ int mo_attend_step(int dtype, int64_t N, int H, int D, int E, float scale, const
 int64_t mo_group_norm_work(const MoNorm* a, int backward) {
     return guarded([&]() -> int64_t {
         if (!norm_sizes(a)) return -1;
-        return 4 * norm_general_work(*a, norm_cut(*a, norm_wide(*a) ? 8 : 1), backward != 0).total;
+        return norm_work(*a, backward != 0);
     });
 }
 
@@ -161,7 +172,7 @@ int mo_group_norm(const MoNorm* a, void* stream) {
         if (a->B == 0) return 0;
         const size_t z = size_of(a->dtype);
         if (!usable(a->x, "x", z) || !usable(a->y, "y", z) || (a->weight && (!usable(a->weight, "weight", 4) || !usable(a->bias, "bias", 4))) ||
-            (a->stats && !usable(a->stats, "stats", 4)) || !usable(a->work, "work", 16))
+            (a->stats && !usable(a->stats, "stats", 4)) || (norm_work(*a, false) && !usable(a->work, "work", 16)))
             return -1;
         return norm_run(*a, false, (hipStream_t)stream);
     });
@@ -175,7 +186,8 @@ int mo_group_norm_backward(const MoNorm* a, void* stream) {
         const size_t z = size_of(a->dtype);
         if (!usable(a->x, "x", z) || !usable(a->dy, "dy", z) || !usable(a->dx, "dx", z) || !usable(a->stats, "stats", 4) ||
             (a->weight && (!usable(a->weight, "weight", 4) || !usable(a->bias, "bias", 4))) ||
-            (a->dweight && (!usable(a->dweight, "dweight", 4) || !usable(a->dbias, "dbias", 4))) || !usable(a->work, "work", 16))
+            (a->dweight && (!usable(a->dweight, "dweight", 4) || !usable(a->dbias, "dbias", 4))) ||
+            (norm_work(*a, true) && !usable(a->work, "work", 16)))
             return -1;
         return norm_run(*a, true, (hipStream_t)stream);
     });

@@ -1,0 +1,265 @@
+// Group norm with an activation where a sample fits a workgroup's registers: read once.
+#pragma once
+#include "norm_general.hpp"
+
+namespace mo {
+
+// A team of W waves takes a sample, holds it as up to R packs of 8 channels a thread and goes on to its next sample. A thread has
+// the packs cv = t % NV (NV: packs a pixel, rounded up to a power of two; threads of packs that are not there idle) of the pixels
+// t / NV, t / NV + 64 W / NV, .., so its channels, their weights and their gradients' sums stay its own. Sums over a group are
+// shuffles over the lanes that hold it, and one exchange through LDS where the team has several waves (MULTI). The variance is
+// that of the values in registers about their mean: exact also where the mean is large.
+// WHOLE: groups are whole packs; else a group is 1, 2 or 4 channels, and sums are kept by channel up to the last step.
+struct Small {
+    MoNorm a;
+    int W, nv, NV, log_nv;     // waves a team; packs a pixel, and rounded up
+    int cg, vpg;               // channels a group; packs a group (WHOLE)
+    float* part;               // (blocks, 2, C): the blocks' sums for dweight and dbias
+};
+
+constexpr int SMALL_PACKS = 8, SMALL_PACKS_BACK = 4;   // packs a thread, at most
+constexpr int SMALL_WAVES = 8;                          // waves a team, at most
+constexpr int small_threads(bool multi) { return multi ? SMALL_WAVES * kWave : 256; }   // (one wave a sample: four samples a block)
+
+// The sums over a group's lanes, pixels and waves of a thread's NS values; x: a set for each of two exchanges in turn, so that
+// one barrier a sum is enough.
+template <bool MULTI, int NS, int SETS>
+__device__ __forceinline__ void group_sum(float (&s)[NS], const Small& k, float (*x)[kWave][NS], int turn) {
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int i = 0; i < NS; i++)
+        for (int m = k.NV; m < kWave; m *= 2) s[i] += __shfl_xor(s[i], m);
+    if (NS == SETS) {                                      // whole packs: a value a set
+        if ((k.vpg & (k.vpg - 1)) == 0) {
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+                for (int m = 1; m < k.vpg; m *= 2) s[i] += __shfl_xor(s[i], m);
+        } else {
+            const int cv = lane & (k.NV - 1), first = lane - cv + cv / k.vpg * k.vpg;
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                float t = 0.f;
+                for (int j = 0; j < k.vpg; j++) t += __shfl(s[i], first + j);
+                s[i] = t;
+            }
+        }
+    } else {                                               // neighbouring channels of a pack
+#pragma unroll
+        for (int m = 1; m < 4; m *= 2) {
+            float t[NS];
+#pragma unroll
+            for (int i = 0; i < NS; i++) t[i] = s[i] + s[i ^ m];
+#pragma unroll
+            for (int i = 0; i < NS; i++) s[i] = m < k.cg ? t[i] : s[i];
+        }
+    }
+    if (!MULTI) return;
+    x += turn * SMALL_WAVES;
+#pragma unroll
+    for (int i = 0; i < NS; i++) x[threadIdx.x / kWave][lane][i] = s[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NS; i++) s[i] = 0.f;
+    for (int j = 0; j < k.W; j++)
+#pragma unroll
+        for (int i = 0; i < NS; i++) s[i] += x[j][lane][i];
+}
+
+template <class T, bool MULTI, int R, int ACT, bool WHOLE>
+__global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
+    constexpr int NS = WHOLE ? 1 : 8;
+    typedef Pack<T, 8> P;
+    __shared__ float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][NS];
+    const MoNorm& a = k.a;
+    const int W = MULTI ? k.W : 1, TT = W * kWave, teams = MULTI ? 1 : 4;
+    const int t = MULTI ? threadIdx.x : threadIdx.x % kWave, cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
+    const bool live = cv < k.nv;
+    float w[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        w[i] = live && a.weight ? a.weight[cv * 8 + i] : 1.f;
+        s[i] = live && a.bias ? a.bias[cv * 8 + i] : 0.f;
+    }
+    const float by = 1.f / ((float)a.S * (float)k.cg);
+    for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / kWave); b < a.B; b += (int64_t)gridDim.x * teams) {
+        const T* in = (const T*)a.x + b * a.S * a.C + cv * 8;
+        P v[R];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (live && pl + r * PL < S) v[r] = *(const P*)(in + (int64_t)(pl + r * PL) * a.C);
+        float mean[NS] = {}, var[NS] = {};
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (live && pl + r * PL < S)
+#pragma unroll
+                for (int i = 0; i < 8; i++) mean[i % NS] += as_f32(v[r].v[i]);
+        group_sum<MULTI, NS, 1>(mean, k, x, 0);
+#pragma unroll
+        for (int i = 0; i < NS; i++) mean[i] *= by;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (live && pl + r * PL < S)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float d = as_f32(v[r].v[i]) - mean[i % NS];
+                    var[i % NS] = fmaf(d, d, var[i % NS]);
+                }
+        group_sum<MULTI, NS, 1>(var, k, x, 1);
+        float rstd[NS];
+#pragma unroll
+        for (int i = 0; i < NS; i++) rstd[i] = 1.f / sqrtf(fmaf(var[i], by, a.eps));
+        if (a.stats && pl == 0 && live)
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+                if ((cv * 8 + i) % k.cg == 0) {
+                    float* to = a.stats + 2 * (b * a.groups + (cv * 8 + i) / k.cg);
+                    to[0] = mean[i];
+                    to[1] = rstd[i];
+                }
+        T* out = (T*)a.y + b * a.S * a.C + cv * 8;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (live && pl + r * PL < S) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    v[r].v[i] = as<T>(act<ACT>(fmaf((as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS], w[i], s[i])));
+                *(P*)(out + (int64_t)(pl + r * PL) * a.C) = v[r];
+            }
+    }
+}
+
+template <class T, bool MULTI, int R, int ACT, bool WHOLE>
+__global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small_back(Small k) {
+    constexpr int NS = WHOLE ? 1 : 8;
+    typedef Pack<T, 8> P;
+    __shared__ union { float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][2 * NS]; float sums[MULTI ? SMALL_WAVES : 4][kWave][8]; } lds;
+    const MoNorm& a = k.a;
+    const int W = MULTI ? k.W : 1, TT = W * kWave, teams = MULTI ? 1 : 4, waves = MULTI ? k.W : 4;
+    const int t = MULTI ? threadIdx.x : threadIdx.x % kWave, cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
+    const bool live = cv < k.nv;
+    float w[8], s[8], dw[8] = {}, db[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        w[i] = live && a.weight ? a.weight[cv * 8 + i] : 1.f;
+        s[i] = live && a.bias ? a.bias[cv * 8 + i] : 0.f;
+    }
+    const float by = 1.f / ((float)a.S * (float)k.cg);
+    int turn = 0;
+    for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / kWave); b < a.B; b += (int64_t)gridDim.x * teams) {
+        const int64_t at = b * a.S * a.C + cv * 8;
+        P v[R], dy[R];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (live && pl + r * PL < S) {
+                v[r] = *(const P*)((const T*)a.x + at + (int64_t)(pl + r * PL) * a.C);
+                dy[r] = *(const P*)((const T*)a.dy + at + (int64_t)(pl + r * PL) * a.C);
+            }
+        float mean[NS], rstd[NS], m[2 * NS] = {};          // m: the sums of dh, then those of dh h
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const float* st = a.stats + 2 * (b * a.groups + (live ? (cv * 8 + i) / k.cg : 0));
+            mean[i] = st[0];
+            rstd[i] = st[1];
+        }
+        float h[R][8], dh[R][8];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (live && pl + r * PL < S)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    h[r][i] = (as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS];
+                    const float dz = as_f32(dy[r].v[i]) * act_grad<ACT>(fmaf(h[r][i], w[i], s[i]));
+                    dw[i] = fmaf(dz, h[r][i], dw[i]);
+                    db[i] += dz;
+                    dh[r][i] = dz * w[i];
+                    m[i % NS] += dh[r][i];
+                    m[NS + i % NS] = fmaf(dh[r][i], h[r][i], m[NS + i % NS]);
+                }
+        group_sum<MULTI, 2 * NS, 2>(m, k, lds.x, turn);
+        turn ^= 1;
+#pragma unroll
+        for (int i = 0; i < 2 * NS; i++) m[i] *= by;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (live && pl + r * PL < S) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    v[r].v[i] = as<T>(rstd[i % NS] * (dh[r][i] - fmaf(h[r][i], m[NS + i % NS], m[i % NS])));
+                *(P*)((T*)a.dx + at + (int64_t)(pl + r * PL) * a.C) = v[r];
+            }
+    }
+    if (!k.part) return;
+    // the block's sums for dweight and dbias: over the pixel lanes, then over its waves in order
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        for (int m = k.NV; m < kWave; m *= 2) {
+            dw[i] += __shfl_xor(dw[i], m);
+            db[i] += __shfl_xor(db[i], m);
+        }
+    for (int half = 0; half < 2; half++) {
+        __syncthreads();
+        if (threadIdx.x % kWave < k.NV)
+#pragma unroll
+            for (int i = 0; i < 8; i++) lds.sums[threadIdx.x / kWave][threadIdx.x % kWave][i] = half ? db[i] : dw[i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
+            float sum = 0.f;
+            for (int j = 0; j < waves; j++) sum += lds.sums[j][c / 8][c % 8];
+            k.part[((int64_t)blockIdx.x * 2 + half) * a.C + c] = sum;
+        }
+    }
+}
+
+// ---- host side
+struct SmallCut { int W, R, blocks; };
+
+// Whole packs a pixel, groups of whole packs or of 1, 2 or 4 channels, a pixel's packs within a wave, and a sample within a
+// team's registers; otherwise the sample goes through memory twice (norm_general).
+inline bool norm_small_takes(const MoNorm& a, bool backward, SmallCut& c) {
+    const int cg = a.C / a.groups;
+    if (!norm_wide(a) || a.C > 8 * kWave || (cg % 8 && 8 % cg)) return false;
+    int NV = 1;
+    while (NV < a.C / 8) NV *= 2;
+    const int most = backward ? SMALL_PACKS_BACK : SMALL_PACKS;
+    const int64_t packs = a.S * NV;
+    if (packs > (int64_t)SMALL_WAVES * kWave * most) return false;
+    for (c.W = 1; packs > (int64_t)c.W * kWave * most; c.W *= 2) {}
+    for (c.R = 1; packs > (int64_t)c.W * kWave * c.R; c.R *= 2) {}
+    const int per_block = c.W == 1 ? 4 : 1, waves = c.W == 1 ? 4 : c.W;
+    const int64_t blocks = (a.B + per_block - 1) / per_block, fill = (int64_t)compute_units() * std::max(1, (backward ? 16 : 32) / waves);
+    c.blocks = (int)std::min(blocks, fill);
+    return true;
+}
+
+template <class T, bool MULTI, int R, int ACT> int norm_small_run(const Small& k, const SmallCut& c, bool backward, hipStream_t s) {
+    const dim3 block(MULTI ? c.W * kWave : 256);
+    const auto go = [&](auto whole) {
+        constexpr bool G = decltype(whole)::value;
+        if (!backward) hipLaunchKernelGGL((k_norm_small<T, MULTI, R, ACT, G>), dim3(c.blocks), block, 0, s, k);
+        else if constexpr (R <= SMALL_PACKS_BACK) hipLaunchKernelGGL((k_norm_small_back<T, MULTI, R, ACT, G>), dim3(c.blocks), block, 0, s, k);
+        return launched("k_norm_small");
+    };
+    return k.cg % 8 == 0 ? go(std::true_type{}) : go(std::false_type{});
+}
+
+template <class T, int ACT> int norm_small(const MoNorm& a, const SmallCut& c, bool backward, hipStream_t s) {
+    const int cg = a.C / a.groups;
+    Small k{a, c.W, a.C / 8, 1, 0, cg, std::max(1, cg / 8), nullptr};
+    while (k.NV < k.nv) { k.NV *= 2; k.log_nv++; }
+    if (backward && a.dweight) k.part = (float*)a.work;
+    int rc;
+    if (c.W == 1 && c.R == 1) rc = norm_small_run<T, false, 1, ACT>(k, c, backward, s);
+    else if (c.W == 1 && c.R == 2) rc = norm_small_run<T, false, 2, ACT>(k, c, backward, s);
+    else if (c.W == 1 && c.R == 4) rc = norm_small_run<T, false, 4, ACT>(k, c, backward, s);
+    else if (c.W == 1) rc = norm_small_run<T, false, 8, ACT>(k, c, backward, s);
+    else if (backward) rc = norm_small_run<T, true, 4, ACT>(k, c, backward, s);
+    else rc = norm_small_run<T, true, 8, ACT>(k, c, backward, s);
+    if (rc || !k.part) return rc;
+    return norm_colsum(a, k.part, c.blocks, k.part + (int64_t)c.blocks * 2 * a.C, s);
+}
+
+inline int64_t norm_small_work(const MoNorm& a, const SmallCut& c, bool backward) {   // in floats
+    return backward && a.dweight ? ((int64_t)c.blocks + NORM_SUM_ROWS) * 2 * a.C : 0;
+}
+
+}  // namespace mo

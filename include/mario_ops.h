@@ -77,6 +77,7 @@ int mo_attend_step(int dtype, int64_t N, int H, int D, int E, float scale, const
  *   stats         (B, groups, 2) float32: mean and rstd out, for the gradient; NULL: not wanted
  *   work          mo_group_norm_work() bytes, 16-byte aligned (NULL if 0), free once the queued work is done
  * The gradient: dy (B, S, C) in, stats from the forward call; dx (B, S, C), dweight and dbias (C; both NULL: not wanted) out.
+ * work's size goes by the sizes, by the buffers' alignment and by whether dweight is wanted: set them before asking.
  * The sums over samples and pixels have a fixed order: the same inputs give the same bits. With B = 0 nothing is written. */
 typedef struct MoNorm {
     int32_t dtype, act, C, groups;
