@@ -19,11 +19,12 @@ template <class T, int P> struct Chunk {
     static constexpr int L = sizeof(T) == 2 ? 64 : 32;
     static constexpr int WAVES = P / 16, NT = WAVES * kWave;
     static constexpr int LT = L / 16, LB = L / 32, PB = P / 32, PT = P / 16;
-    static constexpr int PAD = 16 / sizeof(T), LD = P + PAD, LS = L + PAD;    // LDS row strides: 16 bytes past a power of two
-    static constexpr int EPV = 16 / sizeof(T), VPR = P / EPV, RV = L * VPR / NT;   // 16-byte accesses: a row's, a thread's
-    static constexpr int TILES = LT == 4 ? 12 : 4;                            // score tiles up to the diagonal's 32-blocks
-    static_assert(RV == 2 && L * VPR % NT == 0, "");
-    typedef T Tile[L][LD];
+    typedef mo::Tile<T, P> Rows;      // a chunk of q, k, v, ..
+    typedef mo::Tile<T, L> Scores;
+    static constexpr int STEP = NT / Rows::PIECES, RV = L / STEP;   // rows that the workgroup brings at a time, and times
+    static constexpr int TILES = LT == 4 ? 12 : 4;            // score tiles up to the diagonal's 32-blocks
+    static constexpr int TPW = (TILES + WAVES - 1) / WAVES;   // a wave's
+    static_assert(RV == 2 && STEP % 8 == 0, "");
 
     static __device__ __forceinline__ void score_tile(int idx, int& it, int& jt) {
         if (LT == 2 || idx < 4) { it = idx >> 1; jt = idx & 1; }
@@ -31,42 +32,52 @@ template <class T, int P> struct Chunk {
     }
 };
 
-// What a thread brings of one operand's tile: its 16-byte pieces, of which pieces past the chunk's end or the head's size
-// are zeros.
-template <class T, int P> struct Rows {
+// What a thread brings of one operand's chunk: a 16-byte piece of row `row` and of the one STEP further, straight into LDS.
+// Pieces past the chunk's end or the head's size are zeros (these go through registers).
+template <class T, int P> struct Bring {
     typedef Chunk<T, P> C;
-    const T* p[C::RV];
+    typedef typename C::Rows Rows;
+    const T* p;
     int64_t st;
-    int row[C::RV], col;
-    uint4 x[C::RV];
-    __device__ __forceinline__ void init(const MoRows& r, int64_t n, int h, int d) {
+    int col;                   // P where the head ends before the piece
+    bool whole;                // the head fills the rows
+    __device__ __forceinline__ Bring(const MoRows& r, int64_t n, int h, int d) {
+        const int row = threadIdx.x / Rows::PIECES;
+        col = ((int)(threadIdx.x % Rows::PIECES) ^ Rows::turn(row)) * C::Rows::EPV;
         st = r.st;
-        col = (int)(threadIdx.x % C::VPR) * C::EPV;
-#pragma unroll
-        for (int i = 0; i < C::RV; i++) {
-            row[i] = (int)threadIdx.x / C::VPR + i * (C::NT / C::VPR);
-            p[i] = (const T*)r.p + n * r.sn + h * r.sh + row[i] * r.st + col;
-            if (col >= d) row[i] = C::L;
-        }
+        p = (const T*)r.p + n * r.sn + h * r.sh + row * st + col;
+        whole = d == P;
+        if (col >= d) col = P;
     }
-    __device__ __forceinline__ void load(int64_t t0, int n) {
+    __device__ __forceinline__ void chunk(T* tile, int64_t t0, int n) const {
+        const T* from = p + t0 * st;
+        if (whole && n == C::L) {
+            // (a wave's 64 pieces land one after another from the address of its first)
+            T* to = tile + threadIdx.x / kWave * (kWave * Rows::EPV);
+            typedef __attribute__((address_space(3))) void* Lds;
+            typedef const __attribute__((address_space(1))) void* Global;
+#pragma unroll
+            for (int i = 0; i < C::RV; i++)
+                __builtin_amdgcn_global_load_lds((Global)(from + i * C::STEP * st), (Lds)(to + i * C::NT * Rows::EPV), 16, 0, 0);
+            return;
+        }
+        const int row = threadIdx.x / Rows::PIECES;
+        uint4 x[C::RV];
 #pragma unroll
         for (int i = 0; i < C::RV; i++) {
             x[i] = uint4{0, 0, 0, 0};
-            if (row[i] < n) x[i] = *(const uint4*)(p[i] + t0 * st);
+            if (row + i * C::STEP < n && col < P) x[i] = *(const uint4*)(from + i * C::STEP * st);
         }
-    }
-    __device__ __forceinline__ void put(T (*tile)[C::LD]) {
 #pragma unroll
-        for (int i = 0; i < C::RV; i++)
-            *(uint4*)&tile[(int)threadIdx.x / C::VPR + i * (C::NT / C::VPR)][col] = x[i];
-    }
-    __device__ __forceinline__ uint32_t most(uint32_t m) const {
-#pragma unroll
-        for (int i = 0; i < C::RV; i++) m = most_bits(m, x[i], T{});
-        return m;
+        for (int i = 0; i < C::RV; i++) *(uint4*)(tile + ((int)threadIdx.x + i * C::NT) * Rows::EPV) = x[i];
     }
 };
+
+// What the workgroup brought is there, for all of it.
+__device__ __forceinline__ void brought() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
 
 // Four neighbouring values, in one access where the rows allow it.
 __device__ __forceinline__ bool rows_wide(const MoRows& r, size_t bytes) {
@@ -109,180 +120,194 @@ struct Cut {
 
 enum { KEEP_NONE = 0, KEEP_STATES = 1, ONLY_SUMS = 2 };
 
-// MODE: KEEP_STATES leaves the states that enter chunks 1, 2, .. for the gradient in a.saved, (N H, chunks - 1, D, E) in the
+// MODE: KEEP_STATES leaves the states that enter chunks 1, 2, .. for the gradient in a.saved, (N H, chunks - 1, P, P) in the
 // elements' type: there they are operands only. ONLY_SUMS makes a segment's own sum.
+// A wave's 16 columns (from x0) of a head's (D, E) matrix, or of its transpose, as accumulator tiles.
+template <class T, int P, bool TRANSPOSED, class F> __device__ __forceinline__ void each_of_state(const MoAttend& a, int x0, F f) {
+    const int lane = threadIdx.x % kWave, g = lane / 16, x = x0 + lane % 16;
+    if (a.D == P && a.E == P) {
+#pragma unroll
+        for (int t = 0; t < P / 16; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) f(t, r, TRANSPOSED ? x * P + acc_row(t, g, r) : acc_row(t, g, r) * P + x);
+        return;
+    }
+#pragma unroll
+    for (int t = 0; t < P / 16; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int y = acc_row(t, g, r), d = TRANSPOSED ? x : y, e = TRANSPOSED ? y : x;
+            if (d < a.D && e < a.E) f(t, r, d * a.E + e);
+        }
+}
+
+// Where a step does not see another, their product's factor is 0; but 0 times a NaN or an infinity is a NaN, which would reach
+// steps of other episodes. Such a value shows in every sum that it entered, so sums that are not finite are made again over
+// what is seen only, one product after another. (`none` collects 0 times each sum: a NaN, or 0.)
+__device__ __forceinline__ void watch(float& none, const f32x4& x) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) none = fmaf(x[r], 0.f, none);
+}
+__device__ __forceinline__ bool any_not_finite(float none) { return __ballot(none != none) != 0; }
+
 template <class T, int P, int MODE>
-__global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend(MoAttend a, Cut cut) {
+__global__ void __launch_bounds__((Chunk<T, P>::NT), 4) k_attend(MoAttend a, Cut cut) {
     typedef Chunk<T, P> C;
     constexpr int L = C::L;
-    __shared__ __align__(16) T sk[L][C::LD], sv[L][C::LD];
-    __shared__ __align__(16) T sq[MODE == ONLY_SUMS ? 1 : L][C::LD], sp[MODE == ONLY_SUMS ? 1 : L][C::LS];
+    constexpr bool OUT = MODE != ONLY_SUMS;
+    __shared__ __align__(16) T lk[L * P], lv[L * P], lq[OUT ? L * P : 8], lp[OUT ? L * L : 8];
     __shared__ float pw[L + 1];
     __shared__ __align__(16) float wt[L];
-    __shared__ int odd[2];     // a value that is not finite is in the chunk's k or v
-    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, i16 = lane % 16;
+    const typename C::Rows sk{lk}, sv{lv}, sq{lq};
+    const typename C::Scores sp{lp};
+    const int w = threadIdx.x / kWave;
     const int64_t nh = blockIdx.x, env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int e0 = w * 16;     // the wave's columns
     const bool wide_out = rows_wide(a.out, 4 * sizeof(T));
     const int64_t de = (int64_t)a.D * a.E;
+    const Bring<T, P> k(a.k, env, h, a.D), v(a.v, env, h, a.E), q(a.q, env, h, a.D);
 
-    powers<L>(pw, a.decay[h]);
-    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
     f32x4 S[C::PT];
-    const float* in = MODE == ONLY_SUMS ? nullptr : cut.segs > 1 ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : a.state ? a.state + nh * de : nullptr;
 #pragma unroll
-    for (int dt = 0; dt < C::PT; dt++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int d = dt * 16 + 4 * g + r, e = e0 + i16;
-            S[dt][r] = in && d < a.D && e < a.E ? in[d * a.E + e] : 0.f;
-        }
-    Rows<T, P> q, k, v;
-    k.init(a.k, env, h, a.D);
-    v.init(a.v, env, h, a.E);
-    if (MODE != ONLY_SUMS) q.init(a.q, env, h, a.D);
-    const auto steps = [&](int64_t c) { return (int)min((int64_t)L, a.T - c * L); };
-    int starts = 0;
-    const auto fetch = [&](int64_t c) {
-        starts = start_of_lane(a, c * L, steps(c), env);
-        k.load(c * L, steps(c));
-        v.load(c * L, steps(c));
-        if (MODE != ONLY_SUMS) q.load(c * L, steps(c));
-    };
-    if (c0 < c1) fetch(c0);
+    for (int dt = 0; dt < C::PT; dt++) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* in = !OUT ? nullptr : cut.segs > 1 ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : a.state ? a.state + nh * de : nullptr;
+    if (in) each_of_state<T, P, false>(a, e0, [&](int t, int r, int at) { S[t][r] = in[at]; });
+    powers<L>(pw, a.decay[h]);
     bool any_start = false;
     for (int64_t c = c0; c < c1; c++) {
-        const int n = steps(c);
         const int64_t t0 = c * L;
+        const int n = (int)min((int64_t)L, a.T - t0);
         __syncthreads();                                       // the last chunk's tiles are done with
-        k.put(sk);
-        v.put(sv);
-        if (MODE != ONLY_SUMS) q.put(sq);
-        const uint64_t m = __ballot(starts != 0);   // the chunk's starts as bits
+        k.chunk(lk, t0, n);
+        v.chunk(lv, t0, n);
+        if (OUT) q.chunk(lq, t0, n);
+        const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);   // the chunk's starts as bits
         any_start |= m != 0;
         const int last = seen_from(m, L - 1);
         if (threadIdx.x < L) wt[threadIdx.x] = (int)threadIdx.x < n && (int)threadIdx.x >= last ? pw[n - 1 - (int)threadIdx.x] : 0.f;
-        if (not_finite(v.most(k.most(0)), T{})) odd[c & 1] = 1;
-        __syncthreads();
-        if (c + 1 < c1) fetch(c + 1);
-        const bool exact_sums = odd[c & 1];
-        if (threadIdx.x == 0) odd[(c + 1) & 1] = 0;
+        brought();
+        const int lane = lane_here(), g = lane / 16, i16 = lane % 16;
 
-        if (MODE != ONLY_SUMS) {
+        if (OUT) {
             // scores, transposed: a lane has four neighbouring j of one i
-            for (int idx = w; idx < C::TILES; idx += C::WAVES) {
+#pragma unroll
+            for (int x = 0; x < C::TPW; x++) {
+                const int idx = w + x * C::WAVES;
+                if (C::TILES % C::WAVES && idx >= C::TILES) break;
                 int it, jt;
                 C::score_tile(idx, it, jt);
                 f32x4 s = {0.f, 0.f, 0.f, 0.f};
-                if (jt <= it) {
 #pragma unroll
-                    for (int b = 0; b < C::PB; b++)
-                        mma(s, frag_in_order(&sk[jt * 16 + i16][b * 32], g), frag_in_order(&sq[it * 16 + i16][b * 32], g));
-                    const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = seen_from(m, i);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) s[r] = j + r <= i && j + r >= from ? s[r] * pw[max(i - j - r, 0)] : 0.f;
-                }
+                for (int b = 0; b < C::PB; b++) mma(s, sk.along(jt * 16, b * 32, lane), sq.along(it * 16, b * 32, lane));
+                const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = m ? seen_from(m, i) : -1;
                 Pack<T, 4> p;
 #pragma unroll
-                for (int r = 0; r < 4; r++) p.v[r] = as<T>(s[r]);
-                *(Pack<T, 4>*)&sp[it * 16 + i16][jt * 16 + 4 * g] = p;
+                for (int r = 0; r < 4; r++) {
+                    const float f = pw[max(i - j - r, 0)];
+                    p.v[r] = as<T>(j + r <= i && j + r >= from ? s[r] * f : 0.f);
+                }
+                *(Pack<T, 4>*)sp.at(i, j) = p;
             }
-            if (MODE == KEEP_STATES && c > 0) {
-                T* to = (T*)a.saved + (nh * (cut.chunks - 1) + c - 1) * de;
+            if (MODE == KEEP_STATES && c > 0) {                // by rows d, a lane four neighbouring columns
+                T* to = (T*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + i16 * P + e0 + 4 * g;
 #pragma unroll
-                for (int dt = 0; dt < C::PT; dt++)
+                for (int t = 0; t < C::PT; t++) {
+                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                    mma(x, frag_of<T>(S[t & ~1], S[t | 1]), unit_frag<T>(t & 1, lane));
+                    Pack<T, 4> y;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int d = dt * 16 + 4 * g + r, e = e0 + i16;
-                        if (d < a.D && e < a.E) to[d * a.E + e] = as<T>(S[dt][r]);
-                    }
+                    for (int r = 0; r < 4; r++) y.v[r] = as<T>(x[r]);
+                    *(Pack<T, 4>*)(to + t * 16 * P) = y;
+                }
             }
             __syncthreads();
         }
 
         Frag<T> vf[C::LB];
 #pragma unroll
-        for (int b = 0; b < C::LB; b++) vf[b] = frag_down(&sv[b * 32][e0], C::LD, lane);
+        for (int b = 0; b < C::LB; b++) vf[b] = sv.down(b * 32, e0, lane);
 
-        if (MODE != ONLY_SUMS) {
+        if (OUT) {
             // outputs, transposed: a lane has four neighbouring columns of one step
-            f32x4 o[C::LT], x[C::LT];
-#pragma unroll
-            for (int it = 0; it < C::LT; it++) {
-                o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-                x[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int b = 0; b <= it / 2; b++)
-                    if (!exact_sums) mma(o[it], vf[b], frag_in_order(&sp[it * 16 + i16][b * 32], g));
-            }
-            if (exact_sums) {                                  // 0 times a NaN that a step must not see would be one
-#pragma unroll
-                for (int it = 0; it < C::LT; it++) {
-                    const int i = it * 16 + i16;
-                    for (int j = max(seen_from(m, i), 0); j <= i; j++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) o[it][r] = fmaf(as_f32(sp[i][j]), as_f32(sv[j][e0 + 4 * g + r]), o[it][r]);
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < C::PB; b++) {
-                const Frag<T> sf = state_frag<T>(S[2 * b], S[2 * b + 1]);
-#pragma unroll
-                for (int it = 0; it < C::LT; it++) mma(x[it], sf, frag_in_halves(&sq[it * 16 + i16][b * 32], g));
-            }
-            T* out = (T*)a.out.p + env * a.out.sn + h * a.out.sh + e0 + 4 * g;
-#pragma unroll
-            for (int it = 0; it < C::LT; it++) {
+            T* out = (T*)a.out.p + env * a.out.sn + h * a.out.sh + e0 + 4 * g + (t0 + i16) * a.out.st;
+            const auto write = [&](int it, const f32x4& own, const f32x4& far) {
                 const int i = it * 16 + i16;
-                if (i >= n || e0 + 4 * g >= a.E) continue;
-                const bool enters = seen_from(m, i) < 0;
+                const bool enters = !m || seen_from(m, i) < 0;
                 const float f = pw[i + 1];
                 Pack<T, 4> y;
 #pragma unroll
-                for (int r = 0; r < 4; r++) y.v[r] = as<T>(a.scale * (enters ? fmaf(f, x[it][r], o[it][r]) : o[it][r]));
-                put4(out + (t0 + i) * a.out.st, y, wide_out);
+                for (int r = 0; r < 4; r++) y.v[r] = as<T>(a.scale * (enters ? fmaf(f, far[r], own[r]) : own[r]));
+                if (i < n && e0 + 4 * g < a.E) put4(out + it * 16 * a.out.st, y, wide_out);
+            };
+            Frag<T> sf[C::PB];
+#pragma unroll
+            for (int b = 0; b < C::PB; b++) sf[b] = frag_of<T>(S[2 * b], S[2 * b + 1]);
+            float none = 0.f;
+#pragma unroll
+            for (int it = 0; it < C::LT; it++) {
+                f32x4 own = {0.f, 0.f, 0.f, 0.f}, far = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int b = 0; b < C::PB; b++) mma(far, sf[b], sq.along(it * 16, b * 32, lane));
+#pragma unroll
+                for (int b = 0; b <= it / 2; b++) mma(own, vf[b], sp.along(it * 16, b * 32, lane));
+                watch(none, own);
+                write(it, own, far);
+            }
+            if (any_not_finite(none)) {
+#pragma unroll 1
+                for (int it = 0; it < C::LT; it++) {
+                    const int i = it * 16 + i16;
+                    f32x4 own = {0.f, 0.f, 0.f, 0.f}, far = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int b = 0; b < C::PB; b++) mma(far, sf[b], sq.along(it * 16, b * 32, lane));
+#pragma unroll 1
+                    for (int j = max(seen_from(m, i), 0); j <= i; j++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) own[r] = fmaf(as_f32(*sp.at(i, j)), as_f32(*sv.at(j, e0 + 4 * g + r)), own[r]);
+                    write(it, own, far);
+                }
             }
         }
 
-        const float f = last < 0 ? pw[n] : 0.f;
-        if (!exact_sums) {
-            Frag<T> part[C::LB][kParts<T>];
+        f32x4 add[C::PT];
 #pragma unroll
-            for (int b = 0; b < C::LB; b++) scaled_parts(vf[b], &wt[b * 32 + 8 * g], part[b]);
+        for (int dt = 0; dt < C::PT; dt++) add[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < C::LB; b++) {
+            Frag<T> part[kParts<T>];
+            scaled_parts(vf[b], &wt[b * 32 + 8 * g], part);
 #pragma unroll
             for (int dt = 0; dt < C::PT; dt++) {
+                const Frag<T> kf = sk.template down<true>(b * 32, acc_col(dt), lane);
 #pragma unroll
-                for (int r = 0; r < 4; r++) S[dt][r] = last < 0 ? f * S[dt][r] : 0.f;
-#pragma unroll
-                for (int b = 0; b < C::LB; b++) {
-                    const Frag<T> kf = frag_down(&sk[b * 32][dt * 16], C::LD, lane);
-#pragma unroll
-                    for (int p = 0; p < kParts<T>; p++) mma(S[dt], kf, part[b][p]);
-                }
+                for (int p = 0; p < kParts<T>; p++) mma(add[dt], kf, part[p]);
             }
-        } else {
-#pragma unroll
-            for (int dt = 0; dt < C::PT; dt++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float s = last < 0 ? f * S[dt][r] : 0.f;
-                    for (int j = max(last, 0); j < n; j++) s = fmaf(wt[j] * as_f32(sk[j][dt * 16 + 4 * g + r]), as_f32(sv[j][e0 + i16]), s);
-                    S[dt][r] = s;
-                }
         }
-    }
-    float* to = MODE == ONLY_SUMS ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : cut.segs > 1 ? nullptr : a.state_out + nh * de;
-    if (to)
+        float none = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < C::PT; dt++) watch(none, add[dt]);
+        if (any_not_finite(none)) {
+#pragma unroll
+            for (int dt = 0; dt < C::PT; dt++) {
+                add[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                for (int j = max(last, 0); j < n; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        add[dt][r] = fmaf(wt[j] * as_f32(*sk.at(j, acc_row(dt, g, r))), as_f32(*sv.at(j, e0 + i16)), add[dt][r]);
+            }
+        }
+        const float f = pw[n];
 #pragma unroll
         for (int dt = 0; dt < C::PT; dt++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int d = dt * 16 + 4 * g + r, e = e0 + i16;
-                if (d < a.D && e < a.E) to[d * a.E + e] = S[dt][r];
-            }
-    if (MODE == ONLY_SUMS && threadIdx.x == 0) {
+            for (int r = 0; r < 4; r++) S[dt][r] = last < 0 ? fmaf(f, S[dt][r], add[dt][r]) : add[dt][r];
+    }
+    float* to = !OUT ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : cut.segs > 1 ? nullptr : a.state_out + nh * de;
+    if (to) each_of_state<T, P, false>(a, e0, [&](int t, int r, int at) { to[at] = S[t][r]; });
+    if (!OUT && threadIdx.x == 0) {
         const int64_t n = min(c1 * L, a.T) - c0 * L;
         cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : exp2f((float)n * __log2f(a.decay[h]));
     }
@@ -346,6 +371,10 @@ inline Cut attend_cut(const MoAttend& a, int per_cu) {
     c.per_seg = std::max<int64_t>(1, (c.chunks + segs - 1) / segs);
     c.segs = (int)std::max<int64_t>(1, (c.chunks + c.per_seg - 1) / c.per_seg);
     return c;
+}
+inline int64_t saved_bytes(const MoAttend& a) {
+    const int64_t p = padded_head(a);
+    return a.N * a.H * ((a.T + chunk_steps(a) - 1) / chunk_steps(a) - 1) * p * p * (a.dtype == MO_BF16 ? 2 : 4);
 }
 inline int64_t cut_bytes(const MoAttend& a, const Cut& c) {
     return c.segs > 1 ? (int64_t)c.segs * a.N * a.H * (4 * (int64_t)a.D * a.E + 4) : 0;

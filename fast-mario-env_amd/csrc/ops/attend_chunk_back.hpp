@@ -15,12 +15,45 @@ namespace mo {
 // 16-byte pieces straight into operands.
 template <class T, int P> struct BackLds {
     typedef Chunk<T, P> C;
-    T q[C::L][C::LD], k[C::L][C::LD], v[C::L][C::LD], o[C::L][C::LD];   // o: dO
-    T a[C::L][C::LS], b[C::L][C::LS];
-    T r[P][C::LD];
-    float pw[C::L + 4], wt[C::L], ut[C::L];
-    int odd[4];
+    T q[C::L * P], k[C::L * P], v[C::L * P], o[C::L * P];   // o: dO
+    T a[C::L * C::L], b[C::L * C::L];
+    T r[P * P];
+    float wt[C::L], ut[C::L], pw[C::L + 4];
 };
+
+// R += Q^T diag(u) dO of a chunk, as R^T's tiles: `at` the wave's columns (rows of R).
+template <class T, int P>
+__device__ __forceinline__ void add_to_r(f32x4 (&add)[P / 16], const Frag<T> (&qf)[Chunk<T, P>::LB], const Tile<T, P>& so, const Tile<T, P>& sq,
+                                         const float* ut, int x0, int first, int lane) {
+    typedef Chunk<T, P> C;
+    const int g = lane / 16, i16 = lane % 16;
+#pragma unroll
+    for (int et = 0; et < C::PT; et++) add[et] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < C::LB; b++) {
+        Frag<T> part[kParts<T>];
+        scaled_parts(qf[b], &ut[b * 32 + 8 * g], part);
+#pragma unroll
+        for (int et = 0; et < C::PT; et++) {
+            const Frag<T> x = so.template down<true>(b * 32, acc_col(et), lane);
+#pragma unroll
+            for (int p = 0; p < kParts<T>; p++) mma(add[et], x, part[p]);
+        }
+    }
+    float none = 0.f;
+#pragma unroll
+    for (int et = 0; et < C::PT; et++) watch(none, add[et]);
+    if (!any_not_finite(none)) return;
+#pragma unroll
+    for (int et = 0; et < C::PT; et++) {
+        add[et] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int i = 0; i < first; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                add[et][r] = fmaf(ut[i] * as_f32(*sq.at(i, x0 + i16)), as_f32(*so.at(i, acc_row(et, g, r))), add[et][r]);
+    }
+}
 
 template <class T, int P>
 __global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back(MoAttend a, Cut cut) {
@@ -28,253 +61,171 @@ __global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back(MoAttend a, C
     constexpr int L = C::L;
     extern __shared__ __align__(16) char lds[];
     BackLds<T, P>& s = *(BackLds<T, P>*)lds;
-    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, i16 = lane % 16;
+    const typename C::Rows sq{s.q}, sk{s.k}, sv{s.v}, so{s.o}, sr{s.r};
+    const typename C::Scores sa{s.a}, sb{s.b};
+    const int w = threadIdx.x / kWave;
     const int64_t nh = blockIdx.x, env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int x0 = w * 16;     // the wave's rows of R and S, columns of dq and dk; of dv its columns
     const int64_t de = (int64_t)a.D * a.E;
+    const Bring<T, P> q(a.q, env, h, a.D), k(a.k, env, h, a.D), v(a.v, env, h, a.E), o(a.dout, env, h, a.E);
 
     powers<L>(s.pw, a.decay[h]);
-    if (threadIdx.x < 2) s.odd[threadIdx.x] = 0;
     f32x4 R[C::PT];            // R^T: rows e, columns d
+#pragma unroll
+    for (int et = 0; et < C::PT; et++) R[et] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float* in = cut.segs > 1 ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : a.dstate_out ? a.dstate_out + nh * de : nullptr;
-#pragma unroll
-    for (int et = 0; et < C::PT; et++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int d = x0 + i16, e = et * 16 + 4 * g + r;
-            R[et][r] = in && d < a.D && e < a.E ? in[d * a.E + e] : 0.f;
-        }
-    Rows<T, P> q, k, v, o;
-    q.init(a.q, env, h, a.D);
-    k.init(a.k, env, h, a.D);
-    v.init(a.v, env, h, a.E);
-    o.init(a.dout, env, h, a.E);
-    const auto steps = [&](int64_t c) { return (int)min((int64_t)L, a.T - c * L); };
-    int starts = 0;
-    const auto fetch = [&](int64_t c) {
-        const int n = steps(c);
-        starts = start_of_lane(a, c * L, n, env);
-        q.load(c * L, n);
-        k.load(c * L, n);
-        v.load(c * L, n);
-        o.load(c * L, n);
-    };
-    if (c0 < c1) fetch(c1 - 1);
+    if (in) each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { R[t][r] = in[at]; });
     for (int64_t c = c1 - 1; c >= c0; c--) {
-        const int n = steps(c);
         const int64_t t0 = c * L;
+        const int n = (int)min((int64_t)L, a.T - t0);
         __syncthreads();                                       // the last chunk's tiles are done with
-        q.put(s.q);
-        k.put(s.k);
-        v.put(s.v);
-        o.put(s.o);
+        q.chunk(s.q, t0, n);
+        k.chunk(s.k, t0, n);
+        v.chunk(s.v, t0, n);
+        o.chunk(s.o, t0, n);
+        const int lane = lane_here(), g = lane / 16, i16 = lane % 16;
+        // the state that enters the chunk: rows d of the wave, eight neighbouring columns e a lane
+        Frag<T> sf[C::PB];
+        {
+            const int d = x0 + i16;
+            if (c > 0) {
+                const T* kept = (const T*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + d * P + 8 * g;
 #pragma unroll
-        for (int et = 0; et < C::PT; et++) {
-            Pack<T, 4> x;
+                for (int b = 0; b < C::PB; b++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) x.v[r] = as<T>(R[et][r]);
-            *(Pack<T, 4>*)&s.r[x0 + i16][et * 16 + 4 * g] = x;
+                    for (int j = 0; j < 8; j += C::Rows::EPV) *(uint4*)((T*)&sf[b] + j) = *(const uint4*)(kept + b * 32 + j);
+            } else {
+#pragma unroll
+                for (int b = 0; b < C::PB; b++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int e = b * 32 + 8 * g + j;
+                        sf[b].v[j] = as<T>(a.state && d < a.D && e < a.E ? a.state[nh * de + d * a.E + e] : 0.f);
+                    }
+            }
         }
-        const uint64_t m = __ballot(starts != 0);
+#pragma unroll
+        for (int b = 0; b < C::PB; b++) {                      // R by rows d, for K R
+            const Frag<T> x = frag_of<T>(R[2 * b], R[2 * b + 1]);
+#pragma unroll
+            for (int j = 0; j < 8; j += C::Rows::EPV) *(uint4*)sr.at(x0 + i16, b * 32 + 8 * g + j) = *(const uint4*)((const T*)&x + j);
+        }
+        const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);
         const int last = seen_from(m, L - 1);
         if (threadIdx.x < L) {
             const int i = threadIdx.x;
             s.wt[i] = i < n && i >= last ? s.pw[n - 1 - i] : 0.f;
             s.ut[i] = i < n && seen_from(m, i) < 0 ? a.scale * s.pw[i + 1] : 0.f;
         }
-        if (not_finite(q.most(k.most(v.most(o.most(0)))), T{})) s.odd[c & 1] = 1;
-        __syncthreads();
-        if (c > c0) fetch(c - 1);
-        const bool exact_sums = s.odd[c & 1];
-        if (threadIdx.x == 0) s.odd[(c + 1) & 1] = 0;
-        // the state that enters the chunk: rows d of the wave, eight neighbouring columns e a lane
-        Frag<T> sf[C::PB];
-        {
-            const int d = x0 + i16;
-            const T* kept = c > 0 && a.saved ? (const T*)a.saved + (nh * (cut.chunks - 1) + c - 1) * de : nullptr;
-#pragma unroll
-            for (int b = 0; b < C::PB; b++) {
-                const int e = b * 32 + 8 * g;
-                const bool in = d < a.D && e < a.E;
-                if (c > 0) {
-                    union { uint4 u[sizeof(T) / 2]; T x[8]; } y{};
-                    if (in)
-#pragma unroll
-                        for (int j = 0; j < (int)sizeof(T) / 2; j++)
-                            if (e + j * C::EPV < a.E) y.u[j] = *(const uint4*)(kept + d * a.E + e + j * C::EPV);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) sf[b].v[j] = y.x[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        sf[b].v[j] = as<T>(a.state && in && e + j < a.E ? a.state[nh * de + d * a.E + e + j] : 0.f);
-                }
-            }
-        }
+        brought();
 
-        for (int idx = w; idx < C::TILES; idx += C::WAVES) {   // A and B, a lane four neighbouring j of one i
+#pragma unroll
+        for (int z = 0; z < C::TPW; z++) {                     // A and B, a lane four neighbouring j of one i
+            const int idx = w + z * C::WAVES;
+            if (C::TILES % C::WAVES && idx >= C::TILES) break;
             int it, jt;
             C::score_tile(idx, it, jt);
             f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
-            if (jt <= it) {
 #pragma unroll
-                for (int b = 0; b < C::PB; b++) {
-                    mma(x, frag_in_order(&s.k[jt * 16 + i16][b * 32], g), frag_in_order(&s.q[it * 16 + i16][b * 32], g));
-                    mma(y, frag_in_order(&s.v[jt * 16 + i16][b * 32], g), frag_in_order(&s.o[it * 16 + i16][b * 32], g));
-                }
-                const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = seen_from(m, i);
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const bool sees = j + r <= i && j + r >= from;
-                    const float f = a.scale * s.pw[max(i - j - r, 0)];
-                    x[r] = sees ? f * x[r] : 0.f;
-                    y[r] = sees ? f * y[r] : 0.f;
-                }
+            for (int b = 0; b < C::PB; b++) {
+                mma(x, sk.along(jt * 16, b * 32, lane), sq.along(it * 16, b * 32, lane));
+                mma(y, sv.along(jt * 16, b * 32, lane), so.along(it * 16, b * 32, lane));
             }
+            const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = m ? seen_from(m, i) : -1;
             Pack<T, 4> xa, yb;
 #pragma unroll
-            for (int r = 0; r < 4; r++) { xa.v[r] = as<T>(x[r]); yb.v[r] = as<T>(y[r]); }
-            *(Pack<T, 4>*)&s.a[it * 16 + i16][jt * 16 + 4 * g] = xa;
-            *(Pack<T, 4>*)&s.b[it * 16 + i16][jt * 16 + 4 * g] = yb;
+            for (int r = 0; r < 4; r++) {
+                const bool sees = j + r <= i && j + r >= from;
+                const float f = a.scale * s.pw[max(i - j - r, 0)];
+                xa.v[r] = as<T>(sees ? f * x[r] : 0.f);
+                yb.v[r] = as<T>(sees ? f * y[r] : 0.f);
+            }
+            *(Pack<T, 4>*)sa.at(i, j) = xa;
+            *(Pack<T, 4>*)sb.at(i, j) = yb;
         }
         __syncthreads();
 
         // Each output transposed: a lane has four neighbouring columns of one step. `own` the sum over the chunk's steps, `far`
         // what the entering state or its gradient adds, by a factor a step.
-        f32x4 own[C::LT], far[C::LT];
-        const auto clear = [&] {
+        const auto write = [&](const MoRows& to, int size, int t, float f, const f32x4& own, const f32x4& far) {
+            const int i = t * 16 + i16;
+            Pack<T, 4> y;
 #pragma unroll
-            for (int t = 0; t < C::LT; t++) { own[t] = f32x4{0.f, 0.f, 0.f, 0.f}; far[t] = own[t]; }
+            for (int r = 0; r < 4; r++) y.v[r] = as<T>(f == 0.f ? own[r] : fmaf(f, far[r], own[r]));
+            if (i < n && x0 + 4 * g < size)
+                put4((T*)to.p + env * to.sn + h * to.sh + x0 + 4 * g + (t0 + i) * to.st, y, rows_wide(to, 4 * sizeof(T)));
         };
-        const auto write = [&](const MoRows& to, int size, auto factor) {
-            const bool wide = rows_wide(to, 4 * sizeof(T));
-            T* p = (T*)to.p + env * to.sn + h * to.sh + x0 + 4 * g;
-            if (x0 + 4 * g >= size) return;
+        // far + sum over the steps j that step i sees (or that see it) of x_ij y_j, made again one product after another
+        const auto again = [&](const auto& x, bool down, const auto& y, int i, f32x4& own) {
+            own = f32x4{0.f, 0.f, 0.f, 0.f};
+            const int j0 = down ? i : max(seen_from(m, i), 0), j1 = down ? n - 1 : i;
+#pragma unroll 1
+            for (int j = j0; j <= j1 && (!down || seen_from(m, j) <= i); j++)
 #pragma unroll
-            for (int t = 0; t < C::LT; t++) {
-                const int i = t * 16 + i16;
-                if (i >= n) continue;
-                const float f = factor(i);
-                Pack<T, 4> y;
-#pragma unroll
-                for (int r = 0; r < 4; r++) y.v[r] = as<T>(f == 0.f ? own[t][r] : fmaf(f, far[t][r], own[t][r]));
-                put4(p + (t0 + i) * to.st, y, wide);
-            }
+                for (int r = 0; r < 4; r++)
+                    own[r] = fmaf(as_f32(down ? *x.at(j, i) : *x.at(i, j)), as_f32(*y.at(j, x0 + 4 * g + r)), own[r]);
         };
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-        clear();                                               // dQ
-        if (!exact_sums) {
-            Frag<T> kf[C::LB];
+        Frag<T> kf[C::LB];                                     // dQ
 #pragma unroll
-            for (int b = 0; b < C::LB; b++) kf[b] = frag_down(&s.k[b * 32][x0], C::LD, lane);
+        for (int b = 0; b < C::LB; b++) kf[b] = sk.down(b * 32, x0, lane);
 #pragma unroll
-            for (int t = 0; t < C::LT; t++)
+        for (int t = 0; t < C::LT; t++) {
+            f32x4 own = zero, far = zero;
 #pragma unroll
-                for (int b = 0; b <= t / 2; b++) mma(own[t], kf[b], frag_in_order(&s.b[t * 16 + i16][b * 32], g));
-        } else {
+            for (int b = 0; b < C::PB; b++) mma(far, sf[b], so.along(t * 16, b * 32, lane));
 #pragma unroll
-            for (int t = 0; t < C::LT; t++) {
-                const int i = t * 16 + i16;
-                for (int j = max(seen_from(m, i), 0); j <= i; j++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) own[t][r] = fmaf(as_f32(s.b[i][j]), as_f32(s.k[j][x0 + 4 * g + r]), own[t][r]);
-            }
+            for (int b = 0; b <= t / 2; b++) mma(own, kf[b], sb.along(t * 16, b * 32, lane));
+            float none = 0.f;
+            watch(none, own);
+            if (any_not_finite(none)) again(sb, false, sk, t * 16 + i16, own);
+            write(a.dq, a.D, t, s.ut[t * 16 + i16], own, far);
         }
-#pragma unroll
-        for (int b = 0; b < C::PB; b++)
-#pragma unroll
-            for (int t = 0; t < C::LT; t++) mma(far[t], sf[b], frag_in_order(&s.o[t * 16 + i16][b * 32], g));
-        write(a.dq, a.D, [&](int i) { return s.ut[i]; });
 
-        clear();                                               // dK
-        Frag<T> qf[C::LB], of[C::LB];
+        Frag<T> qf[C::LB];                                     // dK
 #pragma unroll
-        for (int b = 0; b < C::LB; b++) qf[b] = frag_down(&s.q[b * 32][x0], C::LD, lane);
-        if (!exact_sums) {
+        for (int b = 0; b < C::LB; b++) qf[b] = sq.down(b * 32, x0, lane);
 #pragma unroll
-            for (int t = 0; t < C::LT; t++)
+        for (int t = 0; t < C::LT; t++) {
+            f32x4 own = zero, far = zero;
 #pragma unroll
-                for (int b = t / 2; b < C::LB; b++) mma(own[t], qf[b], frag_down(&s.b[b * 32][t * 16], C::LS, lane));
-        } else {
+            for (int b = 0; b < C::PB; b++) mma(far, frag_of<T>(R[2 * b], R[2 * b + 1]), sv.along(t * 16, b * 32, lane));
 #pragma unroll
-            for (int t = 0; t < C::LT; t++) {
-                const int j = t * 16 + i16;
-                for (int i = j; i < n && seen_from(m, i) <= j; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) own[t][r] = fmaf(as_f32(s.b[i][j]), as_f32(s.q[i][x0 + 4 * g + r]), own[t][r]);
-            }
+            for (int b = t / 2; b < C::LB; b++) mma(own, qf[b], sb.down(b * 32, t * 16, lane));
+            float none = 0.f;
+            watch(none, own);
+            if (any_not_finite(none)) again(sb, true, sq, t * 16 + i16, own);
+            write(a.dk, a.D, t, s.wt[t * 16 + i16], own, far);
         }
-#pragma unroll
-        for (int b = 0; b < C::PB; b++) {
-            const Frag<T> rf = state_frag<T>(R[2 * b], R[2 * b + 1]);
-#pragma unroll
-            for (int t = 0; t < C::LT; t++) mma(far[t], rf, frag_in_halves(&s.v[t * 16 + i16][b * 32], g));
-        }
-        write(a.dk, a.D, [&](int i) { return s.wt[i]; });
 
-        clear();                                               // dV
-        if (!exact_sums) {
+        Frag<T> of[C::LB];                                     // dV
 #pragma unroll
-            for (int b = 0; b < C::LB; b++) of[b] = frag_down(&s.o[b * 32][x0], C::LD, lane);
+        for (int b = 0; b < C::LB; b++) of[b] = so.down(b * 32, x0, lane);
 #pragma unroll
-            for (int t = 0; t < C::LT; t++)
+        for (int t = 0; t < C::LT; t++) {
+            f32x4 own = zero, far = zero;
 #pragma unroll
-                for (int b = t / 2; b < C::LB; b++) mma(own[t], of[b], frag_down(&s.a[b * 32][t * 16], C::LS, lane));
-        } else {
+            for (int b = 0; b < C::PB; b++) mma(far, sr.down(b * 32, x0, lane), sk.along(t * 16, b * 32, lane));
 #pragma unroll
-            for (int t = 0; t < C::LT; t++) {
-                const int j = t * 16 + i16;
-                for (int i = j; i < n && seen_from(m, i) <= j; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) own[t][r] = fmaf(as_f32(s.a[i][j]), as_f32(s.o[i][x0 + 4 * g + r]), own[t][r]);
-            }
+            for (int b = t / 2; b < C::LB; b++) mma(own, of[b], sa.down(b * 32, t * 16, lane));
+            float none = 0.f;
+            watch(none, own);
+            if (any_not_finite(none)) again(sa, true, so, t * 16 + i16, own);
+            write(a.dv, a.E, t, s.wt[t * 16 + i16], own, far);
         }
-#pragma unroll
-        for (int b = 0; b < C::PB; b++) {
-            const Frag<T> rf = frag_down(&s.r[b * 32][x0], C::LD, lane);
-#pragma unroll
-            for (int t = 0; t < C::LT; t++) mma(far[t], rf, frag_in_order(&s.k[t * 16 + i16][b * 32], g));
-        }
-        write(a.dv, a.E, [&](int i) { return s.wt[i]; });
 
-        const float f = s.pw[n];                               // R'
-        if (!exact_sums) {
-            Frag<T> part[C::LB][kParts<T>];
+        f32x4 add[C::PT];                                      // R'
+        add_to_r<T, P>(add, qf, so, sq, s.ut, x0, m ? (int)__ffsll((long long)m) - 1 : n, lane);
+        const float f = s.pw[n];
 #pragma unroll
-            for (int b = 0; b < C::LB; b++) scaled_parts(qf[b], &s.ut[b * 32 + 8 * g], part[b]);
+        for (int et = 0; et < C::PT; et++)
 #pragma unroll
-            for (int et = 0; et < C::PT; et++) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) R[et][r] = m ? 0.f : f * R[et][r];
-#pragma unroll
-                for (int b = 0; b < C::LB; b++) {
-                    const Frag<T> x = frag_down(&s.o[b * 32][et * 16], C::LD, lane);
-#pragma unroll
-                    for (int p = 0; p < kParts<T>; p++) mma(R[et], x, part[b][p]);
-                }
-            }
-        } else {
-            const int first = m ? (int)__ffsll((long long)m) - 1 : n;
-#pragma unroll
-            for (int et = 0; et < C::PT; et++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float x = m ? 0.f : f * R[et][r];
-                    for (int i = 0; i < first; i++) x = fmaf(s.ut[i] * as_f32(s.q[i][x0 + i16]), as_f32(s.o[i][et * 16 + 4 * g + r]), x);
-                    R[et][r] = x;
-                }
-        }
+            for (int r = 0; r < 4; r++) R[et][r] = m ? add[et][r] : fmaf(f, R[et][r], add[et][r]);
     }
-    if (!a.dstate || cut.segs > 1) return;
-#pragma unroll
-    for (int et = 0; et < C::PT; et++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int d = x0 + i16, e = et * 16 + 4 * g + r;
-            if (d < a.D && e < a.E) a.dstate[nh * de + d * a.E + e] = R[et][r];
-        }
+    if (a.dstate && cut.segs == 1) each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { a.dstate[nh * de + at] = R[t][r]; });
 }
 
 // A segment's own sum of R' (see R' above) and what it leaves of a gradient that comes from behind it.
@@ -282,81 +233,45 @@ template <class T, int P>
 __global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back_sums(MoAttend a, Cut cut) {
     typedef Chunk<T, P> C;
     constexpr int L = C::L;
-    __shared__ __align__(16) T sq[L][C::LD], so[L][C::LD];
+    __shared__ __align__(16) T lq[L * P], lo[L * P];
     __shared__ float pw[L + 1];
     __shared__ __align__(16) float ut[L];
-    __shared__ int odd[2];
-    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, i16 = lane % 16;
+    const typename C::Rows sq{lq}, so{lo};
+    const int w = threadIdx.x / kWave;
     const int64_t nh = blockIdx.x, env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int x0 = w * 16;
+    const Bring<T, P> q(a.q, env, h, a.D), o(a.dout, env, h, a.E);
     powers<L>(pw, a.decay[h]);
-    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
     f32x4 R[C::PT];
 #pragma unroll
     for (int et = 0; et < C::PT; et++) R[et] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Rows<T, P> q, o;
-    q.init(a.q, env, h, a.D);
-    o.init(a.dout, env, h, a.E);
-    const auto steps = [&](int64_t c) { return (int)min((int64_t)L, a.T - c * L); };
-    int starts = 0;
-    const auto fetch = [&](int64_t c) {
-        starts = start_of_lane(a, c * L, steps(c), env);
-        q.load(c * L, steps(c));
-        o.load(c * L, steps(c));
-    };
-    if (c0 < c1) fetch(c1 - 1);
     bool any_start = false;
     for (int64_t c = c1 - 1; c >= c0; c--) {
-        const int n = steps(c);
+        const int64_t t0 = c * L;
+        const int n = (int)min((int64_t)L, a.T - t0);
         __syncthreads();
-        q.put(sq);
-        o.put(so);
-        const uint64_t m = __ballot(starts != 0);
+        q.chunk(lq, t0, n);
+        o.chunk(lo, t0, n);
+        const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);
         any_start |= m != 0;
         if (threadIdx.x < L) ut[threadIdx.x] = (int)threadIdx.x < n && seen_from(m, threadIdx.x) < 0 ? a.scale * pw[threadIdx.x + 1] : 0.f;
-        if (not_finite(q.most(o.most(0)), T{})) odd[c & 1] = 1;
-        __syncthreads();
-        if (c > c0) fetch(c - 1);
-        const bool exact_sums = odd[c & 1];
-        if (threadIdx.x == 0) odd[(c + 1) & 1] = 0;
+        brought();
+        const int lane = lane_here();
+        Frag<T> qf[C::LB];
+#pragma unroll
+        for (int b = 0; b < C::LB; b++) qf[b] = sq.down(b * 32, x0, lane);
+        f32x4 add[C::PT];
+        add_to_r<T, P>(add, qf, so, sq, ut, x0, m ? (int)__ffsll((long long)m) - 1 : n, lane);
         const float f = pw[n];
-        if (!exact_sums) {
-            Frag<T> part[C::LB][kParts<T>];
 #pragma unroll
-            for (int b = 0; b < C::LB; b++) scaled_parts(frag_down(&sq[b * 32][x0], C::LD, lane), &ut[b * 32 + 8 * g], part[b]);
+        for (int et = 0; et < C::PT; et++)
 #pragma unroll
-            for (int et = 0; et < C::PT; et++) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) R[et][r] = m ? 0.f : f * R[et][r];
-#pragma unroll
-                for (int b = 0; b < C::LB; b++) {
-                    const Frag<T> x = frag_down(&so[b * 32][et * 16], C::LD, lane);
-#pragma unroll
-                    for (int p = 0; p < kParts<T>; p++) mma(R[et], x, part[b][p]);
-                }
-            }
-        } else {
-            const int first = m ? (int)__ffsll((long long)m) - 1 : n;
-#pragma unroll
-            for (int et = 0; et < C::PT; et++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float x = m ? 0.f : f * R[et][r];
-                    for (int i = 0; i < first; i++) x = fmaf(ut[i] * as_f32(sq[i][x0 + i16]), as_f32(so[i][et * 16 + 4 * g + r]), x);
-                    R[et][r] = x;
-                }
-        }
+            for (int r = 0; r < 4; r++) R[et][r] = m ? add[et][r] : fmaf(f, R[et][r], add[et][r]);
     }
     float* to = cut.enter + ((int64_t)seg * a.N * a.H + nh) * a.D * a.E;
-#pragma unroll
-    for (int et = 0; et < C::PT; et++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int d = x0 + i16, e = et * 16 + 4 * g + r;
-            if (d < a.D && e < a.E) to[d * a.E + e] = R[et][r];
-        }
+    each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { to[at] = R[t][r]; });
     if (threadIdx.x == 0) {
         const int64_t n = min(c1 * L, a.T) - c0 * L;
         cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : exp2f((float)n * __log2f(a.decay[h]));

@@ -99,7 +99,7 @@ const char* mo_last_error(void) { return g_err.c_str(); }
 int64_t mo_attend_saved(const MoAttend* a) {
     return guarded([&]() -> int64_t {
         if (!attend_sizes(a)) return -1;
-        return chunks_take(*a, false) ? a->N * a->H * (attend_cut(*a, 1).chunks - 1) * a->D * a->E * (int64_t)size_of(a->dtype) : 0;
+        return chunks_take(*a, false) ? saved_bytes(*a) : 0;
     });
 }
 

@@ -242,36 +242,48 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_dx(NormArgs k) {
     }
 }
 
-// Sums the rows of `in` (rows, cols) that belong to block row blockIdx.y: 64 columns by 4 row lanes, joined in order. The last
-// round (one block row) writes the first half of the columns to dweight and the rest to dbias.
-__global__ void __launch_bounds__(256) k_norm_colsum(const float* in, int64_t rows, int cols, float* out, float* dweight, float* dbias) {
-    __shared__ float s[4][64];
-    const int c = blockIdx.x * 64 + threadIdx.x % 64, r0 = threadIdx.x / 64;
+// Sums the rows of `in` (rows, cols) that belong to block row blockIdx.y: 16 columns by 64 row lanes, each eight loads ahead,
+// joined in order. The last round (one block row) writes the first half of the columns to dweight and the rest to dbias.
+constexpr int SUM_COLS = 16, SUM_LANES = 64;
+__global__ void __launch_bounds__(SUM_COLS * SUM_LANES) k_norm_colsum(const float* in, int64_t rows, int cols, float* out, float* dweight,
+                                                                     float* dbias) {
+    __shared__ float s[SUM_LANES][SUM_COLS];
+    const int cl = threadIdx.x % SUM_COLS, c = blockIdx.x * SUM_COLS + cl, rl = threadIdx.x / SUM_COLS;
+    const int64_t step = (int64_t)SUM_LANES * gridDim.y;
     float sum = 0.f;
     if (c < cols)
-        for (int64_t r = (int64_t)blockIdx.y * 4 + r0; r < rows; r += 4 * (int64_t)gridDim.y) sum += in[r * cols + c];
-    s[r0][threadIdx.x % 64] = sum;
-    __syncthreads();
-    if (r0 || c >= cols) return;
-    sum = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
+        for (int64_t r = (int64_t)blockIdx.y * SUM_LANES + rl; r < rows; r += 8 * step) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = r + i * step < rows ? in[(r + i * step) * cols + c] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum += x[i];
+        }
+    s[rl][cl] = sum;
+    for (int m = SUM_LANES / 2; m; m /= 2) {
+        __syncthreads();
+        if (rl < m) s[rl][cl] += s[rl + m][cl];
+    }
+    if (rl || c >= cols) return;
+    sum = s[0][cl];
     if (out) out[(int64_t)blockIdx.y * cols + c] = sum;
     else if (c < cols / 2) dweight[c] = sum;
     else dbias[c - cols / 2] = sum;
 }
 
-constexpr int NORM_SUM_ROWS = 256;   // rows that the first round of column sums leaves
+constexpr int NORM_SUM_ROWS = 64;   // rows that the first round of column sums leaves
 
-// rows of (2, C) sums -> dweight, dbias, in two rounds where there are many rows; `spare` holds NORM_SUM_ROWS rows.
+// rows of (2, C) sums -> dweight, dbias, in two rounds where a block would go through many rows; `spare` holds NORM_SUM_ROWS rows.
 inline int norm_colsum(const MoNorm& a, const float* rows_of, int64_t rows, float* spare, hipStream_t s) {
     const int cols = 2 * a.C;
-    const dim3 grid((unsigned)((cols + 63) / 64));
-    if (rows > NORM_SUM_ROWS) {
-        hipLaunchKernelGGL(k_norm_colsum, dim3(grid.x, NORM_SUM_ROWS), dim3(256), 0, s, rows_of, rows, cols, spare, nullptr, nullptr);
+    const unsigned blocks = (unsigned)((cols + SUM_COLS - 1) / SUM_COLS);
+    if (rows > 4096) {
+        hipLaunchKernelGGL(k_norm_colsum, dim3(blocks, NORM_SUM_ROWS), dim3(SUM_COLS * SUM_LANES), 0, s, rows_of, rows, cols, spare, nullptr, nullptr);
         if (launched("k_norm_colsum")) return -1;
         rows_of = spare;
         rows = NORM_SUM_ROWS;
     }
-    hipLaunchKernelGGL(k_norm_colsum, grid, dim3(256), 0, s, rows_of, rows, cols, nullptr, a.dweight, a.dbias);
+    hipLaunchKernelGGL(k_norm_colsum, dim3(blocks), dim3(SUM_COLS * SUM_LANES), 0, s, rows_of, rows, cols, nullptr, a.dweight, a.dbias);
     return launched("k_norm_colsum");
 }
 

@@ -6,13 +6,9 @@ namespace mo {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
-// An operand of a product over 32 indices: lane l has row (of A) or column (of B) l % 16 and eight of the indices. Which eight
-// is up to the caller, as long as A and B agree: 8 (l / 16) + 0..7 ("in order"), or 4 (l / 16) + 0..3 and the same + 16
-// ("in halves"): the rows that a lane holds of two stacked accumulator tiles, so that an accumulator becomes an operand in place.
+// An operand of a product over 32 indices: lane l has row (of A) or column (of B) l % 16 and the indices 8 (l / 16) + 0..7.
 template <class T> struct Frag;
 template <> struct Frag<bf16> { bf16x8 v; };
 template <> struct Frag<float> { float v[8]; };
@@ -26,60 +22,81 @@ __device__ __forceinline__ void mma(f32x4& acc, const Frag<float>& a, const Frag
     for (int i = 0; i < 8; i++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], acc, 0, 0, 0);
 }
 
-// p: row l % 16 of the operand at its first index; the lane's eight indices in order or in halves.
-__device__ __forceinline__ Frag<bf16> frag_in_order(const bf16* p, int g) { return {*(const bf16x8*)(p + 8 * g)}; }
-__device__ __forceinline__ Frag<float> frag_in_order(const float* p, int g) {
-    Frag<float> f;
-    *(f32x4*)f.v = *(const f32x4*)(p + 8 * g);
-    *(f32x4*)(f.v + 4) = *(const f32x4*)(p + 8 * g + 4);
-    return f;
-}
-__device__ __forceinline__ Frag<bf16> frag_in_halves(const bf16* p, int g) {
-    const bf16x4 a = *(const bf16x4*)(p + 4 * g), b = *(const bf16x4*)(p + 16 + 4 * g);
-    return {__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)};
-}
-__device__ __forceinline__ Frag<float> frag_in_halves(const float* p, int g) {
-    Frag<float> f;
-    *(f32x4*)f.v = *(const f32x4*)(p + 4 * g);
-    *(f32x4*)(f.v + 4) = *(const f32x4*)(p + 16 + 4 * g);
-    return f;
-}
+// A tile in LDS of W elements a row, in 16-byte pieces. The pieces of a row are exchanged among each other by the row's number,
+// so that the same piece of eight neighbouring rows, and two neighbouring pieces of four, lie in different banks: the pieces come
+// straight from memory to where they are read, and rows need no padding.
+template <class T, int W> struct Tile {
+    static constexpr int EPV = 16 / sizeof(T), PIECES = W / EPV;
+    static_assert(PIECES >= 4, "");
+    T* p;
+    static __device__ __forceinline__ int turn(int row) {
+        return PIECES == 4 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
+    }
+    __device__ __forceinline__ T* at(int row, int col) const { return p + row * W + (((col / EPV) ^ turn(row)) * EPV | (col % EPV)); }
 
-// The operand whose indices run down the rows of a tile: p its first row at the operand's first row or column, ld its row
-// stride. In order. bf16 takes the transposing LDS read: 16 lanes read 4 rows of 16 and each gets a column.
-__device__ __forceinline__ Frag<bf16> frag_down(const bf16* p, int ld, int lane) {
-    typedef __attribute__((address_space(3))) i16x4* Lds;
+    // indices along the rows: `row` the operand's first, its indices from col
+    __device__ __forceinline__ Frag<T> along(int row, int col, int lane) const;
+    // indices down the rows from `row`; the operand's rows or columns are the tile's columns from col, or (SPREAD) four of each
+    // eight: column c of the operand is col + 8 (c / 4) + c % 4
+    template <bool SPREAD = false> __device__ __forceinline__ Frag<T> down(int row, int col, int lane) const;
+};
+template <class T, int W> __device__ __forceinline__ Frag<T> Tile<T, W>::along(int row, int col, int lane) const {
+    const int r = row + lane % 16, c = col + 8 * (lane / 16);
+    if constexpr (sizeof(T) == 2) {
+        return {*(const bf16x8*)at(r, c)};
+    } else {
+        Frag<T> f;
+        *(f32x4*)f.v = *(const f32x4*)at(r, c);
+        *(f32x4*)(f.v + 4) = *(const f32x4*)at(r, c + 4);
+        return f;
+    }
+}
+template <class T, int W> template <bool SPREAD> __device__ __forceinline__ Frag<T> Tile<T, W>::down(int row, int col, int lane) const {
     const int g = lane / 16, i = lane % 16;
-    const bf16* q = p + (8 * g + i / 4) * ld + (i % 4) * 4;
-    union { i16x4 h[2]; Frag<bf16> f; } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)q);
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 4 * ld));
-    return u.f;
-}
-__device__ __forceinline__ Frag<float> frag_down(const float* p, int ld, int lane) {
-    const float* q = p + 8 * (lane / 16) * ld + lane % 16;
-    Frag<float> f;
+    if constexpr (sizeof(T) == 2) {   // the transposing LDS read: 16 lanes read four neighbours of each of 4 rows and get a column each
+        typedef __attribute__((address_space(3))) i16x4* Lds;
+        const int r = row + 8 * g + i / 4, c = col + (i % 4) * (SPREAD ? 8 : 4);
+        union { i16x4 h[2]; Frag<bf16> f; } u;
+        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at(r, c));
+        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at(r + 4, c));
+        return u.f;
+    } else {
+        const int c = col + (SPREAD ? 8 * (i / 4) + i % 4 : i);
+        Frag<T> f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) f.v[i] = q[i * ld];
+        for (int e = 0; e < 8; e++) f.v[e] = *at(row + 8 * g + e, c);
+        return f;
+    }
+}
+
+// Accumulator tiles as an operand in place. A matrix's rows are dealt to its tiles so that this needs no exchange between lanes:
+// row 4 g + r of tile t is row acc_row(t, g, r), and tiles 2 b and 2 b + 1 of a lane are its eight indices of block b. (An
+// operand that makes such a tile takes its columns SPREAD.) This is the one rounding of what the tiles hold.
+__device__ __forceinline__ constexpr int acc_row(int t, int g, int r) { return 32 * (t / 2) + 8 * g + 4 * (t % 2) + r; }
+__device__ __forceinline__ constexpr int acc_col(int t) { return 32 * (t / 2) + 4 * (t % 2); }   // its first column there
+template <class T> __device__ __forceinline__ Frag<T> frag_of(const f32x4& a, const f32x4& b) {
+    Frag<T> f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) { f.v[i] = as<T>(a[i]); f.v[4 + i] = as<T>(b[i]); }
     return f;
 }
 
-// Two stacked accumulator tiles as an operand, indices in halves: the one rounding of what they hold.
-__device__ __forceinline__ Frag<bf16> frag_of(const f32x4& a, const f32x4& b) {
-    Frag<bf16> f;
+// B's operand of a product that gives columns 16 half .. 16 half + 15 of A's 32 indices back: A's rows by lanes become its
+// columns by lanes, exactly.
+template <class T> __device__ __forceinline__ Frag<T> unit_frag(int half, int lane) {
+    Frag<T> f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) { f.v[i] = (bf16)a[i]; f.v[4 + i] = (bf16)b[i]; }
+    for (int i = 0; i < 8; i++) f.v[i] = as<T>(8 * (lane / 16) + i == 16 * half + lane % 16 ? 1.f : 0.f);
     return f;
 }
-__device__ __forceinline__ Frag<float> frag_of_f32(const f32x4& a, const f32x4& b) {
-    Frag<float> f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) { f.v[i] = a[i]; f.v[4 + i] = b[i]; }
-    return f;
+
+// The lane's number, not known to be the same from one pass of a loop to the next: what follows from it (addresses, mostly) is
+// then made where it is used, instead of being kept in registers over the whole loop, which costs more in waves than it saves.
+__device__ __forceinline__ int lane_here() {
+    int lane = threadIdx.x % kWave;
+    asm volatile("" : "+v"(lane));
+    return lane;
 }
-template <class T> __device__ __forceinline__ Frag<T> state_frag(const f32x4& a, const f32x4& b);
-template <> __device__ __forceinline__ Frag<bf16> state_frag<bf16>(const f32x4& a, const f32x4& b) { return frag_of(a, b); }
-template <> __device__ __forceinline__ Frag<float> state_frag<float>(const f32x4& a, const f32x4& b) { return frag_of_f32(a, b); }
 
 // acc += A (w B), w a factor for each index, with float32's precision: w B is split into bf16 parts of 8 bits of significand
 // each, three of which leave 2^-27 of it. (Where w is 0 the value is left out, whatever it is.)
@@ -100,21 +117,5 @@ __device__ __forceinline__ void scaled_parts(const Frag<float>& b, const float* 
 }
 template <class T> constexpr int kParts = 1;
 template <> inline constexpr int kParts<bf16> = 3;
-
-// Whether any of the 16 bytes' values is infinite or a NaN: the largest magnitude's bits so far, and what they say.
-__device__ __forceinline__ uint32_t most_bits(uint32_t most, const uint4& x, bf16) {
-    union { uint32_t u; u16x2 h; } m{most};
-    for (uint32_t w : {x.x, x.y, x.z, x.w}) {
-        union { uint32_t u; u16x2 h; } y{w & 0x7fff7fffu};
-        m.h = __builtin_elementwise_max(m.h, y.h);
-    }
-    return m.u;
-}
-__device__ __forceinline__ uint32_t most_bits(uint32_t most, const uint4& x, float) {
-    for (uint32_t w : {x.x, x.y, x.z, x.w}) most = max(most, w & 0x7fffffffu);
-    return most;
-}
-__device__ __forceinline__ bool not_finite(uint32_t most, bf16) { return (most >> 16) >= 0x7f80u || (most & 0xffffu) >= 0x7f80u; }
-__device__ __forceinline__ bool not_finite(uint32_t most, float) { return most >= 0x7f800000u; }
 
 }  // namespace mo

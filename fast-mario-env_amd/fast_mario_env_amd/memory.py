@@ -14,7 +14,7 @@ queued on torch's current stream. CPU tensors, and what torch traces or transfor
 """
 from __future__ import annotations
 
-import ctypes
+import contextlib
 
 from .rollout import _torch, _transformed
 
@@ -60,6 +60,12 @@ def _work(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _on(device):
+    """The device made current for launches and allocations (nothing to do where it is: a context costs more than the check)."""
+    torch = _torch()
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _stream(device):
     return _torch().cuda.current_stream(device).cuda_stream
 
@@ -102,7 +108,7 @@ def _attend_forward(q, k, v, decay, start, state, scale, keep):
     torch = _torch()
     from ._native import ops_check, ops_lib
     L, dev = ops_lib(), q.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         a = _attend_args(q, k, v, decay, start, scale)
         out = torch.empty(q.shape[:3] + v.shape[-1:], dtype=q.dtype, device=dev)
         state_out = torch.empty(q.shape[1:] + v.shape[-1:], dtype=torch.float32, device=dev)
@@ -118,7 +124,7 @@ def _attend_backward(q, k, v, decay, start, state, saved, scale, dout, dstate_ou
     torch = _torch()
     from ._native import ops_check, ops_lib
     L, dev = ops_lib(), q.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         a = _attend_args(q, k, v, decay, start, scale)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         dstate = torch.empty(q.shape[1:] + v.shape[-1:], dtype=torch.float32, device=dev) if want_dstate else None
@@ -165,16 +171,16 @@ def _function(name):
     class Norm(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, groups, weight, bias, eps, act):
-            y, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
-            ctx.save_for_backward(x, weight, bias, stats)
+            y, rows, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
+            ctx.save_for_backward(rows, weight, bias, stats)
             ctx.how = (groups, eps, act)
             return y
 
         @staticmethod
         @once
         def backward(ctx, dy):
-            x, weight, bias, stats = ctx.saved_tensors
-            dx, dw, db = _norm_backward(x, weight, bias, stats, dy.contiguous(), *ctx.how, any(ctx.needs_input_grad[2:4]))
+            rows, weight, bias, stats = ctx.saved_tensors
+            dx, dw, db = _norm_backward(rows, weight, bias, stats, dy, *ctx.how, any(ctx.needs_input_grad[2:4]))
             return dx, None, dw, db, None, None
 
     _functions.update(attend=Attend, norm=Norm)
@@ -247,7 +253,7 @@ def linear_attention_step(q, k, v, decay, state, start=None, scale=None):
     decay = decay.contiguous()
     start = None if start is None else start.contiguous()
     N, H, D = q.shape
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
         ops_check(ops_lib().mo_attend_step(_dtype(q), N, H, D, v.shape[-1], scale, _rows(q), _rows(k), _rows(v), decay.data_ptr(),
                                            _ptr(start), state.data_ptr(), _rows(out), _stream(q.device)), "mo_attend_step")
@@ -255,44 +261,49 @@ def linear_attention_step(q, k, v, decay, state, start=None, scale=None):
 
 
 # ---------------------------------------------------------------- group norm and activation
-def _norm_args(x, groups, weight, bias, eps, act):
+def _channels_last(x):
+    """x (B, C, ...) as its channels-last rows (B, ..., C), contiguous (a copy where it lies otherwise)."""
+    return (x.movedim(1, -1) if x.dim() > 2 else x).contiguous()
+
+
+def _norm_args(rows, groups, weight, bias, eps, act):
     from ._native import MoNorm
-    B, C = x.shape[0], x.shape[-1]
-    return MoNorm(dtype=_dtype(x), act=ACTS[act], C=C, groups=groups, B=B, S=x.shape[1], eps=eps, x=x.data_ptr(),
-                  weight=_ptr(weight), bias=_ptr(bias))
+    B, C = rows.shape[0], rows.shape[-1]
+    return MoNorm(dtype=_dtype(rows), act=ACTS[act], C=C, groups=groups, B=B, S=max(1, rows.numel() // max(1, B * C)), eps=eps,
+                  x=rows.data_ptr(), weight=_ptr(weight), bias=_ptr(bias))
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, keep):
-    """y and, if `keep`, each group's mean and 1 / deviation, of x (B, S, C) contiguous."""
+    """y, x's rows, and, if `keep`, each group's mean and 1 / deviation."""
     torch = _torch()
     from ._native import ops_check, ops_lib
-    L, dev = ops_lib(), x.device
-    with torch.cuda.device(dev):
-        y = torch.empty_like(x)
-        stats = torch.empty(x.shape[0], groups, 2, dtype=torch.float32, device=dev) if keep else None
-        a = _norm_args(x, groups, weight, bias, eps, act)
+    L, dev, rows = ops_lib(), x.device, _channels_last(x)
+    with _on(dev):
+        y = torch.empty_like(rows)
+        stats = torch.empty(rows.shape[0], groups, 2, dtype=torch.float32, device=dev) if keep else None
+        a = _norm_args(rows, groups, weight, bias, eps, act)
         a.y, a.stats = y.data_ptr(), _ptr(stats)
         work = _work(ops_check(L.mo_group_norm_work(a, 0), "mo_group_norm_work"), dev)
         a.work = _ptr(work)
         ops_check(L.mo_group_norm(a, _stream(dev)), "mo_group_norm")
-    return y, stats
+    return y.movedim(-1, 1) if x.dim() > 2 else y, rows, stats
 
 
-def _norm_backward(x, weight, bias, stats, dy, groups, eps, act, want_params):
+def _norm_backward(rows, weight, bias, stats, dy, groups, eps, act, want_params):
     torch = _torch()
     from ._native import ops_check, ops_lib
-    L, dev = ops_lib(), x.device
-    with torch.cuda.device(dev):
-        dx = torch.empty_like(x)
+    L, dev, dy = ops_lib(), rows.device, _channels_last(dy)
+    with _on(dev):
+        dx = torch.empty_like(rows)
         dw = db = None
         if want_params and weight is not None:
-            dw, db = (torch.empty if x.shape[0] else torch.zeros)((2,) + weight.shape, dtype=torch.float32, device=dev)
-        a = _norm_args(x, groups, weight, bias, eps, act)
+            dw, db = (torch.empty if rows.shape[0] else torch.zeros)((2,) + weight.shape, dtype=torch.float32, device=dev)
+        a = _norm_args(rows, groups, weight, bias, eps, act)
         a.stats, a.dy, a.dx, a.dweight, a.dbias = stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db)
         work = _work(ops_check(L.mo_group_norm_work(a, 1), "mo_group_norm_work"), dev)
         a.work = _ptr(work)
         ops_check(L.mo_group_norm_backward(a, _stream(dev)), "mo_group_norm_backward")
-    return dx, dw, db
+    return dx.movedim(-1, 1) if dx.dim() > 2 else dx, dw, db
 
 
 def _norm_plain(x, groups, weight, bias, eps, act):
@@ -328,17 +339,13 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
         raise ValueError("group_norm_act: weight and bias go together")
     if weight is not None and any(tuple(p.shape) != (C,) or not p.is_floating_point() or p.device != x.device for p in (weight, bias)):
         raise ValueError(f"group_norm_act: weight and bias must be ({C},) on the device of x ({x.device})")
-    if x.dim() > 2 and x[0, 0].numel() == 0 if x.shape[0] else False:
+    if 0 in x.shape[2:]:
         raise ValueError("group_norm_act: a sample has no positions")
     every = [t for t in (x, weight, bias) if t is not None]
     if not _kernel_takes(*every):
         return _norm_plain(x, groups, weight, bias, eps, act)
-    last = x.movedim(1, -1)
-    rows = last.contiguous().view(x.shape[0], -1, C) if x.shape[0] else last.reshape(0, 1, C)
     if weight is not None:
         weight, bias = weight.float().contiguous(), bias.float().contiguous()
     if torch.is_grad_enabled() and any(t.requires_grad for t in every):
-        y = _function("norm").apply(rows, groups, weight, bias, eps, act)
-    else:
-        y = _norm_forward(rows, groups, weight, bias, eps, act, False)[0]
-    return y.view(last.shape).movedim(-1, 1)
+        return _function("norm").apply(x, groups, weight, bias, eps, act)
+    return _norm_forward(x, groups, weight, bias, eps, act, False)[0]
