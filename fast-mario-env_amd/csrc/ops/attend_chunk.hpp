@@ -15,16 +15,19 @@ namespace mo {
 //
 // T: element type. P: head size rounded up to 32, 64 or 128; columns past D or E are zeros. L: 64 for bf16; 32 for float32,
 // whose matrix instructions are 16 times slower, so that the products of a chunk with itself stay short.
-template <class T, int P> struct Chunk {
+//
+// W: waves of the workgroup.
+template <class T, int P, int W> struct Chunk {
     static constexpr int L = sizeof(T) == 2 ? 64 : 32;
-    static constexpr int WAVES = P / 16, NT = WAVES * kWave;
+    static constexpr int WAVES = W, NT = W * kWave;
+    static constexpr int CT = P / 16 / W;                     // 16-column tiles of S of a wave
     static constexpr int LT = L / 16, LB = L / 32, PB = P / 32, PT = P / 16;
-    typedef mo::Tile<T, P> Rows;      // a chunk of q, k, v, ..
-    typedef mo::Tile<T, L> Scores;
-    static constexpr int STEP = NT / Rows::PIECES, RV = L / STEP;   // rows that the workgroup brings at a time, and times
+    typedef Tile<T, P> Rows;          // a chunk of q, k, v, ..
+    typedef Tile<T, L> Scores;
+    static constexpr int STEP = NT / Rows::PIECES, RV = L / STEP;   // rows that the workgroup moves at a time, and times
     static constexpr int TILES = LT == 4 ? 12 : 4;            // score tiles up to the diagonal's 32-blocks
-    static constexpr int TPW = (TILES + WAVES - 1) / WAVES;   // a wave's
-    static_assert(RV == 2 && STEP % 8 == 0, "");
+    static constexpr int TPW = (TILES + W - 1) / W;           // a wave's
+    static_assert(CT * W * 16 == P && RV * STEP == L && STEP % 8 == 0, "");
 
     static __device__ __forceinline__ void score_tile(int idx, int& it, int& jt) {
         if (LT == 2 || idx < 4) { it = idx >> 1; jt = idx & 1; }
@@ -32,62 +35,71 @@ template <class T, int P> struct Chunk {
     }
 };
 
-// What a thread brings of one operand's chunk: a 16-byte piece of row `row` and of the one STEP further, straight into LDS.
-// Pieces past the chunk's end or the head's size are zeros (these go through registers).
-template <class T, int P> struct Bring {
-    typedef Chunk<T, P> C;
-    typedef typename C::Rows Rows;
-    const T* p;
+// The thread's number, not known to be the same from one pass of a loop to the next: what follows from it (addresses, mostly) is
+// then made where it is used, instead of being kept in registers over the whole loop, which costs more in waves than it saves.
+__device__ __forceinline__ unsigned thread_here() {
+    unsigned t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+// The rows of one operand or result of an env's head, d wide. A thread moves a 16-byte piece of row t / PIECES and of every
+// STEP-th after it.
+template <class T, class C> struct HeadRows {
+    typedef typename C::Rows Tl;
+    T* p;
     int64_t st;
-    int col;                   // P where the head ends before the piece
-    bool whole;                // the head fills the rows
-    __device__ __forceinline__ Bring(const MoRows& r, int64_t n, int h, int d) {
-        const int row = threadIdx.x / Rows::PIECES;
-        col = ((int)(threadIdx.x % Rows::PIECES) ^ Rows::turn(row)) * C::Rows::EPV;
-        st = r.st;
-        p = (const T*)r.p + n * r.sn + h * r.sh + row * st + col;
-        whole = d == P;
-        if (col >= d) col = P;
-    }
-    __device__ __forceinline__ void chunk(T* tile, int64_t t0, int n) const {
-        const T* from = p + t0 * st;
+    int d;
+    bool whole;                // 16-byte pieces only: the head fills the tile's rows; of a result: its rows lie on 16 bytes
+    __device__ __forceinline__ HeadRows(const MoRows& r, int64_t n, int h, int size, bool w) : p((T*)r.p + n * r.sn + h * r.sh), st(r.st), d(size), whole(w) {}
+
+    // Straight into LDS, where a wave's 64 pieces land one after another. (Rows past the chunk's end and columns past the
+    // head's size are zeros; such chunks go through registers.)
+    __device__ __forceinline__ void bring(T* tile, int64_t t0, int n) const {
+        const unsigned t = thread_here(), row = t / Tl::PIECES, col = ((t % Tl::PIECES) ^ Tl::turn(row)) * Tl::EPV;
+        const T* from = p + (t0 + row) * st + col;
         if (whole && n == C::L) {
-            // (a wave's 64 pieces land one after another from the address of its first)
-            T* to = tile + threadIdx.x / kWave * (kWave * Rows::EPV);
+            T* to = tile + threadIdx.x / kWave * (kWave * Tl::EPV);
             typedef __attribute__((address_space(3))) void* Lds;
             typedef const __attribute__((address_space(1))) void* Global;
 #pragma unroll
             for (int i = 0; i < C::RV; i++)
-                __builtin_amdgcn_global_load_lds((Global)(from + i * C::STEP * st), (Lds)(to + i * C::NT * Rows::EPV), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((Global)(from + i * C::STEP * st), (Lds)(to + i * C::NT * Tl::EPV), 16, 0, 0);
             return;
         }
-        const int row = threadIdx.x / Rows::PIECES;
-        uint4 x[C::RV];
 #pragma unroll
         for (int i = 0; i < C::RV; i++) {
-            x[i] = uint4{0, 0, 0, 0};
-            if (row + i * C::STEP < n && col < P) x[i] = *(const uint4*)(from + i * C::STEP * st);
+            uint4 x = {0, 0, 0, 0};
+            if ((int)row + i * C::STEP < n && (int)col < d) x = *(const uint4*)(from + i * C::STEP * st);
+            *(uint4*)(tile + (t + i * C::NT) * Tl::EPV) = x;
         }
+    }
+
+    // Results from LDS. (Straight from the accumulators, four values of each of 16 rows at a time, the stores of the forward
+    // pass took longer than its loads and products together.)
+    __device__ __forceinline__ void take(const T* tile, int64_t t0, int n) const {
+        typedef Pack<T, Tl::EPV> Piece;
+        const unsigned t = thread_here(), row = t / Tl::PIECES, col = ((t % Tl::PIECES) ^ Tl::turn(row)) * Tl::EPV;
+        T* to = p + (t0 + row) * st + col;
 #pragma unroll
-        for (int i = 0; i < C::RV; i++) *(uint4*)(tile + ((int)threadIdx.x + i * C::NT) * Rows::EPV) = x[i];
+        for (int i = 0; i < C::RV; i++) {
+            const Piece x = *(const Piece*)(tile + (t + i * C::NT) * Tl::EPV);
+            if ((int)row + i * C::STEP >= n || (int)col >= d) continue;
+            if (whole) *(Piece*)(to + i * C::STEP * st) = x;
+            else
+#pragma unroll
+                for (int j = 0; j < Tl::EPV; j++) to[i * C::STEP * st + j] = x.v[j];
+        }
     }
 };
+template <class T> __device__ __forceinline__ bool on_pieces(const MoRows& r) {
+    return ((uintptr_t)r.p % 16 == 0) & ((uint64_t)(r.st | r.sn | r.sh) % (16 / sizeof(T)) == 0);
+}
 
 // What the workgroup brought is there, for all of it.
 __device__ __forceinline__ void brought() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-}
-
-// Four neighbouring values, in one access where the rows allow it.
-__device__ __forceinline__ bool rows_wide(const MoRows& r, size_t bytes) {
-    return ((uintptr_t)r.p % bytes == 0) & ((uint64_t)(r.st | r.sn | r.sh) % 4 == 0);
-}
-template <class T> __device__ __forceinline__ void put4(T* p, const Pack<T, 4>& y, bool wide) {
-    if (wide) *(Pack<T, 4>*)p = y;
-    else
-#pragma unroll
-        for (int r = 0; r < 4; r++) p[r] = y.v[r];
 }
 
 // The latest start at or before step i of a chunk whose starts are the bits of m, or -1: step i sees the steps from there on.
@@ -102,11 +114,19 @@ __device__ __forceinline__ int start_of_lane(const MoAttend& a, int64_t t0, int 
     return a.start && lane < n ? a.start[(t0 + lane) * a.N + env] : 0;
 }
 
-// g^0 .. g^L. (g^0 is 1 for g = 0 too.)
-template <int L> __device__ __forceinline__ void powers(float* pw, float g) {
-    const float lg = __log2f(g);
-    for (int i = threadIdx.x; i <= L; i += blockDim.x) pw[i] = i ? exp2f((float)i * lg) : 1.f;
-}
+// g^0 .. g^L (g^0 is 1 for g = 0 too), and the factors by which step i sees step j, scale g^(i-j) or 0, of all i - j.
+template <int L> struct Powers {
+    float pw[L + 1], seen[2 * L];
+    __device__ __forceinline__ void fill(float g, float scale) {
+        const float lg = __log2f(g);
+        for (int i = threadIdx.x; i <= L; i += blockDim.x) {
+            const float x = i ? exp2f((float)i * lg) : 1.f;
+            pw[i] = x;
+            if (i < L) { seen[i] = 0.f; seen[L + i] = scale * x; }
+        }
+    }
+    __device__ __forceinline__ const float* sees(int i, int j) const { return &seen[L + i - j]; }
+};
 
 // A long sequence is cut into segments of whole chunks, a workgroup each, so that few sequences fill the chip. First each
 // segment's own sum and what it leaves of an entering state (`keep`: g^steps, or -1 where an episode starts inside), then the
@@ -143,170 +163,218 @@ template <class T, int P, bool TRANSPOSED, class F> __device__ __forceinline__ v
 
 // Where a step does not see another, their product's factor is 0; but 0 times a NaN or an infinity is a NaN, which would reach
 // steps of other episodes. Such a value shows in every sum that it entered, so sums that are not finite are made again over
-// what is seen only, one product after another. (`none` collects 0 times each sum: a NaN, or 0.)
-__device__ __forceinline__ void watch(float& none, const f32x4& x) {
-#pragma unroll
-    for (int r = 0; r < 4; r++) none = fmaf(x[r], 0.f, none);
-}
-__device__ __forceinline__ bool any_not_finite(float none) { return __ballot(none != none) != 0; }
+// what is seen only, one product after another. (`all` adds the sums up: it is not finite if one of them is not.)
+__device__ __forceinline__ void watch(float& all, const f32x4& x) { all += (x[0] + x[1]) + (x[2] + x[3]); }
+__device__ __forceinline__ bool any_not_finite(float all) { return __ballot(!(fabsf(all) < INFINITY)) != 0; }
+
+template <int P> constexpr int kForwardWaves = P / 16 < 4 ? P / 16 : 4;
+template <int P> constexpr int kForwardPerSimd = P == 128 ? 2 : 3;   // waves a SIMD: what LDS leaves room for
 
 template <class T, int P, int MODE>
-__global__ void __launch_bounds__((Chunk<T, P>::NT), 4) k_attend(MoAttend a, Cut cut) {
-    typedef Chunk<T, P> C;
-    constexpr int L = C::L;
+__global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P>)) k_attend(MoAttend a, Cut cut) {
+    typedef Chunk<T, P, kForwardWaves<P>> C;
+    typedef HeadRows<T, C> Head;
+    constexpr int L = C::L, CT = C::CT;
     constexpr bool OUT = MODE != ONLY_SUMS;
-    __shared__ __align__(16) T lk[L * P], lv[L * P], lq[OUT ? L * P : 8], lp[OUT ? L * L : 8];
-    __shared__ float pw[L + 1];
+    __shared__ __align__(16) T lk[L * P], lv[L * P], lq[OUT ? L * P : 8], lp[OUT ? L * L : 8], ly[OUT ? L * P : 8];
+    __shared__ Powers<L> pw;
     __shared__ __align__(16) float wt[L];
-    const typename C::Rows sk{lk}, sv{lv}, sq{lq};
+    __shared__ float rt[OUT ? L : 1];   // what a step has of the entering state: scale g^(i+1), or 0
+    const typename C::Rows sk{lk}, sv{lv}, sq{lq}, sy{ly};
     const typename C::Scores sp{lp};
     const int w = threadIdx.x / kWave;
     const int64_t nh = blockIdx.x, env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
-    const int e0 = w * 16;     // the wave's columns
-    const bool wide_out = rows_wide(a.out, 4 * sizeof(T));
+    const int e0 = w * CT * 16;   // the wave's columns
     const int64_t de = (int64_t)a.D * a.E;
-    const Bring<T, P> k(a.k, env, h, a.D), v(a.v, env, h, a.E), q(a.q, env, h, a.D);
+    const Head k(a.k, env, h, a.D, a.D == P), v(a.v, env, h, a.E, a.E == P), q(a.q, env, h, a.D, a.D == P), out(a.out, env, h, a.E, on_pieces<T>(a.out));
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-    f32x4 S[C::PT];
+    f32x4 S[CT][C::PT];
 #pragma unroll
-    for (int dt = 0; dt < C::PT; dt++) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+        for (int dt = 0; dt < C::PT; dt++) S[ct][dt] = zero;
     const float* in = !OUT ? nullptr : cut.segs > 1 ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : a.state ? a.state + nh * de : nullptr;
-    if (in) each_of_state<T, P, false>(a, e0, [&](int t, int r, int at) { S[t][r] = in[at]; });
-    powers<L>(pw, a.decay[h]);
+    if (in)
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) each_of_state<T, P, false>(a, e0 + 16 * ct, [&](int t, int r, int at) { S[ct][t][r] = in[at]; });
+    pw.fill(a.decay[h], a.scale);
     bool any_start = false;
     for (int64_t c = c0; c < c1; c++) {
         const int64_t t0 = c * L;
         const int n = (int)min((int64_t)L, a.T - t0);
-        __syncthreads();                                       // the last chunk's tiles are done with
-        k.chunk(lk, t0, n);
-        v.chunk(lv, t0, n);
-        if (OUT) q.chunk(lq, t0, n);
+        __syncthreads();                                       // the last chunk's tiles are done with, its outputs in theirs
+        k.bring(lk, t0, n);
+        v.bring(lv, t0, n);
+        if (OUT) q.bring(lq, t0, n);
+        if (OUT && c > c0) out.take(ly, t0 - L, L);
         const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);   // the chunk's starts as bits
         any_start |= m != 0;
         const int last = seen_from(m, L - 1);
-        if (threadIdx.x < L) wt[threadIdx.x] = (int)threadIdx.x < n && (int)threadIdx.x >= last ? pw[n - 1 - (int)threadIdx.x] : 0.f;
+        if (threadIdx.x < L) {
+            const int i = threadIdx.x;
+            wt[i] = i < n && i >= last ? pw.pw[n - 1 - i] : 0.f;
+            if (OUT) rt[i] = seen_from(m, i) < 0 ? a.scale * pw.pw[i + 1] : 0.f;
+        }
         brought();
-        const int lane = lane_here(), g = lane / 16, i16 = lane % 16;
+        const unsigned lane = thread_here() % kWave, g = lane / 16, i16 = lane % 16;
 
         if (OUT) {
             // scores, transposed: a lane has four neighbouring j of one i
+            const auto scores = [&](auto starts) {
 #pragma unroll
-            for (int x = 0; x < C::TPW; x++) {
-                const int idx = w + x * C::WAVES;
-                if (C::TILES % C::WAVES && idx >= C::TILES) break;
-                int it, jt;
-                C::score_tile(idx, it, jt);
-                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                for (int x = 0; x < C::TPW; x++) {
+                    const int idx = w + x * C::WAVES;
+                    if (C::TILES % C::WAVES && idx >= C::TILES) break;
+                    int it, jt;
+                    C::score_tile(idx, it, jt);
+                    f32x4 s = zero;
 #pragma unroll
-                for (int b = 0; b < C::PB; b++) mma(s, sk.along(jt * 16, b * 32, lane), sq.along(it * 16, b * 32, lane));
-                const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = m ? seen_from(m, i) : -1;
-                Pack<T, 4> p;
+                    for (int b = 0; b < C::PB; b++) mma(s, sk.along(jt * 16, b * 32, lane), sq.along(it * 16, b * 32, lane));
+                    const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = starts ? seen_from(m, i) : 0;
+                    const float* f = pw.sees(i, j);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float f = pw[max(i - j - r, 0)];
-                    p.v[r] = as<T>(j + r <= i && j + r >= from ? s[r] * f : 0.f);
+                    for (int r = 0; r < 4; r++) s[r] = !starts || j + r >= from ? s[r] * f[-r] : 0.f;
+                    *(Pack<T, 4>*)sp.at(i, j) = pack4(s, T{});
                 }
-                *(Pack<T, 4>*)sp.at(i, j) = p;
-            }
+            };
+            if (m) scores(std::true_type{});
+            else scores(std::false_type{});
             if (MODE == KEEP_STATES && c > 0) {                // by rows d, a lane four neighbouring columns
                 T* to = (T*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + i16 * P + e0 + 4 * g;
 #pragma unroll
-                for (int t = 0; t < C::PT; t++) {
-                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                    mma(x, frag_of<T>(S[t & ~1], S[t | 1]), unit_frag<T>(t & 1, lane));
-                    Pack<T, 4> y;
+                for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) y.v[r] = as<T>(x[r]);
-                    *(Pack<T, 4>*)(to + t * 16 * P) = y;
-                }
+                    for (int t = 0; t < C::PT; t++) {
+                        f32x4 x = zero;
+                        mma(x, frag_of<T>(S[ct][t & ~1], S[ct][t | 1]), unit_frag<T>(t & 1, lane));
+                        *(Pack<T, 4>*)(to + t * 16 * P + ct * 16) = pack4(x, T{});
+                    }
             }
             __syncthreads();
         }
 
-        Frag<T> vf[C::LB];
+        Frag<T> vf[CT][C::LB];
 #pragma unroll
-        for (int b = 0; b < C::LB; b++) vf[b] = sv.down(b * 32, e0, lane);
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int b = 0; b < C::LB; b++) vf[ct][b] = sv.down(b * 32, e0 + 16 * ct, lane);
 
         if (OUT) {
             // outputs, transposed: a lane has four neighbouring columns of one step
-            T* out = (T*)a.out.p + env * a.out.sn + h * a.out.sh + e0 + 4 * g + (t0 + i16) * a.out.st;
-            const auto write = [&](int it, const f32x4& own, const f32x4& far) {
-                const int i = it * 16 + i16;
-                const bool enters = !m || seen_from(m, i) < 0;
-                const float f = pw[i + 1];
-                Pack<T, 4> y;
+            const auto write = [&](int it, int ct, const f32x4& own, const f32x4& far) {
+                const float f = rt[it * 16 + i16];
+                f32x4 x;
 #pragma unroll
-                for (int r = 0; r < 4; r++) y.v[r] = as<T>(a.scale * (enters ? fmaf(f, far[r], own[r]) : own[r]));
-                if (i < n && e0 + 4 * g < a.E) put4(out + it * 16 * a.out.st, y, wide_out);
+                for (int r = 0; r < 4; r++) x[r] = fmaf(f, far[r], own[r]);
+                if (m && f == 0.f) x = own;                    // (a state that is not seen may be anything)
+                *(Pack<T, 4>*)sy.at(it * 16 + i16, e0 + 16 * ct + 4 * g) = pack4(x, T{});
             };
-            Frag<T> sf[C::PB];
+            float all = 0.f;
+            {
+                Frag<T> sf[CT][C::PB];
 #pragma unroll
-            for (int b = 0; b < C::PB; b++) sf[b] = frag_of<T>(S[2 * b], S[2 * b + 1]);
-            float none = 0.f;
+                for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-            for (int it = 0; it < C::LT; it++) {
-                f32x4 own = {0.f, 0.f, 0.f, 0.f}, far = {0.f, 0.f, 0.f, 0.f};
+                    for (int b = 0; b < C::PB; b++) sf[ct][b] = frag_of<T>(S[ct][2 * b], S[ct][2 * b + 1]);
 #pragma unroll
-                for (int b = 0; b < C::PB; b++) mma(far, sf[b], sq.along(it * 16, b * 32, lane));
-#pragma unroll
-                for (int b = 0; b <= it / 2; b++) mma(own, vf[b], sp.along(it * 16, b * 32, lane));
-                watch(none, own);
-                write(it, own, far);
-            }
-            if (any_not_finite(none)) {
-#pragma unroll 1
                 for (int it = 0; it < C::LT; it++) {
-                    const int i = it * 16 + i16;
-                    f32x4 own = {0.f, 0.f, 0.f, 0.f}, far = {0.f, 0.f, 0.f, 0.f};
+                    f32x4 own[CT], far[CT];
 #pragma unroll
-                    for (int b = 0; b < C::PB; b++) mma(far, sf[b], sq.along(it * 16, b * 32, lane));
-#pragma unroll 1
-                    for (int j = max(seen_from(m, i), 0); j <= i; j++)
+                    for (int ct = 0; ct < CT; ct++) { own[ct] = zero; far[ct] = zero; }
 #pragma unroll
-                        for (int r = 0; r < 4; r++) own[r] = fmaf(as_f32(*sp.at(i, j)), as_f32(*sv.at(j, e0 + 4 * g + r)), own[r]);
-                    write(it, own, far);
+                    for (int b = 0; b < C::PB; b++) {
+                        const Frag<T> x = sq.along(it * 16, b * 32, lane);
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) mma(far[ct], sf[ct][b], x);
+                    }
+#pragma unroll
+                    for (int b = 0; b <= it / 2; b++) {
+                        const Frag<T> x = sp.along(it * 16, b * 32, lane);
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) mma(own[ct], vf[ct][b], x);
+                    }
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        watch(all, own[ct]);
+                        write(it, ct, own[ct], far[ct]);
+                    }
                 }
+            }
+            if (any_not_finite(all)) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll 1
+                    for (int it = 0; it < C::LT; it++) {
+                        const int i = it * 16 + i16;
+                        f32x4 own = zero, far = zero;
+#pragma unroll
+                        for (int b = 0; b < C::PB; b++) mma(far, frag_of<T>(S[ct][2 * b], S[ct][2 * b + 1]), sq.along(it * 16, b * 32, lane));
+#pragma unroll 1
+                        for (int j = max(seen_from(m, i), 0); j <= i; j++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                own[r] = fmaf(as_f32(*sp.at(i, j)), as_f32(*sv.at(j, e0 + 16 * ct + 4 * g + r)), own[r]);
+                        write(it, ct, own, far);
+                    }
             }
         }
 
-        f32x4 add[C::PT];
+        f32x4 add[CT][C::PT];
 #pragma unroll
-        for (int dt = 0; dt < C::PT; dt++) add[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int dt = 0; dt < C::PT; dt++) add[ct][dt] = zero;
 #pragma unroll
         for (int b = 0; b < C::LB; b++) {
-            Frag<T> part[kParts<T>];
-            scaled_parts(vf[b], &wt[b * 32 + 8 * g], part);
+            Frag<T> part[CT][kParts<T>];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) scaled_parts(vf[ct][b], &wt[b * 32 + 8 * g], part[ct]);
 #pragma unroll
             for (int dt = 0; dt < C::PT; dt++) {
                 const Frag<T> kf = sk.template down<true>(b * 32, acc_col(dt), lane);
 #pragma unroll
-                for (int p = 0; p < kParts<T>; p++) mma(add[dt], kf, part[p]);
+                for (int p = 0; p < kParts<T>; p++)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) mma(add[ct][dt], kf, part[ct][p]);
             }
         }
-        float none = 0.f;
+        float all = 0.f;
 #pragma unroll
-        for (int dt = 0; dt < C::PT; dt++) watch(none, add[dt]);
-        if (any_not_finite(none)) {
+        for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-            for (int dt = 0; dt < C::PT; dt++) {
-                add[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int dt = 0; dt < C::PT; dt++) watch(all, add[ct][dt]);
+        if (any_not_finite(all)) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int dt = 0; dt < C::PT; dt++) {
+                    add[ct][dt] = zero;
 #pragma unroll 1
-                for (int j = max(last, 0); j < n; j++)
+                    for (int j = max(last, 0); j < n; j++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        add[dt][r] = fmaf(wt[j] * as_f32(*sk.at(j, acc_row(dt, g, r))), as_f32(*sv.at(j, e0 + i16)), add[dt][r]);
-            }
+                        for (int r = 0; r < 4; r++)
+                            add[ct][dt][r] = fmaf(wt[j] * as_f32(*sk.at(j, acc_row(dt, g, r))), as_f32(*sv.at(j, e0 + 16 * ct + i16)), add[ct][dt][r]);
+                }
         }
-        const float f = pw[n];
+        const float f = pw.pw[n];
 #pragma unroll
-        for (int dt = 0; dt < C::PT; dt++)
+        for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) S[dt][r] = last < 0 ? fmaf(f, S[dt][r], add[dt][r]) : add[dt][r];
+            for (int dt = 0; dt < C::PT; dt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) S[ct][dt][r] = last < 0 ? fmaf(f, S[ct][dt][r], add[ct][dt][r]) : add[ct][dt][r];
+    }
+    if (OUT && c0 < c1) {
+        __syncthreads();
+        out.take(ly, (c1 - 1) * L, (int)min((int64_t)L, a.T - (c1 - 1) * L));
     }
     float* to = !OUT ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : cut.segs > 1 ? nullptr : a.state_out + nh * de;
-    if (to) each_of_state<T, P, false>(a, e0, [&](int t, int r, int at) { to[at] = S[t][r]; });
+    if (to)
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) each_of_state<T, P, false>(a, e0 + 16 * ct, [&](int t, int r, int at) { to[at] = S[ct][t][r]; });
     if (!OUT && threadIdx.x == 0) {
         const int64_t n = min(c1 * L, a.T) - c0 * L;
         cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : exp2f((float)n * __log2f(a.decay[h]));
@@ -395,7 +463,7 @@ constexpr int FORWARD_PER_CU = 4;
 template <class T, int P> int attend_chunks(const MoAttend& a, hipStream_t s) {
     Cut c = attend_cut(a, FORWARD_PER_CU);
     cut_place(a, c);
-    const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(Chunk<T, P>::NT);
+    const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(kForwardWaves<P> * kWave);
     if (c.segs > 1) {
         hipLaunchKernelGGL((k_attend<T, P, ONLY_SUMS>), grid, block, 0, s, a, c);
         if (launched("k_attend sums") || enter_states(a, c, a.state, a.state_out, false, s)) return -1;

@@ -13,26 +13,32 @@ namespace mo {
 // q, k, v and dO are read once for all of them. Wave w holds the 16 rows of R from 16 w, as the accumulator tiles of R^T, which
 // are the operand of V R^T as they lie; K R takes R from LDS. S comes from the forward pass (a.saved), each wave its rows, in
 // 16-byte pieces straight into operands.
+template <class T, int P> using BackChunk = Chunk<T, P, P / 16>;
 template <class T, int P> struct BackLds {
-    typedef Chunk<T, P> C;
-    T q[C::L * P], k[C::L * P], v[C::L * P], o[C::L * P];   // o: dO
-    T a[C::L * C::L], b[C::L * C::L];
-    T r[P * P];
-    float wt[C::L], ut[C::L], pw[C::L + 4];
+    typedef BackChunk<T, P> C;
+    static constexpr int L = C::L, ROWS = L * P;
+    T q[ROWS], k[ROWS], v[ROWS], o[ROWS];        // o: dO
+    T a[L * L], b[L * L], y[ROWS];               // y: dV
+    T r[P * P > ROWS ? P * P : ROWS];
+    float wt[L], ut[L];
+    Powers<L> pw;
+    // Once dV is there, A and R's tile make room for dQ and dK.
+    __device__ __forceinline__ T* dq() { return r; }
+    __device__ __forceinline__ T* dk() { return P <= L ? a : r + ROWS; }
+    static_assert(P <= L || P * P >= 2 * ROWS, "");
 };
 
-// R += Q^T diag(u) dO of a chunk, as R^T's tiles: `at` the wave's columns (rows of R).
+// The sum over a chunk's steps of Q^T diag(u) dO, as R^T's tiles of the wave's columns from x0.
 template <class T, int P>
-__device__ __forceinline__ void add_to_r(f32x4 (&add)[P / 16], const Frag<T> (&qf)[Chunk<T, P>::LB], const Tile<T, P>& so, const Tile<T, P>& sq,
-                                         const float* ut, int x0, int first, int lane) {
-    typedef Chunk<T, P> C;
-    const int g = lane / 16, i16 = lane % 16;
+__device__ __forceinline__ void add_to_r(f32x4 (&add)[P / 16], const Tile<T, P>& so, const Tile<T, P>& sq, const float* ut, int x0, int first, unsigned lane) {
+    typedef BackChunk<T, P> C;
+    const unsigned g = lane / 16, i16 = lane % 16;
 #pragma unroll
     for (int et = 0; et < C::PT; et++) add[et] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < C::LB; b++) {
         Frag<T> part[kParts<T>];
-        scaled_parts(qf[b], &ut[b * 32 + 8 * g], part);
+        scaled_parts(sq.down(b * 32, x0, lane), &ut[b * 32 + 8 * g], part);
 #pragma unroll
         for (int et = 0; et < C::PT; et++) {
             const Frag<T> x = so.template down<true>(b * 32, acc_col(et), lane);
@@ -40,10 +46,10 @@ __device__ __forceinline__ void add_to_r(f32x4 (&add)[P / 16], const Frag<T> (&q
             for (int p = 0; p < kParts<T>; p++) mma(add[et], x, part[p]);
         }
     }
-    float none = 0.f;
+    float all = 0.f;
 #pragma unroll
-    for (int et = 0; et < C::PT; et++) watch(none, add[et]);
-    if (!any_not_finite(none)) return;
+    for (int et = 0; et < C::PT; et++) watch(all, add[et]);
+    if (!any_not_finite(all)) return;
 #pragma unroll
     for (int et = 0; et < C::PT; et++) {
         add[et] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -56,8 +62,9 @@ __device__ __forceinline__ void add_to_r(f32x4 (&add)[P / 16], const Frag<T> (&q
 }
 
 template <class T, int P>
-__global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back(MoAttend a, Cut cut) {
-    typedef Chunk<T, P> C;
+__global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAttend a, Cut cut) {
+    typedef BackChunk<T, P> C;
+    typedef HeadRows<T, C> Head;
     constexpr int L = C::L;
     extern __shared__ __align__(16) char lds[];
     BackLds<T, P>& s = *(BackLds<T, P>*)lds;
@@ -69,23 +76,31 @@ __global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back(MoAttend a, C
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int x0 = w * 16;     // the wave's rows of R and S, columns of dq and dk; of dv its columns
     const int64_t de = (int64_t)a.D * a.E;
-    const Bring<T, P> q(a.q, env, h, a.D), k(a.k, env, h, a.D), v(a.v, env, h, a.E), o(a.dout, env, h, a.E);
+    const Head q(a.q, env, h, a.D, a.D == P), k(a.k, env, h, a.D, a.D == P), v(a.v, env, h, a.E, a.E == P), o(a.dout, env, h, a.E, a.E == P);
+    const Head dq(a.dq, env, h, a.D, on_pieces<T>(a.dq)), dk(a.dk, env, h, a.D, on_pieces<T>(a.dk)), dv(a.dv, env, h, a.E, on_pieces<T>(a.dv));
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-    powers<L>(s.pw, a.decay[h]);
+    s.pw.fill(a.decay[h], a.scale);
     f32x4 R[C::PT];            // R^T: rows e, columns d
 #pragma unroll
-    for (int et = 0; et < C::PT; et++) R[et] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int et = 0; et < C::PT; et++) R[et] = zero;
     const float* in = cut.segs > 1 ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : a.dstate_out ? a.dstate_out + nh * de : nullptr;
     if (in) each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { R[t][r] = in[at]; });
     for (int64_t c = c1 - 1; c >= c0; c--) {
         const int64_t t0 = c * L;
         const int n = (int)min((int64_t)L, a.T - t0);
-        __syncthreads();                                       // the last chunk's tiles are done with
-        q.chunk(s.q, t0, n);
-        k.chunk(s.k, t0, n);
-        v.chunk(s.v, t0, n);
-        o.chunk(s.o, t0, n);
-        const int lane = lane_here(), g = lane / 16, i16 = lane % 16;
+        __syncthreads();                                       // the last chunk's tiles are done with, its results in theirs
+        q.bring(s.q, t0, n);
+        k.bring(s.k, t0, n);
+        v.bring(s.v, t0, n);
+        o.bring(s.o, t0, n);
+        if (c < c1 - 1) {
+            const int n1 = (int)min((int64_t)L, a.T - t0 - L);
+            dq.take(s.dq(), t0 + L, n1);
+            dk.take(s.dk(), t0 + L, n1);
+            dv.take(s.y, t0 + L, n1);
+        }
+        const unsigned lane = thread_here() % kWave, g = lane / 16, i16 = lane % 16;
         // the state that enters the chunk: rows d of the wave, eight neighbouring columns e a lane
         Frag<T> sf[C::PB];
         {
@@ -106,144 +121,165 @@ __global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back(MoAttend a, C
                     }
             }
         }
+        const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);
+        const int last = seen_from(m, L - 1);
+        if (threadIdx.x < L) {
+            const int i = threadIdx.x;
+            s.wt[i] = i < n && i >= last ? s.pw.pw[n - 1 - i] : 0.f;
+            s.ut[i] = i < n && seen_from(m, i) < 0 ? a.scale * s.pw.pw[i + 1] : 0.f;
+        }
+        brought();
+
 #pragma unroll
         for (int b = 0; b < C::PB; b++) {                      // R by rows d, for K R
             const Frag<T> x = frag_of<T>(R[2 * b], R[2 * b + 1]);
 #pragma unroll
             for (int j = 0; j < 8; j += C::Rows::EPV) *(uint4*)sr.at(x0 + i16, b * 32 + 8 * g + j) = *(const uint4*)((const T*)&x + j);
         }
-        const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);
-        const int last = seen_from(m, L - 1);
-        if (threadIdx.x < L) {
-            const int i = threadIdx.x;
-            s.wt[i] = i < n && i >= last ? s.pw[n - 1 - i] : 0.f;
-            s.ut[i] = i < n && seen_from(m, i) < 0 ? a.scale * s.pw[i + 1] : 0.f;
-        }
-        brought();
-
+        const auto scores = [&](auto starts) {                 // A and B, a lane four neighbouring j of one i
 #pragma unroll
-        for (int z = 0; z < C::TPW; z++) {                     // A and B, a lane four neighbouring j of one i
-            const int idx = w + z * C::WAVES;
-            if (C::TILES % C::WAVES && idx >= C::TILES) break;
-            int it, jt;
-            C::score_tile(idx, it, jt);
-            f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+            for (int z = 0; z < C::TPW; z++) {
+                const int idx = w + z * C::WAVES;
+                if (C::TILES % C::WAVES && idx >= C::TILES) break;
+                int it, jt;
+                C::score_tile(idx, it, jt);
+                f32x4 x = zero, y = zero;
 #pragma unroll
-            for (int b = 0; b < C::PB; b++) {
-                mma(x, sk.along(jt * 16, b * 32, lane), sq.along(it * 16, b * 32, lane));
-                mma(y, sv.along(jt * 16, b * 32, lane), so.along(it * 16, b * 32, lane));
+                for (int b = 0; b < C::PB; b++) {
+                    mma(x, sk.along(jt * 16, b * 32, lane), sq.along(it * 16, b * 32, lane));
+                    mma(y, sv.along(jt * 16, b * 32, lane), so.along(it * 16, b * 32, lane));
+                }
+                const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = starts ? seen_from(m, i) : 0;
+                const float* f = s.pw.sees(i, j);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const bool sees = !starts || j + r >= from;
+                    x[r] = sees ? x[r] * f[-r] : 0.f;
+                    y[r] = sees ? y[r] * f[-r] : 0.f;
+                }
+                *(Pack<T, 4>*)sa.at(i, j) = pack4(x, T{});
+                *(Pack<T, 4>*)sb.at(i, j) = pack4(y, T{});
             }
-            const int i = it * 16 + i16, j = jt * 16 + 4 * g, from = m ? seen_from(m, i) : -1;
-            Pack<T, 4> xa, yb;
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const bool sees = j + r <= i && j + r >= from;
-                const float f = a.scale * s.pw[max(i - j - r, 0)];
-                xa.v[r] = as<T>(sees ? f * x[r] : 0.f);
-                yb.v[r] = as<T>(sees ? f * y[r] : 0.f);
-            }
-            *(Pack<T, 4>*)sa.at(i, j) = xa;
-            *(Pack<T, 4>*)sb.at(i, j) = yb;
-        }
+        };
+        if (m) scores(std::true_type{});
+        else scores(std::false_type{});
         __syncthreads();
 
-        // Each output transposed: a lane has four neighbouring columns of one step. `own` the sum over the chunk's steps, `far`
-        // what the entering state or its gradient adds, by a factor a step.
-        const auto write = [&](const MoRows& to, int size, int t, float f, const f32x4& own, const f32x4& far) {
-            const int i = t * 16 + i16;
-            Pack<T, 4> y;
+        // Each result transposed: a lane has four neighbouring columns of one step. `own` the sum over the chunk's steps, `far`
+        // what the entering state or its gradient adds, by a factor f a step.
+        const auto write = [&](const typename C::Rows& to, int t, float f, const f32x4& own, const f32x4& far) {
+            f32x4 y;
 #pragma unroll
-            for (int r = 0; r < 4; r++) y.v[r] = as<T>(f == 0.f ? own[r] : fmaf(f, far[r], own[r]));
-            if (i < n && x0 + 4 * g < size)
-                put4((T*)to.p + env * to.sn + h * to.sh + x0 + 4 * g + (t0 + i) * to.st, y, rows_wide(to, 4 * sizeof(T)));
+            for (int r = 0; r < 4; r++) y[r] = fmaf(f, far[r], own[r]);
+            if (m && f == 0.f) y = own;                        // (what is not seen may be anything)
+            *(Pack<T, 4>*)to.at(t * 16 + i16, x0 + 4 * g) = pack4(y, T{});
         };
-        // far + sum over the steps j that step i sees (or that see it) of x_ij y_j, made again one product after another
-        const auto again = [&](const auto& x, bool down, const auto& y, int i, f32x4& own) {
-            own = f32x4{0.f, 0.f, 0.f, 0.f};
+        // `own` again, one product after another: over the steps j that step i sees (or that see it) of x_ij y_j
+        const auto again = [&](const typename C::Scores& x, bool down, const typename C::Rows& y, int i) {
+            f32x4 own = zero;
             const int j0 = down ? i : max(seen_from(m, i), 0), j1 = down ? n - 1 : i;
 #pragma unroll 1
             for (int j = j0; j <= j1 && (!down || seen_from(m, j) <= i); j++)
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     own[r] = fmaf(as_f32(down ? *x.at(j, i) : *x.at(i, j)), as_f32(*y.at(j, x0 + 4 * g + r)), own[r]);
+            return own;
         };
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-        Frag<T> kf[C::LB];                                     // dQ
+        {                                                      // dV
+            Frag<T> of[C::LB], rf[C::PB];
 #pragma unroll
-        for (int b = 0; b < C::LB; b++) kf[b] = sk.down(b * 32, x0, lane);
+            for (int b = 0; b < C::LB; b++) of[b] = so.down(b * 32, x0, lane);
 #pragma unroll
-        for (int t = 0; t < C::LT; t++) {
-            f32x4 own = zero, far = zero;
+            for (int b = 0; b < C::PB; b++) rf[b] = sr.down(b * 32, x0, lane);
+            const typename C::Rows sy{s.y};
 #pragma unroll
-            for (int b = 0; b < C::PB; b++) mma(far, sf[b], so.along(t * 16, b * 32, lane));
+            for (int t = 0; t < C::LT; t++) {
+                f32x4 own = zero, far = zero;
 #pragma unroll
-            for (int b = 0; b <= t / 2; b++) mma(own, kf[b], sb.along(t * 16, b * 32, lane));
-            float none = 0.f;
-            watch(none, own);
-            if (any_not_finite(none)) again(sb, false, sk, t * 16 + i16, own);
-            write(a.dq, a.D, t, s.ut[t * 16 + i16], own, far);
+                for (int b = 0; b < C::PB; b++) mma(far, rf[b], sk.along(t * 16, b * 32, lane));
+#pragma unroll
+                for (int b = t / 2; b < C::LB; b++) mma(own, of[b], sa.down(b * 32, t * 16, lane));
+                float all = 0.f;
+                watch(all, own);
+                if (any_not_finite(all)) own = again(sa, true, so, t * 16 + i16);
+                write(sy, t, s.wt[t * 16 + i16], own, far);
+            }
         }
-
-        Frag<T> qf[C::LB];                                     // dK
+        __syncthreads();                                       // A and R's tile are done with
+        {                                                      // dQ
+            Frag<T> kf[C::LB];
 #pragma unroll
-        for (int b = 0; b < C::LB; b++) qf[b] = sq.down(b * 32, x0, lane);
+            for (int b = 0; b < C::LB; b++) kf[b] = sk.down(b * 32, x0, lane);
+            const typename C::Rows sy{s.dq()};
 #pragma unroll
-        for (int t = 0; t < C::LT; t++) {
-            f32x4 own = zero, far = zero;
+            for (int t = 0; t < C::LT; t++) {
+                f32x4 own = zero, far = zero;
 #pragma unroll
-            for (int b = 0; b < C::PB; b++) mma(far, frag_of<T>(R[2 * b], R[2 * b + 1]), sv.along(t * 16, b * 32, lane));
+                for (int b = 0; b < C::PB; b++) mma(far, sf[b], so.along(t * 16, b * 32, lane));
 #pragma unroll
-            for (int b = t / 2; b < C::LB; b++) mma(own, qf[b], sb.down(b * 32, t * 16, lane));
-            float none = 0.f;
-            watch(none, own);
-            if (any_not_finite(none)) again(sb, true, sq, t * 16 + i16, own);
-            write(a.dk, a.D, t, s.wt[t * 16 + i16], own, far);
+                for (int b = 0; b <= t / 2; b++) mma(own, kf[b], sb.along(t * 16, b * 32, lane));
+                float all = 0.f;
+                watch(all, own);
+                if (any_not_finite(all)) own = again(sb, false, sk, t * 16 + i16);
+                write(sy, t, s.ut[t * 16 + i16], own, far);
+            }
         }
-
-        Frag<T> of[C::LB];                                     // dV
+        {                                                      // dK
+            Frag<T> qf[C::LB], rf[C::PB];
 #pragma unroll
-        for (int b = 0; b < C::LB; b++) of[b] = so.down(b * 32, x0, lane);
+            for (int b = 0; b < C::LB; b++) qf[b] = sq.down(b * 32, x0, lane);
 #pragma unroll
-        for (int t = 0; t < C::LT; t++) {
-            f32x4 own = zero, far = zero;
+            for (int b = 0; b < C::PB; b++) rf[b] = frag_of<T>(R[2 * b], R[2 * b + 1]);
+            const typename C::Rows sy{s.dk()};
 #pragma unroll
-            for (int b = 0; b < C::PB; b++) mma(far, sr.down(b * 32, x0, lane), sk.along(t * 16, b * 32, lane));
+            for (int t = 0; t < C::LT; t++) {
+                f32x4 own = zero, far = zero;
 #pragma unroll
-            for (int b = t / 2; b < C::LB; b++) mma(own, of[b], sa.down(b * 32, t * 16, lane));
-            float none = 0.f;
-            watch(none, own);
-            if (any_not_finite(none)) again(sa, true, so, t * 16 + i16, own);
-            write(a.dv, a.E, t, s.wt[t * 16 + i16], own, far);
+                for (int b = 0; b < C::PB; b++) mma(far, rf[b], sv.along(t * 16, b * 32, lane));
+#pragma unroll
+                for (int b = t / 2; b < C::LB; b++) mma(own, qf[b], sb.down(b * 32, t * 16, lane));
+                float all = 0.f;
+                watch(all, own);
+                if (any_not_finite(all)) own = again(sb, true, sq, t * 16 + i16);
+                write(sy, t, s.wt[t * 16 + i16], own, far);
+            }
         }
 
         f32x4 add[C::PT];                                      // R'
-        add_to_r<T, P>(add, qf, so, sq, s.ut, x0, m ? (int)__ffsll((long long)m) - 1 : n, lane);
-        const float f = s.pw[n];
+        add_to_r<T, P>(add, so, sq, s.ut, x0, m ? (int)__ffsll((long long)m) - 1 : n, lane);
+        const float f = s.pw.pw[n];
 #pragma unroll
         for (int et = 0; et < C::PT; et++)
 #pragma unroll
             for (int r = 0; r < 4; r++) R[et][r] = m ? add[et][r] : fmaf(f, R[et][r], add[et][r]);
+    }
+    if (c0 < c1) {
+        __syncthreads();
+        const int n = (int)min((int64_t)L, a.T - c0 * L);
+        dq.take(s.dq(), c0 * L, n);
+        dk.take(s.dk(), c0 * L, n);
+        dv.take(s.y, c0 * L, n);
     }
     if (a.dstate && cut.segs == 1) each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { a.dstate[nh * de + at] = R[t][r]; });
 }
 
 // A segment's own sum of R' (see R' above) and what it leaves of a gradient that comes from behind it.
 template <class T, int P>
-__global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back_sums(MoAttend a, Cut cut) {
-    typedef Chunk<T, P> C;
+__global__ void __launch_bounds__((BackChunk<T, P>::NT)) k_attend_back_sums(MoAttend a, Cut cut) {
+    typedef BackChunk<T, P> C;
+    typedef HeadRows<T, C> Head;
     constexpr int L = C::L;
     __shared__ __align__(16) T lq[L * P], lo[L * P];
-    __shared__ float pw[L + 1];
+    __shared__ Powers<L> pw;
     __shared__ __align__(16) float ut[L];
     const typename C::Rows sq{lq}, so{lo};
-    const int w = threadIdx.x / kWave;
     const int64_t nh = blockIdx.x, env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
-    const int x0 = w * 16;
-    const Bring<T, P> q(a.q, env, h, a.D), o(a.dout, env, h, a.E);
-    powers<L>(pw, a.decay[h]);
+    const int x0 = threadIdx.x / kWave * 16;
+    const Head q(a.q, env, h, a.D, a.D == P), o(a.dout, env, h, a.E, a.E == P);
+    pw.fill(a.decay[h], a.scale);
     f32x4 R[C::PT];
 #pragma unroll
     for (int et = 0; et < C::PT; et++) R[et] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -252,19 +288,15 @@ __global__ void __launch_bounds__((Chunk<T, P>::NT)) k_attend_back_sums(MoAttend
         const int64_t t0 = c * L;
         const int n = (int)min((int64_t)L, a.T - t0);
         __syncthreads();
-        q.chunk(lq, t0, n);
-        o.chunk(lo, t0, n);
+        q.bring(lq, t0, n);
+        o.bring(lo, t0, n);
         const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);
         any_start |= m != 0;
-        if (threadIdx.x < L) ut[threadIdx.x] = (int)threadIdx.x < n && seen_from(m, threadIdx.x) < 0 ? a.scale * pw[threadIdx.x + 1] : 0.f;
+        if (threadIdx.x < L) ut[threadIdx.x] = (int)threadIdx.x < n && seen_from(m, threadIdx.x) < 0 ? a.scale * pw.pw[threadIdx.x + 1] : 0.f;
         brought();
-        const int lane = lane_here();
-        Frag<T> qf[C::LB];
-#pragma unroll
-        for (int b = 0; b < C::LB; b++) qf[b] = sq.down(b * 32, x0, lane);
         f32x4 add[C::PT];
-        add_to_r<T, P>(add, qf, so, sq, ut, x0, m ? (int)__ffsll((long long)m) - 1 : n, lane);
-        const float f = pw[n];
+        add_to_r<T, P>(add, so, sq, ut, x0, m ? (int)__ffsll((long long)m) - 1 : n, thread_here() % kWave);
+        const float f = pw.pw[n];
 #pragma unroll
         for (int et = 0; et < C::PT; et++)
 #pragma unroll
@@ -283,7 +315,7 @@ constexpr int BACKWARD_PER_CU = 2;
 template <class T, int P> int attend_back_chunks(const MoAttend& a, hipStream_t s) {
     Cut c = attend_cut(a, BACKWARD_PER_CU);
     cut_place(a, c);
-    const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(Chunk<T, P>::NT);
+    const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(BackChunk<T, P>::NT);
     if (c.segs > 1) {
         hipLaunchKernelGGL((k_attend_back_sums<T, P>), grid, block, 0, s, a, c);
         if (launched("k_attend_back_sums") || enter_states(a, c, a.dstate_out, a.dstate, true, s)) return -1;

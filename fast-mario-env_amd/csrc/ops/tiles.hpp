@@ -6,6 +6,7 @@ namespace mo {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 // An operand of a product over 32 indices: lane l has row (of A) or column (of B) l % 16 and the indices 8 (l / 16) + 0..7.
@@ -29,19 +30,21 @@ template <class T, int W> struct Tile {
     static constexpr int EPV = 16 / sizeof(T), PIECES = W / EPV;
     static_assert(PIECES >= 4, "");
     T* p;
-    static __device__ __forceinline__ int turn(int row) {
+    static __device__ __forceinline__ unsigned turn(unsigned row) {
         return PIECES == 4 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
     }
-    __device__ __forceinline__ T* at(int row, int col) const { return p + row * W + (((col / EPV) ^ turn(row)) * EPV | (col % EPV)); }
+    __device__ __forceinline__ T* at(unsigned row, unsigned col) const {
+        return p + (row * W + (((col / EPV) ^ turn(row)) * EPV | (col % EPV)));
+    }
 
     // indices along the rows: `row` the operand's first, its indices from col
-    __device__ __forceinline__ Frag<T> along(int row, int col, int lane) const;
+    __device__ __forceinline__ Frag<T> along(unsigned row, unsigned col, unsigned lane) const;
     // indices down the rows from `row`; the operand's rows or columns are the tile's columns from col, or (SPREAD) four of each
     // eight: column c of the operand is col + 8 (c / 4) + c % 4
-    template <bool SPREAD = false> __device__ __forceinline__ Frag<T> down(int row, int col, int lane) const;
+    template <bool SPREAD = false> __device__ __forceinline__ Frag<T> down(unsigned row, unsigned col, unsigned lane) const;
 };
-template <class T, int W> __device__ __forceinline__ Frag<T> Tile<T, W>::along(int row, int col, int lane) const {
-    const int r = row + lane % 16, c = col + 8 * (lane / 16);
+template <class T, int W> __device__ __forceinline__ Frag<T> Tile<T, W>::along(unsigned row, unsigned col, unsigned lane) const {
+    const unsigned r = row + lane % 16, c = col + 8 * (lane / 16);
     if constexpr (sizeof(T) == 2) {
         return {*(const bf16x8*)at(r, c)};
     } else {
@@ -51,17 +54,17 @@ template <class T, int W> __device__ __forceinline__ Frag<T> Tile<T, W>::along(i
         return f;
     }
 }
-template <class T, int W> template <bool SPREAD> __device__ __forceinline__ Frag<T> Tile<T, W>::down(int row, int col, int lane) const {
-    const int g = lane / 16, i = lane % 16;
+template <class T, int W> template <bool SPREAD> __device__ __forceinline__ Frag<T> Tile<T, W>::down(unsigned row, unsigned col, unsigned lane) const {
+    const unsigned g = lane / 16, i = lane % 16;
     if constexpr (sizeof(T) == 2) {   // the transposing LDS read: 16 lanes read four neighbours of each of 4 rows and get a column each
         typedef __attribute__((address_space(3))) i16x4* Lds;
-        const int r = row + 8 * g + i / 4, c = col + (i % 4) * (SPREAD ? 8 : 4);
+        const unsigned r = row + 8 * g + i / 4, c = col + (i % 4) * (SPREAD ? 8 : 4);
         union { i16x4 h[2]; Frag<bf16> f; } u;
         u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at(r, c));
         u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at(r + 4, c));
         return u.f;
     } else {
-        const int c = col + (SPREAD ? 8 * (i / 4) + i % 4 : i);
+        const unsigned c = col + (SPREAD ? 8 * (i / 4) + i % 4 : i);
         Frag<T> f;
 #pragma unroll
         for (int e = 0; e < 8; e++) f.v[e] = *at(row + 8 * g + e, c);
@@ -74,46 +77,58 @@ template <class T, int W> template <bool SPREAD> __device__ __forceinline__ Frag
 // operand that makes such a tile takes its columns SPREAD.) This is the one rounding of what the tiles hold.
 __device__ __forceinline__ constexpr int acc_row(int t, int g, int r) { return 32 * (t / 2) + 8 * g + 4 * (t % 2) + r; }
 __device__ __forceinline__ constexpr int acc_col(int t) { return 32 * (t / 2) + 4 * (t % 2); }   // its first column there
+__device__ __forceinline__ Pack<float, 4> pack4(const f32x4& x, float) { return *(const Pack<float, 4>*)&x; }
+__device__ __forceinline__ Pack<bf16, 4> pack4(const f32x4& x, bf16) {   // two conversions an instruction
+    const bf16x4 y = __builtin_convertvector(x, bf16x4);
+    return *(const Pack<bf16, 4>*)&y;
+}
 template <class T> __device__ __forceinline__ Frag<T> frag_of(const f32x4& a, const f32x4& b) {
-    Frag<T> f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) { f.v[i] = as<T>(a[i]); f.v[4 + i] = as<T>(b[i]); }
-    return f;
+    union { Pack<T, 4> h[2]; Frag<T> f; } u{};
+    u.h[0] = pack4(a, T{});
+    u.h[1] = pack4(b, T{});
+    return u.f;
 }
 
 // B's operand of a product that gives columns 16 half .. 16 half + 15 of A's 32 indices back: A's rows by lanes become its
 // columns by lanes, exactly.
-template <class T> __device__ __forceinline__ Frag<T> unit_frag(int half, int lane) {
+template <class T> __device__ __forceinline__ Frag<T> unit_frag(unsigned half, unsigned lane) {
     Frag<T> f;
 #pragma unroll
     for (int i = 0; i < 8; i++) f.v[i] = as<T>(8 * (lane / 16) + i == 16 * half + lane % 16 ? 1.f : 0.f);
     return f;
 }
 
-// The lane's number, not known to be the same from one pass of a loop to the next: what follows from it (addresses, mostly) is
-// then made where it is used, instead of being kept in registers over the whole loop, which costs more in waves than it saves.
-__device__ __forceinline__ int lane_here() {
-    int lane = threadIdx.x % kWave;
-    asm volatile("" : "+v"(lane));
-    return lane;
-}
-
-// acc += A (w B), w a factor for each index, with float32's precision: w B is split into bf16 parts of 8 bits of significand
-// each, three of which leave 2^-27 of it. (Where w is 0 the value is left out, whatever it is.)
+// The parts of w B, w a factor for each index, that keep float32's precision in products with bf16 operands: bf16 parts of 8 bits
+// of significand each, three of which leave 2^-27 of it.
 __device__ __forceinline__ void scaled_parts(const Frag<bf16>& b, const float* w, Frag<bf16>* part) {
+    union { uint4 u; Frag<bf16> f; } in{};
+    in.f = b;
+    const uint32_t word[4] = {in.u.x, in.u.y, in.u.z, in.u.w};
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float x = w[i] == 0.f ? 0.f : w[i] * (float)b.v[i];
+    for (int h = 0; h < 2; h++) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t y = word[2 * h + i / 2];
+            x[i] = w[4 * h + i] * __uint_as_float(i % 2 ? y & 0xffff0000u : y << 16);
+        }
 #pragma unroll
         for (int p = 0; p < 3; p++) {
-            part[p].v[i] = (bf16)x;
-            x -= (float)part[p].v[i];
+            union { bf16x4 v; uint2 u; } y{};
+            y.v = __builtin_convertvector(x, bf16x4);
+            ((uint2*)&part[p])[h] = y.u;
+            if (p < 2) {
+                x[0] -= __uint_as_float(y.u.x << 16);
+                x[1] -= __uint_as_float(y.u.x & 0xffff0000u);
+                x[2] -= __uint_as_float(y.u.y << 16);
+                x[3] -= __uint_as_float(y.u.y & 0xffff0000u);
+            }
         }
     }
 }
 __device__ __forceinline__ void scaled_parts(const Frag<float>& b, const float* w, Frag<float>* part) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) part[0].v[i] = w[i] == 0.f ? 0.f : w[i] * b.v[i];
+    for (int i = 0; i < 8; i++) part[0].v[i] = w[i] * b.v[i];
 }
 template <class T> constexpr int kParts = 1;
 template <> inline constexpr int kParts<bf16> = 3;
