@@ -64,7 +64,7 @@ template <class T, class C> struct HeadRows {
             typedef const __attribute__((address_space(1))) void* Global;
 #pragma unroll
             for (int i = 0; i < C::RV; i++)
-                __builtin_amdgcn_global_load_lds((Global)(from + i * C::STEP * st), (Lds)(to + i * C::NT * Tl::EPV), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((Global)(from + i * C::STEP * st), (Lds)(to + i * C::NT * Tl::EPV), 16, 0, 2 /* nt: read once */);
             return;
         }
 #pragma unroll
@@ -85,7 +85,7 @@ template <class T, class C> struct HeadRows {
         for (int i = 0; i < C::RV; i++) {
             const Piece x = *(const Piece*)(tile + (t + i * C::NT) * Tl::EPV);
             if ((int)row + i * C::STEP >= n || (int)col >= d) continue;
-            if (whole) *(Piece*)(to + i * C::STEP * st) = x;
+            if (whole) stream((Piece*)(to + i * C::STEP * st), x);
             else
 #pragma unroll
                 for (int j = 0; j < Tl::EPV; j++) to[i * C::STEP * st + j] = x.v[j];
@@ -128,6 +128,15 @@ template <int L> struct Powers {
     __device__ __forceinline__ const float* sees(int i, int j) const { return &seen[L + i - j]; }
 };
 
+// The env and head of a workgroup. Workgroups go to the 8 XCDs in turn; XCD_RUN neighbouring heads (whose rows of a step lie
+// together) go to one of them, so that what one L2 fetches lies together too.
+constexpr int XCD_RUN = 16;
+__device__ __forceinline__ int64_t head_of_block(int64_t heads) {
+    const int64_t b = blockIdx.x, round = 8 * XCD_RUN;
+    if (b >= heads / round * round) return b;
+    return b / round * round + b % 8 * XCD_RUN + b % round / 8;
+}
+
 // A long sequence is cut into segments of whole chunks, a workgroup each, so that few sequences fill the chip. First each
 // segment's own sum and what it leaves of an entering state (`keep`: g^steps, or -1 where an episode starts inside), then the
 // states that enter the segments one after another, then the outputs from there.
@@ -142,23 +151,41 @@ enum { KEEP_NONE = 0, KEEP_STATES = 1, ONLY_SUMS = 2 };
 
 // MODE: KEEP_STATES leaves the states that enter chunks 1, 2, .. for the gradient in a.saved, (N H, chunks - 1, P, P) in the
 // elements' type: there they are operands only. ONLY_SUMS makes a segment's own sum.
-// A wave's 16 columns (from x0) of a head's (D, E) matrix, or of its transpose, as accumulator tiles.
-template <class T, int P, bool TRANSPOSED, class F> __device__ __forceinline__ void each_of_state(const MoAttend& a, int x0, F f) {
+// A wave's 16 columns (from x0) of a head's float32 (D, E) matrix, or of its transpose, to and from accumulator tiles. Of the
+// transpose a lane has four neighbours, moved together (E is a multiple of 4).
+struct alignas(4) Four { float v[4]; };
+template <int P, bool TRANSPOSED, class F> __device__ __forceinline__ void each_of_state(const MoAttend& a, int x0, F f) {
     const int lane = threadIdx.x % kWave, g = lane / 16, x = x0 + lane % 16;
-    if (a.D == P && a.E == P) {
+    const auto tiles = [&](auto whole) {                       // (whole heads without a test and with known strides)
+        const int E = whole ? P : a.E;
 #pragma unroll
-        for (int t = 0; t < P / 16; t++)
+        for (int t = 0; t < P / 16; t++) {
+            const int y = acc_row(t, g, 0);
+            if (TRANSPOSED) {
+                if (whole || (x < a.D && y < a.E)) f(t, 0, x * E + y);
+            } else {
 #pragma unroll
-            for (int r = 0; r < 4; r++) f(t, r, TRANSPOSED ? x * P + acc_row(t, g, r) : acc_row(t, g, r) * P + x);
-        return;
-    }
-#pragma unroll
-    for (int t = 0; t < P / 16; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int y = acc_row(t, g, r), d = TRANSPOSED ? x : y, e = TRANSPOSED ? y : x;
-            if (d < a.D && e < a.E) f(t, r, d * a.E + e);
+                for (int r = 0; r < 4; r++)
+                    if (whole || (y + r < a.D && x < a.E)) f(t, r, (y + r) * E + x);
+            }
         }
+    };
+    if (!TRANSPOSED && a.D == P && a.E == P) tiles(std::true_type{});
+    else tiles(std::false_type{});
+}
+template <int P, bool TRANSPOSED> __device__ __forceinline__ void load_state(const MoAttend& a, const float* from, int x0, f32x4 (&S)[P / 16]) {
+    each_of_state<P, TRANSPOSED>(a, x0, [&](int t, int r, int at) {
+        if (!TRANSPOSED) { S[t][r] = from[at]; return; }
+        const Four q = *(const Four*)(from + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) S[t][i] = q.v[i];
+    });
+}
+template <int P, bool TRANSPOSED> __device__ __forceinline__ void store_state(const MoAttend& a, float* to, int x0, const f32x4 (&S)[P / 16]) {
+    each_of_state<P, TRANSPOSED>(a, x0, [&](int t, int r, int at) {
+        if (!TRANSPOSED) to[at] = S[t][r];
+        else *(Four*)(to + at) = Four{{S[t][0], S[t][1], S[t][2], S[t][3]}};
+    });
 }
 
 // Where a step does not see another, their product's factor is 0; but 0 times a NaN or an infinity is a NaN, which would reach
@@ -183,7 +210,7 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
     const typename C::Rows sk{lk}, sv{lv}, sq{lq}, sy{ly};
     const typename C::Scores sp{lp};
     const int w = threadIdx.x / kWave;
-    const int64_t nh = blockIdx.x, env = nh / a.H;
+    const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int e0 = w * CT * 16;   // the wave's columns
@@ -199,7 +226,7 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
     const float* in = !OUT ? nullptr : cut.segs > 1 ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : a.state ? a.state + nh * de : nullptr;
     if (in)
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) each_of_state<T, P, false>(a, e0 + 16 * ct, [&](int t, int r, int at) { S[ct][t][r] = in[at]; });
+        for (int ct = 0; ct < CT; ct++) load_state<P, false>(a, in, e0 + 16 * ct, S[ct]);
     pw.fill(a.decay[h], a.scale);
     bool any_start = false;
     for (int64_t c = c0; c < c1; c++) {
@@ -374,7 +401,7 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
     float* to = !OUT ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : cut.segs > 1 ? nullptr : a.state_out + nh * de;
     if (to)
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) each_of_state<T, P, false>(a, e0 + 16 * ct, [&](int t, int r, int at) { to[at] = S[ct][t][r]; });
+        for (int ct = 0; ct < CT; ct++) store_state<P, false>(a, to, e0 + 16 * ct, S[ct]);
     if (!OUT && threadIdx.x == 0) {
         const int64_t n = min(c1 * L, a.T) - c0 * L;
         cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : exp2f((float)n * __log2f(a.decay[h]));

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
     const typename C::Rows sq{s.q}, sk{s.k}, sv{s.v}, so{s.o}, sr{s.r};
     const typename C::Scores sa{s.a}, sb{s.b};
     const int w = threadIdx.x / kWave;
-    const int64_t nh = blockIdx.x, env = nh / a.H;
+    const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int x0 = w * 16;     // the wave's rows of R and S, columns of dq and dk; of dv its columns
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
 #pragma unroll
     for (int et = 0; et < C::PT; et++) R[et] = zero;
     const float* in = cut.segs > 1 ? cut.enter + ((int64_t)seg * a.N * a.H + nh) * de : a.dstate_out ? a.dstate_out + nh * de : nullptr;
-    if (in) each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { R[t][r] = in[at]; });
+    if (in) load_state<P, true>(a, in, x0, R);
     for (int64_t c = c1 - 1; c >= c0; c--) {
         const int64_t t0 = c * L;
         const int n = (int)min((int64_t)L, a.T - t0);
@@ -165,85 +165,91 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
         else scores(std::false_type{});
         __syncthreads();
 
-        // Each result transposed: a lane has four neighbouring columns of one step. `own` the sum over the chunk's steps, `far`
-        // what the entering state or its gradient adds, by a factor f a step.
-        const auto write = [&](const typename C::Rows& to, int t, float f, const f32x4& own, const f32x4& far) {
-            f32x4 y;
+        // A result, transposed: a lane has four neighbouring columns of one step. own_of: the sum over the chunk's steps, x its
+        // scores and y its rows; far_of: what the entering state or its gradient adds, by a factor a step.
+        const auto result = [&](T* to, const float* factor, auto far_of, auto own_of, const typename C::Scores& x, bool down, const typename C::Rows& y) {
+            const typename C::Rows tile{to};
+            const auto write = [&](int t, const f32x4& own, const f32x4& far) {
+                const float f = factor[t * 16 + i16];
+                f32x4 z;
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = fmaf(f, far[r], own[r]);
-            if (m && f == 0.f) y = own;                        // (what is not seen may be anything)
-            *(Pack<T, 4>*)to.at(t * 16 + i16, x0 + 4 * g) = pack4(y, T{});
-        };
-        // `own` again, one product after another: over the steps j that step i sees (or that see it) of x_ij y_j
-        const auto again = [&](const typename C::Scores& x, bool down, const typename C::Rows& y, int i) {
-            f32x4 own = zero;
-            const int j0 = down ? i : max(seen_from(m, i), 0), j1 = down ? n - 1 : i;
+                for (int r = 0; r < 4; r++) z[r] = fmaf(f, far[r], own[r]);
+                if (m && f == 0.f) z = own;                    // (what is not seen may be anything)
+                *(Pack<T, 4>*)tile.at(t * 16 + i16, x0 + 4 * g) = pack4(z, T{});
+            };
+            float all = 0.f;
+#pragma unroll
+            for (int t = 0; t < C::LT; t++) {
+                const f32x4 far = far_of(t), own = own_of(t);
+                watch(all, own);
+                write(t, own, far);
+            }
+            if (!any_not_finite(all)) return;
 #pragma unroll 1
-            for (int j = j0; j <= j1 && (!down || seen_from(m, j) <= i); j++)
+            for (int t = 0; t < C::LT; t++) {                  // over the steps j that step i sees (or that see it) of x_ij y_j
+                const int i = t * 16 + i16, j0 = down ? i : max(seen_from(m, i), 0), j1 = down ? n - 1 : i;
+                f32x4 own = zero;
+#pragma unroll 1
+                for (int j = j0; j <= j1 && (!down || seen_from(m, j) <= i); j++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    own[r] = fmaf(as_f32(down ? *x.at(j, i) : *x.at(i, j)), as_f32(*y.at(j, x0 + 4 * g + r)), own[r]);
-            return own;
+                    for (int r = 0; r < 4; r++)
+                        own[r] = fmaf(as_f32(down ? *x.at(j, i) : *x.at(i, j)), as_f32(*y.at(j, x0 + 4 * g + r)), own[r]);
+                write(t, own, far_of(t));
+            }
         };
 
-        {                                                      // dV
+        {
             Frag<T> of[C::LB], rf[C::PB];
 #pragma unroll
             for (int b = 0; b < C::LB; b++) of[b] = so.down(b * 32, x0, lane);
 #pragma unroll
             for (int b = 0; b < C::PB; b++) rf[b] = sr.down(b * 32, x0, lane);
-            const typename C::Rows sy{s.y};
-#pragma unroll
-            for (int t = 0; t < C::LT; t++) {
-                f32x4 own = zero, far = zero;
+            result(s.y, s.wt, [&](int t) {
+                f32x4 far = zero;
 #pragma unroll
                 for (int b = 0; b < C::PB; b++) mma(far, rf[b], sk.along(t * 16, b * 32, lane));
+                return far;
+            }, [&](int t) {
+                f32x4 own = zero;
 #pragma unroll
                 for (int b = t / 2; b < C::LB; b++) mma(own, of[b], sa.down(b * 32, t * 16, lane));
-                float all = 0.f;
-                watch(all, own);
-                if (any_not_finite(all)) own = again(sa, true, so, t * 16 + i16);
-                write(sy, t, s.wt[t * 16 + i16], own, far);
-            }
+                return own;
+            }, sa, true, so);
         }
         __syncthreads();                                       // A and R's tile are done with
-        {                                                      // dQ
+        {
             Frag<T> kf[C::LB];
 #pragma unroll
             for (int b = 0; b < C::LB; b++) kf[b] = sk.down(b * 32, x0, lane);
-            const typename C::Rows sy{s.dq()};
-#pragma unroll
-            for (int t = 0; t < C::LT; t++) {
-                f32x4 own = zero, far = zero;
+            result(s.dq(), s.ut, [&](int t) {
+                f32x4 far = zero;
 #pragma unroll
                 for (int b = 0; b < C::PB; b++) mma(far, sf[b], so.along(t * 16, b * 32, lane));
+                return far;
+            }, [&](int t) {
+                f32x4 own = zero;
 #pragma unroll
                 for (int b = 0; b <= t / 2; b++) mma(own, kf[b], sb.along(t * 16, b * 32, lane));
-                float all = 0.f;
-                watch(all, own);
-                if (any_not_finite(all)) own = again(sb, false, sk, t * 16 + i16);
-                write(sy, t, s.ut[t * 16 + i16], own, far);
-            }
+                return own;
+            }, sb, false, sk);
         }
-        {                                                      // dK
+        {
             Frag<T> qf[C::LB], rf[C::PB];
 #pragma unroll
             for (int b = 0; b < C::LB; b++) qf[b] = sq.down(b * 32, x0, lane);
 #pragma unroll
             for (int b = 0; b < C::PB; b++) rf[b] = frag_of<T>(R[2 * b], R[2 * b + 1]);
-            const typename C::Rows sy{s.dk()};
-#pragma unroll
-            for (int t = 0; t < C::LT; t++) {
-                f32x4 own = zero, far = zero;
+            result(s.dk(), s.wt, [&](int t) {
+                f32x4 far = zero;
 #pragma unroll
                 for (int b = 0; b < C::PB; b++) mma(far, rf[b], sv.along(t * 16, b * 32, lane));
+                return far;
+            }, [&](int t) {
+                f32x4 own = zero;
 #pragma unroll
                 for (int b = t / 2; b < C::LB; b++) mma(own, qf[b], sb.down(b * 32, t * 16, lane));
-                float all = 0.f;
-                watch(all, own);
-                if (any_not_finite(all)) own = again(sb, true, sq, t * 16 + i16);
-                write(sy, t, s.wt[t * 16 + i16], own, far);
-            }
+                return own;
+            }, sb, true, sq);
         }
 
         f32x4 add[C::PT];                                      // R'
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
         dk.take(s.dk(), c0 * L, n);
         dv.take(s.y, c0 * L, n);
     }
-    if (a.dstate && cut.segs == 1) each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { a.dstate[nh * de + at] = R[t][r]; });
+    if (a.dstate && cut.segs == 1) store_state<P, true>(a, a.dstate + nh * de, x0, R);
 }
 
 // A segment's own sum of R' (see R' above) and what it leaves of a gradient that comes from behind it.
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT)) k_attend_back_sums(MoAt
     __shared__ Powers<L> pw;
     __shared__ __align__(16) float ut[L];
     const typename C::Rows sq{lq}, so{lo};
-    const int64_t nh = blockIdx.x, env = nh / a.H;
+    const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int x0 = threadIdx.x / kWave * 16;
@@ -303,7 +309,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT)) k_attend_back_sums(MoAt
             for (int r = 0; r < 4; r++) R[et][r] = m ? add[et][r] : fmaf(f, R[et][r], add[et][r]);
     }
     float* to = cut.enter + ((int64_t)seg * a.N * a.H + nh) * a.D * a.E;
-    each_of_state<T, P, true>(a, x0, [&](int t, int r, int at) { to[at] = R[t][r]; });
+    store_state<P, true>(a, to, x0, R);
     if (threadIdx.x == 0) {
         const int64_t n = min(c1 * L, a.T) - c0 * L;
         cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : exp2f((float)n * __log2f(a.decay[h]));

@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) k_step_state(Step a) {
                 x[r].v[c] = cut ? kk[r] * vv[c] : fmaf(g, x[r].v[c], kk[r] * vv[c]);
                 o[c] = fmaf(qq[r], x[r].v[c], o[c]);
             }
-            *(P*)(S + (int64_t)(d0 + r) * a.E + e) = x[r];
+            stream((P*)(S + (int64_t)(d0 + r) * a.E + e), x[r]);
         }
     }
 #pragma unroll

@@ -23,6 +23,27 @@ template <class T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N
 
 constexpr int kWave = 64;
 
+// What is written once, in whole cache lines, leaves past the caches' reuse order (nontemporal): strided rows of 128 bytes then
+// reach memory at 4.0 instead of 2.9 TB/s (linear attention's gradient, 1,024 steps of 257 envs), a group norm's output at 5.3
+// instead of 4.0 (4096 x 32 x 20 x 20). Parts of lines are slower that way, not faster.
+template <class P> __device__ __forceinline__ void stream(P* to, const P& x) {
+    if constexpr (sizeof(P) == 16) {
+        typedef unsigned U __attribute__((ext_vector_type(4), aligned(4)));   // (aligned to elements is enough)
+        __builtin_nontemporal_store(*(const U*)&x, (U*)to);
+    } else if constexpr (sizeof(P) == 32) {
+        typedef unsigned U __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(((const U*)&x)[0], (U*)to);
+        __builtin_nontemporal_store(((const U*)&x)[1], (U*)to + 1);
+    } else if constexpr (sizeof(P) == 8) {
+        typedef unsigned U __attribute__((ext_vector_type(2)));
+        __builtin_nontemporal_store(*(const U*)&x, (U*)to);
+    } else if constexpr (sizeof(P) == 4) {
+        __builtin_nontemporal_store(*(const unsigned*)&x, (unsigned*)to);
+    } else {
+        *to = x;
+    }
+}
+
 // ---- host side
 inline thread_local std::string g_err;
 

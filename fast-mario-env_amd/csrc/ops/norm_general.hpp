@@ -49,7 +49,8 @@ struct NormArgs {
 
 constexpr int NORM_THREADS = 256;
 
-// Each channel's mean and squared deviations over a slab, into part.
+// Each channel's mean and squared deviations over a slab, into part. A thread sums about its first value, and the threads' sets are
+// joined as moments, so neither a large mean nor a far value costs digits.
 template <class T, int V>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
     __shared__ float sm[NORM_THREADS][V], s2[NORM_THREADS][V], sn[NORM_THREADS];
@@ -60,33 +61,50 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
     for (int c0 = 0; c0 < k.c.nv; c0 += k.c.LN) {
         const int cv = c0 + t % k.c.LN;
         const bool live = pl < k.c.PL && cv < k.c.nv;
-        float mean[V] = {}, m2[V] = {}, n = 0.f;
+        float about[V] = {}, sum[V] = {}, sq[V] = {}, n = 0.f;
         if (live)
             for (int64_t p = p0 + pl; p < p1; p += k.c.PL) {
                 const Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + (b * a.S + p) * a.C + cv * V);
-                n += 1.f;
-                const float r = 1.f / n;
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    const float v = as_f32(x.v[i]), d = v - mean[i];
-                    mean[i] = fmaf(d, r, mean[i]);
-                    m2[i] = fmaf(d, v - mean[i], m2[i]);
+                    if (n == 0.f) about[i] = as_f32(x.v[i]);
+                    const float d = as_f32(x.v[i]) - about[i];
+                    sum[i] += d;
+                    sq[i] = fmaf(d, d, sq[i]);
                 }
+                n += 1.f;
             }
         __syncthreads();
+        const float r = n > 0.f ? 1.f / n : 0.f;
 #pragma unroll
-        for (int i = 0; i < V; i++) { sm[t][i] = mean[i]; s2[t][i] = m2[i]; }
+        for (int i = 0; i < V; i++) {
+            const float d = sum[i] * r;
+            sm[t][i] = about[i] + d;
+            s2[t][i] = fmaxf(fmaf(-d, sum[i], sq[i]), 0.f) + (sq[i] - sq[i]);   // (what is not finite stays so)
+        }
         sn[t] = n;
-        __syncthreads();
-        if (live && pl == 0) {                            // the pixel lanes in their order
+        for (int m = 1; m < k.c.PL; m *= 2) {                  // pixel lanes j and j + m
+            __syncthreads();
+            if (live && pl % (2 * m) == 0 && pl + m < k.c.PL) {
+                const int o = t + m * k.c.LN;
+                const float na = sn[t], nb = sn[o], nt = na + nb, w = nt > 0.f ? nb / nt : 0.f;
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                Moments m{sn[t], sm[t][i], s2[t][i]};
-                for (int j = 1; j < k.c.PL; j++) m.join({sn[t + j * k.c.LN], sm[t + j * k.c.LN][i], s2[t + j * k.c.LN][i]});
-                part[cv * V + i] = m.mean;
-                part[a.C + cv * V + i] = m.m2;
+                for (int i = 0; i < V; i++) {
+                    const float d = sm[o][i] - sm[t][i];
+                    if (nb > 0.f) {
+                        sm[t][i] = fmaf(d, w, sm[t][i]);
+                        s2[t][i] += s2[o][i] + d * d * na * w;
+                    }
+                }
+                sn[t] = nt;
             }
         }
+        if (live && pl == 0)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                part[cv * V + i] = sm[t][i];
+                part[a.C + cv * V + i] = s2[t][i];
+            }
     }
 }
 
@@ -134,7 +152,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(NormArgs k) {
             Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + at);
 #pragma unroll
             for (int i = 0; i < V; i++) x.v[i] = as<T>(act<ACT>(fmaf(as_f32(x.v[i]) - mean[i], w[i], s[i])));
-            *(Pack<T, V>*)((T*)a.y + at) = x;
+            stream((Pack<T, V>*)((T*)a.y + at), x);
         }
     }
 }
@@ -176,15 +194,21 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(NormArgs k) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < V; i++) { sw[t][i] = dw[i]; sb[t][i] = db[i]; }
-        __syncthreads();
-        if (live && pl == 0) {
+        for (int m = 1; m < k.c.PL; m *= 2) {                  // pixel lanes j and j + m
+            __syncthreads();
+            if (live && pl % (2 * m) == 0 && pl + m < k.c.PL)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    sw[t][i] += sw[t + m * k.c.LN][i];
+                    sb[t][i] += sb[t + m * k.c.LN][i];
+                }
+        }
+        if (live && pl == 0)
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                for (int j = 1; j < k.c.PL; j++) { dw[i] += sw[t + j * k.c.LN][i]; db[i] += sb[t + j * k.c.LN][i]; }
-                part[cv * V + i] = dw[i];
-                part[a.C + cv * V + i] = db[i];
+                part[cv * V + i] = sw[t][i];
+                part[a.C + cv * V + i] = sb[t][i];
             }
-        }
     }
 }
 
@@ -237,7 +261,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_dx(NormArgs k) {
                 const float h = (as_f32(x.v[i]) - mean[i]) * r[i], dz = as_f32(dy.v[i]) * act_grad<ACT>(fmaf(h, w[i], s[i]));
                 dy.v[i] = as<T>(r[i] * (w[i] * dz - m1[i] - h * m2[i]));
             }
-            *(Pack<T, V>*)((T*)a.dx + at) = dy;
+            stream((Pack<T, V>*)((T*)a.dx + at), dy);
         }
     }
 }

@@ -4,15 +4,15 @@
 
 namespace mo {
 
-// A team of W waves takes a sample, holds it as up to R packs of 8 channels a thread and goes on to its next sample. A thread has
+// A team of threads (W waves, or of a small sample a part of one) takes a sample, holds it as up to R packs of 8 channels a thread and goes on to its next sample. A thread has
 // the packs cv = t % NV (NV: packs a pixel, rounded up to a power of two; threads of packs that are not there idle) of the pixels
-// t / NV, t / NV + 64 W / NV, .., so its channels, their weights and their gradients' sums stay its own. Sums over a group are
+// t / NV, t / NV + TT / NV, .. (TT: the team's threads), so its channels, their weights and their gradients' sums stay its own. Sums over a group are
 // shuffles over the lanes that hold it, and one exchange through LDS where the team has several waves (MULTI). The variance is
 // that of the values in registers about their mean: exact also where the mean is large.
 // WHOLE: groups are whole packs; else a group is 1, 2 or 4 channels, and sums are kept by channel up to the last step.
 struct Small {
     MoNorm a;
-    int W, nv, NV, log_nv;     // waves a team; packs a pixel, and rounded up
+    int W, TT, nv, NV, log_nv; // waves and threads a team; packs a pixel, and rounded up
     int cg, vpg;               // channels a group; packs a group (WHOLE)
     float* part;               // (blocks, 2, C): the blocks' sums for dweight and dbias
 };
@@ -28,7 +28,7 @@ __device__ __forceinline__ void group_sum(float (&s)[NS], const Small& k, float 
     const int lane = threadIdx.x % kWave;
 #pragma unroll
     for (int i = 0; i < NS; i++)
-        for (int m = k.NV; m < kWave; m *= 2) s[i] += __shfl_xor(s[i], m);
+        for (int m = k.NV; m < (MULTI ? kWave : k.TT); m *= 2) s[i] += __shfl_xor(s[i], m);
     if (NS == SETS) {                                      // whole packs: a value a set
         if ((k.vpg & (k.vpg - 1)) == 0) {
 #pragma unroll
@@ -71,8 +71,8 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
     typedef Pack<T, 8> P;
     __shared__ float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][NS];
     const MoNorm& a = k.a;
-    const int W = MULTI ? k.W : 1, TT = W * kWave, teams = MULTI ? 1 : 4;
-    const int t = MULTI ? threadIdx.x : threadIdx.x % kWave, cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
+    const int TT = k.TT, teams = MULTI ? 1 : 256 / TT;
+    const int t = threadIdx.x & (TT - 1), cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
     const bool live = cv < k.nv;
     float w[8], s[8];
 #pragma unroll
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
         s[i] = live && a.bias ? a.bias[cv * 8 + i] : 0.f;
     }
     const float by = 1.f / ((float)a.S * (float)k.cg);
-    for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / kWave); b < a.B; b += (int64_t)gridDim.x * teams) {
+    for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / TT); b < a.B; b += (int64_t)gridDim.x * teams) {
         const T* in = (const T*)a.x + b * a.S * a.C + cv * 8;
         P v[R];
 #pragma unroll
@@ -123,19 +123,19 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
                     v[r].v[i] = as<T>(act<ACT>(fmaf((as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS], w[i], s[i])));
-                *(P*)(out + (int64_t)(pl + r * PL) * a.C) = v[r];
+                stream((P*)(out + (int64_t)(pl + r * PL) * a.C), v[r]);
             }
     }
 }
 
 template <class T, bool MULTI, int R, int ACT, bool WHOLE>
-__global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small_back(Small k) {
+__global__ void __launch_bounds__(small_threads(MULTI), 4) k_norm_small_back(Small k) {
     constexpr int NS = WHOLE ? 1 : 8;
     typedef Pack<T, 8> P;
     __shared__ union { float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][2 * NS]; float sums[MULTI ? SMALL_WAVES : 4][kWave][8]; } lds;
     const MoNorm& a = k.a;
-    const int W = MULTI ? k.W : 1, TT = W * kWave, teams = MULTI ? 1 : 4, waves = MULTI ? k.W : 4;
-    const int t = MULTI ? threadIdx.x : threadIdx.x % kWave, cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
+    const int TT = k.TT, teams = MULTI ? 1 : 256 / TT, waves = MULTI ? k.W : 4;
+    const int t = threadIdx.x & (TT - 1), cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
     const bool live = cv < k.nv;
     float w[8], s[8], dw[8] = {}, db[8] = {};
 #pragma unroll
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small_back(Small 
     }
     const float by = 1.f / ((float)a.S * (float)k.cg);
     int turn = 0;
-    for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / kWave); b < a.B; b += (int64_t)gridDim.x * teams) {
+    for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / TT); b < a.B; b += (int64_t)gridDim.x * teams) {
         const int64_t at = b * a.S * a.C + cv * 8;
         P v[R], dy[R];
 #pragma unroll
@@ -161,19 +161,19 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small_back(Small 
             mean[i] = st[0];
             rstd[i] = st[1];
         }
-        float h[R][8], dh[R][8];
+        float dh[R][8];
 #pragma unroll
         for (int r = 0; r < R; r++)
             if (live && pl + r * PL < S)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    h[r][i] = (as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS];
-                    const float dz = as_f32(dy[r].v[i]) * act_grad<ACT>(fmaf(h[r][i], w[i], s[i]));
-                    dw[i] = fmaf(dz, h[r][i], dw[i]);
+                    const float h = (as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS];
+                    const float dz = as_f32(dy[r].v[i]) * act_grad<ACT>(fmaf(h, w[i], s[i]));
+                    dw[i] = fmaf(dz, h, dw[i]);
                     db[i] += dz;
                     dh[r][i] = dz * w[i];
                     m[i % NS] += dh[r][i];
-                    m[NS + i % NS] = fmaf(dh[r][i], h[r][i], m[NS + i % NS]);
+                    m[NS + i % NS] = fmaf(dh[r][i], h, m[NS + i % NS]);
                 }
         group_sum<MULTI, 2 * NS, 2>(m, k, lds.x, turn);
         turn ^= 1;
@@ -183,9 +183,11 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small_back(Small 
         for (int r = 0; r < R; r++)
             if (live && pl + r * PL < S) {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    v[r].v[i] = as<T>(rstd[i % NS] * (dh[r][i] - fmaf(h[r][i], m[NS + i % NS], m[i % NS])));
-                *(P*)((T*)a.dx + at + (int64_t)(pl + r * PL) * a.C) = v[r];
+                for (int i = 0; i < 8; i++) {
+                    const float h = (as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS];
+                    v[r].v[i] = as<T>(rstd[i % NS] * (dh[r][i] - fmaf(h, m[NS + i % NS], m[i % NS])));
+                }
+                stream((P*)((T*)a.dx + at + (int64_t)(pl + r * PL) * a.C), v[r]);
             }
     }
     if (!k.part) return;
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small_back(Small 
 }
 
 // ---- host side
-struct SmallCut { int W, R, blocks; };
+struct SmallCut { int W, TT, R, blocks; };
 
 // Whole packs a pixel, groups of whole packs or of 1, 2 or 4 channels, a pixel's packs within a wave, and a sample within a
 // team's registers; otherwise the sample goes through memory twice (norm_general).
@@ -225,7 +227,8 @@ inline bool norm_small_takes(const MoNorm& a, bool backward, SmallCut& c) {
     if (packs > (int64_t)SMALL_WAVES * kWave * most) return false;
     for (c.W = 1; packs > (int64_t)c.W * kWave * most; c.W *= 2) {}
     for (c.R = 1; packs > (int64_t)c.W * kWave * c.R; c.R *= 2) {}
-    const int per_block = c.W == 1 ? 4 : 1, waves = c.W == 1 ? 4 : c.W;
+    for (c.TT = NV; c.TT < c.W * kWave && c.TT < packs; c.TT *= 2) {}
+    const int per_block = c.W == 1 ? 256 / c.TT : 1, waves = c.W == 1 ? 4 : c.W;
     const int64_t blocks = (a.B + per_block - 1) / per_block, fill = (int64_t)compute_units() * std::max(1, (backward ? 16 : 32) / waves);
     c.blocks = (int)std::min(blocks, fill);
     return true;
@@ -244,7 +247,7 @@ template <class T, bool MULTI, int R, int ACT> int norm_small_run(const Small& k
 
 template <class T, int ACT> int norm_small(const MoNorm& a, const SmallCut& c, bool backward, hipStream_t s) {
     const int cg = a.C / a.groups;
-    Small k{a, c.W, a.C / 8, 1, 0, cg, std::max(1, cg / 8), nullptr};
+    Small k{a, c.W, c.TT, a.C / 8, 1, 0, cg, std::max(1, cg / 8), nullptr};
     while (k.NV < k.nv) { k.NV *= 2; k.log_nv++; }
     if (backward && a.dweight) k.part = (float*)a.work;
     int rc;
