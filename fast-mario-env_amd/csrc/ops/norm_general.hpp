@@ -38,18 +38,20 @@ struct Moments {
 struct NormCut {
     int64_t slabs, px;
     int nv, LN, PL;   // packs of V channels a pixel; channel lanes; pixel lanes
+    bool by_group;    // a block sees whole pixels, and joins its channels' sums to the groups'
 };
 
 struct NormArgs {
     MoNorm a;
     NormCut c;
-    float* part;      // per (sample, slab): [2][C], or the same summed
+    float* part;      // per (sample, slab): [2][C], each channel's two sums
+    float* group;     // per (sample, slab): [2][groups], each group's (by_group)
     float* means;     // (B, groups, 2): mean and rstd; going back, mean(dh) and mean(dh h)
 };
 
 constexpr int NORM_THREADS = 256;
 
-// Each channel's mean and squared deviations over a slab, into part. A thread sums about its first value, and the threads' sets are
+// Each channel's (or group's) mean and squared deviations over a slab. A thread sums about its first value, and the threads' sets are
 // joined as moments, so neither a large mean nor a far value costs digits.
 template <class T, int V>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
@@ -99,35 +101,58 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
                 sn[t] = nt;
             }
         }
-        if (live && pl == 0)
+        if (!k.c.by_group) {
+            if (live && pl == 0)
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                part[cv * V + i] = sm[t][i];
-                part[a.C + cv * V + i] = s2[t][i];
+                for (int i = 0; i < V; i++) {
+                    part[cv * V + i] = sm[t][i];
+                    part[a.C + cv * V + i] = s2[t][i];
+                }
+            continue;
+        }
+        __syncthreads();
+        const int cg = a.C / a.groups;                         // channels of one count: a mean of means
+        float* group = k.group + (int64_t)blockIdx.x * 2 * a.groups;
+        for (int g = t / kWave; g < a.groups; g += NORM_THREADS / kWave) {
+            float mean = 0.f, m2 = 0.f;
+            for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) mean += sm[c / V][c % V];
+            for (int s = 1; s < kWave; s *= 2) mean += __shfl_xor(mean, s);
+            mean /= (float)cg;
+            for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) {
+                const float d = sm[c / V][c % V] - mean;
+                m2 += s2[c / V][c % V] + sn[0] * d * d;
             }
+            for (int s = 1; s < kWave; s *= 2) m2 += __shfl_xor(m2, s);
+            if (t % kWave == 0) {
+                group[g] = mean;
+                group[a.groups + g] = m2;
+            }
+        }
     }
 }
 
-// Mean and rstd of a sample's group, a wave each, from its channels' moments in every slab.
-__global__ void __launch_bounds__(kWave) k_norm_means(NormArgs k) {
+// Mean and rstd of a sample's group, a block each, from the moments of every slab (of its channels, or its own).
+__global__ void __launch_bounds__(NORM_THREADS) k_norm_means(NormArgs k) {
+    __shared__ Moments of[NORM_THREADS];
     const MoNorm& a = k.a;
     const int64_t b = blockIdx.x / a.groups;
-    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups;
+    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups, t = threadIdx.x;
+    const int per = k.c.by_group ? 1 : cg, width = k.c.by_group ? a.groups : a.C;
+    const float* from = (k.c.by_group ? k.group : k.part) + b * k.c.slabs * 2 * width + g * per;
     Moments m{0.f, 0.f, 0.f};
-    for (int64_t i = threadIdx.x; i < k.c.slabs * cg; i += kWave) {
-        const int64_t slab = i / cg;
-        const float* p = k.part + (b * k.c.slabs + slab) * 2 * a.C + g * cg + i % cg;
-        m.join({(float)(min((slab + 1) * k.c.px, a.S) - slab * k.c.px), p[0], p[a.C]});
+    for (int64_t i = t; i < k.c.slabs * per; i += NORM_THREADS) {
+        const int64_t slab = i / per;
+        const float* p = from + slab * 2 * width + i % per;
+        m.join({(float)(min((slab + 1) * k.c.px, a.S) - slab * k.c.px) * (float)(cg / per), p[0], p[width]});
     }
-    for (int s = 1; s < kWave; s *= 2) {
-        const Moments o{__shfl_xor(m.n, s), __shfl_xor(m.mean, s), __shfl_xor(m.m2, s)};
-        Moments lo = (threadIdx.x & s) ? o : m;           // every lane joins the two in the same order
-        lo.join((threadIdx.x & s) ? m : o);
-        m = lo;
+    of[t] = m;
+    for (int s = 1; s < NORM_THREADS; s *= 2) {
+        __syncthreads();
+        if (t % (2 * s) == 0) of[t].join(of[t + s]);
     }
-    if (threadIdx.x == 0) {
-        k.means[2 * blockIdx.x] = m.mean;
-        k.means[2 * blockIdx.x + 1] = 1.f / sqrtf(m.m2 / m.n + a.eps);
+    if (t == 0) {
+        k.means[2 * blockIdx.x] = of[0].mean;
+        k.means[2 * blockIdx.x + 1] = 1.f / sqrtf(of[0].m2 / of[0].n + a.eps);
     }
 }
 
@@ -157,7 +182,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(NormArgs k) {
     }
 }
 
-// Each channel's sums of dz h and of dz over a slab, into part.
+// Each channel's sums of dz h and of dz over a slab, into part, and each group's of dh and dh h.
 template <class T, int V, int ACT>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(NormArgs k) {
     __shared__ float sw[NORM_THREADS][V], sb[NORM_THREADS][V];
@@ -203,33 +228,62 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(NormArgs k) {
                     sb[t][i] += sb[t + m * k.c.LN][i];
                 }
         }
-        if (live && pl == 0)
+        if (live && pl == 0 && (a.dweight || !k.c.by_group))
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 part[cv * V + i] = sw[t][i];
                 part[a.C + cv * V + i] = sb[t][i];
             }
+        if (!k.c.by_group) continue;
+        __syncthreads();
+        float* group = k.group + (int64_t)blockIdx.x * 2 * a.groups;
+        for (int g = t / kWave; g < a.groups; g += NORM_THREADS / kWave) {
+            float m1 = 0.f, m2 = 0.f;
+            for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) {
+                const float w = a.weight ? a.weight[c] : 1.f;
+                m1 = fmaf(w, sb[c / V][c % V], m1);
+                m2 = fmaf(w, sw[c / V][c % V], m2);
+            }
+            for (int s = 1; s < kWave; s *= 2) { m1 += __shfl_xor(m1, s); m2 += __shfl_xor(m2, s); }
+            if (t % kWave == 0) {
+                group[g] = m1;
+                group[a.groups + g] = m2;
+            }
+        }
     }
 }
 
-// mean(dh) and mean(dh h) of a sample's group, a wave each, from its channels' sums.
-__global__ void __launch_bounds__(kWave) k_norm_dmeans(NormArgs k) {
+// mean(dh) and mean(dh h) of a sample's group, a block each, from the sums of every slab (of its channels, or its own).
+__global__ void __launch_bounds__(NORM_THREADS) k_norm_dmeans(NormArgs k) {
+    __shared__ float s1[NORM_THREADS], s2[NORM_THREADS];
     const MoNorm& a = k.a;
     const int64_t b = blockIdx.x / a.groups;
-    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups;
+    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups, t = threadIdx.x;
     float m1 = 0.f, m2 = 0.f;
-    for (int64_t i = threadIdx.x; i < k.c.slabs * cg; i += kWave) {
-        const int c = g * cg + (int)(i % cg);
-        const float* p = k.part + (b * k.c.slabs + i / cg) * 2 * a.C + c;
-        const float w = a.weight ? a.weight[c] : 1.f;
-        m2 = fmaf(w, p[0], m2);
-        m1 = fmaf(w, p[a.C], m1);
+    if (k.c.by_group)
+        for (int64_t slab = t; slab < k.c.slabs; slab += NORM_THREADS) {
+            const float* p = k.group + (b * k.c.slabs + slab) * 2 * a.groups + g;
+            m1 += p[0];
+            m2 += p[a.groups];
+        }
+    else
+        for (int64_t i = t; i < k.c.slabs * cg; i += NORM_THREADS) {
+            const int c = g * cg + (int)(i % cg);
+            const float* p = k.part + (b * k.c.slabs + i / cg) * 2 * a.C + c;
+            const float w = a.weight ? a.weight[c] : 1.f;
+            m2 = fmaf(w, p[0], m2);
+            m1 = fmaf(w, p[a.C], m1);
+        }
+    s1[t] = m1;
+    s2[t] = m2;
+    for (int s = NORM_THREADS / 2; s; s /= 2) {
+        __syncthreads();
+        if (t < s) { s1[t] += s1[t + s]; s2[t] += s2[t + s]; }
     }
-    for (int s = 1; s < kWave; s *= 2) { m1 += __shfl_xor(m1, s); m2 += __shfl_xor(m2, s); }
-    if (threadIdx.x == 0) {
+    if (t == 0) {
         const float by = 1.f / ((float)a.S * (float)cg);
-        k.means[2 * blockIdx.x] = m1 * by;
-        k.means[2 * blockIdx.x + 1] = m2 * by;
+        k.means[2 * blockIdx.x] = s1[0] * by;
+        k.means[2 * blockIdx.x + 1] = s2[0] * by;
     }
 }
 
@@ -321,43 +375,46 @@ inline bool norm_wide(const MoNorm& a) {   // 8 channels an access (of 16 bytes,
 inline NormCut norm_cut(const MoNorm& a, int V) {
     NormCut c;
     const int64_t per_px = (int64_t)a.C * (a.dtype == MO_BF16 ? 2 : 4);
-    const int64_t most = std::max<int64_t>(1, a.S * per_px / (16 << 10)), want = std::max<int64_t>(1, 4096 / std::max<int64_t>(1, a.B));
+    const int64_t most = std::max<int64_t>(1, a.S * per_px / (16 << 10)), want = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, a.B));
     c.px = (a.S + std::min(most, want) - 1) / std::min(most, want);
     c.slabs = (a.S + c.px - 1) / c.px;
     c.nv = a.C / V;
     c.LN = std::min(c.nv, NORM_THREADS);
     c.PL = NORM_THREADS / c.LN;
+    c.by_group = c.nv == c.LN;
     return c;
 }
 
-struct NormWork { int64_t part, means, spare, total; };   // in floats
+struct NormWork { int64_t part, group, means, spare, total; };   // in floats
 inline NormWork norm_general_work(const MoNorm& a, const NormCut& c, bool backward) {
     NormWork w;
-    w.part = a.B * c.slabs * 2 * a.C;
+    w.part = c.by_group && !(backward && a.dweight) ? 0 : a.B * c.slabs * 2 * a.C;
+    w.group = c.by_group ? a.B * c.slabs * 2 * a.groups : 0;
     w.means = a.B * a.groups * 2;
     w.spare = backward ? (int64_t)NORM_SUM_ROWS * 2 * a.C : 0;
-    w.total = w.part + w.means + w.spare;
+    w.total = w.part + w.group + w.means + w.spare;
     return w;
 }
 
 template <class T, int V, int ACT> int norm_general(const MoNorm& a, bool backward, hipStream_t s) {
-    NormArgs k{a, norm_cut(a, V), nullptr, nullptr};
+    NormArgs k{a, norm_cut(a, V), nullptr, nullptr, nullptr};
     const NormWork w = norm_general_work(a, k.c, backward);
     k.part = (float*)a.work;
-    k.means = k.part + w.part;
+    k.group = k.part + w.part;
+    k.means = k.group + w.group;
     const dim3 grid((unsigned)(a.B * k.c.slabs)), per_group((unsigned)(a.B * a.groups));
     if (!backward) {
         if (a.stats) k.means = a.stats;
         hipLaunchKernelGGL((k_norm_moments<T, V>), grid, dim3(NORM_THREADS), 0, s, k);
-        hipLaunchKernelGGL(k_norm_means, per_group, dim3(kWave), 0, s, k);
+        hipLaunchKernelGGL(k_norm_means, per_group, dim3(NORM_THREADS), 0, s, k);
         hipLaunchKernelGGL((k_norm_apply<T, V, ACT>), grid, dim3(NORM_THREADS), 0, s, k);
         return launched("k_norm_apply");
     }
     hipLaunchKernelGGL((k_norm_sums<T, V, ACT>), grid, dim3(NORM_THREADS), 0, s, k);
-    hipLaunchKernelGGL(k_norm_dmeans, per_group, dim3(kWave), 0, s, k);
+    hipLaunchKernelGGL(k_norm_dmeans, per_group, dim3(NORM_THREADS), 0, s, k);
     hipLaunchKernelGGL((k_norm_dx<T, V, ACT>), grid, dim3(NORM_THREADS), 0, s, k);
     if (launched("k_norm_dx")) return -1;
-    return a.dweight ? norm_colsum(a, k.part, a.B * k.c.slabs, k.part + w.part + w.means, s) : 0;
+    return a.dweight ? norm_colsum(a, k.part, a.B * k.c.slabs, k.means + w.means, s) : 0;
 }
 
 }  // namespace mo

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
 }
 
 template <class T, bool MULTI, int R, int ACT, bool WHOLE>
-__global__ void __launch_bounds__(small_threads(MULTI), 4) k_norm_small_back(Small k) {
+__global__ void __launch_bounds__(small_threads(MULTI), (WHOLE && sizeof(T) == 2 ? 4 : 2)) k_norm_small_back(Small k) {
     constexpr int NS = WHOLE ? 1 : 8;
     typedef Pack<T, 8> P;
     __shared__ union { float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][2 * NS]; float sums[MULTI ? SMALL_WAVES : 4][kWave][8]; } lds;
