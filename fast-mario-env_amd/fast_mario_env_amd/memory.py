@@ -9,6 +9,9 @@ memory of fixed size per env goes on where the stack ends:
 - `group_norm_act`: group norm and an activation over channels-last features: of the memory's output (a group a head; its size
   grows with the episode) and of convolutions; with its gradients.
 
+`make_memory_net` is an actor-critic that uses them, and `Rollout` (rollout.py) runs it: `act` steps the memories along with the
+envs, and calling the network on a stored rollout gives the same policy and values, with gradients.
+
 Float32 or bf16 in and out, sums and states in float32. On the GPU they are HIP kernels (libmario_ops.so, include/mario_ops.h),
 queued on torch's current stream. CPU tensors, and what torch traces or transforms, take torch operations.
 """
@@ -16,7 +19,9 @@ from __future__ import annotations
 
 import contextlib
 
-from .rollout import _torch, _transformed
+import math
+
+from .rollout import N_ACTIONS, _torch, _transformed, policy_input
 
 ACTS = {"none": 0, "relu": 1, "silu": 2}
 MAX_HEAD = 128
@@ -349,3 +354,98 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
     if torch.is_grad_enabled() and any(t.requires_grad for t in every):
         return _function("norm").apply(x, groups, weight, bias, eps, act)
     return _norm_forward(x, groups, weight, bias, eps, act, False)[0]
+
+
+# ---------------------------------------------------------------- an actor-critic with a memory
+def make_memory_net(n_actions: int = N_ACTIONS, in_ch: int = 4, heads: int = 8, seed: int = 0, device="cuda"):
+    """The Nature trunk of `make_net` with a group norm after each convolution, and between its features and the two heads a
+    memory: projection to q, k and v, linear attention with `heads` decaying memories of 512 / heads, group norm a head,
+    projection, added to the features. Random weights. On the GPU the trunk and the memory run in bf16 (the memories
+    themselves and the heads in float32), on the CPU everything in float32."""
+    torch = _torch()
+    nn = torch.nn
+    F = torch.nn.functional
+    width = 512
+    if heads < 1 or width % heads or width // heads > MAX_HEAD:
+        raise ValueError(f"make_memory_net: heads must divide {width} into heads of at most {MAX_HEAD}")
+
+    class MemoryAC(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.heads = heads
+            self.convs = nn.ModuleList([nn.Conv2d(in_ch, 32, 8, 4), nn.Conv2d(32, 64, 4, 2), nn.Conv2d(64, 64, 3, 1)])
+            self.norms = nn.ModuleList([nn.GroupNorm(8, c) for c in (32, 64, 64)])   # (parameters; group_norm_act computes)
+            self.fc = nn.Linear(64 * 7 * 7, width)
+            self.qkv = nn.Linear(width, 3 * width, bias=False)
+            self.norm = nn.GroupNorm(heads, width)
+            self.out = nn.Linear(width, width, bias=False)
+            self.pi = nn.Linear(width, n_actions)
+            self.vf = nn.Linear(width, 1)
+            self.register_buffer("decay", head_decays(heads, "cpu"))
+            for m in list(self.convs) + [self.fc]:
+                nn.init.orthogonal_(m.weight, math.sqrt(2.0))
+                nn.init.zeros_(m.bias)
+            for m, gain in ((self.qkv, 1.0), (self.out, 1.0), (self.pi, 0.01), (self.vf, 1.0)):
+                nn.init.orthogonal_(m.weight, gain)
+            nn.init.zeros_(self.pi.bias)
+            nn.init.zeros_(self.vf.bias)
+
+        def initial_state(self, n: int):
+            """The memories of n envs before anything: (n, heads, D, D) float32 zeros."""
+            d = width // heads
+            return torch.zeros(n, heads, d, d, device=self.decay.device)
+
+        def _autocast(self):
+            on = self.decay.is_cuda
+            return torch.autocast("cuda" if on else "cpu", dtype=torch.bfloat16, enabled=on)
+
+        def _features(self, obs_u8):
+            """uint8 (B, k, 84, 84) -> the projected features and q, k, v of each, (B, 512) and (B, heads, D)."""
+            if obs_u8.is_cuda:
+                x = torch.empty(obs_u8.shape, dtype=torch.bfloat16, device=obs_u8.device).to(memory_format=torch.channels_last)
+                policy_input(obs_u8.contiguous(), x)
+            else:
+                x = obs_u8.float().mul_(1.0 / 255.0)
+            with self._autocast():
+                for c, g in zip(self.convs, self.norms):
+                    x = group_norm_act(c(x), g.num_groups, g.weight, g.bias, eps=g.eps, act="silu")
+                h = F.silu(self.fc(x.flatten(1)))
+                q, k, v = (y.unflatten(-1, (heads, -1)) for y in self.qkv(h).chunk(3, -1))
+            return h, q, k, v
+
+        def _heads(self, h, memory):
+            with self._autocast():
+                y = group_norm_act(memory.flatten(1), heads, self.norm.weight, self.norm.bias, eps=self.norm.eps, act="silu")
+                h = h + self.out(y)
+            h = h.float()
+            return self.pi(h), self.vf(h).squeeze(-1)
+
+        def forward(self, obs_u8, start=None, state=None):
+            """A rollout: obs_u8 (T, N, k, 84, 84) uint8, start (T, N) bool and state (N, heads, D, D), the memories before it ->
+            logits (T, N, A), values (T, N), the memories after it."""
+            T, N = obs_u8.shape[:2]
+            h, q, k, v = self._features(obs_u8.flatten(0, 1))
+            out, state = linear_attention(*(y.unflatten(0, (T, N)) for y in (q, k, v)), self.decay, start, state)
+            logits, value = self._heads(h, out.flatten(0, 1))
+            return logits.unflatten(0, (T, N)), value.unflatten(0, (T, N)), state
+
+        @torch.no_grad()
+        def step(self, obs_u8, start, state):
+            """One step: obs_u8 (N, k, 84, 84), start (N,) bool or None; state is updated. Logits (N, A), values (N,)."""
+            h, q, k, v = self._features(obs_u8)
+            return self._heads(h, linear_attention_step(q, k, v, self.decay, state, start))
+
+        @torch.no_grad()
+        def act(self, obs_u8, generator=None, start=None, state=None):
+            """Action (Gumbel-max sample), its log-probability and the value, as NatureAC.act; state is updated."""
+            logits, value = self.step(obs_u8, start, state)
+            logp = F.log_softmax(logits, -1)
+            u = torch.rand(logits.shape, generator=generator, device=logits.device).clamp_(1e-20, 1.0)
+            a = (logp - torch.log(-torch.log(u))).argmax(-1)
+            return a, logp.gather(-1, a[:, None]).squeeze(-1), value
+
+    torch.manual_seed(seed)
+    net = MemoryAC().to(device)
+    if torch.device(device).type == "cuda":
+        net = net.to(memory_format=torch.channels_last)
+    return net

@@ -13,6 +13,8 @@ half of its trainer (src/fast_mario_env/ppo/backends.py:127-162, ppo/train.py:12
 - Timeout bootstrap (train.py:414-431, the device-backend branch): where an episode was truncated by the time
   limit and not terminated, the stored reward is r + gamma * V(final_obs), V evaluated on the final
   observation stacks of those envs. As in the reference, finding them costs one small host sync per step.
+- A network with a memory (memory.py's `make_memory_net`) steps its memories along with the envs, cleared at episode starts;
+  `sequence` gives what it was shown, and the memories it began with, for training.
 - `gae`: generalized advantage estimation over the stored rewards, values and episode starts, with the
   reference's convention (train.py:140-150): the bootstrap of step t is cut where step t + 1 starts an episode.
 
@@ -354,6 +356,8 @@ class Rollout:
         self.next_val = torch.zeros(n, device=dev)
         self.next_start = torch.zeros(n, dtype=torch.bool, device=dev)
         self._starting = torch.ones(n, dtype=torch.bool, device=dev)   # the current obs is a reset stack
+        self.memory = net.initial_state(n) if hasattr(net, "initial_state") else None   # now, and when the rollout began
+        self.memory0 = None if self.memory is None else self.memory.clone()
         self.env_ms = 0.0
 
     def collect(self):
@@ -362,11 +366,13 @@ class Rollout:
         torch, env = self.torch, self.env
         ev = [(torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)) for _ in range(self.T)]
         self.first.copy_(env.obs)
+        if self.memory is not None:
+            self.memory0.copy_(self.memory)
         for t in range(self.T):
             obs = env.obs                                    # the env's buffer, read in place
             self.frames[t].copy_(obs[:, -1])
             self.start[t].copy_(self._starting)
-            a, lp, v = self.net.act(obs, self.gen)
+            a, lp, v = self._act(obs, self.memory)
             self.act[t].copy_(a)
             self.logp[t].copy_(lp)
             self.val[t].copy_(v)
@@ -377,12 +383,17 @@ class Rollout:
             if self.bootstrap_timeouts:
                 self._bootstrap(t, term, trunc)
             torch.logical_or(term, trunc, out=self._starting)   # the next obs is a reset stack
-        _, _, v = self.net.act(env.obs, self.gen)
+        _, _, v = self._act(env.obs, None if self.memory is None else self.memory.clone())   # (the next rollout steps from here)
         self.next_val.copy_(v)
         self.next_start.copy_(self._starting)
         torch.cuda.synchronize(env.dev)
         self.env_ms = sum(a.elapsed_time(b) for a, b in ev)
         return self.env_ms
+
+    def _act(self, obs, memory):
+        if memory is None:
+            return self.net.act(obs, self.gen)
+        return self.net.act(obs, self.gen, start=self._starting, state=memory)
 
     def _bootstrap(self, t: int, term, trunc):
         """rew[t] += gamma * V(final_obs) where the time limit cut an episode that did not terminate."""
@@ -392,22 +403,31 @@ class Rollout:
             return
         ti = tmask.nonzero().squeeze(-1)
         with torch.no_grad():
-            _, v = self.net(self.env.final_obs[ti])
+            final = self.env.final_obs[ti]
+            _, v = self.net(final) if self.memory is None else self.net.step(final, None, self.memory[ti])
         self.rew[t, ti] += self.gamma * v
 
-    def obs(self, t: int):
-        """The (N, k, 84, 84) observation stack of step t, rebuilt from the stored frames."""
+    def obs(self, t: int, envs=slice(None)):
+        """The (N, k, 84, 84) observation stack of step t (of `envs`, an index), rebuilt from the stored frames."""
         torch = self.torch
-        out = torch.zeros_like(self.first)
-        out[:, -1] = self.frames[t]
-        alive = ~self.start[t]               # the stack still continues one step further back
+        first = self.first[envs]
+        out = torch.zeros_like(first)
+        out[:, -1] = self.frames[t][envs]
+        alive = ~self.start[t][envs]         # the stack still continues one step further back
         for j in range(1, self.k):
             if t - j >= 0:
-                out[:, -1 - j] = torch.where(alive[:, None, None], self.frames[t - j], 0)
-                alive = alive & ~self.start[t - j]
+                out[:, -1 - j] = torch.where(alive[:, None, None], self.frames[t - j][envs], 0)
+                alive = alive & ~self.start[t - j][envs]
             else:                            # before the rollout: the stack of step 0
-                out[:, -1 - j] = torch.where(alive[:, None, None], self.first[:, -1 - (j - t)], 0)
+                out[:, -1 - j] = torch.where(alive[:, None, None], first[:, -1 - (j - t)], 0)
         return out
+
+    def sequence(self, envs):
+        """What a network with a memory was shown in this rollout, of `envs` (an index): the observations (T, n, k, 84, 84), the
+        episode starts (T, n) and the memories before the first step. `net(*sequence)` computes the rollout again."""
+        torch = self.torch
+        return (torch.stack([self.obs(t, envs) for t in range(self.T)]), self.start[:, envs].contiguous(),
+                None if self.memory0 is None else self.memory0[envs])
 
     def advantages(self, gamma: float | None = None, lam: float = 0.95):
         g = self.gamma if gamma is None else gamma

@@ -571,3 +571,84 @@ def test_norm_gradients_are_differences():
             d, want = (f(up) - f(down)) / (2 * h), (grad.double() * u).sum()
             # rounding 2^-24 sqrt(n) |y dy| / h, and the cubic term h^2 with a third derivative of order one
             assert abs(d - want) <= 2.0 ** -22 * dy.norm() / h + 2 * h ** 2 * (grad.double() * u).norm() * t.numel() ** 0.5, i
+
+
+# ---------------------------------------------------------------- the network that uses them
+def test_memory_net_on_cpu():
+    """Steps and the whole sequence agree, memories are cleared at starts, and every parameter gets a gradient."""
+    torch.manual_seed(0)
+    T, N = 5, 3
+    net = memory.make_memory_net(heads=4, device="cpu")
+    obs = torch.randint(0, 256, (T, N, 4, 84, 84), dtype=torch.uint8)
+    start = torch.zeros(T, N, dtype=torch.bool)
+    start[0], start[3, 1] = True, True
+    logits, value, last = net(obs, start)
+    state = net.initial_state(N) + 7.0                       # what a first step's env remembers is not seen
+    for t in range(T):
+        lg, v = net.step(obs[t], start[t], state)
+        assert torch.allclose(lg, logits[t], atol=1e-5) and torch.allclose(v, value[t], atol=1e-4)
+    assert torch.allclose(state, last, atol=1e-4)
+    alone, _, _ = net(obs[3:, 1:2], None, None)              # an episode from its start on
+    assert torch.allclose(alone, logits[3:, 1:2], atol=1e-5)
+    (logits.sum() + value.sum()).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in net.parameters())
+    with pytest.raises(ValueError, match="heads"):
+        memory.make_memory_net(heads=3, device="cpu")
+
+
+@pytest.mark.gpu
+def test_memory_net_gradients_as_on_cpu():
+    """The network's loss and gradients on the GPU (bf16 trunk and memory) against the same weights on the CPU in float32."""
+    T, N = 70, 3
+    g = torch.Generator().manual_seed(1)
+    obs = torch.randint(0, 256, (T, N, 4, 84, 84), dtype=torch.uint8, generator=g)
+    start = torch.rand(T, N, generator=g) < 0.05
+    nets = [memory.make_memory_net(seed=3, device=d) for d in ("cpu", "cuda")]
+    assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(nets[0].parameters(), nets[1].parameters()))
+    grads = []
+    for net, dev in zip(nets, ("cpu", "cuda")):
+        state = torch.randn(N, 8, 64, 64, generator=torch.Generator().manual_seed(2)).to(dev).requires_grad_()
+        logits, value, last = net(obs.to(dev), start.to(dev), state)
+        (torch.log_softmax(logits, -1)[..., 2].mean() + value.square().mean() + 1e-3 * last.square().mean()).backward()
+        grads.append([p.grad.float().cpu() for p in net.parameters()] + [state.grad.cpu()])
+    for name, a, b in zip([n for n, _ in nets[0].named_parameters()] + ["state"], *grads):
+        # a bf16 network of about ten layers: each rounds by 2^-9 at most, forth and back
+        assert (a - b).norm() <= 0.1 * a.norm() + 1e-6, (name, ((a - b).norm() / a.norm()).item())
+
+
+@pytest.mark.gpu
+def test_rollout_with_a_memory_is_computed_again():
+    """A rollout under the network: its stored log-probabilities and values come out again from the stored sequence, episodes
+    ending inside; a second rollout goes on from the memories of the first; training steps change the policy."""
+    from build_roms import rom_path
+    from fast_mario_env_amd import HipVecEnv
+    from fast_mario_env_amd.rollout import Rollout
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("memory_policy", os.path.join(ROOT, "examples", "memory_policy.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    n, T = 24, 20
+    env = HipVecEnv("1-1", n, seed=0, sticky=0.25, noop_max=30, max_steps=13, maxpool=True, rom=open(rom_path("vanilla"), "rb").read())
+    env.reset()
+    net = memory.make_memory_net(seed=0)
+    ro = Rollout(env, net, T=T, seed=3)
+    for _ in range(2):
+        before = ro.memory.clone()
+        ro.collect()
+        assert torch.equal(ro.memory0, before)
+        envs = torch.arange(n, device="cuda")
+        with torch.no_grad():
+            logits, value, last = net(*ro.sequence(envs))
+        logp = torch.log_softmax(logits, -1).gather(-1, ro.act[..., None]).squeeze(-1)
+        # (the convolutions of another batch size may take other kernels, and the memory another order of sums: bf16 either way)
+        assert torch.allclose(logp, ro.logp, atol=2e-2) and torch.allclose(value, ro.val, atol=0.1, rtol=0.05)
+        assert (last - ro.memory).norm() <= 0.03 * last.norm()
+        assert ro.start[1:].any()
+    with torch.no_grad():                                    # a share of the envs, by index
+        part, _, _ = net(*ro.sequence(torch.tensor([5, 2], device="cuda")))
+    assert torch.allclose(torch.log_softmax(part, -1), torch.log_softmax(logits[:, [5, 2]], -1), atol=2e-2)
+    opt = torch.optim.Adam(net.parameters(), 1e-3)
+    old = [p.detach().clone() for p in net.parameters()]
+    assert torch.isfinite(example.update(net, opt, ro))
+    assert all(not torch.equal(a, b) for a, b in zip(old, net.parameters()))
+    env.close()
