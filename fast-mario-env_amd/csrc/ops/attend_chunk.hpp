@@ -457,13 +457,14 @@ inline bool chunks_take(const MoAttend& a, bool backward) {
 inline int chunk_steps(const MoAttend& a) { return a.dtype == MO_BF16 ? 64 : 32; }
 inline int padded_head(const MoAttend& a) { const int m = std::max(a.D, a.E); return m <= 32 ? 32 : m <= 64 ? 64 : 128; }
 
-// Segments: where the sequences alone would leave compute units without `per_cu` workgroups.
-inline Cut attend_cut(const MoAttend& a, int per_cu) {
+// Segments: up to two workgroups a compute unit, of two chunks at least. Two segments are not worth it: k, v (or q, dO) are read
+// twice and two more kernels run. (16,001 steps of 16 heads of 128: 1,266 us in one piece, 132 in 32; 2,000 steps of 512 heads of
+// 64: 136 in one piece, 208 in two; 300 steps of 32 heads of 128: 32 in one, 37 in two.)
+inline Cut attend_cut(const MoAttend& a) {
     Cut c{};
     c.chunks = (a.T + chunk_steps(a) - 1) / chunk_steps(a);
-    const int64_t want = (int64_t)compute_units() * per_cu / std::max<int64_t>(1, a.N * a.H);
-    const int64_t segs = std::max<int64_t>(1, std::min(want, c.chunks / 2));
-    c.per_seg = std::max<int64_t>(1, (c.chunks + segs - 1) / segs);
+    const int64_t segs = std::min<int64_t>(2 * (int64_t)compute_units() / std::max<int64_t>(1, a.N * a.H), c.chunks / 2);
+    c.per_seg = segs < 3 ? std::max<int64_t>(1, c.chunks) : (c.chunks + segs - 1) / segs;
     c.segs = (int)std::max<int64_t>(1, (c.chunks + c.per_seg - 1) / c.per_seg);
     return c;
 }
@@ -485,10 +486,8 @@ inline int enter_states(const MoAttend& a, const Cut& c, const float* first, flo
     return launched("k_attend_enter");
 }
 
-constexpr int FORWARD_PER_CU = 4;
-
 template <class T, int P> int attend_chunks(const MoAttend& a, hipStream_t s) {
-    Cut c = attend_cut(a, FORWARD_PER_CU);
+    Cut c = attend_cut(a);
     cut_place(a, c);
     const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(kForwardWaves<P> * kWave);
     if (c.segs > 1) {

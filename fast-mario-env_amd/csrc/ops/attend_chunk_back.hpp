@@ -316,10 +316,8 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT)) k_attend_back_sums(MoAt
     }
 }
 
-constexpr int BACKWARD_PER_CU = 2;
-
 template <class T, int P> int attend_back_chunks(const MoAttend& a, hipStream_t s) {
-    Cut c = attend_cut(a, BACKWARD_PER_CU);
+    Cut c = attend_cut(a);
     cut_place(a, c);
     const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(BackChunk<T, P>::NT);
     if (c.segs > 1) {

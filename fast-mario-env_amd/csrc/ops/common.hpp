@@ -23,6 +23,25 @@ template <class T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N
 
 constexpr int kWave = 64;
 
+// What is larger than the last-level cache and read once comes past the caches' reuse order.
+constexpr int64_t LAST_LEVEL_CACHE = 256 << 20;
+template <class P> __device__ __forceinline__ P streamed(const P* from) {
+    P x;
+    if constexpr (sizeof(P) == 16) {
+        typedef unsigned U __attribute__((ext_vector_type(4)));
+        *(U*)&x = __builtin_nontemporal_load((const U*)from);
+    } else if constexpr (sizeof(P) == 32) {
+        typedef unsigned U __attribute__((ext_vector_type(4)));
+        ((U*)&x)[0] = __builtin_nontemporal_load((const U*)from);
+        ((U*)&x)[1] = __builtin_nontemporal_load((const U*)from + 1);
+    } else if constexpr (sizeof(P) == 4) {
+        *(unsigned*)&x = __builtin_nontemporal_load((const unsigned*)from);
+    } else {
+        x = *from;
+    }
+    return x;
+}
+
 // What is written once, in whole cache lines, leaves past the caches' reuse order (nontemporal): strided rows of 128 bytes then
 // reach memory at 4.0 instead of 2.9 TB/s (linear attention's gradient, 1,024 steps of 257 envs), a group norm's output at 5.3
 // instead of 4.0 (4096 x 32 x 20 x 20). Parts of lines are slower that way, not faster.

@@ -51,7 +51,7 @@ template <class T> int attend_forward(const MoAttend& a, hipStream_t s) {
     return p == 32 ? attend_chunks<T, 32>(a, s) : p == 64 ? attend_chunks<T, 64>(a, s) : attend_chunks<T, 128>(a, s);
 }
 template <class T> int attend_back(const MoAttend& a, hipStream_t s) {
-    if (!chunks_take(a, true) || (!a.saved && attend_cut(a, 1).chunks > 1)) return walk_backward<T>(a, s);
+    if (!chunks_take(a, true) || (!a.saved && attend_cut(a).chunks > 1)) return walk_backward<T>(a, s);
     const int p = padded_head(a);
     return p == 32 ? attend_back_chunks<T, 32>(a, s) : p == 64 ? attend_back_chunks<T, 64>(a, s) : attend_back_chunks<T, 128>(a, s);
 }
@@ -106,7 +106,7 @@ int64_t mo_attend_saved(const MoAttend* a) {
 int64_t mo_attend_work(const MoAttend* a, int backward) {
     return guarded([&]() -> int64_t {
         if (!attend_sizes(a)) return -1;
-        return chunks_take(*a, backward) ? cut_bytes(*a, attend_cut(*a, backward ? BACKWARD_PER_CU : FORWARD_PER_CU)) : 0;
+        return chunks_take(*a, backward) ? cut_bytes(*a, attend_cut(*a)) : 0;
     });
 }
 

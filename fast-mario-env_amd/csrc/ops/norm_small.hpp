@@ -14,6 +14,8 @@ struct Small {
     MoNorm a;
     int W, TT, nv, NV, log_nv; // waves and threads a team; packs a pixel, and rounded up
     int cg, vpg;               // channels a group; packs a group (WHOLE)
+    bool far;                  // rows (R = 1) of an x that fills the last-level cache come past it (262,144 x 512 bf16: gradient 186 ->
+                               // 176 us); a smaller x may be there from its maker, and larger samples gain nothing
     float* part;               // (blocks, 2, C): the blocks' sums for dweight and dbias
 };
 
@@ -86,7 +88,10 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
         P v[R];
 #pragma unroll
         for (int r = 0; r < R; r++)
-            if (live && pl + r * PL < S) v[r] = *(const P*)(in + (int64_t)(pl + r * PL) * a.C);
+            if (live && pl + r * PL < S) {
+                const P* p = (const P*)(in + (int64_t)(pl + r * PL) * a.C);
+                v[r] = R == 1 && k.far ? streamed(p) : *p;
+            }
         float mean[NS] = {}, var[NS] = {};
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -151,8 +156,9 @@ __global__ void __launch_bounds__(small_threads(MULTI), (WHOLE && sizeof(T) == 2
 #pragma unroll
         for (int r = 0; r < R; r++)
             if (live && pl + r * PL < S) {
-                v[r] = *(const P*)((const T*)a.x + at + (int64_t)(pl + r * PL) * a.C);
-                dy[r] = *(const P*)((const T*)a.dy + at + (int64_t)(pl + r * PL) * a.C);
+                const P *p = (const P*)((const T*)a.x + at + (int64_t)(pl + r * PL) * a.C), *d = (const P*)((const T*)a.dy + at + (int64_t)(pl + r * PL) * a.C);
+                v[r] = R == 1 && k.far ? streamed(p) : *p;
+                dy[r] = R == 1 && k.far ? streamed(d) : *d;
             }
         float mean[NS], rstd[NS], m[2 * NS] = {};          // m: the sums of dh, then those of dh h
 #pragma unroll
@@ -247,7 +253,8 @@ template <class T, bool MULTI, int R, int ACT> int norm_small_run(const Small& k
 
 template <class T, int ACT> int norm_small(const MoNorm& a, const SmallCut& c, bool backward, hipStream_t s) {
     const int cg = a.C / a.groups;
-    Small k{a, c.W, c.TT, a.C / 8, 1, 0, cg, std::max(1, cg / 8), nullptr};
+    Small k{a, c.W, c.TT, a.C / 8, 1, 0, cg, std::max(1, cg / 8),
+            a.B * a.S * a.C * (int64_t)sizeof(T) >= LAST_LEVEL_CACHE, nullptr};
     while (k.NV < k.nv) { k.NV *= 2; k.log_nv++; }
     if (backward && a.dweight) k.part = (float*)a.work;
     int rc;
