@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 LIB_ENV_VAR = "MARIO_HIP_LIB"
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -88,20 +89,11 @@ def lib() -> ctypes.CDLL:
     return L
 
 
-class MoRows(ctypes.Structure):
-    _fields_ = [("p", _P), ("st", _i64), ("sn", _i64), ("sh", _i64)]
-
-
-class MoAttend(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "H", "D", "E")] + [("T", _i64), ("N", _i64), ("scale", ctypes.c_float)]
-                + [(n, MoRows) for n in ("q", "k", "v", "out")]
-                + [(n, _P) for n in ("decay", "start", "state", "state_out", "saved", "work")]
-                + [(n, MoRows) for n in ("dout", "dq", "dk", "dv")] + [("dstate_out", _P), ("dstate", _P)])
-
-
-class MoNorm(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "act", "C", "groups")] + [("B", _i64), ("S", _i64), ("eps", ctypes.c_float)]
-                + [(n, _P) for n in ("x", "weight", "bias", "y", "stats", "work", "dy", "dx", "dweight", "dbias")])
+# The structures of include/mario_ops.h, as the bytes that a call hands over (made in one go: a call of these operators is a few
+# microseconds of host work, of which ctypes structures were a third).
+ROWS = struct.Struct("=Qqqq")                                                       # MoRows: p, st, sn, sh
+ATTEND = struct.Struct("=4i2qf4x" + 4 * "Qqqq" + "6Q" + 4 * "Qqqq" + "2Q")          # MoAttend, its fields in order
+NORM = struct.Struct("=4i2qf4x10Q")                                                 # MoNorm
 
 
 def ops_lib() -> ctypes.CDLL:
@@ -116,17 +108,15 @@ def ops_lib() -> ctypes.CDLL:
             f"g.build()\"` from the repository root (needs hipcc with gfx950 support).")
     L = ctypes.CDLL(path)
     L.mo_last_error.restype = ctypes.c_char_p
-    attend, norm = ctypes.POINTER(MoAttend), ctypes.POINTER(MoNorm)
     L.mo_attend_saved.restype = L.mo_attend_work.restype = L.mo_group_norm_work.restype = _i64
-    L.mo_attend_saved.argtypes = [attend]
-    L.mo_attend_work.argtypes = [attend, _i32]
+    L.mo_attend_saved.argtypes = [_P]
+    L.mo_attend_work.argtypes = [_P, _i32]
     for f in (L.mo_attend, L.mo_attend_backward):
-        f.argtypes = [attend, _P]
-    rows = ctypes.POINTER(MoRows)
-    L.mo_attend_step.argtypes = [_i32, _i64, _i32, _i32, _i32, ctypes.c_float, rows, rows, rows, _P, _P, _P, rows, _P]
-    L.mo_group_norm_work.argtypes = [norm, _i32]
+        f.argtypes = [_P, _P]
+    L.mo_attend_step.argtypes = [_i32, _i64, _i32, _i32, _i32, ctypes.c_float] + [_P] * 8
+    L.mo_group_norm_work.argtypes = [_P, _i32]
     for f in (L.mo_group_norm, L.mo_group_norm_backward):
-        f.argtypes = [norm, _P]
+        f.argtypes = [_P, _P]
     _ops = L
     return L
 

@@ -18,183 +18,151 @@ queued on torch's current stream. CPU tensors, and what torch traces or transfor
 from __future__ import annotations
 
 import contextlib
-
 import math
 
-from .rollout import N_ACTIONS, _torch, _transformed, policy_input
+import torch
+
+from ._native import ATTEND, NORM, ROWS, ops_check, ops_lib
+from .rollout import N_ACTIONS, _transformed, policy_input
 
 ACTS = {"none": 0, "relu": 1, "silu": 2}
 MAX_HEAD = 128
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_NO_ROWS = (0, 0, 0, 0)
 
 
 def _kernel_takes(*ts):
     """Whether a kernel called by address computes these: plain tensors on a GPU that nothing traces or transforms."""
-    torch = _torch()
-    return (all(type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and not t.is_neg() for t in ts)
-            and not _transformed(*ts))
-
-
-def _dtype(t):
-    return {_torch().float32: 0, _torch().bfloat16: 1}[t.dtype]
+    for t in ts:
+        if type(t) not in (torch.Tensor, torch.nn.Parameter) or not t.is_cuda or t.is_neg():
+            return False
+    return not _transformed(*ts)
 
 
 def _rows(t):
-    """The tensor's head vectors (T, N, H, d) or (N, H, d) as the library takes them; the last dimension is contiguous."""
-    from ._native import MoRows
-    st = t.stride() if t.dim() == 4 else (0,) + t.stride()
-    return MoRows(t.data_ptr(), *st[:3])
+    """The tensor's head vectors (T, N, H, d) or (N, H, d) as the library takes them (MoRows); the last dimension is contiguous."""
+    return (t.data_ptr(), *t.stride()[:3]) if t.dim() == 4 else (t.data_ptr(), 0, *t.stride()[:2])
 
 
 def _as_rows(t):
     """The tensor as the kernels take it: head vectors contiguous, and on 16-byte boundaries where their size allows it (they are
     copied otherwise: a copy costs less than going step by step)."""
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] != 1:
         return t.contiguous()
     whole = 16 // t.element_size()
-    if t.shape[-1] % whole == 0 and (t.data_ptr() % 16 or any(s % whole for s in t.stride()[:-1])):
-        return t.clone(memory_format=_torch().contiguous_format)
+    if t.shape[-1] % whole == 0 and (t.data_ptr() % 16 or any(s % whole for s in st[:-1])):
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _work(nbytes, device):
-    torch = _torch()
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _on(device):
     """The device made current for launches and allocations (nothing to do where it is: a context costs more than the check)."""
-    torch = _torch()
     return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def head_decays(heads: int, device="cuda"):
     """Factors (heads,) whose memories last from about 22 steps (half-life) to about 1,400: 1 - 2^-5 .. 1 - 2^-11."""
-    torch = _torch()
     return (1.0 - 2.0 ** -torch.linspace(5.0, 11.0, heads, dtype=torch.float64)).float().to(device)
 
 
 # ---------------------------------------------------------------- linear attention
 def _check_attend(name, lead, q, k, v, decay, start, state):
-    torch = _torch()
-    H, D, E = q.shape[-2], q.shape[-1], v.shape[-1]
-    if (q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype or tuple(k.shape) != tuple(q.shape)
-            or tuple(v.shape[:-1]) != tuple(q.shape[:-1]) or not (1 <= D <= MAX_HEAD and 1 <= E <= MAX_HEAD) or H < 1):
+    shape, dt, dev = q.shape, q.dtype, q.device
+    H, D, E = shape[-2], shape[-1], v.shape[-1]
+    if (dt not in _DTYPES or k.dtype != dt or v.dtype != dt or k.shape != shape or v.shape[:-1] != shape[:-1]
+            or not (1 <= D <= MAX_HEAD and 1 <= E <= MAX_HEAD) or H < 1):
         raise ValueError(f"{name}: q and k must be ({lead}, H, D), v ({lead}, H, E), all float32 or all bf16, head sizes 1 .. {MAX_HEAD}")
-    if decay.dtype != torch.float32 or tuple(decay.shape) != (H,):
+    if decay.dtype != torch.float32 or decay.shape != (H,):
         raise ValueError(f"{name}: decay must be ({H},) float32")
     if decay.requires_grad:
         raise ValueError(f"{name}: decay is a constant of the heads: it has no gradient here")
-    if start is not None and (start.dtype != torch.bool or tuple(start.shape) != tuple(q.shape[:-2])):
+    if start is not None and (start.dtype != torch.bool or start.shape != shape[:-2]):
         raise ValueError(f"{name}: start must be ({lead}) bool")
-    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != (q.shape[-3], H, D, E)):
-        raise ValueError(f"{name}: state must be (N, H, D, E) = {(q.shape[-3], H, D, E)} float32")
-    if any(t is not None and t.device != q.device for t in (k, v, decay, start, state)):
-        raise ValueError(f"{name}: all tensors must be on the device of q ({q.device})")
-
-
-def _attend_args(q, k, v, decay, start, scale):
-    from ._native import MoAttend
-    T, N, H, D = q.shape
-    a = MoAttend(dtype=_dtype(q), H=H, D=D, E=v.shape[-1], T=T, N=N, scale=scale, q=_rows(q), k=_rows(k), v=_rows(v),
-                 decay=decay.data_ptr(), start=_ptr(start))
-    return a
+    if state is not None and (state.dtype != torch.float32 or state.shape != (shape[-3], H, D, E)):
+        raise ValueError(f"{name}: state must be (N, H, D, E) = {(shape[-3], H, D, E)} float32")
+    for t in (k, v, decay, start, state):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: all tensors must be on the device of q ({dev})")
 
 
 def _attend_forward(q, k, v, decay, start, state, scale, keep):
     """out, state_out and what the gradient takes up (None unless `keep`)."""
-    torch = _torch()
-    from ._native import ops_check, ops_lib
     L, dev = ops_lib(), q.device
+    (T, N, H, D), E = q.shape, v.shape[-1]
     with _on(dev):
-        a = _attend_args(q, k, v, decay, start, scale)
-        out = torch.empty(q.shape[:3] + v.shape[-1:], dtype=q.dtype, device=dev)
-        state_out = torch.empty(q.shape[1:] + v.shape[-1:], dtype=torch.float32, device=dev)
-        a.out, a.state, a.state_out = _rows(out), _ptr(state), state_out.data_ptr()
+        out = torch.empty((T, N, H, E), dtype=q.dtype, device=dev)
+        state_out = torch.empty((N, H, D, E), dtype=torch.float32, device=dev)
+
+        def args(saved, work):
+            return ATTEND.pack(_DTYPES[q.dtype], H, D, E, T, N, scale, *_rows(q), *_rows(k), *_rows(v), *_rows(out), decay.data_ptr(), _ptr(start),
+                               _ptr(state), state_out.data_ptr(), saved, work, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0)
+
+        a = args(0, 0)
         saved = _work(ops_check(L.mo_attend_saved(a), "mo_attend_saved"), dev) if keep else None
         work = _work(ops_check(L.mo_attend_work(a, 0), "mo_attend_work"), dev)
-        a.saved, a.work = _ptr(saved), _ptr(work)
+        if saved is not None or work is not None:
+            a = args(_ptr(saved), _ptr(work))
         ops_check(L.mo_attend(a, _stream(dev)), "mo_attend")
     return out, state_out, saved
 
 
 def _attend_backward(q, k, v, decay, start, state, saved, scale, dout, dstate_out, want_dstate):
-    torch = _torch()
-    from ._native import ops_check, ops_lib
     L, dev = ops_lib(), q.device
+    (T, N, H, D), E = q.shape, v.shape[-1]
     with _on(dev):
-        a = _attend_args(q, k, v, decay, start, scale)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        dstate = torch.empty(q.shape[1:] + v.shape[-1:], dtype=torch.float32, device=dev) if want_dstate else None
-        a.state, a.saved, a.dstate_out, a.dstate = _ptr(state), _ptr(saved), _ptr(dstate_out), _ptr(dstate)
-        a.dout, a.dq, a.dk, a.dv = _rows(dout), _rows(dq), _rows(dk), _rows(dv)
+        dstate = torch.empty((N, H, D, E), dtype=torch.float32, device=dev) if want_dstate else None
+
+        def args(work):
+            return ATTEND.pack(_DTYPES[q.dtype], H, D, E, T, N, scale, *_rows(q), *_rows(k), *_rows(v), *_NO_ROWS, decay.data_ptr(), _ptr(start),
+                               _ptr(state), 0, _ptr(saved), work, *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), _ptr(dstate_out),
+                               _ptr(dstate))
+
+        a = args(0)
         work = _work(ops_check(L.mo_attend_work(a, 1), "mo_attend_work"), dev)
-        a.work = _ptr(work)
+        if work is not None:
+            a = args(work.data_ptr())
         ops_check(L.mo_attend_backward(a, _stream(dev)), "mo_attend_backward")
     return dq, dk, dv, dstate
 
 
-_functions = {}
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, decay, start, state, scale):
+        out, state_out, saved = _attend_forward(q, k, v, decay, start, state, scale, True)
+        ctx.save_for_backward(q, k, v, decay, start, state, saved)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, state_out
 
-
-def _function(name):
-    """The autograd functions, made on first use (torch is imported late throughout this package)."""
-    if _functions:
-        return _functions[name]
-    torch = _torch()
-    once = torch.autograd.function.once_differentiable
-
-    class Attend(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, q, k, v, decay, start, state, scale):
-            out, state_out, saved = _attend_forward(q, k, v, decay, start, state, scale, True)
-            ctx.save_for_backward(q, k, v, decay, start, state, saved)
-            ctx.scale = scale
-            ctx.set_materialize_grads(False)
-            return out, state_out
-
-        @staticmethod
-        @once
-        def backward(ctx, dout, dstate_out):
-            q, k, v, decay, start, state, saved = ctx.saved_tensors
-            if dout is None:
-                dout = torch.zeros(1, dtype=q.dtype, device=q.device).expand(v.shape)
-            dout = _as_rows(dout)
-            if dstate_out is not None:
-                dstate_out = dstate_out.contiguous()
-            dq, dk, dv, dstate = _attend_backward(q, k, v, decay, start, state, saved, ctx.scale, dout, dstate_out,
-                                                  state is not None and ctx.needs_input_grad[5])
-            return dq, dk, dv, None, None, dstate, None
-
-    class Norm(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, groups, weight, bias, eps, act):
-            y, rows, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
-            ctx.save_for_backward(rows, weight, bias, stats)
-            ctx.how = (groups, eps, act)
-            return y
-
-        @staticmethod
-        @once
-        def backward(ctx, dy):
-            rows, weight, bias, stats = ctx.saved_tensors
-            dx, dw, db = _norm_backward(rows, weight, bias, stats, dy, *ctx.how, any(ctx.needs_input_grad[2:4]))
-            return dx, None, dw, db, None, None
-
-    _functions.update(attend=Attend, norm=Norm)
-    return _functions[name]
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dstate_out):
+        q, k, v, decay, start, state, saved = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros(1, dtype=q.dtype, device=q.device).expand(v.shape)
+        if dstate_out is not None:
+            dstate_out = dstate_out.contiguous()
+        dq, dk, dv, dstate = _attend_backward(q, k, v, decay, start, state, saved, ctx.scale, _as_rows(dout), dstate_out,
+                                              state is not None and ctx.needs_input_grad[5])
+        return dq, dk, dv, None, None, dstate, None
 
 
 def _attend_plain(q, k, v, decay, start, state, scale):
     """The recurrence step by step in torch operations, in float32."""
-    torch = _torch()
     S = q.new_zeros(q.shape[1:] + v.shape[-1:], dtype=torch.float32) if state is None else state
     g, out = decay[:, None, None], []
     for t in range(q.shape[0]):
@@ -220,7 +188,6 @@ def linear_attention(q, k, v, decay, start=None, state=None, scale=None):
 
     Sums and states are float32. With bf16 inputs the masked products of a chunk and the state that multiplies q are rounded to
     bf16 where they enter a matrix product; the state itself is not."""
-    torch = _torch()
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("linear_attention: q, k and v must be (T, N, H, head size)")
     _check_attend("linear_attention", "T, N", q, k, v, decay, start, state)
@@ -228,40 +195,38 @@ def linear_attention(q, k, v, decay, start=None, state=None, scale=None):
     every = [t for t in (q, k, v, decay, start, state) if t is not None]
     if not _kernel_takes(*every):
         return _attend_plain(q, k, v, decay, start, state, scale)
-    q, k, v = (_as_rows(t) for t in (q, k, v))
-    decay = decay.contiguous()
+    q, k, v, decay = _as_rows(q), _as_rows(k), _as_rows(v), decay.contiguous()
     start = None if start is None else start.contiguous()
     state = None if state is None else state.contiguous()
     if torch.is_grad_enabled() and any(t.requires_grad for t in every):
-        return _function("attend").apply(q, k, v, decay, start, state, scale)
+        return _Attend.apply(q, k, v, decay, start, state, scale)
     return _attend_forward(q, k, v, decay, start, state, scale, False)[:2]
 
 
 def linear_attention_step(q, k, v, decay, state, start=None, scale=None):
     """One step of `linear_attention` for every env: q, k (N, H, D), v (N, H, E), start (N,) bool or None; state (N, H, D, E)
     float32, contiguous, is updated in place. Returns out (N, H, E) in the type of q. No gradient."""
-    torch = _torch()
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("linear_attention_step: q, k and v must be (N, H, head size)")
     _check_attend("linear_attention_step", "N", q, k, v, decay, start, state)
     if not state.is_contiguous():
         raise ValueError("linear_attention_step: state is updated in place and must be contiguous")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise ValueError("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention to train")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if not _kernel_takes(*(t for t in (q, k, v, decay, state, start) if t is not None)):
+    every = (q, k, v, decay, state) if start is None else (q, k, v, decay, state, start)
+    if not _kernel_takes(*every):
         out, S = _attend_plain(q[None], k[None], v[None], decay, None if start is None else start[None], state, scale)
         state.copy_(S)
         return out[0]
-    from ._native import ops_check, ops_lib
-    q, k, v = (_as_rows(t) for t in (q, k, v))
-    decay = decay.contiguous()
+    q, k, v, decay = _as_rows(q), _as_rows(k), _as_rows(v), decay.contiguous()
     start = None if start is None else start.contiguous()
-    N, H, D = q.shape
-    with _on(q.device):
-        out = torch.empty_like(v, memory_format=torch.contiguous_format)
-        ops_check(ops_lib().mo_attend_step(_dtype(q), N, H, D, v.shape[-1], scale, _rows(q), _rows(k), _rows(v), decay.data_ptr(),
-                                           _ptr(start), state.data_ptr(), _rows(out), _stream(q.device)), "mo_attend_step")
+    (N, H, D), E, dev = q.shape, v.shape[-1], q.device
+    with _on(dev):
+        out = torch.empty((N, H, E), dtype=q.dtype, device=dev)
+        ops_check(ops_lib().mo_attend_step(_DTYPES[q.dtype], N, H, D, E, scale, ROWS.pack(*_rows(q)), ROWS.pack(*_rows(k)), ROWS.pack(*_rows(v)),
+                                           decay.data_ptr(), _ptr(start), state.data_ptr(), ROWS.pack(*_rows(out)), _stream(dev)),
+                  "mo_attend_step")
     return out
 
 
@@ -271,49 +236,62 @@ def _channels_last(x):
     return (x.movedim(1, -1) if x.dim() > 2 else x).contiguous()
 
 
-def _norm_args(rows, groups, weight, bias, eps, act):
-    from ._native import MoNorm
+def _norm_sizes(rows, groups, eps, act):
     B, C = rows.shape[0], rows.shape[-1]
-    return MoNorm(dtype=_dtype(rows), act=ACTS[act], C=C, groups=groups, B=B, S=max(1, rows.numel() // max(1, B * C)), eps=eps,
-                  x=rows.data_ptr(), weight=_ptr(weight), bias=_ptr(bias))
+    return _DTYPES[rows.dtype], ACTS[act], C, groups, B, max(1, rows.numel() // max(1, B * C)), eps
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, keep):
     """y, x's rows, and, if `keep`, each group's mean and 1 / deviation."""
-    torch = _torch()
-    from ._native import ops_check, ops_lib
     L, dev, rows = ops_lib(), x.device, _channels_last(x)
     with _on(dev):
         y = torch.empty_like(rows)
-        stats = torch.empty(rows.shape[0], groups, 2, dtype=torch.float32, device=dev) if keep else None
-        a = _norm_args(rows, groups, weight, bias, eps, act)
-        a.y, a.stats = y.data_ptr(), _ptr(stats)
+        stats = torch.empty((rows.shape[0], groups, 2), dtype=torch.float32, device=dev) if keep else None
+        sizes = _norm_sizes(rows, groups, eps, act) + (rows.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats))
+        a = NORM.pack(*sizes, 0, 0, 0, 0, 0)
         work = _work(ops_check(L.mo_group_norm_work(a, 0), "mo_group_norm_work"), dev)
-        a.work = _ptr(work)
+        if work is not None:
+            a = NORM.pack(*sizes, work.data_ptr(), 0, 0, 0, 0)
         ops_check(L.mo_group_norm(a, _stream(dev)), "mo_group_norm")
     return y.movedim(-1, 1) if x.dim() > 2 else y, rows, stats
 
 
 def _norm_backward(rows, weight, bias, stats, dy, groups, eps, act, want_params):
-    torch = _torch()
-    from ._native import ops_check, ops_lib
     L, dev, dy = ops_lib(), rows.device, _channels_last(dy)
     with _on(dev):
         dx = torch.empty_like(rows)
         dw = db = None
         if want_params and weight is not None:
             dw, db = (torch.empty if rows.shape[0] else torch.zeros)((2,) + weight.shape, dtype=torch.float32, device=dev)
-        a = _norm_args(rows, groups, weight, bias, eps, act)
-        a.stats, a.dy, a.dx, a.dweight, a.dbias = stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db)
+        sizes = _norm_sizes(rows, groups, eps, act) + (rows.data_ptr(), _ptr(weight), _ptr(bias), 0, stats.data_ptr())
+        rest = (dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db))
+        a = NORM.pack(*sizes, 0, *rest)
         work = _work(ops_check(L.mo_group_norm_work(a, 1), "mo_group_norm_work"), dev)
-        a.work = _ptr(work)
+        if work is not None:
+            a = NORM.pack(*sizes, work.data_ptr(), *rest)
         ops_check(L.mo_group_norm_backward(a, _stream(dev)), "mo_group_norm_backward")
     return dx.movedim(-1, 1) if dx.dim() > 2 else dx, dw, db
 
 
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, eps, act):
+        y, rows, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
+        ctx.save_for_backward(rows, weight, bias, stats)
+        ctx.how = (groups, eps, act)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        rows, weight, bias, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = _norm_backward(rows, weight, bias, stats, dy, *ctx.how, need[2] or need[3])
+        return dx, None, dw, db, None, None
+
+
 def _norm_plain(x, groups, weight, bias, eps, act):
     """The same in torch operations, in float32."""
-    torch = _torch()
     y = x.float().reshape(x.shape[0], groups, x.shape[1] // groups, -1)
     d = y - y.mean((2, 3), keepdim=True)
     z = (d * torch.rsqrt(d.square().mean((2, 3), keepdim=True) + eps)).reshape(x.shape)
@@ -330,8 +308,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
     bias (C,) (both or neither; float32, other float types are converted), then act: "none", "relu" or "silu". All in float32,
     rounded once. The result has x's type and lies channels last, as x does (`memory_format=torch.channels_last`, or (B, C));
     an x that lies otherwise is copied first. Differentiable once."""
-    torch = _torch()
-    if x.dim() < 2 or x.dtype not in (torch.float32, torch.bfloat16):
+    if x.dim() < 2 or x.dtype not in _DTYPES:
         raise ValueError("group_norm_act: x must be (B, C, ...) float32 or bf16")
     C = x.shape[1]
     if not isinstance(groups, int) or groups < 1 or C < 1 or C % groups:
@@ -342,17 +319,17 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
         raise ValueError("group_norm_act: eps must be >= 0")
     if (weight is None) != (bias is None):
         raise ValueError("group_norm_act: weight and bias go together")
-    if weight is not None and any(tuple(p.shape) != (C,) or not p.is_floating_point() or p.device != x.device for p in (weight, bias)):
+    if weight is not None and any(p.shape != (C,) or not p.is_floating_point() or p.device != x.device for p in (weight, bias)):
         raise ValueError(f"group_norm_act: weight and bias must be ({C},) on the device of x ({x.device})")
     if 0 in x.shape[2:]:
         raise ValueError("group_norm_act: a sample has no positions")
-    every = [t for t in (x, weight, bias) if t is not None]
+    every = (x,) if weight is None else (x, weight, bias)
     if not _kernel_takes(*every):
         return _norm_plain(x, groups, weight, bias, eps, act)
     if weight is not None:
         weight, bias = weight.float().contiguous(), bias.float().contiguous()
     if torch.is_grad_enabled() and any(t.requires_grad for t in every):
-        return _function("norm").apply(x, groups, weight, bias, eps, act)
+        return _Norm.apply(x, groups, weight, bias, eps, act)
     return _norm_forward(x, groups, weight, bias, eps, act, False)[0]
 
 
@@ -362,9 +339,7 @@ def make_memory_net(n_actions: int = N_ACTIONS, in_ch: int = 4, heads: int = 8, 
     memory: projection to q, k and v, linear attention with `heads` decaying memories of 512 / heads, group norm a head,
     projection, added to the features. Random weights. On the GPU the trunk and the memory run in bf16 (the memories
     themselves and the heads in float32), on the CPU everything in float32."""
-    torch = _torch()
-    nn = torch.nn
-    F = torch.nn.functional
+    nn, F = torch.nn, torch.nn.functional
     width = 512
     if heads < 1 or width % heads or width // heads > MAX_HEAD:
         raise ValueError(f"make_memory_net: heads must divide {width} into heads of at most {MAX_HEAD}")

@@ -6,7 +6,7 @@ one; N_TERMS covers the terms, the decay's powers and the joining of chunks. bf1
 significand, each at most 2^-9 of what it rounds: that of a masked product, that of the state that meets q (the two act on parts of
 one sum), and the result's own. So a bf16 result is within 3 * 2^-9 of the exact one in norm and, element by element, within
 3 * 2^-9 of the sum of absolute values."""
-import ctypes
+
 import os
 import re
 
@@ -211,13 +211,16 @@ def test_ops_library_exports_and_bindings():
     bound = open(os.path.join(ROOT, "fast-mario-env_amd", "fast_mario_env_amd", "_native.py")).read()
     for s in names:
         assert hasattr(L, s) and s in bound, s
-    a = _native.MoAttend(dtype=1, H=2, D=200, E=8, T=1, N=1)
+    rows, none = (0, 0, 0, 0), (0,) * 6
+    a = _native.ATTEND.pack(1, 2, 200, 8, 1, 1, 1.0, *rows * 4, *none, *rows * 4, 0, 0)   # a head size of 200
+    assert len(a) == 360 and _native.NORM.size == 120 and _native.ROWS.size == 32
     assert L.mo_attend(a, None) == -1 and b"head sizes" in L.mo_last_error()
     assert L.mo_attend_work(a, 0) == -1
-    m = _native.MoNorm(dtype=1, act=0, C=10, groups=3, B=1, S=1, eps=1e-5)
+    m = _native.NORM.pack(1, 0, 10, 3, 1, 1, 1e-5, *(0,) * 10)
     assert L.mo_group_norm(m, None) == -1 and b"groups" in L.mo_last_error()
     host = np.zeros(64, np.float32)
-    m = _native.MoNorm(dtype=0, act=0, C=8, groups=1, B=1, S=1, eps=1e-5, x=host.ctypes.data, y=host.ctypes.data, work=host.ctypes.data)
+    at = host.ctypes.data
+    m = _native.NORM.pack(0, 0, 8, 1, 1, 1, 1e-5, at, 0, 0, at, 0, at, 0, 0, 0, 0)
     assert L.mo_group_norm(m, None) == -1 and L.mo_last_error()   # pageable host memory (or no GPU at all)
 
 
