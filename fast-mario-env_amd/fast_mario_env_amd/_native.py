@@ -9,12 +9,10 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 
 LIB_ENV_VAR = "MARIO_HIP_LIB"
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libmario_hip.so"
-OPS_LIB_NAME = "libmario_ops.so"
 
 _P = ctypes.c_void_p
 _i64, _i32, _dbl = ctypes.c_int64, ctypes.c_int, ctypes.c_double
@@ -89,42 +87,19 @@ def lib() -> ctypes.CDLL:
     return L
 
 
-# The structures of include/mario_ops.h, as the bytes that a call hands over (made in one go: a call of these operators is a few
-# microseconds of host work, of which ctypes structures were a third).
-ROWS = struct.Struct("=Qqqq")                                                       # MoRows: p, st, sn, sh
-ATTEND = struct.Struct("=4i2qf4x" + 4 * "Qqqq" + "6Q" + 4 * "Qqqq" + "2Q")          # MoAttend, its fields in order
-NORM = struct.Struct("=4i2qf4x10Q")                                                 # MoNorm
-
-
-def ops_lib() -> ctypes.CDLL:
-    """libmario_ops.so: the operators of a policy with a memory (include/mario_ops.h)."""
+def ops():
+    """The extension module that runs libmario_ops.so (include/mario_ops.h) on torch tensors: csrc/ops/torch_ops.cpp."""
     global _ops
-    if _ops is not None:
-        return _ops
-    path = os.path.join(HERE, OPS_LIB_NAME)
-    if not os.path.isfile(path):
-        raise NativeLibraryError(
-            f"fast_mario_env_amd: {path} is missing. Build it with `python -c \"import __graft_entry__ as g; "
-            f"g.build()\"` from the repository root (needs hipcc with gfx950 support).")
-    L = ctypes.CDLL(path)
-    L.mo_last_error.restype = ctypes.c_char_p
-    L.mo_attend_saved.restype = L.mo_attend_work.restype = L.mo_group_norm_work.restype = _i64
-    L.mo_attend_saved.argtypes = [_P]
-    L.mo_attend_work.argtypes = [_P, _i32]
-    for f in (L.mo_attend, L.mo_attend_backward):
-        f.argtypes = [_P, _P]
-    L.mo_attend_step.argtypes = [_i32, _i64, _i32, _i32, _i32, ctypes.c_float] + [_P] * 8
-    L.mo_group_norm_work.argtypes = [_P, _i32]
-    for f in (L.mo_group_norm, L.mo_group_norm_backward):
-        f.argtypes = [_P, _P]
-    _ops = L
-    return L
-
-
-def ops_check(rc: int, what: str) -> int:
-    if rc < 0:
-        raise RuntimeError(f"{what} failed: {ops_lib().mo_last_error().decode(errors='replace')}")
-    return rc
+    if _ops is None:
+        try:
+            import torch  # noqa: F401  (its libraries first)
+            from . import _mario_ops_torch
+        except ImportError as e:
+            raise NativeLibraryError(
+                f"fast_mario_env_amd: the operators in {HERE} cannot be loaded ({e}). Build them with `python -c \"import "
+                f"__graft_entry__ as g; g.build()\"` from the repository root (needs hipcc with gfx950 support).") from e
+        _ops = _mario_ops_torch
+    return _ops
 
 
 def check(rc: int, what: str) -> None:

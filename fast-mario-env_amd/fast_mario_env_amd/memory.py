@@ -17,18 +17,16 @@ queued on torch's current stream. CPU tensors, and what torch traces or transfor
 """
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
 
-from ._native import ATTEND, NORM, ROWS, ops_check, ops_lib
+from ._native import ops
 from .rollout import N_ACTIONS, _transformed, policy_input
 
 ACTS = {"none": 0, "relu": 1, "silu": 2}
 MAX_HEAD = 128
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
-_NO_ROWS = (0, 0, 0, 0)
+_DTYPES = (torch.float32, torch.bfloat16)
 
 
 def _kernel_takes(*ts):
@@ -37,40 +35,6 @@ def _kernel_takes(*ts):
         if type(t) not in (torch.Tensor, torch.nn.Parameter) or not t.is_cuda or t.is_neg():
             return False
     return not _transformed(*ts)
-
-
-def _rows(t):
-    """The tensor's head vectors (T, N, H, d) or (N, H, d) as the library takes them (MoRows); the last dimension is contiguous."""
-    return (t.data_ptr(), *t.stride()[:3]) if t.dim() == 4 else (t.data_ptr(), 0, *t.stride()[:2])
-
-
-def _as_rows(t):
-    """The tensor as the kernels take it: head vectors contiguous, and on 16-byte boundaries where their size allows it (they are
-    copied otherwise: a copy costs less than going step by step)."""
-    st = t.stride()
-    if st[-1] != 1 and t.shape[-1] != 1:
-        return t.contiguous()
-    whole = 16 // t.element_size()
-    if t.shape[-1] % whole == 0 and (t.data_ptr() % 16 or any(s % whole for s in st[:-1])):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _work(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _on(device):
-    """The device made current for launches and allocations (nothing to do where it is: a context costs more than the check)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 def head_decays(heads: int, device="cuda"):
@@ -96,69 +60,6 @@ def _check_attend(name, lead, q, k, v, decay, start, state):
     for t in (k, v, decay, start, state):
         if t is not None and t.device != dev:
             raise ValueError(f"{name}: all tensors must be on the device of q ({dev})")
-
-
-def _attend_forward(q, k, v, decay, start, state, scale, keep):
-    """out, state_out and what the gradient takes up (None unless `keep`)."""
-    L, dev = ops_lib(), q.device
-    (T, N, H, D), E = q.shape, v.shape[-1]
-    with _on(dev):
-        out = torch.empty((T, N, H, E), dtype=q.dtype, device=dev)
-        state_out = torch.empty((N, H, D, E), dtype=torch.float32, device=dev)
-
-        def args(saved, work):
-            return ATTEND.pack(_DTYPES[q.dtype], H, D, E, T, N, scale, *_rows(q), *_rows(k), *_rows(v), *_rows(out), decay.data_ptr(), _ptr(start),
-                               _ptr(state), state_out.data_ptr(), saved, work, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0)
-
-        a = args(0, 0)
-        saved = _work(ops_check(L.mo_attend_saved(a), "mo_attend_saved"), dev) if keep else None
-        work = _work(ops_check(L.mo_attend_work(a, 0), "mo_attend_work"), dev)
-        if saved is not None or work is not None:
-            a = args(_ptr(saved), _ptr(work))
-        ops_check(L.mo_attend(a, _stream(dev)), "mo_attend")
-    return out, state_out, saved
-
-
-def _attend_backward(q, k, v, decay, start, state, saved, scale, dout, dstate_out, want_dstate):
-    L, dev = ops_lib(), q.device
-    (T, N, H, D), E = q.shape, v.shape[-1]
-    with _on(dev):
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        dstate = torch.empty((N, H, D, E), dtype=torch.float32, device=dev) if want_dstate else None
-
-        def args(work):
-            return ATTEND.pack(_DTYPES[q.dtype], H, D, E, T, N, scale, *_rows(q), *_rows(k), *_rows(v), *_NO_ROWS, decay.data_ptr(), _ptr(start),
-                               _ptr(state), 0, _ptr(saved), work, *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), _ptr(dstate_out),
-                               _ptr(dstate))
-
-        a = args(0)
-        work = _work(ops_check(L.mo_attend_work(a, 1), "mo_attend_work"), dev)
-        if work is not None:
-            a = args(work.data_ptr())
-        ops_check(L.mo_attend_backward(a, _stream(dev)), "mo_attend_backward")
-    return dq, dk, dv, dstate
-
-
-class _Attend(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, decay, start, state, scale):
-        out, state_out, saved = _attend_forward(q, k, v, decay, start, state, scale, True)
-        ctx.save_for_backward(q, k, v, decay, start, state, saved)
-        ctx.scale = scale
-        ctx.set_materialize_grads(False)
-        return out, state_out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, dstate_out):
-        q, k, v, decay, start, state, saved = ctx.saved_tensors
-        if dout is None:
-            dout = torch.zeros(1, dtype=q.dtype, device=q.device).expand(v.shape)
-        if dstate_out is not None:
-            dstate_out = dstate_out.contiguous()
-        dq, dk, dv, dstate = _attend_backward(q, k, v, decay, start, state, saved, ctx.scale, _as_rows(dout), dstate_out,
-                                              state is not None and ctx.needs_input_grad[5])
-        return dq, dk, dv, None, None, dstate, None
 
 
 def _attend_plain(q, k, v, decay, start, state, scale):
@@ -192,15 +93,9 @@ def linear_attention(q, k, v, decay, start=None, state=None, scale=None):
         raise ValueError("linear_attention: q, k and v must be (T, N, H, head size)")
     _check_attend("linear_attention", "T, N", q, k, v, decay, start, state)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    every = [t for t in (q, k, v, decay, start, state) if t is not None]
-    if not _kernel_takes(*every):
+    if not _kernel_takes(*(t for t in (q, k, v, decay, start, state) if t is not None)):
         return _attend_plain(q, k, v, decay, start, state, scale)
-    q, k, v, decay = _as_rows(q), _as_rows(k), _as_rows(v), decay.contiguous()
-    start = None if start is None else start.contiguous()
-    state = None if state is None else state.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in every):
-        return _Attend.apply(q, k, v, decay, start, state, scale)
-    return _attend_forward(q, k, v, decay, start, state, scale, False)[:2]
+    return ops().attend(q, k, v, decay, start, state, scale)
 
 
 def linear_attention_step(q, k, v, decay, state, start=None, scale=None):
@@ -219,77 +114,10 @@ def linear_attention_step(q, k, v, decay, state, start=None, scale=None):
         out, S = _attend_plain(q[None], k[None], v[None], decay, None if start is None else start[None], state, scale)
         state.copy_(S)
         return out[0]
-    q, k, v, decay = _as_rows(q), _as_rows(k), _as_rows(v), decay.contiguous()
-    start = None if start is None else start.contiguous()
-    (N, H, D), E, dev = q.shape, v.shape[-1], q.device
-    with _on(dev):
-        out = torch.empty((N, H, E), dtype=q.dtype, device=dev)
-        ops_check(ops_lib().mo_attend_step(_DTYPES[q.dtype], N, H, D, E, scale, ROWS.pack(*_rows(q)), ROWS.pack(*_rows(k)), ROWS.pack(*_rows(v)),
-                                           decay.data_ptr(), _ptr(start), state.data_ptr(), ROWS.pack(*_rows(out)), _stream(dev)),
-                  "mo_attend_step")
-    return out
+    return ops().attend_step(q, k, v, decay, state, start, scale)
 
 
 # ---------------------------------------------------------------- group norm and activation
-def _channels_last(x):
-    """x (B, C, ...) as its channels-last rows (B, ..., C), contiguous (a copy where it lies otherwise)."""
-    return (x.movedim(1, -1) if x.dim() > 2 else x).contiguous()
-
-
-def _norm_sizes(rows, groups, eps, act):
-    B, C = rows.shape[0], rows.shape[-1]
-    return _DTYPES[rows.dtype], ACTS[act], C, groups, B, max(1, rows.numel() // max(1, B * C)), eps
-
-
-def _norm_forward(x, groups, weight, bias, eps, act, keep):
-    """y, x's rows, and, if `keep`, each group's mean and 1 / deviation."""
-    L, dev, rows = ops_lib(), x.device, _channels_last(x)
-    with _on(dev):
-        y = torch.empty_like(rows)
-        stats = torch.empty((rows.shape[0], groups, 2), dtype=torch.float32, device=dev) if keep else None
-        sizes = _norm_sizes(rows, groups, eps, act) + (rows.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats))
-        a = NORM.pack(*sizes, 0, 0, 0, 0, 0)
-        work = _work(ops_check(L.mo_group_norm_work(a, 0), "mo_group_norm_work"), dev)
-        if work is not None:
-            a = NORM.pack(*sizes, work.data_ptr(), 0, 0, 0, 0)
-        ops_check(L.mo_group_norm(a, _stream(dev)), "mo_group_norm")
-    return y.movedim(-1, 1) if x.dim() > 2 else y, rows, stats
-
-
-def _norm_backward(rows, weight, bias, stats, dy, groups, eps, act, want_params):
-    L, dev, dy = ops_lib(), rows.device, _channels_last(dy)
-    with _on(dev):
-        dx = torch.empty_like(rows)
-        dw = db = None
-        if want_params and weight is not None:
-            dw, db = (torch.empty if rows.shape[0] else torch.zeros)((2,) + weight.shape, dtype=torch.float32, device=dev)
-        sizes = _norm_sizes(rows, groups, eps, act) + (rows.data_ptr(), _ptr(weight), _ptr(bias), 0, stats.data_ptr())
-        rest = (dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db))
-        a = NORM.pack(*sizes, 0, *rest)
-        work = _work(ops_check(L.mo_group_norm_work(a, 1), "mo_group_norm_work"), dev)
-        if work is not None:
-            a = NORM.pack(*sizes, work.data_ptr(), *rest)
-        ops_check(L.mo_group_norm_backward(a, _stream(dev)), "mo_group_norm_backward")
-    return dx.movedim(-1, 1) if dx.dim() > 2 else dx, dw, db
-
-
-class _Norm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, groups, weight, bias, eps, act):
-        y, rows, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
-        ctx.save_for_backward(rows, weight, bias, stats)
-        ctx.how = (groups, eps, act)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        rows, weight, bias, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = _norm_backward(rows, weight, bias, stats, dy, *ctx.how, need[2] or need[3])
-        return dx, None, dw, db, None, None
-
-
 def _norm_plain(x, groups, weight, bias, eps, act):
     """The same in torch operations, in float32."""
     y = x.float().reshape(x.shape[0], groups, x.shape[1] // groups, -1)
@@ -323,14 +151,9 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
         raise ValueError(f"group_norm_act: weight and bias must be ({C},) on the device of x ({x.device})")
     if 0 in x.shape[2:]:
         raise ValueError("group_norm_act: a sample has no positions")
-    every = (x,) if weight is None else (x, weight, bias)
-    if not _kernel_takes(*every):
+    if not _kernel_takes(*((x,) if weight is None else (x, weight, bias))):
         return _norm_plain(x, groups, weight, bias, eps, act)
-    if weight is not None:
-        weight, bias = weight.float().contiguous(), bias.float().contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in every):
-        return _Norm.apply(x, groups, weight, bias, eps, act)
-    return _norm_forward(x, groups, weight, bias, eps, act, False)[0]
+    return ops().group_norm_act(x, groups, weight, bias, eps, ACTS[act])
 
 
 # ---------------------------------------------------------------- an actor-critic with a memory

@@ -7,8 +7,10 @@ significand, each at most 2^-9 of what it rounds: that of a masked product, that
 one sum), and the result's own. So a bf16 result is within 3 * 2^-9 of the exact one in norm and, element by element, within
 3 * 2^-9 of the sum of absolute values."""
 
+import ctypes
 import os
 import re
+import struct
 
 import numpy as np
 import pytest
@@ -203,25 +205,29 @@ def test_refusals():
             group_norm_act(*args, **kw)
 
 
-def test_ops_library_exports_and_bindings():
-    """libmario_ops.so loads without a GPU, exports what include/mario_ops.h declares, and checks sizes before any device."""
-    names = set(re.findall(r"\b(mo_\w+)\s*\(", open(os.path.join(ROOT, "include", "mario_ops.h")).read())) - {"mo_attend_saved()"}
+def test_ops_library_exports_and_checks():
+    """libmario_ops.so loads without a GPU, exports what include/mario_ops.h declares (all of which the torch module calls), and
+    checks sizes before any device."""
+    package = os.path.dirname(_native.__file__)
+    names = set(re.findall(r"\b(mo_\w+)\s*\(", open(os.path.join(ROOT, "include", "mario_ops.h")).read()))
     assert len(names) >= 8
-    L = _native.ops_lib()
-    bound = open(os.path.join(ROOT, "fast-mario-env_amd", "fast_mario_env_amd", "_native.py")).read()
+    L = ctypes.CDLL(os.path.join(package, "libmario_ops.so"))
+    L.mo_last_error.restype = ctypes.c_char_p
+    L.mo_attend_work.restype = ctypes.c_int64
+    calls = open(os.path.join(ROOT, "fast-mario-env_amd", "csrc", "ops", "torch_ops.cpp")).read()
     for s in names:
-        assert hasattr(L, s) and s in bound, s
-    rows, none = (0, 0, 0, 0), (0,) * 6
-    a = _native.ATTEND.pack(1, 2, 200, 8, 1, 1, 1.0, *rows * 4, *none, *rows * 4, 0, 0)   # a head size of 200
-    assert len(a) == 360 and _native.NORM.size == 120 and _native.ROWS.size == 32
+        assert hasattr(L, s) and s in calls, s
+    attend, norm = struct.Struct("=4i2qf4x" + 4 * "Qqqq" + "6Q" + 4 * "Qqqq" + "2Q"), struct.Struct("=4i2qf4x10Q")   # MoAttend, MoNorm
+    a = attend.pack(1, 2, 200, 8, 1, 1, 1.0, *(0,) * 16, *(0,) * 6, *(0,) * 16, 0, 0)      # a head size of 200
     assert L.mo_attend(a, None) == -1 and b"head sizes" in L.mo_last_error()
     assert L.mo_attend_work(a, 0) == -1
-    m = _native.NORM.pack(1, 0, 10, 3, 1, 1, 1e-5, *(0,) * 10)
+    m = norm.pack(1, 0, 10, 3, 1, 1, 1e-5, *(0,) * 10)
     assert L.mo_group_norm(m, None) == -1 and b"groups" in L.mo_last_error()
     host = np.zeros(64, np.float32)
     at = host.ctypes.data
-    m = _native.NORM.pack(0, 0, 8, 1, 1, 1, 1e-5, at, 0, 0, at, 0, at, 0, 0, 0, 0)
+    m = norm.pack(0, 0, 8, 1, 1, 1, 1e-5, at, 0, 0, at, 0, at, 0, 0, 0, 0)
     assert L.mo_group_norm(m, None) == -1 and L.mo_last_error()   # pageable host memory (or no GPU at all)
+    assert all(hasattr(_native.ops(), f) for f in ("attend", "attend_step", "group_norm_act"))
 
 
 # ---------------------------------------------------------------- linear attention on the GPU
@@ -436,6 +442,18 @@ def test_attention_same_bits_and_other_streams(T, N, H, D):
     torch.cuda.synchronize()
     for a, b, c in zip(first, other, again):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_operators_are_differentiable_once():
+    q, k, v, decay, start, state, do, ds = attend_inputs(5, 2, 2, 16, 16, torch.float32)
+    x, w, b, dy = norm_inputs(3, 16, (3, 3), torch.float32)
+    q, x = q.requires_grad_(), x.requires_grad_()
+    for y, leaf, g in ((linear_attention(q, k, v, decay, start, state)[0], q, do), (group_norm_act(x, 2, w, b, act="silu"), x, dy)):
+        (first,) = torch.autograd.grad(y, leaf, g, create_graph=True)
+        assert torch.isfinite(first).all()
+        with pytest.raises(RuntimeError, match="once"):
+            first.square().sum().backward()
 
 
 @pytest.mark.gpu
