@@ -114,13 +114,21 @@ __device__ __forceinline__ int start_of_lane(const MoAttend& a, int64_t t0, int 
     return a.start && lane < n ? a.start[(t0 + lane) * a.N + env] : 0;
 }
 
-// g^0 .. g^L (g^0 is 1 for g = 0 too), and the factors by which step i sees step j, scale g^(i-j) or 0, of all i - j.
+// g^n, 1 for n = 0, rounded once: squares in float64. (A logarithm's rounding would grow with the memory's length: with g = 1 - x
+// it enters a state as its error over x.)
+__device__ __forceinline__ float power(float g, int64_t n) {
+    double p = 1.0;
+    for (double x = g; n; n >>= 1, x *= x)
+        if (n & 1) p *= x;
+    return (float)p;
+}
+
+// g^0 .. g^L, and the factors by which step i sees step j, scale g^(i-j) or 0, of all i - j.
 template <int L> struct Powers {
     float pw[L + 1], seen[2 * L];
     __device__ __forceinline__ void fill(float g, float scale) {
-        const float lg = __log2f(g);
         for (int i = threadIdx.x; i <= L; i += blockDim.x) {
-            const float x = i ? exp2f((float)i * lg) : 1.f;
+            const float x = power(g, i);
             pw[i] = x;
             if (i < L) { seen[i] = 0.f; seen[L + i] = scale * x; }
         }
@@ -132,7 +140,7 @@ template <int L> struct Powers {
 // together) go to one of them, so that what one L2 fetches lies together too.
 constexpr int XCD_RUN = 16;
 __device__ __forceinline__ int64_t head_of_block(int64_t heads) {
-    const int64_t b = blockIdx.x, round = 8 * XCD_RUN;
+    const int64_t b = block_here(), round = 8 * XCD_RUN;
     if (b >= heads / round * round) return b;
     return b / round * round + b % 8 * XCD_RUN + b % round / 8;
 }
@@ -211,6 +219,7 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
     const typename C::Scores sp{lp};
     const int w = threadIdx.x / kWave;
     const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
+    if (nh >= a.N * a.H) return;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int e0 = w * CT * 16;   // the wave's columns
@@ -404,7 +413,7 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
         for (int ct = 0; ct < CT; ct++) store_state<P, false>(a, to, e0 + 16 * ct, S[ct]);
     if (!OUT && threadIdx.x == 0) {
         const int64_t n = min(c1 * L, a.T) - c0 * L;
-        cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : exp2f((float)n * __log2f(a.decay[h]));
+        cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : power(a.decay[h], n);
     }
 }
 
@@ -489,7 +498,7 @@ inline int enter_states(const MoAttend& a, const Cut& c, const float* first, flo
 template <class T, int P> int attend_chunks(const MoAttend& a, hipStream_t s) {
     Cut c = attend_cut(a);
     cut_place(a, c);
-    const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(kForwardWaves<P> * kWave);
+    const dim3 grid = grid_of(a.N * a.H, c.segs), block(kForwardWaves<P> * kWave);
     if (c.segs > 1) {
         hipLaunchKernelGGL((k_attend<T, P, ONLY_SUMS>), grid, block, 0, s, a, c);
         if (launched("k_attend sums") || enter_states(a, c, a.state, a.state_out, false, s)) return -1;

@@ -72,6 +72,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
     const typename C::Scores sa{s.a}, sb{s.b};
     const int w = threadIdx.x / kWave;
     const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
+    if (nh >= a.N * a.H) return;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int x0 = w * 16;     // the wave's rows of R and S, columns of dq and dk; of dv its columns
@@ -281,6 +282,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT)) k_attend_back_sums(MoAt
     __shared__ __align__(16) float ut[L];
     const typename C::Rows sq{lq}, so{lo};
     const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
+    if (nh >= a.N * a.H) return;
     const int h = (int)(nh % a.H), seg = blockIdx.y;
     const int64_t c0 = seg * cut.per_seg, c1 = min(c0 + cut.per_seg, cut.chunks);
     const int x0 = threadIdx.x / kWave * 16;
@@ -312,14 +314,14 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT)) k_attend_back_sums(MoAt
     store_state<P, true>(a, to, x0, R);
     if (threadIdx.x == 0) {
         const int64_t n = min(c1 * L, a.T) - c0 * L;
-        cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : exp2f((float)n * __log2f(a.decay[h]));
+        cut.keep[(int64_t)seg * a.N * a.H + nh] = any_start ? -1.f : power(a.decay[h], n);
     }
 }
 
 template <class T, int P> int attend_back_chunks(const MoAttend& a, hipStream_t s) {
     Cut c = attend_cut(a);
     cut_place(a, c);
-    const dim3 grid((unsigned)(a.N * a.H), (unsigned)c.segs), block(BackChunk<T, P>::NT);
+    const dim3 grid = grid_of(a.N * a.H, c.segs), block(BackChunk<T, P>::NT);
     if (c.segs > 1) {
         hipLaunchKernelGGL((k_attend_back_sums<T, P>), grid, block, 0, s, a, c);
         if (launched("k_attend_back_sums") || enter_states(a, c, a.dstate_out, a.dstate, true, s)) return -1;

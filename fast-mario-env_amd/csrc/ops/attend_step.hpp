@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256) k_step_state(Step a) {
     constexpr int RG = kWave / CG, WAVES = 256 / kWave;
     __shared__ float sq[WAVES][MO_MAX_HEAD], sk[WAVES][MO_MAX_HEAD];
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, cg = lane % CG, rg = lane / CG;
-    const int64_t nh = (int64_t)blockIdx.x * WAVES + w;
+    const int64_t nh = block_here() * WAVES + w;
     if (nh >= a.N * a.H) return;
     const int64_t n = nh / a.H;
     const int h = (int)(nh % a.H), e = (blockIdx.y * CG + cg) * V;
@@ -88,12 +88,12 @@ __global__ void __launch_bounds__(256) k_step_state(Step a) {
 
 // Four columns a lane where the state's rows allow 16-byte accesses, else one (and two launch rows where 64 lanes do not span them).
 template <class T, bool FAR> int step_by_width(const Step& a, hipStream_t s) {
-    const unsigned blocks = (unsigned)((a.N * a.H + 256 / kWave - 1) / (256 / kWave));
+    const int64_t blocks = (a.N * a.H + 256 / kWave - 1) / (256 / kWave);
     const bool wide = a.E % 4 == 0 && (uintptr_t)a.state % 16 == 0;
-    if (wide && a.E <= 32) hipLaunchKernelGGL((k_step_state<T, 4, 8, FAR>), dim3(blocks), dim3(256), 0, s, a);
-    else if (wide && a.E <= 64) hipLaunchKernelGGL((k_step_state<T, 4, 16, FAR>), dim3(blocks), dim3(256), 0, s, a);
-    else if (wide) hipLaunchKernelGGL((k_step_state<T, 4, 32, FAR>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_step_state<T, 1, 64, FAR>), dim3(blocks, (unsigned)((a.E + 63) / 64)), dim3(256), 0, s, a);
+    if (wide && a.E <= 32) hipLaunchKernelGGL((k_step_state<T, 4, 8, FAR>), grid_of(blocks), dim3(256), 0, s, a);
+    else if (wide && a.E <= 64) hipLaunchKernelGGL((k_step_state<T, 4, 16, FAR>), grid_of(blocks), dim3(256), 0, s, a);
+    else if (wide) hipLaunchKernelGGL((k_step_state<T, 4, 32, FAR>), grid_of(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_step_state<T, 1, 64, FAR>), grid_of(blocks, (a.E + 63) / 64), dim3(256), 0, s, a);
     return launched("k_step_state");
 }
 template <class T> int step(const Step& a, hipStream_t s) {

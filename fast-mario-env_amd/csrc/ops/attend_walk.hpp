@@ -27,8 +27,9 @@ constexpr int WALK_STEPS = 16;   // steps whose w and z lie in LDS at a time
 template <class T, int BP, bool BACK>
 __global__ void __launch_bounds__(kWave) k_walk(Walk k) {
     __shared__ float ws[WALK_STEPS][BP], zs[WALK_STEPS][BP];
-    const int lane = threadIdx.x, h = blockIdx.x % k.H, a = blockIdx.y * kWave + lane;
-    const int64_t n = blockIdx.x / k.H;
+    const int64_t nh = block_here(), n = nh / k.H;
+    if (n >= k.N) return;
+    const int lane = threadIdx.x, h = (int)(nh % k.H), a = blockIdx.y * kWave + lane;
     const bool live = a < k.A;
     const auto at = [&](const MoRows& r, int64_t t) { return (T*)r.p + t * r.st + n * r.sn + h * r.sh; };
     const float g = k.decay[h];
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kWave) k_walk(Walk k) {
 }
 
 template <class T, bool BACK> int walk(const Walk& k, hipStream_t s) {
-    const dim3 grid((unsigned)(k.N * k.H), (unsigned)((k.A + kWave - 1) / kWave));
+    const dim3 grid = grid_of(k.N * k.H, (k.A + kWave - 1) / kWave);
     if (k.B <= 32) hipLaunchKernelGGL((k_walk<T, 32, BACK>), grid, dim3(kWave), 0, s, k);
     else if (k.B <= 64) hipLaunchKernelGGL((k_walk<T, 64, BACK>), grid, dim3(kWave), 0, s, k);
     else hipLaunchKernelGGL((k_walk<T, 128, BACK>), grid, dim3(kWave), 0, s, k);

@@ -23,6 +23,14 @@ template <class T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N
 
 constexpr int kWave = 64;
 
+// A launch has fewer than 2^32 threads along x: past 2^22 blocks it goes on along z. Blocks past the last one have nothing to do.
+constexpr int kGridBits = 22;
+__device__ __forceinline__ int64_t block_here() { return ((int64_t)blockIdx.z << kGridBits) + blockIdx.x; }
+inline dim3 grid_of(int64_t blocks, int64_t y = 1) {
+    const int64_t x = std::min(blocks, (int64_t)1 << kGridBits);
+    return dim3((unsigned)x, (unsigned)y, (unsigned)((blocks + x - 1) / x));
+}
+
 // What is larger than the last-level cache and read once comes past the caches' reuse order.
 constexpr int64_t LAST_LEVEL_CACHE = 256 << 20;
 template <class P> __device__ __forceinline__ P streamed(const P* from) {

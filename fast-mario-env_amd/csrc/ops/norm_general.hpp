@@ -57,9 +57,10 @@ template <class T, int V>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
     __shared__ float sm[NORM_THREADS][V], s2[NORM_THREADS][V], sn[NORM_THREADS];
     const MoNorm& a = k.a;
-    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int64_t at_block = block_here(), b = at_block / k.c.slabs, slab = at_block % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    if (b >= a.B) return;
     const int t = threadIdx.x, pl = t / k.c.LN;
-    float* part = k.part + (int64_t)blockIdx.x * 2 * a.C;
+    float* part = k.part + at_block * 2 * a.C;
     for (int c0 = 0; c0 < k.c.nv; c0 += k.c.LN) {
         const int cv = c0 + t % k.c.LN;
         const bool live = pl < k.c.PL && cv < k.c.nv;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
         }
         __syncthreads();
         const int cg = a.C / a.groups;                         // channels of one count: a mean of means
-        float* group = k.group + (int64_t)blockIdx.x * 2 * a.groups;
+        float* group = k.group + at_block * 2 * a.groups;
         for (int g = t / kWave; g < a.groups; g += NORM_THREADS / kWave) {
             float mean = 0.f, m2 = 0.f;
             for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) mean += sm[c / V][c % V];
@@ -135,8 +136,9 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_means(NormArgs k) {
     __shared__ Moments of[NORM_THREADS];
     const MoNorm& a = k.a;
-    const int64_t b = blockIdx.x / a.groups;
-    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups, t = threadIdx.x;
+    const int64_t bg = block_here(), b = bg / a.groups;
+    if (b >= a.B) return;
+    const int g = (int)(bg % a.groups), cg = a.C / a.groups, t = threadIdx.x;
     const int per = k.c.by_group ? 1 : cg, width = k.c.by_group ? a.groups : a.C;
     const float* from = (k.c.by_group ? k.group : k.part) + b * k.c.slabs * 2 * width + g * per;
     Moments m{0.f, 0.f, 0.f};
@@ -151,15 +153,16 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_means(NormArgs k) {
         if (t % (2 * s) == 0) of[t].join(of[t + s]);
     }
     if (t == 0) {
-        k.means[2 * blockIdx.x] = of[0].mean;
-        k.means[2 * blockIdx.x + 1] = 1.f / sqrtf(of[0].m2 / of[0].n + a.eps);
+        k.means[2 * bg] = of[0].mean;
+        k.means[2 * bg + 1] = 1.f / sqrtf(of[0].m2 / of[0].n + a.eps);
     }
 }
 
 template <class T, int V, int ACT>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_apply(NormArgs k) {
     const MoNorm& a = k.a;
-    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int64_t at_block = block_here(), b = at_block / k.c.slabs, slab = at_block % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    if (b >= a.B) return;
     const int t = threadIdx.x, pl = t / k.c.LN, cg = a.C / a.groups;
     if (pl >= k.c.PL) return;
     for (int cv = t % k.c.LN; cv < k.c.nv; cv += k.c.LN) {
@@ -187,9 +190,10 @@ template <class T, int V, int ACT>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(NormArgs k) {
     __shared__ float sw[NORM_THREADS][V], sb[NORM_THREADS][V];
     const MoNorm& a = k.a;
-    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int64_t at_block = block_here(), b = at_block / k.c.slabs, slab = at_block % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    if (b >= a.B) return;
     const int t = threadIdx.x, pl = t / k.c.LN, cg = a.C / a.groups;
-    float* part = k.part + (int64_t)blockIdx.x * 2 * a.C;
+    float* part = k.part + at_block * 2 * a.C;
     for (int c0 = 0; c0 < k.c.nv; c0 += k.c.LN) {
         const int cv = c0 + t % k.c.LN;
         const bool live = pl < k.c.PL && cv < k.c.nv;
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(NormArgs k) {
             }
         if (!k.c.by_group) continue;
         __syncthreads();
-        float* group = k.group + (int64_t)blockIdx.x * 2 * a.groups;
+        float* group = k.group + at_block * 2 * a.groups;
         for (int g = t / kWave; g < a.groups; g += NORM_THREADS / kWave) {
             float m1 = 0.f, m2 = 0.f;
             for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) {
@@ -257,8 +261,9 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_sums(NormArgs k) {
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_dmeans(NormArgs k) {
     __shared__ float s1[NORM_THREADS], s2[NORM_THREADS];
     const MoNorm& a = k.a;
-    const int64_t b = blockIdx.x / a.groups;
-    const int g = (int)(blockIdx.x % a.groups), cg = a.C / a.groups, t = threadIdx.x;
+    const int64_t bg = block_here(), b = bg / a.groups;
+    if (b >= a.B) return;
+    const int g = (int)(bg % a.groups), cg = a.C / a.groups, t = threadIdx.x;
     float m1 = 0.f, m2 = 0.f;
     if (k.c.by_group)
         for (int64_t slab = t; slab < k.c.slabs; slab += NORM_THREADS) {
@@ -282,15 +287,16 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_dmeans(NormArgs k) {
     }
     if (t == 0) {
         const float by = 1.f / ((float)a.S * (float)cg);
-        k.means[2 * blockIdx.x] = s1[0] * by;
-        k.means[2 * blockIdx.x + 1] = s2[0] * by;
+        k.means[2 * bg] = s1[0] * by;
+        k.means[2 * bg + 1] = s2[0] * by;
     }
 }
 
 template <class T, int V, int ACT>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_dx(NormArgs k) {
     const MoNorm& a = k.a;
-    const int64_t b = blockIdx.x / k.c.slabs, slab = blockIdx.x % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    const int64_t at_block = block_here(), b = at_block / k.c.slabs, slab = at_block % k.c.slabs, p0 = slab * k.c.px, p1 = min(p0 + k.c.px, a.S);
+    if (b >= a.B) return;
     const int t = threadIdx.x, pl = t / k.c.LN, cg = a.C / a.groups;
     if (pl >= k.c.PL) return;
     for (int cv = t % k.c.LN; cv < k.c.nv; cv += k.c.LN) {
@@ -402,7 +408,7 @@ template <class T, int V, int ACT> int norm_general(const MoNorm& a, bool backwa
     k.part = (float*)a.work;
     k.group = k.part + w.part;
     k.means = k.group + w.group;
-    const dim3 grid((unsigned)(a.B * k.c.slabs)), per_group((unsigned)(a.B * a.groups));
+    const dim3 grid = grid_of(a.B * k.c.slabs), per_group = grid_of(a.B * a.groups);
     if (!backward) {
         if (a.stats) k.means = a.stats;
         hipLaunchKernelGGL((k_norm_moments<T, V>), grid, dim3(NORM_THREADS), 0, s, k);

@@ -151,6 +151,7 @@ Tensor attend_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const T
     ok(mo_attend_step(dtype_of(q), q.size(0), (int)q.size(1), (int)q.size(2), (int)v.size(2), (float)scale, &rq, &rk, &rv, data(decay),
                       data<uint8_t>(start), data(state), &ro, stream_of(q)),
        "mo_attend_step");
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();   // (what saved it for a gradient notices)
     return out;
 }
 

@@ -264,6 +264,28 @@ def test_attention_many(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,E", [(4, 4), (5, 4)])
+def test_attention_more_heads_than_a_row_of_blocks(D, E):
+    check_attend(*attend_inputs(2, 2 ** 22 + 37, 1, D, E, torch.float32, starts=0.3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N", [(20000, 1), (4000, 300)])
+def test_attention_decays_near_one(T, N, dtype):
+    """Nothing is added, so the states decay by g^T and back: a rounding of a factor and of a product a chunk (of 32 steps at
+    least) and a segment, however near to one the factor is."""
+    q, k, v, _, _, state, do, ds = attend_inputs(T, N, 4, 16, 16, dtype, starts=None)
+    decay = torch.tensor([1 - 2.0 ** -20, 0.99999, 0.999, 1.0], device="cuda")
+    state.requires_grad_()
+    out, last = linear_attention(q, torch.zeros_like(k), v, decay, None, state)
+    (dstate,) = torch.autograd.grad((out, last), state, (torch.zeros_like(do), ds))
+    f = (decay.double() ** T)[:, None, None]
+    for got, want in ((last, f * state.double()), (dstate, f * ds.double())):
+        assert ((got.double() - want).abs() <= 2 * (T / 32 + 8) * 2.0 ** -24 * want.abs()).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_decays_zero_and_one(dtype):
     a = list(attend_inputs(150, 2, 4, 32, 32, dtype))
@@ -410,6 +432,30 @@ def test_step_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_step_more_heads_than_a_row_of_blocks():
+    N, D = 2 ** 24 + 5, 4
+    q, k, v = (torch.randn(N, 1, D, device="cuda") for _ in range(3))
+    state, decay = torch.randn(N, 1, D, D, device="cuda"), torch.tensor([0.5], device="cuda")
+    want = 0.5 * state.double() + k.double()[..., :, None] * v.double()[..., None, :]
+    out = linear_attention_step(q, k, v, decay, state)
+    assert ((state.double() - want).abs() <= 2.0 ** -22 * (1 + want.abs())).all()
+    assert ((out.double() - (q.double()[..., :, None] * want).sum(-2) / 2).abs() <= 2.0 ** -20 * (1 + (q[..., :, None].abs() * want.abs()).sum(-2))).all()
+
+
+@pytest.mark.gpu
+def test_step_tells_who_saved_its_state():
+    q = torch.randn(3, 2, 8, device="cuda")
+    w, state = torch.randn(3, 2, 8, 8, device="cuda", requires_grad=True), torch.randn(3, 2, 8, 8, device="cuda")
+    y = (w * state).sum()
+    with torch.no_grad():
+        linear_attention_step(q, q, q, head_decays(2), state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        linear_attention_step(q, q, q, head_decays(2), torch.zeros(3, 2, 8, 8, device="cuda"))
+
+
+@pytest.mark.gpu
 def test_attention_past_32_bits():
     """Steps 2^30 elements apart in one buffer: offsets past 2^31 elements and 2^32 bytes."""
     T, N, H, D = 3, 2, 2, 64
@@ -503,6 +549,12 @@ def test_norm_vs_float64(B, C, sp, groups, dtype):
     for act in ("none", "silu"):
         check_norm(x, groups, w, b, act, dy)
     check_norm(x, groups, None, None, "silu", dy)
+
+
+@pytest.mark.gpu
+def test_norm_more_samples_than_a_row_of_blocks():
+    x, w, b, dy = norm_inputs(2 ** 22 + 9, 6, (), torch.float32)
+    check_norm(x, 2, w, b, "silu", dy)
 
 
 @pytest.mark.gpu
