@@ -6,6 +6,7 @@
 #include "attend_step.hpp"
 #include "attend_walk.hpp"
 #include "common.hpp"
+#include "norm_rows.hpp"
 #include "norm_small.hpp"
 
 using namespace mo;
@@ -78,7 +79,9 @@ int norm_run(const MoNorm& a, bool backward, hipStream_t s) {
         return by_act(a.act, [&](auto act) {
             constexpr int A = decltype(act)::value;
             SmallCut c;
+            RowsCut r;
             if (norm_small_takes(a, backward, c)) return norm_small<T, A>(a, c, backward, s);
+            if (norm_rows_takes(a, r)) return norm_rows<T, A>(a, r, backward, s);
             return norm_wide(a) ? norm_general<T, 8, A>(a, backward, s) : norm_general<T, 1, A>(a, backward, s);
         });
     });
@@ -86,7 +89,9 @@ int norm_run(const MoNorm& a, bool backward, hipStream_t s) {
 
 int64_t norm_work(const MoNorm& a, bool backward) {
     SmallCut c;
+    RowsCut r;
     if (norm_small_takes(a, backward, c)) return 4 * norm_small_work(a, c, backward);
+    if (norm_rows_takes(a, r)) return 4 * norm_rows_work(a, r, backward);
     return 4 * norm_general_work(a, norm_cut(a, norm_wide(a) ? 8 : 1), backward).total;
 }
 

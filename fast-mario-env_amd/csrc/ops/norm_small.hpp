@@ -9,11 +9,11 @@ namespace mo {
 // t / NV, t / NV + TT / NV, .. (TT: the team's threads), so its channels, their weights and their gradients' sums stay its own. Sums over a group are
 // shuffles over the lanes that hold it, and one exchange through LDS where the team has several waves (MULTI). The variance is
 // that of the values in registers about their mean: exact also where the mean is large.
-// WHOLE: groups are whole packs; else a group is 1, 2 or 4 channels, and sums are kept by channel up to the last step.
+// NS: groups of a pack, each with sums of its own: 1 (a group is whole packs), 2, 4 or 8.
 struct Small {
     MoNorm a;
     int W, TT, nv, NV, log_nv; // waves and threads a team; packs a pixel, and rounded up
-    int cg, vpg;               // channels a group; packs a group (WHOLE)
+    int cg, vpg;               // channels a group; packs a group (at least 1)
     bool far;                  // rows (R = 1) of an x that fills the last-level cache come past it (262,144 x 512 bf16: gradient 186 ->
                                // 176 us); a smaller x may be there from its maker, and larger samples gain nothing
     float* part;               // (blocks, 2, C): the blocks' sums for dweight and dbias
@@ -45,15 +45,6 @@ __device__ __forceinline__ void group_sum(float (&s)[NS], const Small& k, float 
                 s[i] = t;
             }
         }
-    } else {                                               // neighbouring channels of a pack
-#pragma unroll
-        for (int m = 1; m < 4; m *= 2) {
-            float t[NS];
-#pragma unroll
-            for (int i = 0; i < NS; i++) t[i] = s[i] + s[i ^ m];
-#pragma unroll
-            for (int i = 0; i < NS; i++) s[i] = m < k.cg ? t[i] : s[i];
-        }
     }
     if (!MULTI) return;
     x += turn * SMALL_WAVES;
@@ -67,9 +58,9 @@ __device__ __forceinline__ void group_sum(float (&s)[NS], const Small& k, float 
         for (int i = 0; i < NS; i++) s[i] += x[j][lane][i];
 }
 
-template <class T, bool MULTI, int R, int ACT, bool WHOLE>
+template <class T, bool MULTI, int R, int ACT, int NS>
 __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
-    constexpr int NS = WHOLE ? 1 : 8;
+    constexpr int PER = 8 / NS;   // a pack's channels of one group
     typedef Pack<T, 8> P;
     __shared__ float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][NS];
     const MoNorm& a = k.a;
@@ -82,7 +73,7 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
         w[i] = live && a.weight ? a.weight[cv * 8 + i] : 1.f;
         s[i] = live && a.bias ? a.bias[cv * 8 + i] : 0.f;
     }
-    const float by = 1.f / ((float)a.S * (float)k.cg);
+    const float n = (float)a.S * (float)k.cg, by = 1.f / n;
     for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / TT); b < a.B; b += (int64_t)gridDim.x * teams) {
         const T* in = (const T*)a.x + b * a.S * a.C + cv * 8;
         P v[R];
@@ -97,17 +88,17 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
         for (int r = 0; r < R; r++)
             if (live && pl + r * PL < S)
 #pragma unroll
-                for (int i = 0; i < 8; i++) mean[i % NS] += as_f32(v[r].v[i]);
+                for (int i = 0; i < 8; i++) mean[i / PER] += as_f32(v[r].v[i]);
         group_sum<MULTI, NS, 1>(mean, k, x, 0);
 #pragma unroll
-        for (int i = 0; i < NS; i++) mean[i] *= by;
+        for (int i = 0; i < NS; i++) mean[i] /= n;            // (rounded once: equal values have no deviations)
 #pragma unroll
         for (int r = 0; r < R; r++)
             if (live && pl + r * PL < S)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float d = as_f32(v[r].v[i]) - mean[i % NS];
-                    var[i % NS] = fmaf(d, d, var[i % NS]);
+                    const float d = as_f32(v[r].v[i]) - mean[i / PER];
+                    var[i / PER] = fmaf(d, d, var[i / PER]);
                 }
         group_sum<MULTI, NS, 1>(var, k, x, 1);
         float rstd[NS];
@@ -116,8 +107,8 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
         if (a.stats && pl == 0 && live)
 #pragma unroll
             for (int i = 0; i < NS; i++)
-                if ((cv * 8 + i) % k.cg == 0) {
-                    float* to = a.stats + 2 * (b * a.groups + (cv * 8 + i) / k.cg);
+                if ((cv * 8 + i * PER) % k.cg == 0) {
+                    float* to = a.stats + 2 * (b * a.groups + (cv * 8 + i * PER) / k.cg);
                     to[0] = mean[i];
                     to[1] = rstd[i];
                 }
@@ -127,15 +118,15 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
             if (live && pl + r * PL < S) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    v[r].v[i] = as<T>(act<ACT>(fmaf((as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS], w[i], s[i])));
+                    v[r].v[i] = as<T>(act<ACT>(fmaf((as_f32(v[r].v[i]) - mean[i / PER]) * rstd[i / PER], w[i], s[i])));
                 stream((P*)(out + (int64_t)(pl + r * PL) * a.C), v[r]);
             }
     }
 }
 
-template <class T, bool MULTI, int R, int ACT, bool WHOLE>
-__global__ void __launch_bounds__(small_threads(MULTI), (WHOLE && sizeof(T) == 2 ? 4 : 2)) k_norm_small_back(Small k) {
-    constexpr int NS = WHOLE ? 1 : 8;
+template <class T, bool MULTI, int R, int ACT, int NS>
+__global__ void __launch_bounds__(small_threads(MULTI), (NS <= 2 && sizeof(T) == 2 ? 4 : 2)) k_norm_small_back(Small k) {
+    constexpr int PER = 8 / NS;   // a pack's channels of one group
     typedef Pack<T, 8> P;
     __shared__ union { float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][2 * NS]; float sums[MULTI ? SMALL_WAVES : 4][kWave][8]; } lds;
     const MoNorm& a = k.a;
@@ -163,7 +154,7 @@ __global__ void __launch_bounds__(small_threads(MULTI), (WHOLE && sizeof(T) == 2
         float mean[NS], rstd[NS], m[2 * NS] = {};          // m: the sums of dh, then those of dh h
 #pragma unroll
         for (int i = 0; i < NS; i++) {
-            const float* st = a.stats + 2 * (b * a.groups + (live ? (cv * 8 + i) / k.cg : 0));
+            const float* st = a.stats + 2 * (b * a.groups + (live ? (cv * 8 + i * PER) / k.cg : 0));
             mean[i] = st[0];
             rstd[i] = st[1];
         }
@@ -173,13 +164,13 @@ __global__ void __launch_bounds__(small_threads(MULTI), (WHOLE && sizeof(T) == 2
             if (live && pl + r * PL < S)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float h = (as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS];
+                    const float h = (as_f32(v[r].v[i]) - mean[i / PER]) * rstd[i / PER];
                     const float dz = as_f32(dy[r].v[i]) * act_grad<ACT>(fmaf(h, w[i], s[i]));
                     dw[i] = fmaf(dz, h, dw[i]);
                     db[i] += dz;
                     dh[r][i] = dz * w[i];
-                    m[i % NS] += dh[r][i];
-                    m[NS + i % NS] = fmaf(dh[r][i], h, m[NS + i % NS]);
+                    m[i / PER] += dh[r][i];
+                    m[NS + i / PER] = fmaf(dh[r][i], h, m[NS + i / PER]);
                 }
         group_sum<MULTI, 2 * NS, 2>(m, k, lds.x, turn);
         turn ^= 1;
@@ -190,8 +181,8 @@ __global__ void __launch_bounds__(small_threads(MULTI), (WHOLE && sizeof(T) == 2
             if (live && pl + r * PL < S) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float h = (as_f32(v[r].v[i]) - mean[i % NS]) * rstd[i % NS];
-                    v[r].v[i] = as<T>(rstd[i % NS] * (dh[r][i] - fmaf(h, m[NS + i % NS], m[i % NS])));
+                    const float h = (as_f32(v[r].v[i]) - mean[i / PER]) * rstd[i / PER];
+                    v[r].v[i] = as<T>(rstd[i / PER] * (dh[r][i] - fmaf(h, m[NS + i / PER], m[i / PER])));
                 }
                 stream((P*)((T*)a.dx + at + (int64_t)(pl + r * PL) * a.C), v[r]);
             }
@@ -242,13 +233,14 @@ inline bool norm_small_takes(const MoNorm& a, bool backward, SmallCut& c) {
 
 template <class T, bool MULTI, int R, int ACT> int norm_small_run(const Small& k, const SmallCut& c, bool backward, hipStream_t s) {
     const dim3 block(MULTI ? c.W * kWave : 256);
-    const auto go = [&](auto whole) {
-        constexpr bool G = decltype(whole)::value;
-        if (!backward) hipLaunchKernelGGL((k_norm_small<T, MULTI, R, ACT, G>), dim3(c.blocks), block, 0, s, k);
-        else if constexpr (R <= SMALL_PACKS_BACK) hipLaunchKernelGGL((k_norm_small_back<T, MULTI, R, ACT, G>), dim3(c.blocks), block, 0, s, k);
+    const auto go = [&](auto ns) {
+        constexpr int NS = decltype(ns)::value;
+        if (!backward) hipLaunchKernelGGL((k_norm_small<T, MULTI, R, ACT, NS>), dim3(c.blocks), block, 0, s, k);
+        else if constexpr (R <= SMALL_PACKS_BACK) hipLaunchKernelGGL((k_norm_small_back<T, MULTI, R, ACT, NS>), dim3(c.blocks), block, 0, s, k);
         return launched("k_norm_small");
     };
-    return k.cg % 8 == 0 ? go(std::true_type{}) : go(std::false_type{});
+    return k.cg % 8 == 0 ? go(std::integral_constant<int, 1>{}) : k.cg == 4 ? go(std::integral_constant<int, 2>{})
+         : k.cg == 2 ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 8>{});
 }
 
 template <class T, int ACT> int norm_small(const MoNorm& a, const SmallCut& c, bool backward, hipStream_t s) {

@@ -543,7 +543,8 @@ def test_operators_under_graph_capture():
     (1, 8, (), 1), (3, 512, (), 8), (70, 64, (), 1), (5, 512, (), 64), (200, 24, (), 3), (7, 64, (9, 9), 8), (9, 64, (7, 7), 64),
     (4, 32, (20, 20), 4), (3, 32, (20, 20), 8), (6, 16, (3, 3), 4), (2, 48, (84, 84), 6), (2, 96, (11, 5), 4), (3, 30, (5, 4), 5),
     (2, 24, (6, 6), 2), (1, 64, (130, 117), 4), (2, 3, (41, 41), 1), (2, 1, (9, 9), 1), (3, 1024, (4, 4), 32), (2, 2304, (2,), 3),
-    (300, 128, (3,), 2)])
+    (300, 128, (3,), 2), (700, 24, (), 2), (40000, 30, (), 10), (50, 1024, (), 8), (9, 2304, (), 3), (5, 2040, (), 2), (300, 96, (3, 3), 16),
+    (60, 12, (9, 9), 2), (5, 130, (2,), 10), (3000, 32, (9, 9), 16), (900, 32, (9, 9), 8), (20, 64, (20, 20), 32)])
 def test_norm_vs_float64(B, C, sp, groups, dtype):
     x, w, b, dy = norm_inputs(B, C, sp, dtype, seed=C)
     for act in ("none", "silu"):
@@ -567,7 +568,7 @@ def test_norm_relu_and_its_gradient():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,C,sp", [(3, 64, (9, 9)), (2, 64, (130, 117)), (4, 24, (6, 6))])
+@pytest.mark.parametrize("B,C,sp", [(3, 64, (9, 9)), (2, 64, (130, 117)), (4, 24, (6, 6)), (3, 48, (5, 5)), (30, 1200, ())])
 def test_norm_large_mean_and_constants(B, C, sp):
     x, w, b, dy = norm_inputs(B, C, sp, torch.float32, offset=3000.0)
     check_norm(x, 4, w, b, "silu", dy)
@@ -580,7 +581,7 @@ def test_norm_large_mean_and_constants(B, C, sp):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,C,sp", [(3, 64, (9, 9)), (40, 512, ()), (2, 64, (130, 117))])
+@pytest.mark.parametrize("B,C,sp", [(3, 64, (9, 9)), (40, 512, ()), (2, 64, (130, 117)), (3, 48, (5, 5)), (40, 1200, ()), (40, 48, ())])
 def test_norm_what_is_not_finite_stays_in_its_group(B, C, sp):
     x, w, b, dy = norm_inputs(B, C, sp, torch.bfloat16)
     clean = group_norm_act(x, 8, w, b, act="relu")
@@ -619,7 +620,8 @@ def test_norm_takes_views_and_other_types():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,C,sp,groups", [(2000, 64, (9, 9), 8), (20000, 512, (), 8), (2, 64, (130, 117), 4)])
+@pytest.mark.parametrize("B,C,sp,groups", [(2000, 64, (9, 9), 8), (20000, 512, (), 8), (2, 64, (130, 117), 4),
+                                             (20000, 24, (3, 3), 4), (9000, 1024, (), 8)])
 def test_norm_same_bits(B, C, sp, groups):
     x, w, b, dy = norm_inputs(B, C, sp, torch.bfloat16)
     x, w, b = (t.requires_grad_() for t in (x, w, b))
