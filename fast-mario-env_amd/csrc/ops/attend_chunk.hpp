@@ -11,7 +11,13 @@ namespace mo {
 // A workgroup takes one env's head and walks its chunks (or a cut of them) with S in registers: wave w holds the 16 columns
 // of S from 16 w, all rows, as accumulator tiles, which are the operand of Q S as they lie. Everything is read once and
 // written once; a chunk is three products over 32-step blocks of at most L x L x P, far below what the matrix cores do in the
-// time its rows take to come, so the pass is bound by memory as long as enough workgroups wait for it at once.
+// time its rows take to come, so the pass is bound by memory as long as enough workgroups wait for it at once: three fit a
+// compute unit (two of heads of 128).
+//
+// Measured, bf16, D = E = 64 and 8 heads, 128 steps of 4,096 envs: 723 us for 3.2 GB, 4.45 TB/s, where a copy of 1 GiB reaches 5.2.
+// (Step by step, k_walk: 4,889 us.) 1,000 envs with heads of 128: 335 us, 3.9 TB/s; the same with heads of 64 in float32: 286 us.
+// Where a step's rows lie a multiple of 2 MiB apart (N H D a power of two), a chunk's requests meet in the same memory channels:
+// storing the states for the gradient, 2,048 envs take 424 us, 2,056 take 341.
 //
 // T: element type. P: head size rounded up to 32, 64 or 128; columns past D or E are zeros. L: 64 for bf16; 32 for float32,
 // whose matrix instructions are 16 times slower, so that the products of a chunk with itself stay short.
@@ -137,7 +143,8 @@ template <int L> struct Powers {
 };
 
 // The env and head of a workgroup. Workgroups go to the 8 XCDs in turn; XCD_RUN neighbouring heads (whose rows of a step lie
-// together) go to one of them, so that what one L2 fetches lies together too.
+// together) go to one of them, so that what one L2 fetches lies together too. (256 steps of 2,000 envs, 8 heads of 32, bf16: 312 us,
+// 472 with one; 128 steps of 2,056 envs, 8 heads of 64: 256 and 267.)
 constexpr int XCD_RUN = 16;
 __device__ __forceinline__ int64_t head_of_block(int64_t heads) {
     const int64_t b = block_here(), round = 8 * XCD_RUN;
@@ -147,7 +154,8 @@ __device__ __forceinline__ int64_t head_of_block(int64_t heads) {
 
 // A long sequence is cut into segments of whole chunks, a workgroup each, so that few sequences fill the chip. First each
 // segment's own sum and what it leaves of an entering state (`keep`: g^steps, or -1 where an episode starts inside), then the
-// states that enter the segments one after another, then the outputs from there.
+// states that enter the segments one after another, then the outputs from there. (16,001 steps of 2 envs with 8 heads of 128, bf16: 45
+// us for the sums, 14 for the states between, 76 for the outputs; k and v are read twice.)
 struct Cut {
     int64_t chunks, per_seg;   // chunks of a sequence and of a segment
     int segs;
@@ -457,7 +465,8 @@ __global__ void __launch_bounds__(256) k_attend_enter(Enter k) {
 inline bool rows_suit(const MoRows& r, int64_t epv) {   // 16-byte accesses
     return (uintptr_t)r.p % 16 == 0 && r.st % epv == 0 && r.sn % epv == 0 && r.sh % epv == 0;
 }
-// The chunk kernels take heads of whole 16-byte pieces whose rows lie on them; the rest goes step by step (k_walk).
+// The chunk kernels take heads of whole 16-byte pieces whose rows lie on them; the rest goes step by step (k_walk; 128 steps of
+// 1,000 envs, 8 heads, bf16: heads of 40 by chunks 200 us, with the gradient 589; heads of 36 step by step 855 and 3,370).
 inline bool chunks_take(const MoAttend& a, bool backward) {
     const int64_t epv = a.dtype == MO_BF16 ? 8 : 4;
     if (a.T == 0 || a.D % epv || a.E % epv || !rows_suit(a.q, epv) || !rows_suit(a.k, epv) || !rows_suit(a.v, epv)) return false;

@@ -19,7 +19,7 @@ constexpr int STEP_ROWS = 16;   // rows of the state that a lane has in flight
 // S = (start ? 0 : g S) + k v^T and o = scale S^T q of one env and head in one wave. A lane holds V neighbouring columns, CG
 // lanes span the columns, and the 64 / CG lane groups take neighbouring rows, so that an access covers whole rows one after
 // another; q and k go to the lanes through LDS, and the groups' sums of o are joined by shuffles. The state is all there is to
-// move: 8 D E bytes. (32,768 envs, 8 heads of 64, bf16: 1,430 us, 6.0 TB/s; with a lane's rows together instead of an access's, and
+// move: 8 D E bytes, which bound it. (32,768 envs, 8 heads of 64, bf16: 1,440 us, 6.0 TB/s; with a lane's rows together instead of an access's, and
 // q and k straight from memory, 2,310 us.)
 // FAR: the states are more than the last-level cache holds, and go past it (1,523 us without); where they fit, the next step finds
 // them there (2,000 envs: 83 us, 93 going past it).

@@ -11,6 +11,9 @@ namespace mo {
 //   o:  X = S^T, u = v, w = k, z = q, forwards          dq: X = S,   u = k,  w = v, z = do, forwards
 //   dk: X = R,   u = q, w = do, z = v, backwards        dv: X = R^T, u = do, w = q, z = k,  backwards
 // with R_t = (start_{t+1} ? 0 : g R_{t+1}) + scale q_t do_t^T the gradient of S_t.
+// It takes what the chunk kernels do not: head sizes and strides that are not whole 16-byte pieces, no steps at all, and a gradient
+// without what the forward pass saved. Bound by the step after step: a lane's B products and sums wait for LDS reads of w and z that
+// all lanes share (128 steps of 1,000 envs, 8 heads of 36, bf16: 855 us, its gradient 2,500).
 struct Walk {
     MoRows u, w, z, y;
     const float* decay;

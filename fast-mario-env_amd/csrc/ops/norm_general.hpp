@@ -33,6 +33,9 @@ struct Moments {
     }
 };
 
+// For samples that do not fit a team's registers. Three passes: the slabs' moments (back: sums), their joining, and the results, so x
+// is read twice (back: x and dy), the second time from the last-level cache where it holds them. Measured, float32, 37 x 48 x 84 x 84 in 6
+// groups, in microseconds: moments and results 20 each, back sums 30 and results 25, joining 3 each, all bound by memory.
 // A sample is cut into slabs of `px` pixels; a block takes a slab. Its threads are LN lanes along the channels (V each) by
 // pixel lanes, so a thread's channels stay its own.
 struct NormCut {
@@ -357,7 +360,8 @@ __global__ void __launch_bounds__(SUM_COLS * SUM_LANES) k_norm_colsum(const floa
 
 constexpr int NORM_SUM_ROWS = 64;   // rows that the first round of column sums leaves
 
-// rows of (2, C) sums -> dweight, dbias, in two rounds where a block would go through many rows; `spare` holds NORM_SUM_ROWS rows.
+// rows of (2, C) sums -> dweight, dbias, in two rounds where a block would go through many rows (200,000 of 60 columns: 310 us less
+// of a gradient than in one; 1,024 rows of 1,024 columns: 8 us more); `spare` holds NORM_SUM_ROWS rows.
 inline int norm_colsum(const MoNorm& a, const float* rows_of, int64_t rows, float* spare, hipStream_t s) {
     const int cols = 2 * a.C;
     const unsigned blocks = (unsigned)((cols + SUM_COLS - 1) / SUM_COLS);
@@ -377,11 +381,12 @@ inline bool norm_wide(const MoNorm& a) {   // 8 channels an access (of 16 bytes,
     return a.C % 8 == 0 && p % 16 == 0;
 }
 
-// Slabs: enough blocks for the chip where samples are few, and at least 16 KB of a sample in each.
+// Slabs: enough blocks for the chip where samples are few, and at least 16 KB of a sample in each. (37 x 48 x 84 x 84 float32, forward and
+// gradient: 96 us with up to 1,024 blocks, 105 with 2,048, 119 with 4,096; 500 x 32 x 84 x 84 bf16 366, 366 and 374.)
 inline NormCut norm_cut(const MoNorm& a, int V) {
     NormCut c;
     const int64_t per_px = (int64_t)a.C * (a.dtype == MO_BF16 ? 2 : 4);
-    const int64_t most = std::max<int64_t>(1, a.S * per_px / (16 << 10)), want = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, a.B));
+    const int64_t most = std::max<int64_t>(1, a.S * per_px / (16 << 10)), want = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, a.B));
     c.px = (a.S + std::min(most, want) - 1) / std::min(most, want);
     c.slabs = (a.S + c.px - 1) / c.px;
     c.nv = a.C / V;

@@ -99,7 +99,7 @@ template <class T> __device__ __forceinline__ Frag<T> unit_frag(unsigned half, u
 }
 
 // The parts of w B, w a factor for each index, that keep float32's precision in products with bf16 operands: bf16 parts of 8 bits
-// of significand each, three of which leave 2^-27 of it.
+// of significand each, three of which leave at most 2^-26 of it.
 __device__ __forceinline__ void scaled_parts(const Frag<bf16>& b, const float* w, Frag<bf16>* part) {
     union { uint4 u; Frag<bf16> f; } in{};
     in.f = b;

@@ -2,10 +2,10 @@
 group norm with an activation, against their definitions in float64 written out here.
 
 Tolerances. float32: with a the same sums over absolute values, a result of n terms is within about n 2^-24 a of the exact
-one; N_TERMS covers the terms, the decay's powers and the joining of chunks. bf16 results carry three roundings to 8 bits of
-significand, each at most 2^-9 of what it rounds: that of a masked product, that of the state that meets q (the two act on parts of
-one sum), and the result's own. So a bf16 result is within 3 * 2^-9 of the exact one in norm and, element by element, within
-3 * 2^-9 of the sum of absolute values."""
+one; (T + D + E + 16) 2^-23 covers the terms, the decay's powers and the joining of chunks. bf16 results carry three roundings to 8
+bits of significand: that of a masked product, that of the state that meets q (the two act on parts of one sum), and the
+result's own. A rounding is off by at most 2^-8 of its value and by 2^-9 or less for most values, so three of them seldom reach 3 *
+2^-9, which is asked for in norm and, element by element, of the sum of absolute values: tighter than the worst case."""
 
 import ctypes
 import os
