@@ -14,8 +14,9 @@ namespace mo {
 // time its rows take to come, so the pass is bound by memory as long as enough workgroups wait for it at once: three fit a
 // compute unit (two of heads of 128).
 //
-// Measured, bf16, D = E = 64 and 8 heads, 128 steps of 4,096 envs: 723 us for 3.2 GB, 4.45 TB/s, where a copy of 1 GiB reaches 5.2.
-// (Step by step, k_walk: 4,889 us.) 1,000 envs with heads of 128: 335 us, 3.9 TB/s; the same with heads of 64 in float32: 286 us.
+// Measured, bf16, D = E = 64 and 8 heads, 128 steps of 4,096 envs: 730 us for 3.2 GB, 4.4 TB/s, where a copy of 1 GiB reaches 5.2.
+// (Step by step, k_walk: 4,889 us.) From zeros, 2,056 envs: 257 us, 5.2 TB/s; 1,000 envs with heads of 128: 337 us, 4.7 TB/s; with
+// heads of 64 135 us, in float32 292.
 // Where a step's rows lie a multiple of 2 MiB apart (N H D a power of two), a chunk's requests meet in the same memory channels:
 // storing the states for the gradient, 2,048 envs take 424 us, 2,056 take 341.
 //
@@ -154,8 +155,8 @@ __device__ __forceinline__ int64_t head_of_block(int64_t heads) {
 
 // A long sequence is cut into segments of whole chunks, a workgroup each, so that few sequences fill the chip. First each
 // segment's own sum and what it leaves of an entering state (`keep`: g^steps, or -1 where an episode starts inside), then the
-// states that enter the segments one after another, then the outputs from there. (16,001 steps of 2 envs with 8 heads of 128, bf16: 45
-// us for the sums, 14 for the states between, 76 for the outputs; k and v are read twice.)
+// states that enter the segments one after another, then the outputs from there. (16,001 steps of 2 envs with 8 heads of 128, bf16: 50
+// us for the sums, 16 for the states between, 85 for the outputs under the profiler, 126 in all without; k and v are read twice.)
 struct Cut {
     int64_t chunks, per_seg;   // chunks of a sequence and of a segment
     int segs;

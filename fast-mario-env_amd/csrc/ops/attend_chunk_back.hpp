@@ -15,10 +15,10 @@ namespace mo {
 // 16-byte pieces straight into operands.
 //
 // Bound by memory: 4 rows are read and 3 written a step and head. Measured, bf16, 128 steps of 2,056 envs with 8 heads of 64: 705 us, 4.0
-// TB/s (860 us at 2,048 envs, whose steps' rows lie a multiple of 2 MiB apart). Heads of 128, 1,000 envs: 750 us, 3.2 TB/s: the
+// TB/s (860 us at 2,048 envs, whose steps' rows lie a multiple of 2 MiB apart). Heads of 128, 1,000 envs: 713 us, 2.9 TB/s: the
 // tiles leave room for one workgroup a compute unit, whose loads wait while it multiplies. float32 holds half the steps in as much
-// LDS and its matrix instructions take 16 times as long: 97 steps of 64 envs with 8 heads of 64, 34 us. Step by step (k_walk, three walks):
-// 128 steps of 2,048 envs with the forward pass 10,277 us, 1,284 by chunks.
+// LDS and its matrix instructions take 16 times as long: the 1,000 envs with heads of 64 take 712 us, in bf16 252. Step by step (k_walk, three walks):
+// 128 steps of 2,048 envs with the forward pass 10,277 us, 1,290 by chunks.
 template <class T, int P> using BackChunk = Chunk<T, P, P / 16>;
 template <class T, int P> struct BackLds {
     typedef BackChunk<T, P> C;

@@ -35,7 +35,7 @@ struct Moments {
 
 // For samples that do not fit a team's registers. Three passes: the slabs' moments (back: sums), their joining, and the results, so x
 // is read twice (back: x and dy), the second time from the last-level cache where it holds them. Measured, float32, 37 x 48 x 84 x 84 in 6
-// groups, in microseconds: moments and results 20 each, back sums 30 and results 25, joining 3 each, all bound by memory.
+// groups, in microseconds: moments and results 20 each, back sums 25 and results 31, joining 5 each, all bound by memory.
 // A sample is cut into slabs of `px` pixels; a block takes a slab. Its threads are LN lanes along the channels (V each) by
 // pixel lanes, so a thread's channels stay its own.
 struct NormCut {
@@ -382,7 +382,7 @@ inline bool norm_wide(const MoNorm& a) {   // 8 channels an access (of 16 bytes,
 }
 
 // Slabs: enough blocks for the chip where samples are few, and at least 16 KB of a sample in each. (37 x 48 x 84 x 84 float32, forward and
-// gradient: 96 us with up to 1,024 blocks, 105 with 2,048, 119 with 4,096; 500 x 32 x 84 x 84 bf16 366, 366 and 374.)
+// gradient: 97 us with up to 1,024 blocks, 105 with 2,048, 119 with 4,096; 500 x 32 x 84 x 84 bf16 366, 366 and 374.)
 inline NormCut norm_cut(const MoNorm& a, int V) {
     NormCut c;
     const int64_t per_px = (int64_t)a.C * (a.dtype == MO_BF16 ? 2 : 4);

@@ -11,7 +11,7 @@ namespace mo {
 // where the team has several waves (MULTI). The variance is that of the values in registers about their mean: exact also where
 // the mean is large. NS: groups of a pack, each with sums of its own: 1 (a group is whole packs), 2, 4 or 8.
 // Bound by memory, a value read and one written (back: two and one). Measured, bf16, in microseconds: 4,096 x 32 x 20 x 20 in 4 groups 38
-// (5.6 TB/s, partly out of the last-level cache), 104 through norm_general; 262,144 x 512 in 8 groups back 176 (4.6 TB/s); 4,096 x
+// (5.6 TB/s, partly out of the last-level cache), 104 through norm_general; 262,144 x 512 in 8 groups 120 (4.5 TB/s), back 176 (4.6); 4,096 x
 // 64 x 9 x 9 in 8 groups forward 21, back 33; groups of one channel need eight sums a pack and more registers: 16,384 x 32 x 9 x 9
 // forward and back 340 in 32 groups, 99 in 8, 91 in 4.
 struct Small {
