@@ -13,7 +13,7 @@ namespace mo {
 // Bound by memory, a value read and one written (back: two and one). Measured, bf16, in microseconds: 4,096 x 32 x 20 x 20 in 4 groups 38
 // (5.6 TB/s, partly out of the last-level cache), 104 through norm_general; 262,144 x 512 in 8 groups 120 (4.5 TB/s), back 176 (4.6); 4,096 x
 // 64 x 9 x 9 in 8 groups forward 21, back 33; groups of one channel need eight sums a pack and more registers: 16,384 x 32 x 9 x 9
-// forward and back 340 in 32 groups, 99 in 8, 91 in 4.
+// forward and back 212 in 32 groups, 100 in 8, 91 in 4. (LDS by the team's waves: room for eight waves in each block made the 212 340.)
 struct Small {
     MoNorm a;
     int W, TT, nv, NV, log_nv; // waves and threads a team; packs a pixel, and rounded up
@@ -51,7 +51,7 @@ __device__ __forceinline__ void group_sum(float (&s)[NS], const Small& k, float 
         }
     }
     if (!MULTI) return;
-    x += turn * SMALL_WAVES;
+    x += turn * k.W;
 #pragma unroll
     for (int i = 0; i < NS; i++) x[threadIdx.x / kWave][lane][i] = s[i];
     __syncthreads();
@@ -62,11 +62,17 @@ __device__ __forceinline__ void group_sum(float (&s)[NS], const Small& k, float 
         for (int i = 0; i < NS; i++) s[i] += x[j][lane][i];
 }
 
+extern __shared__ __align__(16) float small_lds[];       // MULTI: two exchanges by wave; going back, then the waves' sums for dweight
+inline unsigned small_lds_bytes(bool multi, int waves, int NS, bool backward) {
+    const int exchange = multi ? 2 * waves * kWave * NS * (backward ? 2 : 1) : 0;
+    return 4 * (unsigned)std::max(exchange, backward ? waves * kWave * 8 : 0);
+}
+
 template <class T, bool MULTI, int R, int ACT, int NS>
 __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
     constexpr int PER = 8 / NS;   // a pack's channels of one group
     typedef Pack<T, 8> P;
-    __shared__ float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][NS];
+    float (*x)[kWave][NS] = (float (*)[kWave][NS])small_lds;
     const MoNorm& a = k.a;
     const int TT = k.TT, teams = MULTI ? 1 : 256 / TT;
     const int t = threadIdx.x & (TT - 1), cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
@@ -132,7 +138,7 @@ template <class T, bool MULTI, int R, int ACT, int NS>
 __global__ void __launch_bounds__(small_threads(MULTI), (NS <= 2 && sizeof(T) == 2 ? 4 : 2)) k_norm_small_back(Small k) {
     constexpr int PER = 8 / NS;   // a pack's channels of one group
     typedef Pack<T, 8> P;
-    __shared__ union { float x[MULTI ? 2 * SMALL_WAVES : 1][kWave][2 * NS]; float sums[MULTI ? SMALL_WAVES : 4][kWave][8]; } lds;
+    float (*x)[kWave][2 * NS] = (float (*)[kWave][2 * NS])small_lds, (*sums)[kWave][8] = (float (*)[kWave][8])small_lds;
     const MoNorm& a = k.a;
     const int TT = k.TT, teams = MULTI ? 1 : 256 / TT, waves = MULTI ? k.W : 4;
     const int t = threadIdx.x & (TT - 1), cv = t & (k.NV - 1), pl = t >> k.log_nv, PL = TT >> k.log_nv, S = (int)a.S;
@@ -176,7 +182,7 @@ __global__ void __launch_bounds__(small_threads(MULTI), (NS <= 2 && sizeof(T) ==
                     m[i / PER] += dh[r][i];
                     m[NS + i / PER] = fmaf(dh[r][i], h, m[NS + i / PER]);
                 }
-        group_sum<MULTI, 2 * NS, 2>(m, k, lds.x, turn);
+        group_sum<MULTI, 2 * NS, 2>(m, k, x, turn);
         turn ^= 1;
 #pragma unroll
         for (int i = 0; i < 2 * NS; i++) m[i] *= by;
@@ -203,11 +209,11 @@ __global__ void __launch_bounds__(small_threads(MULTI), (NS <= 2 && sizeof(T) ==
         __syncthreads();
         if (threadIdx.x % kWave < k.NV)
 #pragma unroll
-            for (int i = 0; i < 8; i++) lds.sums[threadIdx.x / kWave][threadIdx.x % kWave][i] = half ? db[i] : dw[i];
+            for (int i = 0; i < 8; i++) sums[threadIdx.x / kWave][threadIdx.x % kWave][i] = half ? db[i] : dw[i];
         __syncthreads();
         for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
             float sum = 0.f;
-            for (int j = 0; j < waves; j++) sum += lds.sums[j][c / 8][c % 8];
+            for (int j = 0; j < waves; j++) sum += sums[j][c / 8][c % 8];
             k.part[((int64_t)blockIdx.x * 2 + half) * a.C + c] = sum;
         }
     }
@@ -239,8 +245,9 @@ template <class T, bool MULTI, int R, int ACT> int norm_small_run(const Small& k
     const dim3 block(MULTI ? c.W * kWave : 256);
     const auto go = [&](auto ns) {
         constexpr int NS = decltype(ns)::value;
-        if (!backward) hipLaunchKernelGGL((k_norm_small<T, MULTI, R, ACT, NS>), dim3(c.blocks), block, 0, s, k);
-        else if constexpr (R <= SMALL_PACKS_BACK) hipLaunchKernelGGL((k_norm_small_back<T, MULTI, R, ACT, NS>), dim3(c.blocks), block, 0, s, k);
+        const unsigned lds = small_lds_bytes(MULTI, MULTI ? c.W : 4, NS, backward);
+        if (!backward) hipLaunchKernelGGL((k_norm_small<T, MULTI, R, ACT, NS>), dim3(c.blocks), block, lds, s, k);
+        else if constexpr (R <= SMALL_PACKS_BACK) hipLaunchKernelGGL((k_norm_small_back<T, MULTI, R, ACT, NS>), dim3(c.blocks), block, lds, s, k);
         return launched("k_norm_small");
     };
     return k.cg % 8 == 0 ? go(std::integral_constant<int, 1>{}) : k.cg == 4 ? go(std::integral_constant<int, 2>{})
