@@ -166,8 +166,8 @@ struct Cut {
 
 enum { KEEP_NONE = 0, KEEP_STATES = 1, ONLY_SUMS = 2 };
 
-// MODE: KEEP_STATES leaves the states that enter chunks 1, 2, .. for the gradient in a.saved, (N H, chunks - 1, P, P) in the
-// elements' type: there they are operands only. ONLY_SUMS makes a segment's own sum.
+// MODE: KEEP_STATES leaves the states that enter chunks 1, 2, .. for the gradient in a.saved, (N H, chunks - 1, P, P) in float32.
+// ONLY_SUMS makes a segment's own sum.
 // A wave's 16 columns (from x0) of a head's float32 (D, E) matrix, or of its transpose, to and from accumulator tiles. Of the
 // transpose a lane has four neighbours, moved together (E is a multiple of 4).
 struct alignas(4) Four { float v[4]; };
@@ -287,16 +287,14 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
             };
             if (m) scores(std::true_type{});
             else scores(std::false_type{});
-            if (MODE == KEEP_STATES && c > 0) {                // by rows d, a lane four neighbouring columns
-                T* to = (T*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + i16 * P + e0 + 4 * g;
+            if (MODE == KEEP_STATES && c > 0) {                // (copied as they lie: what is not finite stays in its row and column)
+                float* to = (float*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + e0 + i16;
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                    for (int t = 0; t < C::PT; t++) {
-                        f32x4 x = zero;
-                        mma(x, frag_of<T>(S[ct][t & ~1], S[ct][t | 1]), unit_frag<T>(t & 1, lane));
-                        *(Pack<T, 4>*)(to + t * 16 * P + ct * 16) = pack4(x, T{});
-                    }
+                    for (int t = 0; t < C::PT; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) to[acc_row(t, g, r) * P + ct * 16] = S[ct][t][r];
             }
             __syncthreads();
         }
@@ -489,7 +487,7 @@ inline Cut attend_cut(const MoAttend& a) {
 }
 inline int64_t saved_bytes(const MoAttend& a) {
     const int64_t p = padded_head(a);
-    return a.N * a.H * ((a.T + chunk_steps(a) - 1) / chunk_steps(a) - 1) * p * p * (a.dtype == MO_BF16 ? 2 : 4);
+    return a.N * a.H * ((a.T + chunk_steps(a) - 1) / chunk_steps(a) - 1) * p * p * 4;
 }
 inline int64_t cut_bytes(const MoAttend& a, const Cut& c) {
     return c.segs > 1 ? (int64_t)c.segs * a.N * a.H * (4 * (int64_t)a.D * a.E + 4) : 0;

@@ -113,11 +113,12 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
         {
             const int d = x0 + i16;
             if (c > 0) {
-                const T* kept = (const T*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + d * P + 8 * g;
+                const float* kept = (const float*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + d * P + 8 * g;
 #pragma unroll
-                for (int b = 0; b < C::PB; b++)
-#pragma unroll
-                    for (int j = 0; j < 8; j += C::Rows::EPV) *(uint4*)((T*)&sf[b] + j) = *(const uint4*)(kept + b * 32 + j);
+                for (int b = 0; b < C::PB; b++) {
+                    const f32x4* x = (const f32x4*)(kept + b * 32);
+                    sf[b] = frag_of<T>(x[0], x[1]);
+                }
             } else {
 #pragma unroll
                 for (int b = 0; b < C::PB; b++)

@@ -89,15 +89,6 @@ template <class T> __device__ __forceinline__ Frag<T> frag_of(const f32x4& a, co
     return u.f;
 }
 
-// B's operand of a product that gives columns 16 half .. 16 half + 15 of A's 32 indices back: A's rows by lanes become its
-// columns by lanes, exactly.
-template <class T> __device__ __forceinline__ Frag<T> unit_frag(unsigned half, unsigned lane) {
-    Frag<T> f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) f.v[i] = as<T>(8 * (lane / 16) + i == 16 * half + lane % 16 ? 1.f : 0.f);
-    return f;
-}
-
 // The parts of w B, w a factor for each index, that keep float32's precision in products with bf16 operands: bf16 parts of 8 bits
 // of significand each, three of which leave at most 2^-26 of it.
 __device__ __forceinline__ void scaled_parts(const Frag<bf16>& b, const float* w, Frag<bf16>* part) {
