@@ -9,7 +9,8 @@ namespace mo {
 //   O  = scale ((Q K^T . G) V + diag(g^(i+1), 0 past the first start) Q S)
 //   S' = (no start in the chunk ? g^n : 0) S + K^T diag(w) V,   w_j = g^(n-1-j), 0 before the last start
 // A workgroup takes one env's head and walks its chunks (or a cut of them) with S in registers: wave w holds the 16 columns
-// of S from 16 w, all rows, as accumulator tiles, which are the operand of Q S as they lie. Everything is read once and
+// of S from 16 w, all rows, as accumulator tiles, which are the operand of Q S as they lie. S and the masked scores go into products in
+// two parts (halves, in tiles.hpp), S' is made from w V in three (scaled_parts). Everything is read once and
 // written once; a chunk is three products over 32-step blocks of at most L x L x P, far below what the matrix cores do in the
 // time its rows take to come, so the pass is bound by memory as long as enough workgroups wait for it at once: three fit a
 // compute unit (two of heads of 128).
@@ -30,7 +31,8 @@ template <class T, int P, int W> struct Chunk {
     static constexpr int CT = P / 16 / W;                     // 16-column tiles of S of a wave
     static constexpr int LT = L / 16, LB = L / 32, PB = P / 32, PT = P / 16;
     typedef Tile<T, P> Rows;          // a chunk of q, k, v, ..
-    typedef Tile<T, L> Scores;
+    typedef ScoreParts<T, L> Scored;
+    static constexpr int SCORES = kHalves<T> * Scores<T, L>::SIZE, K = kHalves<T>;
     static constexpr int STEP = NT / Rows::PIECES, RV = L / STEP;   // rows that the workgroup moves at a time, and times
     static constexpr int TILES = LT == 4 ? 12 : 4;            // score tiles up to the diagonal's 32-blocks
     static constexpr int TPW = (TILES + W - 1) / W;           // a wave's
@@ -218,14 +220,14 @@ template <class T, int P, int MODE>
 __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P>)) k_attend(MoAttend a, Cut cut) {
     typedef Chunk<T, P, kForwardWaves<P>> C;
     typedef HeadRows<T, C> Head;
-    constexpr int L = C::L, CT = C::CT;
+    constexpr int L = C::L, CT = C::CT, K = C::K;
     constexpr bool OUT = MODE != ONLY_SUMS;
-    __shared__ __align__(16) T lk[L * P], lv[L * P], lq[OUT ? L * P : 8], lp[OUT ? L * L : 8], ly[OUT ? L * P : 8];
+    __shared__ __align__(16) T lk[L * P], lv[L * P], lq[OUT ? L * P : 8], lp[OUT ? C::SCORES : 8], ly[OUT ? L * P : 8];
     __shared__ Powers<L> pw;
     __shared__ __align__(16) float wt[L];
     __shared__ float rt[OUT ? L : 1];   // what a step has of the entering state: scale g^(i+1), or 0
     const typename C::Rows sk{lk}, sv{lv}, sq{lq}, sy{ly};
-    const typename C::Scores sp{lp};
+    const typename C::Scored sp(lp);
     const int w = threadIdx.x / kWave;
     const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
     if (nh >= a.N * a.H) return;
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
                     const float* f = pw.sees(i, j);
 #pragma unroll
                     for (int r = 0; r < 4; r++) s[r] = !starts || j + r >= from ? s[r] * f[-r] : 0.f;
-                    *(Pack<T, 4>*)sp.at(i, j) = pack4(s, T{});
+                    sp.put(i, j, s);
                 }
             };
             if (m) scores(std::true_type{});
@@ -317,11 +319,11 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
             };
             float all = 0.f;
             {
-                Frag<T> sf[CT][C::PB];
+                Frag<T> sf[CT][C::PB][K];
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                    for (int b = 0; b < C::PB; b++) sf[ct][b] = frag_of<T>(S[ct][2 * b], S[ct][2 * b + 1]);
+                    for (int b = 0; b < C::PB; b++) halves<T>(S[ct][2 * b], S[ct][2 * b + 1], sf[ct][b]);
 #pragma unroll
                 for (int it = 0; it < C::LT; it++) {
                     f32x4 own[CT], far[CT];
@@ -331,14 +333,18 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
                     for (int b = 0; b < C::PB; b++) {
                         const Frag<T> x = sq.along(it * 16, b * 32, lane);
 #pragma unroll
-                        for (int ct = 0; ct < CT; ct++) mma(far[ct], sf[ct][b], x);
+                        for (int p = 0; p < K; p++)
+#pragma unroll
+                            for (int ct = 0; ct < CT; ct++) mma(far[ct], sf[ct][b][p], x);
                     }
 #pragma unroll
-                    for (int b = 0; b <= it / 2; b++) {
-                        const Frag<T> x = sp.along(it * 16, b * 32, lane);
+                    for (int b = 0; b <= it / 2; b++)
 #pragma unroll
-                        for (int ct = 0; ct < CT; ct++) mma(own[ct], vf[ct][b], x);
-                    }
+                        for (int p = 0; p < K; p++) {
+                            const Frag<T> x = sp.part[p].along(it * 16, b * 32, lane);
+#pragma unroll
+                            for (int ct = 0; ct < CT; ct++) mma(own[ct], vf[ct][b], x);
+                        }
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++) {
                         watch(all, own[ct]);
@@ -354,12 +360,18 @@ __global__ void __launch_bounds__((kForwardWaves<P> * kWave), (kForwardPerSimd<P
                         const int i = it * 16 + i16;
                         f32x4 own = zero, far = zero;
 #pragma unroll
-                        for (int b = 0; b < C::PB; b++) mma(far, frag_of<T>(S[ct][2 * b], S[ct][2 * b + 1]), sq.along(it * 16, b * 32, lane));
+                        for (int b = 0; b < C::PB; b++) {
+                            Frag<T> sf[K];
+                            halves<T>(S[ct][2 * b], S[ct][2 * b + 1], sf);
+                            const Frag<T> x = sq.along(it * 16, b * 32, lane);
+#pragma unroll
+                            for (int p = 0; p < K; p++) mma(far, sf[p], x);
+                        }
 #pragma unroll 1
                         for (int j = max(seen_from(m, i), 0); j <= i; j++)
 #pragma unroll
                             for (int r = 0; r < 4; r++)
-                                own[r] = fmaf(as_f32(*sp.at(i, j)), as_f32(*sv.at(j, e0 + 16 * ct + 4 * g + r)), own[r]);
+                                own[r] = fmaf(sp.get(i, j), as_f32(*sv.at(j, e0 + 16 * ct + 4 * g + r)), own[r]);
                         write(it, ct, own, far);
                     }
             }

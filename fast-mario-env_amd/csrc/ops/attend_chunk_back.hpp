@@ -12,7 +12,8 @@ namespace mo {
 //   R' = (no start in the chunk ? g^n : 0) R + Q^T diag(u) dO,   u_i = scale g^(i+1), 0 past the first start
 // q, k, v and dO are read once for all of them. Wave w holds the 16 rows of R from 16 w, as the accumulator tiles of R^T, which
 // are the operand of V R^T as they lie; K R takes R from LDS. S comes from the forward pass (a.saved), each wave its rows, in
-// 16-byte pieces straight into operands.
+// 16-byte pieces. A, B, R and S go into products in two parts each (halves, in tiles.hpp); to leave LDS room for two workgroups of heads of
+// 64 a compute unit, B waits in registers until A is done with, and dV until R is.
 //
 // Bound by memory: 4 rows are read and 3 written a step and head. Measured, bf16, 128 steps of 2,056 envs with 8 heads of 64: 705 us, 4.0
 // TB/s (860 us at 2,048 envs, whose steps' rows lie a multiple of 2 MiB apart). Heads of 128, 1,000 envs: 713 us, 2.9 TB/s: the
@@ -24,14 +25,14 @@ template <class T, int P> struct BackLds {
     typedef BackChunk<T, P> C;
     static constexpr int L = C::L, ROWS = L * P;
     T q[ROWS], k[ROWS], v[ROWS], o[ROWS];        // o: dO
-    T a[L * L], b[L * L], y[ROWS];               // y: dV
-    T r[P * P > ROWS ? P * P : ROWS];
+    T x[C::SCORES];                              // A, then B
+    T r[C::K * P * P > 3 * ROWS ? C::K * P * P : 3 * ROWS];
     float wt[L], ut[L];
     Powers<L> pw;
-    // Once dV is there, A and R's tile make room for dQ and dK.
-    __device__ __forceinline__ T* dq() { return r; }
-    __device__ __forceinline__ T* dk() { return P <= L ? a : r + ROWS; }
-    static_assert(P <= L || P * P >= 2 * ROWS, "");
+    // Once dV is made, R's tiles have room for the results.
+    __device__ __forceinline__ T* dv() { return r; }
+    __device__ __forceinline__ T* dq() { return r + ROWS; }
+    __device__ __forceinline__ T* dk() { return r + 2 * ROWS; }
 };
 
 // The sum over a chunk's steps of Q^T diag(u) dO, as R^T's tiles of the wave's columns from x0.
@@ -71,11 +72,11 @@ template <class T, int P>
 __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAttend a, Cut cut) {
     typedef BackChunk<T, P> C;
     typedef HeadRows<T, C> Head;
-    constexpr int L = C::L;
+    constexpr int L = C::L, K = C::K;
     extern __shared__ __align__(16) char lds[];
     BackLds<T, P>& s = *(BackLds<T, P>*)lds;
-    const typename C::Rows sq{s.q}, sk{s.k}, sv{s.v}, so{s.o}, sr{s.r};
-    const typename C::Scores sa{s.a}, sb{s.b};
+    const typename C::Rows sq{s.q}, sk{s.k}, sv{s.v}, so{s.o};
+    const typename C::Scored sx(s.x);
     const int w = threadIdx.x / kWave;
     const int64_t nh = head_of_block(a.N * a.H), env = nh / a.H;
     if (nh >= a.N * a.H) return;
@@ -105,30 +106,9 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
             const int n1 = (int)min((int64_t)L, a.T - t0 - L);
             dq.take(s.dq(), t0 + L, n1);
             dk.take(s.dk(), t0 + L, n1);
-            dv.take(s.y, t0 + L, n1);
+            dv.take(s.dv(), t0 + L, n1);
         }
         const unsigned lane = thread_here() % kWave, g = lane / 16, i16 = lane % 16;
-        // the state that enters the chunk: rows d of the wave, eight neighbouring columns e a lane
-        Frag<T> sf[C::PB];
-        {
-            const int d = x0 + i16;
-            if (c > 0) {
-                const float* kept = (const float*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + d * P + 8 * g;
-#pragma unroll
-                for (int b = 0; b < C::PB; b++) {
-                    const f32x4* x = (const f32x4*)(kept + b * 32);
-                    sf[b] = frag_of<T>(x[0], x[1]);
-                }
-            } else {
-#pragma unroll
-                for (int b = 0; b < C::PB; b++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int e = b * 32 + 8 * g + j;
-                        sf[b].v[j] = as<T>(a.state && d < a.D && e < a.E ? a.state[nh * de + d * a.E + e] : 0.f);
-                    }
-            }
-        }
         const uint64_t m = __ballot(start_of_lane(a, t0, n, env) != 0);
         const int last = seen_from(m, L - 1);
         if (threadIdx.x < L) {
@@ -140,10 +120,15 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
 
 #pragma unroll
         for (int b = 0; b < C::PB; b++) {                      // R by rows d, for K R
-            const Frag<T> x = frag_of<T>(R[2 * b], R[2 * b + 1]);
+            Frag<T> x[K];
+            halves<T>(R[2 * b], R[2 * b + 1], x);
 #pragma unroll
-            for (int j = 0; j < 8; j += C::Rows::EPV) *(uint4*)sr.at(x0 + i16, b * 32 + 8 * g + j) = *(const uint4*)((const T*)&x + j);
+            for (int p = 0; p < K; p++)
+#pragma unroll
+                for (int j = 0; j < 8; j += C::Rows::EPV)
+                    *(uint4*)typename C::Rows{s.r + p * P * P}.at(x0 + i16, b * 32 + 8 * g + j) = *(const uint4*)((const T*)&x[p] + j);
         }
+        f32x4 bs[C::TPW];                                      // B, until A is done with
         const auto scores = [&](auto starts) {                 // A and B, a lane four neighbouring j of one i
 #pragma unroll
             for (int z = 0; z < C::TPW; z++) {
@@ -165,25 +150,24 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
                     x[r] = sees ? x[r] * f[-r] : 0.f;
                     y[r] = sees ? y[r] * f[-r] : 0.f;
                 }
-                *(Pack<T, 4>*)sa.at(i, j) = pack4(x, T{});
-                *(Pack<T, 4>*)sb.at(i, j) = pack4(y, T{});
+                sx.put(i, j, x);
+                bs[z] = y;
             }
         };
         if (m) scores(std::true_type{});
         else scores(std::false_type{});
         __syncthreads();
 
-        // A result, transposed: a lane has four neighbouring columns of one step. own_of: the sum over the chunk's steps, x its
-        // scores and y its rows; far_of: what the entering state or its gradient adds, by a factor a step.
-        const auto result = [&](T* to, const float* factor, auto far_of, auto own_of, const typename C::Scores& x, bool down, const typename C::Rows& y) {
-            const typename C::Rows tile{to};
+        // A result, transposed: a lane has four neighbouring columns of one step. own_of: the sum over the chunk's steps, the
+        // scores times y's rows; far_of: what the entering state or its gradient adds, by a factor a step.
+        const auto result = [&](auto put, const float* factor, auto far_of, auto own_of, bool down, const typename C::Rows& y) {
             const auto write = [&](int t, const f32x4& own, const f32x4& far) {
                 const float f = factor[t * 16 + i16];
                 f32x4 z;
 #pragma unroll
                 for (int r = 0; r < 4; r++) z[r] = fmaf(f, far[r], own[r]);
                 if (m && f == 0.f) z = own;                    // (what is not seen may be anything)
-                *(Pack<T, 4>*)tile.at(t * 16 + i16, x0 + 4 * g) = pack4(z, T{});
+                put(t, pack4(z, T{}));
             };
             float all = 0.f;
 #pragma unroll
@@ -200,64 +184,108 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
 #pragma unroll 1
                 for (int j = j0; j <= j1 && (!down || seen_from(m, j) <= i); j++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        own[r] = fmaf(as_f32(down ? *x.at(j, i) : *x.at(i, j)), as_f32(*y.at(j, x0 + 4 * g + r)), own[r]);
+                    for (int r = 0; r < 4; r++) own[r] = fmaf(down ? sx.get(j, i) : sx.get(i, j), as_f32(*y.at(j, x0 + 4 * g + r)), own[r]);
                 write(t, own, far_of(t));
             }
         };
+        const auto to_tile = [&](T* tile) {
+            return [=](int t, const Pack<T, 4>& z) { *(Pack<T, 4>*)typename C::Rows{tile}.at(t * 16 + i16, x0 + 4 * g) = z; };
+        };
+        const auto far_by = [&](const Frag<T> (&x)[C::PB][K], const typename C::Rows& rows) {
+            return [&](int t) {
+                f32x4 far = zero;
+#pragma unroll
+                for (int b = 0; b < C::PB; b++) {
+                    const Frag<T> y = rows.along(t * 16, b * 32, lane);
+#pragma unroll
+                    for (int p = 0; p < K; p++) mma(far, x[b][p], y);
+                }
+                return far;
+            };
+        };
+        const auto own_down = [&](const Frag<T> (&x)[C::LB]) { // over the steps from t's on
+            return [&](int t) {
+                f32x4 own = zero;
+#pragma unroll
+                for (int b = t / 2; b < C::LB; b++)
+#pragma unroll
+                    for (int p = 0; p < K; p++) mma(own, x[b], sx.part[p].down(b * 32, t * 16, lane));
+                return own;
+            };
+        };
 
+        // the state that enters the chunk: rows d of the wave, eight neighbouring columns e a lane (asked for here, used
+        // after dV)
+        f32x4 S[C::PB][2];
         {
-            Frag<T> of[C::LB], rf[C::PB];
+            const int d = x0 + i16;
+            if (c > 0) {
+                const float* kept = (const float*)a.saved + (nh * (cut.chunks - 1) + c - 1) * (P * P) + d * P + 8 * g;
+#pragma unroll
+                for (int b = 0; b < C::PB; b++) {
+                    S[b][0] = *(const f32x4*)(kept + b * 32);
+                    S[b][1] = *(const f32x4*)(kept + b * 32 + 4);
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < C::PB; b++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int e = b * 32 + 8 * g + j;
+                        S[b][j / 4][j % 4] = a.state && d < a.D && e < a.E ? a.state[nh * de + d * a.E + e] : 0.f;
+                    }
+            }
+        }
+
+        Pack<T, 4> held[C::LT];                                // dV, until R's tiles are done with
+        {
+            Frag<T> of[C::LB], rf[C::PB][K];
 #pragma unroll
             for (int b = 0; b < C::LB; b++) of[b] = so.down(b * 32, x0, lane);
 #pragma unroll
-            for (int b = 0; b < C::PB; b++) rf[b] = sr.down(b * 32, x0, lane);
-            result(s.y, s.wt, [&](int t) {
-                f32x4 far = zero;
+            for (int b = 0; b < C::PB; b++)
 #pragma unroll
-                for (int b = 0; b < C::PB; b++) mma(far, rf[b], sk.along(t * 16, b * 32, lane));
-                return far;
-            }, [&](int t) {
-                f32x4 own = zero;
+                for (int p = 0; p < K; p++) rf[b][p] = typename C::Rows{s.r + p * P * P}.down(b * 32, x0, lane);
+            result([&](int t, const Pack<T, 4>& z) {
 #pragma unroll
-                for (int b = t / 2; b < C::LB; b++) mma(own, of[b], sa.down(b * 32, t * 16, lane));
-                return own;
-            }, sa, true, so);
+                for (int u = 0; u < C::LT; u++)
+                    if (u == t) held[u] = z;
+            }, s.wt, far_by(rf, sk), own_down(of), true, so);
         }
-        __syncthreads();                                       // A and R's tile are done with
+        __syncthreads();                                       // A and R's tiles are done with
+#pragma unroll
+        for (int t = 0; t < C::LT; t++) to_tile(s.dv())(t, held[t]);
+#pragma unroll
+        for (int z = 0; z < C::TPW; z++) {
+            const int idx = w + z * C::WAVES;
+            if (C::TILES % C::WAVES && idx >= C::TILES) break;
+            int it, jt;
+            C::score_tile(idx, it, jt);
+            sx.put(it * 16 + i16, jt * 16 + 4 * g, bs[z]);
+        }
+        __syncthreads();
         {
-            Frag<T> kf[C::LB];
+            Frag<T> kf[C::LB], sf[C::PB][K];
 #pragma unroll
             for (int b = 0; b < C::LB; b++) kf[b] = sk.down(b * 32, x0, lane);
-            result(s.dq(), s.ut, [&](int t) {
-                f32x4 far = zero;
 #pragma unroll
-                for (int b = 0; b < C::PB; b++) mma(far, sf[b], so.along(t * 16, b * 32, lane));
-                return far;
-            }, [&](int t) {
+            for (int b = 0; b < C::PB; b++) halves<T>(S[b][0], S[b][1], sf[b]);
+            result(to_tile(s.dq()), s.ut, far_by(sf, so), [&](int t) {
                 f32x4 own = zero;
 #pragma unroll
-                for (int b = 0; b <= t / 2; b++) mma(own, kf[b], sb.along(t * 16, b * 32, lane));
+                for (int b = 0; b <= t / 2; b++)
+#pragma unroll
+                    for (int p = 0; p < K; p++) mma(own, kf[b], sx.part[p].along(t * 16, b * 32, lane));
                 return own;
-            }, sb, false, sk);
+            }, false, sk);
         }
         {
-            Frag<T> qf[C::LB], rf[C::PB];
+            Frag<T> qf[C::LB], rf[C::PB][K];
 #pragma unroll
             for (int b = 0; b < C::LB; b++) qf[b] = sq.down(b * 32, x0, lane);
 #pragma unroll
-            for (int b = 0; b < C::PB; b++) rf[b] = frag_of<T>(R[2 * b], R[2 * b + 1]);
-            result(s.dk(), s.wt, [&](int t) {
-                f32x4 far = zero;
-#pragma unroll
-                for (int b = 0; b < C::PB; b++) mma(far, rf[b], sv.along(t * 16, b * 32, lane));
-                return far;
-            }, [&](int t) {
-                f32x4 own = zero;
-#pragma unroll
-                for (int b = t / 2; b < C::LB; b++) mma(own, qf[b], sb.down(b * 32, t * 16, lane));
-                return own;
-            }, sb, true, sq);
+            for (int b = 0; b < C::PB; b++) halves<T>(R[2 * b], R[2 * b + 1], rf[b]);
+            result(to_tile(s.dk()), s.wt, far_by(rf, sv), own_down(qf), true, sq);
         }
 
         f32x4 add[C::PT];                                      // R'
@@ -273,7 +301,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT), 2) k_attend_back(MoAtte
         const int n = (int)min((int64_t)L, a.T - c0 * L);
         dq.take(s.dq(), c0 * L, n);
         dk.take(s.dk(), c0 * L, n);
-        dv.take(s.y, c0 * L, n);
+        dv.take(s.dv(), c0 * L, n);
     }
     if (a.dstate && cut.segs == 1) store_state<P, true>(a, a.dstate + nh * de, x0, R);
 }

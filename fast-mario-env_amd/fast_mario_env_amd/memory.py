@@ -87,8 +87,8 @@ def linear_attention(q, k, v, decay, start=None, state=None, scale=None):
     float32 or None for zeros; scale: 1/sqrt(D) if None. Returns out (T, N, H, E) in the type of q and the state after the last
     step, float32. Differentiable once in q, k, v and state.
 
-    Sums and states are float32. With bf16 inputs the masked products of a chunk and the state that multiplies q are rounded to
-    bf16 where they enter a matrix product; the state itself is not."""
+    Sums and states are float32, those kept for the gradient among them. With bf16 inputs what enters a matrix product from another
+    one or from a state goes in as two bf16 parts (2^-16 of it is left out), so results are rounded once, at their end."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("linear_attention: q, k and v must be (T, N, H, head size)")
     _check_attend("linear_attention", "T, N", q, k, v, decay, start, state)
