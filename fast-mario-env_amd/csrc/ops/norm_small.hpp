@@ -8,8 +8,8 @@ namespace mo {
 // and goes on to its next sample. A thread has the packs cv = t % NV (NV: packs a pixel, rounded up to a power of two; threads of
 // packs that are not there idle) of the pixels t / NV, t / NV + TT / NV, .. (TT: the team's threads), so its channels, their weights
 // and their gradients' sums stay its own. Sums over a group are shuffles over the lanes that hold it, and one exchange through LDS
-// where the team has several waves (MULTI). The variance is that of the values in registers about their mean: exact also where
-// the mean is large. NS: groups of a pack, each with sums of its own: 1 (a group is whole packs), 2, 4 or 8.
+// where the team has several waves (MULTI). The mean's sum goes about the group's first value, and the variance is that of the
+// values in registers about their mean: a large mean costs neither digits, and equal values have no deviations. NS: groups of a pack, each with sums of its own: 1 (a group is whole packs), 2, 4 or 8.
 // Bound by memory, a value read and one written (back: two and one). Measured, bf16, in microseconds: 4,096 x 32 x 20 x 20 in 4 groups 38
 // (5.6 TB/s, partly out of the last-level cache), 104 through norm_general; 262,144 x 512 in 8 groups 120 (4.5 TB/s), back 176 (4.6); 4,096 x
 // 64 x 9 x 9 in 8 groups forward 21, back 33; groups of one channel need eight sums a pack and more registers: 16,384 x 32 x 9 x 9
@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
         s[i] = live && a.bias ? a.bias[cv * 8 + i] : 0.f;
     }
     const float n = (float)a.S * (float)k.cg, by = 1.f / n;
+    const int first = cv - cv % k.vpg;                         // the pack that the thread's group begins in
     for (int64_t b = (int64_t)blockIdx.x * teams + (MULTI ? 0 : threadIdx.x / TT); b < a.B; b += (int64_t)gridDim.x * teams) {
         const T* in = (const T*)a.x + b * a.S * a.C + cv * 8;
         P v[R];
@@ -93,15 +94,19 @@ __global__ void __launch_bounds__(small_threads(MULTI)) k_norm_small(Small k) {
                 const P* p = (const P*)(in + (int64_t)(pl + r * PL) * a.C);
                 v[r] = R == 1 && k.far ? streamed(p) : *p;
             }
-        float mean[NS] = {}, var[NS] = {};
+        float mean[NS] = {}, var[NS] = {}, x0[NS];             // x0: each group's first value, from the lane that holds it or from memory
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+            x0[i] = !MULTI ? __shfl(as_f32(v[0].v[i * PER]), (threadIdx.x & (kWave - TT)) + first)
+                    : live ? as_f32(((const T*)a.x)[b * a.S * a.C + first * 8 + i * PER]) : 0.f;
 #pragma unroll
         for (int r = 0; r < R; r++)
             if (live && pl + r * PL < S)
 #pragma unroll
-                for (int i = 0; i < 8; i++) mean[i / PER] += as_f32(v[r].v[i]);
+                for (int i = 0; i < 8; i++) mean[i / PER] += as_f32(v[r].v[i]) - x0[i / PER];
         group_sum<MULTI, NS, 1>(mean, k, x, 0);
 #pragma unroll
-        for (int i = 0; i < NS; i++) mean[i] /= n;            // (rounded once: equal values have no deviations)
+        for (int i = 0; i < NS; i++) mean[i] = x0[i] + mean[i] / n;
 #pragma unroll
         for (int r = 0; r < R; r++)
             if (live && pl + r * PL < S)

@@ -122,3 +122,59 @@ def test_attention_what_is_not_finite_stays_in_its_column(dtype):
     want = attend64(q.detach().float(), torch.where(torch.isinf(k), 0.0, k.detach().float()), v.detach(), decay, None, state, D ** -0.5, do, ds)[2]
     assert torch.isfinite(dq[..., good]).all() and not torch.isfinite(dq[5:, ..., 7]).any()
     assert torch.allclose(dq[..., good].double(), want[..., good], rtol=2e-2, atol=2e-2)
+
+
+# ---------------------------------------------------------------- group norm
+PATHS = [(5, 64, (9, 9), 8), (5, 512, (), 8), (4, 32, (20, 20), 4), (3, 64, (9, 9), 64), (3, 64, (9, 9), 32), (3, 64, (9, 9), 16), (5, 24, (), 1),
+         (3, 96, (11, 5), 4), (4, 24, (6, 6), 4), (6, 30, (5, 4), 5), (5, 1200, (), 4), (2, 64, (130, 117), 4), (2, 2304, (2,), 3), (2, 48, (84, 84), 6)]   # samples in registers of a wave and of several, groups in a wave, slabs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,C,sp,groups", PATHS)
+def test_norm_of_a_constant_is_the_bias(B, C, sp, groups):
+    """Sums go about a value of the group, so equal values, of any size, have no deviation at all: h is 0, and dx and dweight are
+    what h = 0 makes of them."""
+    x, w, b, dy = norm_inputs(B, C, sp, torch.float32)
+    w.requires_grad_()
+    for value in (3.3, -1000.1, 3000.1, 7e-7):
+        flat = torch.full_like(x, value).requires_grad_()
+        y = group_norm_act(flat, groups, w, b)
+        assert torch.equal(y, b.view(1, -1, *(1,) * len(sp)).expand_as(y)), value
+        dx, dw = torch.autograd.grad(y, (flat, w), dy)
+        assert (dw == 0).all(), value
+        d = (dy * w.detach().view(1, -1, *(1,) * len(sp))).double().reshape(B, groups, -1)
+        want = (d - d.mean(-1, keepdim=True)).reshape(x.shape) / 1e-5 ** 0.5
+        assert (dx.double() - want).norm() <= 2.0 ** -20 * want.norm(), value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,C,sp,groups", PATHS)
+def test_norm_of_a_large_mean(B, C, sp, groups):
+    """About a mean of 3,000 deviations: h is off by two ulp of the mean (its rounding where it is stored, and its sum's), times rstd, and by a
+    few 2^-24 of itself; silu's slope is below 1.1 and changes by 0.5 at most, and dx and dw follow h by their formulas."""
+    x, w, b, dy = norm_inputs(B, C, sp, torch.float32)
+    x = (x + 3000.0).requires_grad_()
+    w, b = w.requires_grad_(), b.requires_grad_()
+    y = group_norm_act(x, groups, w, b, act="silu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    want = norm64(x.detach(), groups, w.detach(), b.detach(), 1e-5, "silu", dy)
+    x3 = x.detach().double().reshape(B, groups, -1)
+    mean, r = x3.mean(-1), 1.0 / (x3.var(-1, unbiased=False) + 1e-5).sqrt()
+    shift = (2 * 2.0 ** -23 * mean.abs() * r).max().item()
+    few, big = 64 * 2.0 ** -24, w.detach().abs().max().item()
+    assert (y.detach().double() - want[0]).abs().max() <= 1.1 * big * shift + few * (1 + want[0].abs().max())
+    # dx = r (dh - mean dh - h mean(dh h)): dh changes by 0.5 w^2 |dy| shift, the last term by 3 shift of dh's size
+    assert (dx.double() - want[1]).norm() <= (0.5 * big ** 2 + 3 * big + few / shift) * shift * r.max() * 1.1 * dy.double().norm()
+    to_c = lambda t: t.double().abs().sum([0, *range(2, t.dim())])   # noqa: E731
+    assert ((dw.double() - want[2]).abs() <= (1.1 + 0.5 * big * 6) * shift * to_c(dy) + few * 6 * to_c(dy)).all()
+    assert ((db.double() - want[3]).abs() <= 0.5 * big * shift * to_c(dy) + few * to_c(dy)).all()
+
+
+@pytest.mark.gpu
+def test_norm_does_not_go_by_alignment():
+    """The same values off a 16-byte boundary take another kernel, and give the same norm of a large mean."""
+    x, w, b, _ = norm_inputs(5, 64, (9, 9), torch.float32, offset=3000.0)
+    off = torch.empty(x.numel() + 1, device="cuda")[1:].view(5, 9, 9, 64).permute(0, 3, 1, 2)
+    off.copy_(x)
+    d = group_norm_act(x, 8, w, b).double() - group_norm_act(off, 8, w, b).double()
+    assert d.abs().max() <= 4 * 2.0 ** -23 * 3000.0 * 1.6
