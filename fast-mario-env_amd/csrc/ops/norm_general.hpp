@@ -115,13 +115,14 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
             continue;
         }
         __syncthreads();
-        const int cg = a.C / a.groups;                         // channels of one count: a mean of means
+        const int cg = a.C / a.groups;                         // channels of one count: a mean of means, about the first
         float* group = k.group + at_block * 2 * a.groups;
         for (int g = t / kWave; g < a.groups; g += NORM_THREADS / kWave) {
+            const float m0 = sm[g * cg / V][g * cg % V];
             float mean = 0.f, m2 = 0.f;
-            for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) mean += sm[c / V][c % V];
+            for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) mean += sm[c / V][c % V] - m0;
             for (int s = 1; s < kWave; s *= 2) mean += __shfl_xor(mean, s);
-            mean /= (float)cg;
+            mean = m0 + mean / (float)cg;
             for (int c = g * cg + t % kWave; c < (g + 1) * cg; c += kWave) {
                 const float d = sm[c / V][c % V] - mean;
                 m2 += s2[c / V][c % V] + sn[0] * d * d;

@@ -126,7 +126,8 @@ def test_attention_what_is_not_finite_stays_in_its_column(dtype):
 
 # ---------------------------------------------------------------- group norm
 PATHS = [(5, 64, (9, 9), 8), (5, 512, (), 8), (4, 32, (20, 20), 4), (3, 64, (9, 9), 64), (3, 64, (9, 9), 32), (3, 64, (9, 9), 16), (5, 24, (), 1),
-         (3, 96, (11, 5), 4), (4, 24, (6, 6), 4), (6, 30, (5, 4), 5), (5, 1200, (), 4), (2, 64, (130, 117), 4), (2, 2304, (2,), 3), (2, 48, (84, 84), 6)]   # samples in registers of a wave and of several, groups in a wave, slabs
+         (3, 96, (11, 5), 4), (4, 24, (6, 6), 4), (6, 30, (5, 4), 5), (5, 1200, (), 4), (2, 64, (130, 117), 4), (2, 2304, (2,), 3), (2, 48, (84, 84), 6),
+         (2, 56, (60, 50), 2), (2, 21, (90, 70), 3)]   # samples in registers of a wave and of several, groups in a wave, slabs
 
 
 @pytest.mark.gpu
