@@ -54,8 +54,11 @@ struct NormArgs {
 
 constexpr int NORM_THREADS = 256;
 
-// Each channel's (or group's) mean and squared deviations over a slab. A thread sums about its first value, and the threads' sets are
-// joined as moments, so neither a large mean nor a far value costs digits.
+// Each channel's (or group's) mean and squared deviations over a slab. A thread sums runs of NORM_RUN values about their first, and
+// the runs' and the threads' sets are joined as moments. A run's sum of squares about one of its n values is at most n times that
+// about its mean, so a far value costs a run n roundings at most, and a large mean none. (About a thread's first value of all, one that
+// is far off took a thousandth of the variance along.)
+constexpr int NORM_RUN = 16;
 template <class T, int V>
 __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
     __shared__ float sm[NORM_THREADS][V], s2[NORM_THREADS][V], sn[NORM_THREADS];
@@ -67,27 +70,34 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_moments(NormArgs k) {
     for (int c0 = 0; c0 < k.c.nv; c0 += k.c.LN) {
         const int cv = c0 + t % k.c.LN;
         const bool live = pl < k.c.PL && cv < k.c.nv;
-        float about[V] = {}, sum[V] = {}, sq[V] = {}, n = 0.f;
+        float mean[V] = {}, m2[V] = {}, n = 0.f;
         if (live)
-            for (int64_t p = p0 + pl; p < p1; p += k.c.PL) {
-                const Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + (b * a.S + p) * a.C + cv * V);
+            for (int64_t p = p0 + pl; p < p1;) {
+                float about[V], sum[V] = {}, sq[V] = {}, run = 0.f;
+#pragma unroll 4
+                for (int j = 0; j < NORM_RUN && p < p1; j++, p += k.c.PL, run += 1.f) {
+                    const Pack<T, V> x = *(const Pack<T, V>*)((const T*)a.x + (b * a.S + p) * a.C + cv * V);
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        if (j == 0) about[i] = as_f32(x.v[i]);
+                        const float d = as_f32(x.v[i]) - about[i];
+                        sum[i] += d;
+                        sq[i] = fmaf(d, d, sq[i]);
+                    }
+                }
+                n += run;
+                const float r = 1.f / run, w = run / n, both = (n - run) * w;
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    if (n == 0.f) about[i] = as_f32(x.v[i]);
-                    const float d = as_f32(x.v[i]) - about[i];
-                    sum[i] += d;
-                    sq[i] = fmaf(d, d, sq[i]);
+                    const float e = sum[i] * r, here = about[i] + e;
+                    const float d = n == run ? 0.f : here - mean[i];
+                    mean[i] = n == run ? here : fmaf(d, w, mean[i]);
+                    m2[i] += fmaxf(fmaf(-e, sum[i], sq[i]), 0.f) + (sq[i] - sq[i]) + d * d * both;   // (what is not finite stays so)
                 }
-                n += 1.f;
             }
         __syncthreads();
-        const float r = n > 0.f ? 1.f / n : 0.f;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const float d = sum[i] * r;
-            sm[t][i] = about[i] + d;
-            s2[t][i] = fmaxf(fmaf(-d, sum[i], sq[i]), 0.f) + (sq[i] - sq[i]);   // (what is not finite stays so)
-        }
+        for (int i = 0; i < V; i++) { sm[t][i] = mean[i]; s2[t][i] = m2[i]; }
         sn[t] = n;
         for (int m = 1; m < k.c.PL; m *= 2) {                  // pixel lanes j and j + m
             __syncthreads();
