@@ -24,8 +24,9 @@ template <int ACT> __device__ __forceinline__ float act_grad(float z) {
 struct Moments {
     float n, mean, m2;
     __device__ __forceinline__ void join(const Moments& o) {
+        if (o.n == 0.f) return;
+        if (n == 0.f) { *this = o; return; }   // (the square of a large mean is infinite, and times no values a NaN)
         const float t = n + o.n;
-        if (t == 0.f) return;
         const float d = o.mean - mean, w = o.n / t;
         mean = fmaf(d, w, mean);
         m2 = m2 + o.m2 + d * d * n * w;

@@ -137,7 +137,7 @@ def test_norm_of_a_constant_is_the_bias(B, C, sp, groups):
     what h = 0 makes of them."""
     x, w, b, dy = norm_inputs(B, C, sp, torch.float32)
     w.requires_grad_()
-    for value in (3.3, -1000.1, 3000.1, 7e-7):
+    for value in (3.3, -1000.1, 3000.1, 7e-7, 3e30):
         flat = torch.full_like(x, value).requires_grad_()
         y = group_norm_act(flat, groups, w, b)
         assert torch.equal(y, b.view(1, -1, *(1,) * len(sp)).expand_as(y)), value
