@@ -175,10 +175,12 @@ MoNorm norm_args(const Tensor& rows, int64_t groups, const Tensor& weight, const
     return a;
 }
 
+// The result has the channels second and rows' memory order without being a view of another tensor: a view that an autograd
+// function returns may not be changed in place.
 Tensor norm_forward(const Tensor& rows, int64_t groups, const Tensor& weight, const Tensor& bias, double eps, int64_t act, Tensor* stats) {
     const c10::DeviceGuard guard(rows.device());
     MoNorm a = norm_args(rows, groups, weight, bias, eps, act);
-    const Tensor y = at::empty_like(rows);
+    const Tensor second = channels_second(rows), y = at::empty_strided(second.sizes(), second.strides(), rows.options());
     if (stats) *stats = at::empty({a.B, groups, 2}, rows.options().dtype(at::kFloat));
     a.y = y.data_ptr();
     a.stats = stats ? data(*stats) : nullptr;
@@ -198,7 +200,7 @@ struct Norm : torch::autograd::Function<Norm> {
         ctx->saved_data["groups"] = groups;
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["act"] = act;
-        return channels_second(y);
+        return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list s = ctx->get_saved_variables();
@@ -230,7 +232,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const Maybe& weight_, con
         bias = bias_->to(at::kFloat).contiguous();
     }
     if (wants_grad({x, weight, bias})) return Norm::apply(x, groups, maybe(weight), maybe(bias), eps, act);
-    return channels_second(norm_forward(channels_last(x), groups, weight, bias, eps, act, nullptr));
+    return norm_forward(channels_last(x), groups, weight, bias, eps, act, nullptr);
 }
 
 }  // namespace

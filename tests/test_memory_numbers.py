@@ -199,3 +199,24 @@ def test_norm_of_a_far_first_value(rows, far):
         # the rest, far below the standard deviation, is compared as itself: rstd's error shows on all values alike
         limit = 128 * 2.0 ** -24 * want[0].abs().reshape(8, -1) + shift[:, None] + 8 * 2.0 ** -24 * want[0].abs().reshape(8, -1).max(-1, keepdim=True).values / 64
         assert (d.abs() <= limit).all(), (d.abs() / limit).max().item()
+
+
+# ---------------------------------------------------------------- as a program uses them
+@pytest.mark.gpu
+@pytest.mark.parametrize("sp", [(), (3,), (9, 9)])
+def test_outputs_may_be_changed_in_place(sp):
+    """What follows a norm may add to its result or clamp it in place, as it may with torch's own, and the gradient is the same."""
+    x, w, b, dy = norm_inputs(6, 32, sp, torch.float32)
+    r = torch.randn_like(x)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad((group_norm_act(x, 4, w, b, act="silu") * 2 + r).clamp(min=0), leaves, dy)
+    y = group_norm_act(x, 4, w, b, act="silu")
+    y *= 2
+    y += r
+    y.clamp_(min=0)
+    assert all(torch.equal(a, e) for a, e in zip(torch.autograd.grad(y, leaves, dy), want))
+    q, k, v, decay, start, state, do, _ = attend_inputs(7, 2, 2, 16, 16, torch.float32)
+    (dq,) = torch.autograd.grad(linear_attention(q.requires_grad_(), k, v, decay, start, state)[0] * 2, q, do)
+    out = linear_attention(q, k, v, decay, start, state)[0]
+    out *= 2
+    assert torch.equal(torch.autograd.grad(out, q, do)[0], dq)
