@@ -220,3 +220,21 @@ def test_outputs_may_be_changed_in_place(sp):
     out = linear_attention(q, k, v, decay, start, state)[0]
     out *= 2
     assert torch.equal(torch.autograd.grad(out, q, do)[0], dq)
+
+
+def test_build_needs_the_operators_last(monkeypatch):
+    """Where the operators cannot be built (no C++ compiler or torch headers), the emulator and the oracle are built all the same, and
+    build() says what failed."""
+    import __graft_entry__ as entry
+    import build_native
+    import build_ops
+    done = []
+    monkeypatch.setattr(build_native, "build", lambda *a, **k: done.append("emulator"))
+    monkeypatch.setattr(entry.subprocess, "run", lambda *a, **k: done.append("oracle"))
+
+    def fails(*a, **k):
+        raise RuntimeError("no compiler")
+    monkeypatch.setattr(build_ops, "build", fails)
+    with pytest.raises(RuntimeError, match="no compiler"):
+        entry.build()
+    assert done == ["emulator", "oracle"]
