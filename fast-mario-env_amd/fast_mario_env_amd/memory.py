@@ -200,7 +200,7 @@ def make_memory_net(n_actions: int = N_ACTIONS, in_ch: int = 4, heads: int = 8, 
         def _features(self, obs_u8):
             """uint8 (B, k, 84, 84) -> the projected features and q, k, v of each, (B, 512) and (B, heads, D)."""
             if obs_u8.is_cuda:
-                x = torch.empty(obs_u8.shape, dtype=torch.bfloat16, device=obs_u8.device).to(memory_format=torch.channels_last)
+                x = torch.empty(obs_u8.shape, dtype=torch.bfloat16, device=obs_u8.device, memory_format=torch.channels_last)
                 policy_input(obs_u8.contiguous(), x)
             else:
                 x = obs_u8.float().mul_(1.0 / 255.0)

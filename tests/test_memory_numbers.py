@@ -222,6 +222,21 @@ def test_outputs_may_be_changed_in_place(sp):
     assert torch.equal(torch.autograd.grad(out, q, do)[0], dq)
 
 
+@pytest.mark.gpu
+def test_memory_net_makes_its_input_once(monkeypatch):
+    """The scaled observations take one buffer: nothing that is not there yet is copied."""
+    net = memory.make_memory_net()
+    obs = torch.zeros(256, 4, 84, 84, dtype=torch.uint8, device="cuda")
+    state, peak = net.initial_state(256), []
+    net.step(obs, None, state)
+    inner = memory.policy_input
+    monkeypatch.setattr(memory, "policy_input", lambda o, x: peak.append(torch.cuda.max_memory_allocated() - before) or inner(o, x))
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    net.step(obs, None, state)
+    assert peak == [obs.numel() * 2]
+
+
 def test_build_needs_the_operators_last(monkeypatch):
     """Where the operators cannot be built (no C++ compiler or torch headers), the emulator and the oracle are built all the same, and
     build() says what failed."""
