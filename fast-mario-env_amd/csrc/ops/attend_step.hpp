@@ -58,7 +58,9 @@ __global__ void __launch_bounds__(256) k_step_state(Step a) {
     float vv[V], o[V];
 #pragma unroll
     for (int c = 0; c < V; c++) { vv[c] = live ? as_f32(v[e + c]) : 0.f; o[c] = 0.f; }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");     // (other lanes read them; a barrier alone orders no memory)
     __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     for (int d0 = 0; d0 < a.D; d0 += STEP_ROWS * RG) {
         if (d0) load(d0);
 #pragma unroll
