@@ -201,7 +201,89 @@ def test_norm_of_a_far_first_value(rows, far):
         assert (d.abs() <= limit).all(), (d.abs() / limit).max().item()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,C,sp,groups", [(6, 64, (9, 9), 8), (300, 30, (), 5), (40, 24, (9, 9), 4), (50, 1024, (), 8), (2, 64, (130, 117), 4), (2, 21, (90, 70), 3)])
+def test_norm_relu_gradient(B, C, sp, groups, dtype):
+    """relu's gradient jumps where its argument is 0: dy is 0 wherever it is within a rounding of it."""
+    x, w, b, dy = norm_inputs(B, C, sp, dtype)
+    z = norm64(x, groups, w, b, 1e-5, "none")
+    dy = torch.where(z.abs() < 1e-3, torch.zeros_like(dy), dy)
+    x, w, b = (t.requires_grad_() for t in (x, w, b))
+    grads = torch.autograd.grad(group_norm_act(x, groups, w, b, act="relu"), (x, w, b), dy)
+    want = norm64(x.detach(), groups, w.detach(), b.detach(), 1e-5, "relu", dy)[1:]
+    cells = x.numel() // B // groups
+    for a, e in zip(grads, want):
+        rel = 2.0 ** -8 if a.dtype == torch.bfloat16 else 2.0 ** -24 * (32 + 4 * cells ** 0.5) * 8
+        assert (a.double() - e).norm() <= rel * e.norm() + 2.0 ** -20 * x.numel() ** 0.5
+
+
+@pytest.mark.gpu
+def test_norm_of_more_than_the_caches():
+    """One position a sample and more than 256 MiB: x and dy are read past the caches."""
+    B, C = 280000, 512
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, dy = (torch.randn(B, C, generator=g, device="cuda").bfloat16() for _ in range(2))
+    w, b = (torch.randn(C, generator=g, device="cuda") for _ in range(2))
+    x, w, b = (t.requires_grad_() for t in (x, w, b))
+    y = group_norm_act(x, 8, w, b, act="silu")
+    grads = torch.autograd.grad(y, (x, w, b), dy)
+    dw, db = torch.zeros(C, dtype=torch.float64, device="cuda"), torch.zeros(C, dtype=torch.float64, device="cuda")
+    for i in range(0, B, 40000):
+        s = slice(i, i + 40000)
+        want = norm64(x[s].detach(), 8, w.detach(), b.detach(), 1e-5, "silu", dy[s])
+        assert (y[s].double() - want[0]).norm() <= 2.0 ** -8 * want[0].norm()
+        assert (grads[0][s].double() - want[1]).norm() <= 2.0 ** -8 * want[1].norm()
+        dw += want[2]
+        db += want[3]
+    # sums of 280,000 terms in trees of blocks: a few 2^-24 of the sum of absolute values
+    assert (grads[1].double() - dw).abs().max() <= 256 * 2.0 ** -24 * B and (grads[2].double() - db).abs().max() <= 256 * 2.0 ** -24 * B
+
+
+@pytest.mark.gpu
+def test_step_of_odd_heads_past_the_caches():
+    """States of more than 256 MiB whose rows no 16-byte access fits: a column a lane, two rows of blocks, past the caches."""
+    N, D, E = 4300, 128, 127
+    q, k, v, decay, start, state, _, _ = attend_inputs(1, N, 1, D, E, torch.float32, starts=0.2)
+    assert state.numel() * 4 > 256 << 20
+    want, last = attend64(q, k, v, decay, start, state, D ** -0.5)
+    size, lsize = attend64(q.abs(), k.abs(), v.abs(), decay, start, state.abs(), D ** -0.5)
+    out = linear_attention_step(q[0], k[0], v[0], decay, state, start[0])
+    f32 = (16 + D) * 2.0 ** -23
+    assert ((out.double() - want[0]).abs() <= f32 * size[0]).all() and ((state.double() - last).abs() <= f32 * lsize).all()
+
+
 # ---------------------------------------------------------------- as a program uses them
+@pytest.mark.gpu
+def test_operators_run_behind_what_makes_their_inputs():
+    """On a side stream whose inputs come late, behind long products: a launch on any other stream would see the old ones."""
+    q, k, v, decay, start, state, do, ds = attend_inputs(300, 2, 2, 64, 64, torch.bfloat16)
+    x, w, b, dy = norm_inputs(5, 24, (9, 9), torch.bfloat16)
+
+    def work(q, k, v, state, x, S):
+        leaves = [t.requires_grad_() for t in (q, k, v, state, x)]
+        out, last = linear_attention(*leaves[:3], decay, start, leaves[3])
+        y = group_norm_act(leaves[4], 3, w, b, act="silu")
+        grads = torch.autograd.grad((out, last, y), leaves, (do, ds, dy))
+        with torch.no_grad():
+            one = linear_attention_step(leaves[0][0], leaves[1][0], leaves[2][0], decay, S, start[0])
+        return [out.detach(), last.detach(), y.detach(), *grads, one, S]
+
+    want = work(*(t.clone() for t in (q, k, v, state, x, state)))
+    late = [torch.zeros_like(t) for t in (q, k, v, state, x, state)]
+    big = torch.randn(8192, 8192, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(4):
+            big @ big
+        for to, t in zip(late, (q, k, v, state, x, state)):
+            to.copy_(t)
+        got = work(*late)
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("sp", [(), (3,), (9, 9)])
 def test_outputs_may_be_changed_in_place(sp):
