@@ -23,6 +23,7 @@ The env-kernel share of a rollout is timed with events on the stream both run on
 from __future__ import annotations
 
 import ctypes
+import inspect
 import math
 
 import numpy as np
@@ -335,6 +336,12 @@ def gae(rew, val, start, next_val, next_start, gamma: float = 0.99, lam: float =
     return adv, adv + val
 
 
+def _steps_memories(net) -> bool:
+    """Whether net's `act` steps memories that `initial_state` makes, as make_memory_net's does. (A network may have an
+    `initial_state` for other ends, and an `act` of observations alone.)"""
+    return hasattr(net, "initial_state") and {"start", "state"} <= set(inspect.signature(net.act).parameters)
+
+
 class Rollout:
     """T-step rollouts of `env` (a HipVecEnv) under `net`, stored frame-deduplicated on the env's device."""
 
@@ -356,7 +363,7 @@ class Rollout:
         self.next_val = torch.zeros(n, device=dev)
         self.next_start = torch.zeros(n, dtype=torch.bool, device=dev)
         self._starting = torch.ones(n, dtype=torch.bool, device=dev)   # the current obs is a reset stack
-        self.memory = net.initial_state(n) if hasattr(net, "initial_state") else None   # now, and when the rollout began
+        self.memory = net.initial_state(n) if _steps_memories(net) else None   # now, and when the rollout began
         self.memory0 = None if self.memory is None else self.memory.clone()
         self.env_ms = 0.0
 

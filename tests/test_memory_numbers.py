@@ -335,3 +335,21 @@ def test_build_needs_the_operators_last(monkeypatch):
     with pytest.raises(RuntimeError, match="no compiler"):
         entry.build()
     assert done == ["emulator", "oracle"]
+
+
+def test_rollout_takes_networks_without_memories():
+    """A network's own `initial_state` does not make it one whose `act` takes memories."""
+    from types import SimpleNamespace
+    from fast_mario_env_amd.rollout import Rollout
+    env = SimpleNamespace(n=2, dev=torch.device("cpu"), k=4)
+
+    class Recurrent:
+        def initial_state(self, batch, layers):
+            raise AssertionError("not asked for")
+
+        def act(self, obs, generator=None):
+            return obs
+
+    assert Rollout(env, Recurrent(), T=3).memory is None
+    ro = Rollout(env, memory.make_memory_net(device="cpu"), T=3)
+    assert ro.memory.shape == (2, 8, 64, 64) and torch.equal(ro.memory0, ro.memory)
