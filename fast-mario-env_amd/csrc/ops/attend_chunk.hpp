@@ -13,13 +13,14 @@ namespace mo {
 // two parts (halves, in tiles.hpp), S' is made from w V in three (scaled_parts). Everything is read once and
 // written once; a chunk is three products over 32-step blocks of at most L x L x P, far below what the matrix cores do in the
 // time its rows take to come, so the pass is bound by memory as long as enough workgroups wait for it at once: three fit a
-// compute unit (two of heads of 128).
+// compute unit (two of heads of 128, whose 256 registers spill two).
 //
-// Measured, bf16, D = E = 64 and 8 heads, 128 steps of 4,096 envs: 730 us for 3.2 GB, 4.4 TB/s, where a copy of 1 GiB reaches 5.2.
-// (Step by step, k_walk: 4,889 us.) From zeros, 2,056 envs: 257 us, 5.2 TB/s; 1,000 envs with heads of 128: 337 us, 4.7 TB/s; with
-// heads of 64 135 us, in float32 292.
-// Where a step's rows lie a multiple of 2 MiB apart (N H D a power of two), a chunk's requests meet in the same memory channels:
-// storing the states for the gradient, 2,048 envs take 424 us, 2,056 take 341.
+// Measured, bf16, D = E = 64 and 8 heads, 128 steps of 4,096 envs: 753 us for 3.2 GB, 4.3 TB/s, where a copy of 1 GiB reaches 5.2; its
+// bytes cross once, the matrix units are busy 15 % of the time and waves wait 41 % of theirs (counters). (Step by step, k_walk: 4,889
+// us.) From zeros, 2,056 envs: 302 us, 4.5 TB/s (287 with one part of S and scores); 1,000 envs with heads of 128: 371 us, 4.2 TB/s
+// (335); with heads of 64 140 us (130), in float32 281.
+// Where a step's rows lie a multiple of 2 MiB apart (N H D a power of two), a pass takes longer: from zeros and keeping the states
+// for the gradient, 2,048 envs take 385 us, 2,056 take 325.
 //
 // T: element type. P: head size rounded up to 32, 64 or 128; columns past D or E are zeros. L: 64 for bf16; 32 for float32,
 // whose matrix instructions are 16 times slower, so that the products of a chunk with itself stay short.
@@ -146,8 +147,8 @@ template <int L> struct Powers {
 };
 
 // The env and head of a workgroup. Workgroups go to the 8 XCDs in turn; XCD_RUN neighbouring heads (whose rows of a step lie
-// together) go to one of them, so that what one L2 fetches lies together too. (256 steps of 2,000 envs, 8 heads of 32, bf16: 312 us,
-// 472 with one; 128 steps of 2,056 envs, 8 heads of 64: 256 and 267.)
+// together) go to one of them, so that what one L2 fetches lies together too. (256 steps of 2,000 envs, 8 heads of 32, bf16: 337 us,
+// 481 with one; 128 steps of 2,056 envs, 8 heads of 64: 282 and 292.)
 constexpr int XCD_RUN = 16;
 __device__ __forceinline__ int64_t head_of_block(int64_t heads) {
     const int64_t b = block_here(), round = 8 * XCD_RUN;
@@ -157,8 +158,8 @@ __device__ __forceinline__ int64_t head_of_block(int64_t heads) {
 
 // A long sequence is cut into segments of whole chunks, a workgroup each, so that few sequences fill the chip. First each
 // segment's own sum and what it leaves of an entering state (`keep`: g^steps, or -1 where an episode starts inside), then the
-// states that enter the segments one after another, then the outputs from there. (16,001 steps of 2 envs with 8 heads of 128, bf16: 50
-// us for the sums, 16 for the states between, 85 for the outputs under the profiler, 126 in all without; k and v are read twice.)
+// states that enter the segments one after another, then the outputs from there. (16,001 steps of 2 envs with 8 heads of 128, bf16: 48
+// us for the sums, 15 for the states between, 102 for the outputs under the profiler, 144 in all without; k and v are read twice.)
 struct Cut {
     int64_t chunks, per_seg;   // chunks of a sequence and of a segment
     int segs;
@@ -477,7 +478,7 @@ inline bool rows_suit(const MoRows& r, int64_t epv) {   // 16-byte accesses
     return (uintptr_t)r.p % 16 == 0 && r.st % epv == 0 && r.sn % epv == 0 && r.sh % epv == 0;
 }
 // The chunk kernels take heads of whole 16-byte pieces whose rows lie on them; the rest goes step by step (k_walk; 128 steps of
-// 1,000 envs, 8 heads, bf16: heads of 40 by chunks 200 us, with the gradient 589; heads of 36 step by step 855 and 3,370).
+// 1,000 envs, 8 heads, bf16: heads of 40 by chunks 214 us, with the gradient 646; heads of 36 step by step 854 and 3,370).
 inline bool chunks_take(const MoAttend& a, bool backward) {
     const int64_t epv = a.dtype == MO_BF16 ? 8 : 4;
     if (a.T == 0 || a.D % epv || a.E % epv || !rows_suit(a.q, epv) || !rows_suit(a.k, epv) || !rows_suit(a.v, epv)) return false;
@@ -487,8 +488,8 @@ inline int chunk_steps(const MoAttend& a) { return a.dtype == MO_BF16 ? 64 : 32;
 inline int padded_head(const MoAttend& a) { const int m = std::max(a.D, a.E); return m <= 32 ? 32 : m <= 64 ? 64 : 128; }
 
 // Segments: up to two workgroups a compute unit, of two chunks at least. Two segments are not worth it: k, v (or q, dO) are read
-// twice and two more kernels run. (16,001 steps of 16 heads of 128: 1,266 us in one piece, 132 in 32; 2,000 steps of 512 heads of
-// 64: 136 in one piece, 208 in two; 300 steps of 32 heads of 128: 32 in one, 37 in two.)
+// twice and two more kernels run. (16,001 steps of 16 heads of 128: 1,560 us in one piece, 159 in 32; 2,000 steps of 512 heads of
+// 64: 145 in one piece, 210 in two; 300 steps of 32 heads of 128: 35 in one, 41 in two.)
 inline Cut attend_cut(const MoAttend& a) {
     Cut c{};
     c.chunks = (a.T + chunk_steps(a) - 1) / chunk_steps(a);

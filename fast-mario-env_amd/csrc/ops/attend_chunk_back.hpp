@@ -15,11 +15,13 @@ namespace mo {
 // 16-byte pieces. A, B, R and S go into products in two parts each (halves, in tiles.hpp); to leave LDS room for two workgroups of heads of
 // 64 a compute unit, B waits in registers until A is done with, and dV until R is.
 //
-// Bound by memory: 4 rows are read and 3 written a step and head. Measured, bf16, 128 steps of 2,056 envs with 8 heads of 64: 705 us, 4.0
-// TB/s (860 us at 2,048 envs, whose steps' rows lie a multiple of 2 MiB apart). Heads of 128, 1,000 envs: 713 us, 2.9 TB/s: the
-// tiles leave room for one workgroup a compute unit, whose loads wait while it multiplies. float32 holds half the steps in as much
-// LDS and its matrix instructions take 16 times as long: the 1,000 envs with heads of 64 take 712 us, in bf16 252. Step by step (k_walk, three walks):
-// 128 steps of 2,048 envs with the forward pass 10,277 us, 1,290 by chunks.
+// 4 rows are read and 3 written a step and head, and a state a chunk. Measured, bf16, from zeros, the gradient of 128 steps of 2,056 envs with 8
+// heads of 64: 596 us, 3.6 TB/s (500 with one part of A, B, R and S; 730 at 2,048 envs, whose steps' rows lie a multiple of 2 MiB apart):
+// neither memory nor the matrix units (13 % busy) are full, waves wait 43 % of their time with two workgroups a compute unit. Heads of 128,
+// 1,000 envs: 916 us, 2.6 TB/s (702): the tiles leave room for one workgroup a compute unit, whose loads wait while it multiplies, and 256
+// registers spill 12. float32 holds half the steps in as much LDS and its matrix instructions take 16 times as long: the 1,000 envs with heads
+// of 64 take 672 us, in bf16 291; at 97 steps of 64 envs its matrix units are busy 51 % of the time. Step by step (k_walk, three walks): 128
+// steps of 2,048 envs with the forward pass 10,277 us, 1,312 by chunks.
 template <class T, int P> using BackChunk = Chunk<T, P, P / 16>;
 template <class T, int P> struct BackLds {
     typedef BackChunk<T, P> C;
@@ -356,6 +358,7 @@ __global__ void __launch_bounds__((BackChunk<T, P>::NT)) k_attend_back_sums(MoAt
 template <class T, int P> int attend_back_chunks(const MoAttend& a, hipStream_t s) {
     Cut c = attend_cut(a);
     cut_place(a, c);
+    static_assert(sizeof(BackLds<T, P>) <= (160 << 10), "");
     const dim3 grid = grid_of(a.N * a.H, c.segs), block(BackChunk<T, P>::NT);
     if (c.segs > 1) {
         hipLaunchKernelGGL((k_attend_back_sums<T, P>), grid, block, 0, s, a, c);

@@ -35,8 +35,9 @@ struct Moments {
 };
 
 // For samples that do not fit a team's registers. Three passes: the slabs' moments (back: sums), their joining, and the results, so x
-// is read twice (back: x and dy), the second time from the last-level cache where it holds them. Measured, float32, 37 x 48 x 84 x 84 in 6
-// groups, in microseconds: moments and results 20 each, back sums 25 and results 31, joining 5 each, all bound by memory.
+// is read twice (back: x and dy), each time past the L2s (counters; the last-level cache may have it the second time). Measured, float32, 37 x
+// 48 x 84 x 84 in 6 groups, in microseconds under the profiler: moments 17, their joining 4, results 21; back, sums 22, joining 5, results 28,
+// the channels' sums 4; 97 in all without it.
 // A sample is cut into slabs of `px` pixels; a block takes a slab. Its threads are LN lanes along the channels (V each) by
 // pixel lanes, so a thread's channels stay its own.
 struct NormCut {

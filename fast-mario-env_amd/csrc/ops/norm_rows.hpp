@@ -1,5 +1,5 @@
-// Group norm with an activation where a sample's group fits a wave's registers and neither its channels nor their number suit
-// whole 16-byte packs: read once, an element an access.
+// Group norm with an activation where a sample's group fits a wave's registers and norm_small does not take it: channels or groups that are
+// not whole 16-byte packs, buffers off 16 bytes, and pixels of more than 512 channels. Read once, an element an access.
 #pragma once
 #include "norm_general.hpp"
 

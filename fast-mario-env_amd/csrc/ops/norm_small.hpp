@@ -11,9 +11,10 @@ namespace mo {
 // where the team has several waves (MULTI). The mean's sum goes about the group's first value, and the variance is that of the
 // values in registers about their mean: a large mean costs neither digits, and equal values have no deviations. NS: groups of a pack, each with sums of its own: 1 (a group is whole packs), 2, 4 or 8.
 // Bound by memory, a value read and one written (back: two and one). Measured, bf16, in microseconds: 4,096 x 32 x 20 x 20 in 4 groups 38
-// (5.6 TB/s, partly out of the last-level cache), 104 through norm_general; 262,144 x 512 in 8 groups 120 (4.5 TB/s), back 176 (4.6); 4,096 x
+// (5.6 TB/s, partly out of the last-level cache), 104 through norm_general; 262,144 x 512 in 8 groups 120 (4.5 TB/s), with the gradient 275; 4,096 x
 // 64 x 9 x 9 in 8 groups forward 21, back 33; groups of one channel need eight sums a pack and more registers: 16,384 x 32 x 9 x 9
-// forward and back 212 in 32 groups, 100 in 8, 91 in 4. (LDS by the team's waves: room for eight waves in each block made the 212 340.)
+// forward and back 216 in 32 groups, 105 in 8, 95 in 4. (LDS by the team's waves: room for eight waves in each block made the 216 340.) The
+// gradients of four bf16 packs a thread in groups of 4 channels keep 4 to 6 registers in scratch.
 struct Small {
     MoNorm a;
     int W, TT, nv, NV, log_nv; // waves and threads a team; packs a pixel, and rounded up
@@ -227,8 +228,10 @@ __global__ void __launch_bounds__(small_threads(MULTI), (NS <= 2 && sizeof(T) ==
 // ---- host side
 struct SmallCut { int W, TT, R, blocks; };
 
-// Whole packs a pixel, groups of whole packs or of 1, 2 or 4 channels, a pixel's packs within a wave, and a sample within a
-// team's registers; otherwise the sample goes through memory twice (norm_general).
+// Whole packs a pixel, groups of whole packs or of 1, 2 or 4 channels, a pixel's packs within a wave (64 packs, 512 channels: sums are
+// shuffles of a wave, and waves exchange them lane by lane), and a sample within a team's registers. Wider pixels and other groups go to
+// norm_rows, by single elements (65,536 x 1,024 in 8 groups, forward and gradient 429 us; its bytes take 129), and samples that fit neither
+// go through memory twice (norm_general).
 inline bool norm_small_takes(const MoNorm& a, bool backward, SmallCut& c) {
     const int cg = a.C / a.groups;
     if (!norm_wide(a) || a.C > 8 * kWave || (cg % 8 && 8 % cg)) return false;
