@@ -13,6 +13,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 from build_native import ARCH, HERE, hipcc
 
@@ -20,8 +21,8 @@ CSRC = os.path.join(HERE, "csrc", "ops")
 PACKAGE = os.path.join(HERE, "fast_mario_env_amd")
 OUT = os.path.join(PACKAGE, "libmario_ops.so")
 EXTENSION = os.path.join(PACKAGE, "_mario_ops_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
-FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-         "-Wall"]
+SOURCES = ("mario_ops.hip", "selective.hip")
+FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall"]
 
 
 def _run(cmd, out, verbose):
@@ -38,7 +39,12 @@ def _run(cmd, out, verbose):
 
 
 def build(verbose: bool = True) -> str:
-    _run([hipcc(), f"--offload-arch={ARCH}", *FLAGS, os.path.join(CSRC, "mario_ops.hip")], OUT, verbose)
+    objects = [os.path.join(PACKAGE, s.replace(".hip", ".o")) for s in SOURCES]
+    with ThreadPoolExecutor(len(SOURCES)) as pool:   # (each source is a device compilation of its own)
+        list(pool.map(lambda s, o: _run([hipcc(), f"--offload-arch={ARCH}", *FLAGS, "-c", os.path.join(CSRC, s)], o, verbose), SOURCES, objects))
+    _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *objects], OUT, verbose)
+    for o in objects:
+        os.remove(o)
     import torch
     from torch.utils.cpp_extension import include_paths
     lib, rocm = os.path.join(os.path.dirname(torch.__file__), "lib"), os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))

@@ -1,0 +1,124 @@
+// The norm of many tensors together, and their scaling by it.
+#pragma once
+#include "common.hpp"
+
+namespace mo {
+
+// The tensors go into the kernels' arguments, up to TABLE of them a launch. A block takes every gridDim.x-th chunk of the launch's
+// values and leaves one float64 sum of squares; the scaling kernel's blocks each add all blocks' sums, in the same order.
+constexpr int GRADIENT_TABLE = 128, GRADIENT_THREADS = 256, GRADIENT_BLOCKS = 1024;
+constexpr int64_t GRADIENT_CHUNK = 16384;
+struct Gradients {
+    void* p[GRADIENT_TABLE];
+    int64_t n[GRADIENT_TABLE];
+    uint32_t begin[GRADIENT_TABLE + 1];   // the first chunk of each tensor
+    uint8_t bf[GRADIENT_TABLE];
+    int count;
+};
+static_assert(sizeof(Gradients) < 3500, "");
+
+__device__ __forceinline__ int tensor_of(const Gradients& g, unsigned chunk) {
+    int lo = 0, hi = g.count - 1;          // the last tensor that begins at or before the chunk
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (g.begin[mid] <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+__device__ __forceinline__ double block_sum(double x, double* s) {
+    for (int m = kWave / 2; m; m /= 2) x += __shfl_xor(x, m);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = x;
+    __syncthreads();
+    x = 0.0;
+    for (int w = 0; w < GRADIENT_THREADS / kWave; w++) x += s[w];
+    return x;
+}
+
+template <class T> __device__ __forceinline__ double squares(const T* p, int64_t n) {
+    double x = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += GRADIENT_THREADS) {
+        const double v = as_f32(p[i]);
+        x = fma(v, v, x);
+    }
+    return x;
+}
+__global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_squares(Gradients g, double* part) {
+    __shared__ double s[GRADIENT_THREADS / kWave];
+    double x = 0.0;
+    for (unsigned chunk = blockIdx.x; chunk < g.begin[g.count]; chunk += gridDim.x) {
+        const int i = tensor_of(g, chunk);
+        const int64_t at = (int64_t)(chunk - g.begin[i]) * GRADIENT_CHUNK, n = min(GRADIENT_CHUNK, g.n[i] - at);
+        x += g.bf[i] ? squares((const bf16*)g.p[i] + at, n) : squares((const float*)g.p[i] + at, n);
+    }
+    x = block_sum(x, s);
+    if (threadIdx.x == 0) part[blockIdx.x] = x;
+}
+
+__device__ __forceinline__ double norm_of(const double* part, int64_t parts, double* s) {
+    double x = 0.0;
+    for (int64_t i = threadIdx.x; i < parts; i += GRADIENT_THREADS) x += part[i];
+    return sqrt(block_sum(x, s));
+}
+__global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_norm(const double* part, int64_t parts, float* norm) {
+    __shared__ double s[GRADIENT_THREADS / kWave];
+    const double x = norm_of(part, parts, s);
+    if (threadIdx.x == 0) *norm = (float)x;
+}
+template <class T> __device__ __forceinline__ void scale_values(T* p, int64_t n, float by) {
+    for (int64_t i = threadIdx.x; i < n; i += GRADIENT_THREADS) p[i] = as<T>(as_f32(p[i]) * by);
+}
+// (max / (norm + eps) is taken in float64 and the factor rounded once to float32; a norm that is NaN makes everything NaN.)
+__global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_scale(Gradients g, const double* part, int64_t parts, float max_norm, float eps, float* norm) {
+    __shared__ double s[GRADIENT_THREADS / kWave];
+    const double x = norm_of(part, parts, s), f = (double)max_norm / (x + (double)eps);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)x;
+    const float by = f > 1.0 ? 1.f : (float)f;
+    for (unsigned chunk = blockIdx.x; chunk < g.begin[g.count]; chunk += gridDim.x) {
+        const int i = tensor_of(g, chunk);
+        const int64_t at = (int64_t)(chunk - g.begin[i]) * GRADIENT_CHUNK, n = min(GRADIENT_CHUNK, g.n[i] - at);
+        if (g.bf[i]) scale_values((bf16*)g.p[i] + at, n, by);
+        else scale_values((float*)g.p[i] + at, n, by);
+    }
+}
+
+// ---- host side
+inline int64_t gradient_launches(int64_t count) { return std::max<int64_t>(1, (count + GRADIENT_TABLE - 1) / GRADIENT_TABLE); }
+inline int64_t gradient_work(int64_t count) { return 8 * gradient_launches(count) * GRADIENT_BLOCKS; }
+inline int gradient_norm(const MoTensor* t, int64_t count, bool scale, float max_norm, float eps, float* norm, double* part, hipStream_t s) {
+    const int64_t launches = gradient_launches(count);
+    const auto table = [&](int64_t l, Gradients& g) {
+        g = Gradients{};
+        uint64_t chunks = 0;
+        for (int64_t i = l * GRADIENT_TABLE; i < std::min(count, (l + 1) * GRADIENT_TABLE); i++) {
+            const int k = g.count++;
+            g.p[k] = t[i].p;
+            g.n[k] = t[i].n;
+            g.bf[k] = t[i].dtype == MO_BF16;
+            g.begin[k] = (uint32_t)chunks;
+            chunks += (t[i].n + GRADIENT_CHUNK - 1) / GRADIENT_CHUNK;
+        }
+        g.begin[g.count] = (uint32_t)chunks;
+        return (unsigned)std::min<uint64_t>(std::max<uint64_t>(chunks, 1), GRADIENT_BLOCKS);
+    };
+    Gradients g;
+    int64_t parts = 0;
+    for (int64_t l = 0; l < launches; l++) {
+        const unsigned blocks = table(l, g);
+        hipLaunchKernelGGL(k_gradient_squares, dim3(blocks), dim3(GRADIENT_THREADS), 0, s, g, part + parts);
+        parts += blocks;
+    }
+    if (launched("k_gradient_squares")) return -1;
+    if (!scale) {
+        hipLaunchKernelGGL(k_gradient_norm, dim3(1), dim3(GRADIENT_THREADS), 0, s, (const double*)part, parts, norm);
+        return launched("k_gradient_norm");
+    }
+    for (int64_t l = 0; l < launches; l++) {
+        const unsigned blocks = table(l, g);
+        hipLaunchKernelGGL(k_gradient_scale, dim3(blocks), dim3(GRADIENT_THREADS), 0, s, g, (const double*)part, parts, max_norm, eps, l ? nullptr : norm);
+    }
+    return launched("k_gradient_scale");
+}
+
+}  // namespace mo

@@ -1,4 +1,4 @@
-// libmario_ops.so: the operators of a policy with a memory (include/mario_ops.h), gfx950. A library of its own: the emulator's
+// libmario_ops.so: the operators of a policy with a memory (include/mario_ops.h), gfx950; selective.hip is its second part. A library of its own: the emulator's
 // is built for bit-exact float sums and scalar code, these for matrix instructions and memory.
 #include <algorithm>
 
@@ -6,16 +6,13 @@
 #include "attend_step.hpp"
 #include "attend_walk.hpp"
 #include "common.hpp"
+#include "guard.hpp"
 #include "norm_rows.hpp"
 #include "norm_small.hpp"
 
 using namespace mo;
 
 namespace {
-
-constexpr int64_t MAX_GRID = (int64_t)1 << 31;
-
-size_t size_of(int dtype) { return dtype == MO_BF16 ? 2 : 4; }
 
 bool attend_sizes(const MoAttend* a) {
     if (!a || (a->dtype != MO_F32 && a->dtype != MO_BF16) || a->T < 0 || a->N < 0 || a->H < 1 || a->D < 1 || a->D > MO_MAX_HEAD ||
@@ -43,8 +40,6 @@ bool norm_sizes(const MoNorm* a) {
     return true;
 }
 
-template <class F> int by_type(int dtype, F f) { return dtype == MO_BF16 ? f(bf16{}) : f(float{}); }
-
 // Heads in whole 16-byte pieces go by chunks on the matrix cores, the rest step by step.
 template <class T> int attend_forward(const MoAttend& a, hipStream_t s) {
     if (!chunks_take(a, false)) return walk_forward<T>(a, s);
@@ -55,22 +50,6 @@ template <class T> int attend_back(const MoAttend& a, hipStream_t s) {
     if (!chunks_take(a, true) || (!a.saved && attend_cut(a).chunks > 1)) return walk_backward<T>(a, s);
     const int p = padded_head(a);
     return p == 32 ? attend_back_chunks<T, 32>(a, s) : p == 64 ? attend_back_chunks<T, 64>(a, s) : attend_back_chunks<T, 128>(a, s);
-}
-
-// No C++ exception leaves a C entry point.
-template <class F> auto guarded(F f) noexcept -> decltype(f()) {
-    try {
-        return f();
-    } catch (...) {
-        try { fail("out of host memory"); } catch (...) {}
-        return -1;
-    }
-}
-
-template <class F> int by_act(int act, F f) {
-    if (act == MO_ACT_RELU) return f(std::integral_constant<int, MO_ACT_RELU>{});
-    if (act == MO_ACT_SILU) return f(std::integral_constant<int, MO_ACT_SILU>{});
-    return f(std::integral_constant<int, MO_ACT_NONE>{});
 }
 
 int norm_run(const MoNorm& a, bool backward, hipStream_t s) {

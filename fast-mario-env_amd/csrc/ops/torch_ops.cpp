@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 
 #include "../../../include/mario_ops.h"
@@ -56,6 +57,9 @@ bool wants_grad(at::ArrayRef<Tensor> ts) {
     for (const Tensor& t : ts)
         if (t.defined() && t.requires_grad()) return true;
     return false;
+}
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // (what saved it for a gradient notices)
 }
 // Gradients of a pass that has no gradient itself: where one is asked for all the same, an error.
 variable_list once(variable_list grads) {
@@ -151,7 +155,7 @@ Tensor attend_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const T
     ok(mo_attend_step(dtype_of(q), q.size(0), (int)q.size(1), (int)q.size(2), (int)v.size(2), (float)scale, &rq, &rk, &rv, data(decay),
                       data<uint8_t>(start), data(state), &ro, stream_of(q)),
        "mo_attend_step");
-    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();   // (what saved it for a gradient notices)
+    written(state);
     return out;
 }
 
@@ -235,10 +239,242 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const Maybe& weight_, con
     return norm_forward(channels_last(x), groups, weight, bias, eps, act, nullptr);
 }
 
+// ---------------------------------------------------------------- causal convolution and activation
+// Values of channels (T, N, C) or (N, C), the channels contiguous.
+MoRows channel_rows(const Tensor& t) {
+    if (!t.defined()) return MoRows{};
+    const auto st = t.strides();
+    return t.dim() == 3 ? MoRows{t.data_ptr(), st[0], st[1], 0} : MoRows{t.data_ptr(), 0, st[0], 0};
+}
+// As the scan's kernels take them: contiguous along the last dimension.
+Tensor inner(const Tensor& t) { return !t.defined() || t.strides().back() == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor float_param(const Maybe& t) { return t ? t->to(at::kFloat).contiguous() : Tensor(); }
+
+MoConv conv_args(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& start, const Tensor& state, int64_t act) {
+    MoConv a{};
+    a.dtype = dtype_of(x);
+    a.act = (int32_t)act;
+    a.T = x.dim() == 3 ? x.size(0) : 1; a.N = x.size(-2); a.C = (int32_t)x.size(-1); a.K = (int32_t)weight.size(1);
+    a.x = channel_rows(x);
+    a.weight = data(weight);
+    a.bias = data(bias);
+    a.start = data<uint8_t>(start);
+    a.state = data<void>(state);
+    return a;
+}
+std::pair<Tensor, Tensor> conv_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& start, const Tensor& state, int64_t act) {
+    const c10::DeviceGuard guard(x.device());
+    MoConv a = conv_args(x, weight, bias, start, state, act);
+    const Tensor y = at::empty(x.sizes(), x.options()), last = at::empty({a.N, a.K - 1, a.C}, x.options());
+    a.y = channel_rows(y);
+    a.state_out = data<void>(last);
+    ok(mo_conv(&a, stream_of(x)), "mo_conv");
+    return {y, last};
+}
+
+struct Conv : torch::autograd::Function<Conv> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor weight, Maybe bias_, Maybe start_, Maybe state_, int64_t act) {
+        const Tensor bias = sure(bias_), start = sure(start_), state = sure(state_);
+        const auto [y, last] = conv_forward(x, weight, bias, start, state, act);
+        ctx->save_for_backward({x, weight, bias, start, state});
+        ctx->saved_data["act"] = act;
+        ctx->set_materialize_grads(false);
+        return {y, last};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &weight = s[1], &bias = s[2], &start = s[3], &state = s[4];
+        const c10::DeviceGuard guard(x.device());
+        MoConv a = conv_args(x, weight, bias, start, state, ctx->saved_data["act"].toInt());
+        const Tensor dy = as_rows(grads[0].defined() ? grads[0] : at::zeros({1}, x.options()).expand(x.sizes()));
+        const Tensor dlast = contiguous(grads[1]), dx = at::empty(x.sizes(), x.options());
+        // inputs that are there, in their order: x, weight, bias, start, state
+        size_t at = 1;
+        const bool want_weight = ctx->needs_input_grad(at);
+        const bool want_bias = bias.defined() && ctx->needs_input_grad(++at);
+        if (start.defined()) ++at;
+        const Tensor dstate = state.defined() && ctx->needs_input_grad(++at) ? at::empty(state.sizes(), state.options()) : Tensor();
+        Tensor dw, db;
+        if (want_weight || want_bias) {
+            const auto make = [&](at::IntArrayRef size) { return a.N && a.T ? at::empty(size, weight.options()) : at::zeros(size, weight.options()); };
+            dw = make(weight.sizes());
+            db = make({a.C});
+        }
+        a.dy = channel_rows(dy);
+        a.dx = channel_rows(dx);
+        a.dstate_out = data<void>(dlast);
+        a.dstate = data<void>(dstate);
+        a.dweight = data(dw);
+        a.dbias = data(db);
+        const Tensor work = work_of(ok(mo_conv_work(&a), "mo_conv_work"), x);
+        a.work = data<void>(work);
+        ok(mo_conv_backward(&a, stream_of(x)), "mo_conv_backward");
+        return once({dx, dw, bias.defined() ? db : Tensor(), Tensor(), dstate, Tensor()});
+    }
+};
+
+std::tuple<Tensor, Tensor> conv(const Tensor& x_, const Tensor& weight_, const Maybe& bias_, const Maybe& start_, const Maybe& state_, int64_t act) {
+    const Tensor x = as_rows(x_), weight = weight_.to(at::kFloat).contiguous(), bias = float_param(bias_);
+    const Tensor start = contiguous(sure(start_)), state = contiguous(sure(state_));
+    if (wants_grad({x, weight, bias, state})) {
+        const variable_list out = Conv::apply(x, weight, maybe(bias), maybe(start), maybe(state), act);
+        return {out[0], out[1]};
+    }
+    const auto [y, last] = conv_forward(x, weight, bias, start, state, act);
+    return {y, last};
+}
+
+Tensor conv_step(const Tensor& x_, const Tensor& weight_, const Maybe& bias_, const Tensor& state, const Maybe& start_, int64_t act) {
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = as_rows(x_), weight = weight_.to(at::kFloat).contiguous(), bias = float_param(bias_), start = contiguous(sure(start_));
+    MoConv a = conv_args(x, weight, bias, start, Tensor(), act);
+    const Tensor y = at::empty(x.sizes(), x.options());
+    a.y = channel_rows(y);
+    a.state_out = data<void>(state);
+    ok(mo_conv_step(&a, stream_of(x)), "mo_conv_step");
+    written(state);
+    return y;
+}
+
+// ---------------------------------------------------------------- selective state space scan
+struct ScanIn { Tensor x, dt, A, B, C, D, z, bias, start, state; };
+MoScan scan_args(const ScanIn& in) {
+    MoScan a{};
+    a.dtype = dtype_of(in.x);
+    a.T = in.x.dim() == 3 ? in.x.size(0) : 1; a.N = in.x.size(-2); a.C = (int32_t)in.x.size(-1);
+    a.S = (int32_t)in.A.size(1); a.G = (int32_t)in.B.size(-2);
+    a.x = channel_rows(in.x); a.dt = channel_rows(in.dt); a.z = channel_rows(in.z);
+    a.Bt = rows_of(in.B); a.Ct = rows_of(in.C);
+    a.A = data(in.A); a.D = data(in.D); a.dt_bias = data(in.bias);
+    a.start = data<uint8_t>(in.start);
+    a.state = data(in.state);
+    return a;
+}
+Forward scan_forward(const ScanIn& in, bool keep) {
+    const c10::DeviceGuard guard(in.x.device());
+    MoScan a = scan_args(in);
+    Forward f;
+    f.out = at::empty(in.x.sizes(), in.x.options());
+    f.state = at::empty({a.N, a.C, a.S}, in.x.options().dtype(at::kFloat));
+    a.out = channel_rows(f.out);
+    a.state_out = data(f.state);
+    if (keep) f.saved = work_of(ok(mo_scan_saved(&a), "mo_scan_saved"), in.x);
+    a.saved = data<void>(f.saved);
+    const Tensor work = work_of(ok(mo_scan_work(&a, 0), "mo_scan_work"), in.x);
+    a.work = data<void>(work);
+    ok(mo_scan(&a, stream_of(in.x)), "mo_scan");
+    return f;
+}
+
+struct StateScan : torch::autograd::Function<StateScan> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor dt, Tensor A, Tensor B, Tensor C, Maybe D, Maybe z, Maybe bias, Maybe start, Maybe state) {
+        const ScanIn in{x, dt, A, B, C, sure(D), sure(z), sure(bias), sure(start), sure(state)};
+        Forward f = scan_forward(in, true);
+        ctx->save_for_backward({x, dt, A, B, C, in.D, in.z, in.bias, in.start, in.state, f.saved});
+        ctx->set_materialize_grads(false);
+        return {f.out, f.state};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const ScanIn in{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9]};
+        const c10::DeviceGuard guard(in.x.device());
+        MoScan a = scan_args(in);
+        const Tensor dout = inner(grads[0].defined() ? grads[0] : at::zeros({1}, in.x.options()).expand(in.x.sizes()));
+        const Tensor dlast = contiguous(grads[1]);
+        // inputs that are there, in their order
+        size_t at = 5;
+        const auto wants = [&](const Tensor& t) { return t.defined() && ctx->needs_input_grad(at++); };
+        const bool want_D = wants(in.D);
+        wants(in.z);
+        const bool want_bias = wants(in.bias);
+        wants(in.start);
+        const bool want_state = wants(in.state);
+        const auto like = [](const Tensor& t) { return at::empty(t.sizes(), t.options()); };
+        const auto sums = [&](bool want, const Tensor& t) { return !want ? Tensor() : a.N && a.T ? like(t) : at::zeros(t.sizes(), t.options()); };
+        const Tensor dx = like(in.x), ddt = like(in.dt), dB = like(in.B), dC = like(in.C), dz = in.z.defined() ? like(in.z) : Tensor();
+        const Tensor dA = sums(ctx->needs_input_grad(2), in.A), dD = sums(want_D, in.D), dbias = sums(want_bias, in.bias);
+        const Tensor dstate = want_state ? like(in.state) : Tensor();
+        a.saved = data<void>(s[10]);
+        a.dout = channel_rows(dout); a.dx = channel_rows(dx); a.ddt = channel_rows(ddt); a.dz = channel_rows(dz);
+        a.dB = rows_of(dB); a.dC = rows_of(dC);
+        a.dstate_out = data(dlast);
+        a.dstate = data(dstate); a.dA = data(dA); a.dD = data(dD); a.ddt_bias = data(dbias);
+        const Tensor work = work_of(ok(mo_scan_work(&a, 1), "mo_scan_work"), in.x);
+        a.work = data<void>(work);
+        ok(mo_scan_backward(&a, stream_of(in.x)), "mo_scan_backward");
+        return once({dx, ddt, dA, dB, dC, dD, dz, dbias, Tensor(), dstate});
+    }
+};
+
+ScanIn scan_in(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Maybe& D, const Maybe& z, const Maybe& bias,
+               const Maybe& start, const Maybe& state) {
+    return {inner(x), inner(dt), A.to(at::kFloat).contiguous(), inner(B), inner(C), float_param(D), inner(sure(z)), float_param(bias),
+            contiguous(sure(start)), contiguous(sure(state))};
+}
+std::tuple<Tensor, Tensor> scan(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Maybe& D, const Maybe& z,
+                                const Maybe& bias, const Maybe& start, const Maybe& state) {
+    const ScanIn in = scan_in(x, dt, A, B, C, D, z, bias, start, state);
+    if (wants_grad({in.x, in.dt, in.A, in.B, in.C, in.D, in.z, in.bias, in.state})) {
+        const variable_list out = StateScan::apply(in.x, in.dt, in.A, in.B, in.C, maybe(in.D), maybe(in.z), maybe(in.bias), maybe(in.start), maybe(in.state));
+        return {out[0], out[1]};
+    }
+    const Forward f = scan_forward(in, false);
+    return {f.out, f.state};
+}
+
+Tensor scan_step(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Tensor& state, const Maybe& D, const Maybe& z,
+                 const Maybe& bias, const Maybe& start) {
+    const c10::DeviceGuard guard(x.device());
+    const ScanIn in = scan_in(x, dt, A, B, C, D, z, bias, start, std::nullopt);
+    MoScan a = scan_args(in);
+    const Tensor out = at::empty(x.sizes(), x.options());
+    a.out = channel_rows(out);
+    a.state_out = data(state);
+    ok(mo_scan_step(&a, stream_of(x)), "mo_scan_step");
+    written(state);
+    return out;
+}
+
+// ---------------------------------------------------------------- the gradients' norm
+// Tensors that fill their memory without gaps are taken as they lie; others by a copy, which goes back after scaling. What overlaps in memory is refused.
+Tensor gradient_norm(const std::vector<Tensor>& grads, bool scale, double max_norm, double eps) {
+    const Tensor& first = grads[0];
+    const c10::DeviceGuard guard(first.device());
+    std::vector<Tensor> held;
+    std::vector<MoTensor> list;
+    std::vector<std::pair<char*, char*>> spans;
+    held.reserve(grads.size());
+    list.reserve(grads.size());
+    for (const Tensor& g : grads) {
+        held.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
+        list.push_back({held.back().data_ptr(), held.back().numel(), dtype_of(g), 0});
+        if (!scale || !g.numel()) continue;
+        int64_t last = 0;
+        for (int64_t d = 0; d < g.dim(); d++) last += (g.size(d) - 1) * g.stride(d);
+        spans.push_back({(char*)g.data_ptr(), (char*)g.data_ptr() + (last + 1) * g.element_size()});
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); i++)
+        TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "clip_gradients: two gradients share memory");
+    const Tensor norm = at::empty({}, first.options().dtype(at::kFloat)), work = work_of(ok(mo_gradient_work((int64_t)list.size()), "mo_gradient_work"), first);
+    ok(mo_gradient_norm(list.data(), (int64_t)list.size(), scale, (float)max_norm, (float)eps, data(norm), data<void>(work), stream_of(first)), "mo_gradient_norm");
+    if (scale)
+        for (size_t i = 0; i < grads.size(); i++) {
+            if (held[i].unsafeGetTensorImpl() == grads[i].unsafeGetTensorImpl()) written(grads[i]);
+            else grads[i].copy_(held[i]);
+        }
+    return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_mario_ops_torch, m) {
     m.def("attend", &attend, py::call_guard<py::gil_scoped_release>());
     m.def("attend_step", &attend_step, py::call_guard<py::gil_scoped_release>());
     m.def("group_norm_act", &group_norm_act, py::call_guard<py::gil_scoped_release>());
+    m.def("conv", &conv, py::call_guard<py::gil_scoped_release>());
+    m.def("conv_step", &conv_step, py::call_guard<py::gil_scoped_release>());
+    m.def("scan", &scan, py::call_guard<py::gil_scoped_release>());
+    m.def("scan_step", &scan_step, py::call_guard<py::gil_scoped_release>());
+    m.def("gradient_norm", &gradient_norm, py::call_guard<py::gil_scoped_release>());
 }

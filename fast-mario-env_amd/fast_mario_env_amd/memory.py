@@ -6,10 +6,13 @@ memory of fixed size per env goes on where the stack ends:
 - `linear_attention`: over a stored rollout (T, N), each head's memory a matrix that decays by the head's factor each step and
   is cleared where an episode starts; with the gradients of training.
 - `linear_attention_step`: one step of the same for every env, the memories updated in place: what acting needs.
+- `state_scan`: the same for a memory that selects: a few states a channel whose decays and intake come from the input; with its
+  gradients. `state_scan_step`: one step for every env, in place.
+- `causal_conv_act`, `causal_conv_act_step`: the short convolution over the steps that goes before such a scan, and an activation.
 - `group_norm_act`: group norm and an activation over channels-last features: of the memory's output (a group a head; its size
   grows with the episode) and of convolutions; with its gradients.
 
-`make_memory_net` is an actor-critic that uses them, and `Rollout` (rollout.py) runs it: `act` steps the memories along with the
+`make_memory_net` is an actor-critic that uses them, with either memory, and `Rollout` (rollout.py) runs it: `act` steps the memories along with the
 envs, and calling the network on a stored rollout gives the same policy and values, with gradients.
 
 Float32 or bf16 in and out, sums and states in float32. On the GPU they are HIP kernels (libmario_ops.so, include/mario_ops.h),
@@ -25,7 +28,7 @@ from ._native import ops
 from .rollout import N_ACTIONS, _transformed, policy_input
 
 ACTS = {"none": 0, "relu": 1, "silu": 2}
-MAX_HEAD = 128
+MAX_HEAD, MAX_TAPS, MAX_STATES = 128, 8, 64
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
@@ -154,6 +157,162 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
     if not _kernel_takes(*((x,) if weight is None else (x, weight, bias))):
         return _norm_plain(x, groups, weight, bias, eps, act)
     return ops().group_norm_act(x, groups, weight, bias, eps, ACTS[act])
+
+
+# ---------------------------------------------------------------- a memory that selects: causal convolution
+def _check_conv(name, lead, x, weight, bias, start, state, act):
+    C, dev = x.shape[-1], x.device
+    if x.dtype not in _DTYPES or C < 1:
+        raise ValueError(f"{name}: x must be ({lead}, C) float32 or bf16")
+    if weight.dim() != 2 or weight.shape[0] != C or not 1 <= weight.shape[1] <= MAX_TAPS or not weight.is_floating_point():
+        raise ValueError(f"{name}: weight must be (C, K) = ({C}, 1 .. {MAX_TAPS})")
+    if bias is not None and (bias.shape != (C,) or not bias.is_floating_point()):
+        raise ValueError(f"{name}: bias must be ({C},)")
+    if start is not None and (start.dtype != torch.bool or start.shape != x.shape[:-1]):
+        raise ValueError(f"{name}: start must be ({lead}) bool")
+    if state is not None and (state.dtype != x.dtype or state.shape != (x.shape[-2], weight.shape[1] - 1, C)):
+        raise ValueError(f"{name}: state must be (N, K - 1, C) = {(x.shape[-2], weight.shape[1] - 1, C)} in the type of x")
+    if act not in ACTS:
+        raise ValueError(f"{name}: act must be one of {', '.join(ACTS)}")
+    for t in (weight, bias, start, state):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: all tensors must be on the device of x ({dev})")
+
+
+def _conv_plain(x, weight, bias, start, state, act):
+    """The window moved step by step in torch operations, in float32."""
+    K = weight.shape[1]
+    w = weight.float().t()
+    window = x.new_zeros(x.shape[1], K - 1, x.shape[2]) if state is None else state
+    out = []
+    for t in range(x.shape[0]):
+        if start is not None:
+            window = torch.where(start[t][:, None, None], torch.zeros_like(window), window)
+        every = torch.cat([window, x[t][:, None]], 1)
+        p = (every.float() * w).sum(1)
+        p = p if bias is None else p + bias.float()
+        out.append(p.clamp(min=0.0) if act == "relu" else p * torch.sigmoid(p) if act == "silu" else p)
+        window = every[:, 1:]
+    out = torch.stack(out).to(x.dtype) if out else x.new_empty(x.shape)
+    return out, window.clone() if window is state else window
+
+
+def causal_conv_act(x, weight, bias=None, start=None, state=None, act="silu"):
+    """A short convolution of each channel over the steps, then act, over T steps of N envs. With K taps:
+
+        y_t = act(bias + sum_j weight[:, K - 1 - j] x_{t-j}),   j = 0 .. K - 1, of what the episode of step t holds
+
+    x (T, N, C) float32 or bf16, any strides; weight (C, K), K up to 8, and bias (C,) or None float32 (other float types are converted);
+    start (T, N) bool, the steps that start an episode: no tap reaches past one; state (N, K - 1, C) in the type of x, the inputs before
+    the first step, oldest first, None for zeros; act "none", "relu" or "silu". Returns y (T, N, C) in the type of x and the state after
+    the last step (0 for what its episode does not hold). Sums in float32, rounded once. Differentiable once in x, weight, bias and state."""
+    if x.dim() != 3:
+        raise ValueError("causal_conv_act: x must be (T, N, C)")
+    _check_conv("causal_conv_act", "T, N", x, weight, bias, start, state, act)
+    if not _kernel_takes(*(t for t in (x, weight, bias, start, state) if t is not None)):
+        return _conv_plain(x, weight, bias, start, state, act)
+    return ops().conv(x, weight, bias, start, state, ACTS[act])
+
+
+def causal_conv_act_step(x, weight, bias, state, start=None, act="silu"):
+    """One step of `causal_conv_act` for every env: x (N, C), start (N,) bool or None; state (N, K - 1, C), contiguous, moves on by the step in
+    place. Returns y (N, C). No gradient."""
+    if x.dim() != 2:
+        raise ValueError("causal_conv_act_step: x must be (N, C)")
+    _check_conv("causal_conv_act_step", "N", x, weight, bias, start, state, act)
+    if state is None or not state.is_contiguous():
+        raise ValueError("causal_conv_act_step: state is updated in place and must be contiguous")
+    _no_gradient("causal_conv_act_step", "causal_conv_act", x, weight, bias, state)
+    if not _kernel_takes(*(t for t in (x, weight, bias, start, state) if t is not None)):
+        y, last = _conv_plain(x[None], weight, bias, None if start is None else start[None], state, act)
+        state.copy_(last)
+        return y[0]
+    return ops().conv_step(x, weight, bias, state, start, ACTS[act])
+
+
+def _no_gradient(name, instead, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), or {instead} to train")
+
+
+# ---------------------------------------------------------------- a memory that selects: state space scan
+def _check_scan(name, lead, x, dt, A, B, C, D, z, dt_bias, start, state):
+    ch, dev = x.shape[-1], x.device
+    if x.dtype not in _DTYPES or ch < 1 or any(t is not None and (t.dtype != x.dtype or t.shape != x.shape) for t in (dt, z)):
+        raise ValueError(f"{name}: x, dt and z must be ({lead}, C), all float32 or all bf16")
+    if A.dim() != 2 or A.shape[0] != ch or not 1 <= A.shape[1] <= MAX_STATES or not A.is_floating_point():
+        raise ValueError(f"{name}: A must be (C, S) = ({ch}, 1 .. {MAX_STATES})")
+    S = A.shape[1]
+    if (B.dim() != x.dim() + 1 or B.shape != C.shape or B.shape[:-2] != x.shape[:-1] or B.shape[-1] != S or B.dtype != x.dtype
+            or C.dtype != x.dtype or B.shape[-2] < 1 or ch % B.shape[-2]):
+        raise ValueError(f"{name}: B and C must be ({lead}, G, {S}) in the type of x, G a divisor of {ch}")
+    for n, t in (("D", D), ("dt_bias", dt_bias)):
+        if t is not None and (t.shape != (ch,) or not t.is_floating_point()):
+            raise ValueError(f"{name}: {n} must be ({ch},)")
+    if start is not None and (start.dtype != torch.bool or start.shape != x.shape[:-1]):
+        raise ValueError(f"{name}: start must be ({lead}) bool")
+    if state is not None and (state.dtype != torch.float32 or state.shape != (x.shape[-2], ch, S)):
+        raise ValueError(f"{name}: state must be (N, C, S) = {(x.shape[-2], ch, S)} float32")
+    for t in (dt, A, B, C, D, z, dt_bias, start, state):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: all tensors must be on the device of x ({dev})")
+
+
+def _scan_plain(x, dt, A, B, C, D, z, dt_bias, start, state):
+    """The recurrence step by step in torch operations, in float32."""
+    T, N, ch = x.shape
+    h = x.new_zeros((N,) + A.shape, dtype=torch.float32) if state is None else state
+    A, rep, out = A.float(), ch // B.shape[2], []
+    for t in range(T):
+        xt, raw = x[t].float(), dt[t].float() if dt_bias is None else dt[t].float() + dt_bias.float()
+        d = torch.logaddexp(raw, torch.zeros_like(raw))
+        a = torch.exp(d[..., None] * A) * h
+        if start is not None:
+            a = torch.where(start[t][:, None, None], torch.zeros_like(a), a)
+        h = a + (d * xt)[..., None] * B[t].float().repeat_interleave(rep, 1)
+        y = (C[t].float().repeat_interleave(rep, 1) * h).sum(-1)
+        y = y if D is None else y + D.float() * xt
+        if z is not None:
+            zt = z[t].float()
+            y = y * (zt * torch.sigmoid(zt))
+        out.append(y)
+    out = torch.stack(out).to(x.dtype) if out else x.new_empty(x.shape)
+    return out, h.clone() if h is state else h
+
+
+def state_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, start=None, state=None):
+    """A selective state space scan over T steps of N envs: what a channel's states keep and take up depends on the input. Of each env and
+    channel, with d = softplus(dt + dt_bias) and B, C those of the channel's group:
+
+        h_t = (0 where start[t], else exp(d_t A) h_{t-1}) + d_t x_t B_t,    y_t = (C_t . h_t + D x_t) silu(z_t),    h_{-1} = state
+
+    x, dt and z (T, N, C) (z None: no factor), B and C (T, N, G, S), G a divisor of C (groups of C / G neighbouring channels), all float32 or all
+    bf16, any strides; A (C, S), S up to 64, none above 0, D and dt_bias (C,) or None float32 (other float types are converted); start (T, N)
+    bool: nothing of an episode reaches the next one; state (N, C, S) float32 or None for zeros. Returns y (T, N, C) in the type of x and the state
+    after the last step, float32. States, step sizes, decays and sums are float32, results rounded once. Differentiable once in all but start."""
+    if x.dim() != 3:
+        raise ValueError("state_scan: x must be (T, N, C)")
+    _check_scan("state_scan", "T, N", x, dt, A, B, C, D, z, dt_bias, start, state)
+    if not _kernel_takes(*(t for t in (x, dt, A, B, C, D, z, dt_bias, start, state) if t is not None)):
+        return _scan_plain(x, dt, A, B, C, D, z, dt_bias, start, state)
+    return ops().scan(x, dt, A, B, C, D, z, dt_bias, start, state)
+
+
+def state_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, start=None):
+    """One step of `state_scan` for every env: x, dt, z (N, C), B and C (N, G, S), start (N,) bool or None; state (N, C, S) float32,
+    contiguous, is updated in place. Returns y (N, C) in the type of x. No gradient."""
+    if x.dim() != 2:
+        raise ValueError("state_scan_step: x must be (N, C)")
+    _check_scan("state_scan_step", "N", x, dt, A, B, C, D, z, dt_bias, start, state)
+    if state is None or not state.is_contiguous():
+        raise ValueError("state_scan_step: state is updated in place and must be contiguous")
+    _no_gradient("state_scan_step", "state_scan", x, dt, A, B, C, D, z, dt_bias, state)
+    if not _kernel_takes(*(t for t in (x, dt, A, B, C, D, z, dt_bias, start, state) if t is not None)):
+        one = lambda t: None if t is None else t[None]   # noqa: E731
+        y, last = _scan_plain(x[None], dt[None], A, B[None], C[None], D, one(z), dt_bias, one(start), state)
+        state.copy_(last)
+        return y[0]
+    return ops().scan_step(x, dt, A, B, C, state, D, z, dt_bias, start)
 
 
 # ---------------------------------------------------------------- an actor-critic with a memory

@@ -15,6 +15,7 @@ half of its trainer (src/fast_mario_env/ppo/backends.py:127-162, ppo/train.py:12
   observation stacks of those envs. As in the reference, finding them costs one small host sync per step.
 - A network with a memory (memory.py's `make_memory_net`) steps its memories along with the envs, cleared at episode starts;
   `sequence` gives what it was shown, and the memories it began with, for training.
+- `clip_gradients`, `gradient_norm`: the norm of all gradients together, and their scaling by it.
 - `gae`: generalized advantage estimation over the stored rewards, values and episode starts, with the
   reference's convention (train.py:140-150): the bootstrap of step t is cut where step t + 1 starts an episode.
 
@@ -334,6 +335,70 @@ def gae(rew, val, start, next_val, next_start, gamma: float = 0.99, lam: float =
         last = delta + (gamma * lam) * keep * last
         adv[t] = last
     return adv, adv + val
+
+
+def _gradients(parameters, name):
+    """The gradients of tensors (one, or an iterable), each once: float32 or bf16 on one GPU, as the kernels take them, or any on the CPU."""
+    torch = _torch()
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    seen, grads = set(), []
+    for p in parameters:
+        g = p.grad
+        if g is None or id(g) in seen:
+            continue
+        seen.add(id(g))
+        grads.append(g)
+    for g in grads:
+        if g.layout != torch.strided or not g.is_floating_point() or g.device != grads[0].device:
+            raise ValueError(f"{name}: gradients must be dense float tensors on one device")
+        if g.is_cuda and g.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{name}: gradients on the GPU must be float32 or bf16")
+        if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+            raise ValueError(f"{name}: a gradient shares elements with itself (expanded)")
+    return grads
+
+
+def _norm_kernel_takes(grads):
+    torch = _torch()
+    return bool(grads) and all(type(g) is torch.Tensor and g.is_cuda and not g.is_neg() for g in grads) and not _transformed(*grads)
+
+
+def _norm_plain(grads):
+    torch = _torch()
+    if not grads:
+        return torch.zeros((), dtype=torch.float64)
+    return torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt()
+
+
+def gradient_norm(parameters):
+    """The 2-norm of all gradients of `parameters` (a tensor or an iterable) together, a float32 scalar on their device: squares are summed
+    in float64, so neither large nor tiny values overflow or vanish. Parameters without a gradient count nothing, one that is passed twice
+    counts once. Nothing waits for the GPU; with no gradients at all the result is 0, on the CPU."""
+    grads = _gradients(parameters, "gradient_norm")
+    if _norm_kernel_takes(grads):
+        from ._native import ops
+        return ops().gradient_norm(grads, False, 0.0, 0.0)
+    return _norm_plain(grads).float()
+
+
+def clip_gradients(parameters, max_norm: float, eps: float = 1e-6):
+    """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + eps)), norm that of `gradient_norm`, which is returned: what a
+    training step does between backward and the optimizer. A norm that is NaN or infinite makes
+    gradients NaN or 0 by the same formula; look at the norm. Gradients that share memory are refused."""
+    if not (max_norm >= 0 and eps >= 0):
+        raise ValueError("clip_gradients: max_norm and eps must be >= 0")
+    torch = _torch()
+    grads = _gradients(parameters, "clip_gradients")
+    with torch.no_grad():
+        if _norm_kernel_takes(grads):
+            from ._native import ops
+            return ops().gradient_norm(grads, True, float(max_norm), float(eps))
+        norm = _norm_plain(grads)
+        by = (max_norm / (norm + eps)).clamp(max=1.0).float()
+        for g in grads:
+            g.copy_(g.float() * by if g.dtype != torch.float64 else g * by)
+        return norm.float()
 
 
 def _steps_memories(net) -> bool:

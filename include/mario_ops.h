@@ -3,7 +3,8 @@
  * No counterpart in the reference: its policy sees four stacked frames and keeps nothing between steps
  * (ppo/model.py:13-38). These are the operators that a policy needs which remembers the episode: linear attention with a
  * decay for each head, over a stored rollout (with its gradient) and for the single steps of acting, and the group norm with
- * an activation that follows it and the trunk's convolutions.
+ * an activation that follows it and the trunk's convolutions; a memory that selects, a state space scan whose decays come from its
+ * inputs, with the causal convolution before it, in the same forms; and the norm of all gradients, by which training clips them.
  *
  * Conventions, as in mario_hip.h: plain C types; `stream` is a hipStream_t; every buffer is the caller's memory of the
  * current GPU (device, pinned host or managed), aligned to its elements; functions returning int return 0, or -1 with
@@ -96,6 +97,90 @@ typedef struct MoNorm {
 int64_t mo_group_norm_work(const MoNorm* a, int backward);
 int mo_group_norm(const MoNorm* a, void* stream);
 int mo_group_norm_backward(const MoNorm* a, void* stream);
+
+/* Causal convolution of each channel over the steps, with an activation. Of env n and channel c, K taps:
+ *   y_t = act(bias_c + sum_j weight[c, K - 1 - j] x_{t-j}),  j = 0 .. K - 1, of what the episode of step t holds: terms from before
+ * an episode's start are left out, and steps before the first one are the rows of state.
+ *   dtype     MO_F32 or MO_BF16 (of x, y, the states and their gradients);   act MO_ACT_*;   C >= 1, 1 <= K <= MO_MAX_TAPS, T, N >= 0
+ *   x, y      (T, N, C), channels contiguous; MoRows.sh is not used
+ *   weight    (C, K) float32;   bias (C) float32 or NULL
+ *   start     (T, N) bytes, as above, or NULL
+ *   state     (N, K - 1, C) contiguous: the last K - 1 inputs, oldest first; NULL: zeros
+ *   state_out the same after the last step, 0 where its episode holds no input; must not overlap state; NULL: not wanted
+ * The gradient: dy (T, N, C) and dstate_out (N, K - 1, C; NULL: zeros) in; dx (T, N, C), dstate (N, K - 1, C; NULL: not wanted), dweight (C, K)
+ * and dbias (C) (both NULL: not wanted) out; work mo_conv_work() bytes, 16-byte aligned, free once the queued work is done. Sums are
+ * float32 in a fixed order. */
+#define MO_MAX_TAPS 8
+typedef struct MoConv {
+    int32_t dtype, act, C, K;
+    int64_t T, N;
+    MoRows x, y;
+    const float *weight, *bias;
+    const uint8_t* start;
+    const void* state;
+    void* state_out;
+    void* work;
+    MoRows dy, dx;
+    const void* dstate_out;
+    void* dstate;
+    float *dweight, *dbias;
+} MoConv;
+
+int64_t mo_conv_work(const MoConv* a);
+int mo_conv(const MoConv* a, void* stream);
+int mo_conv_backward(const MoConv* a, void* stream);
+
+/* One step of the same: T is not looked at, x, y (N, C), start (N) or NULL; state_out is read, shifted and written (state is not used). */
+int mo_conv_step(const MoConv* a, void* stream);
+
+/* A selective state space scan. Of env n, channel c (in group g of C / G neighbouring ones) and state s:
+ *   d_t = softplus(dt_t + dt_bias_c),   h_t = (0 where start[t, n], else exp(d_t A[c, s]) h_{t-1}) + d_t x_t B_t[g, s],
+ *   out_t = (sum_s C_t[g, s] h_t + D_c x_t) silu(z_t),   h_{-1} = state
+ * States, decays, sums and step sizes d are float32 throughout.
+ *   dtype     MO_F32 or MO_BF16 (of x, dt, z, B, C, out and their gradients)
+ *   C >= 1, 1 <= S <= MO_MAX_STATES, G >= 1 a divisor of C, T >= 0, N >= 0
+ *   x, dt, z, out  (T, N, C), channels contiguous, MoRows.sh not used; z.p NULL: no factor of z
+ *   Bt, Ct    (T, N, G, S), states contiguous, MoRows.sh the groups' stride
+ *   A         (C, S) float32, none above 0 (a memory that grows may overflow earlier than step by step);   D, dt_bias (C) float32 or NULL (0)
+ *   start, state, state_out  as for linear attention, states (N, C, S) float32 contiguous
+ *   saved     mo_scan_saved() bytes, 16-byte aligned, for mo_scan_backward to take up, or NULL: no gradient is wanted
+ *   work      mo_scan_work() bytes, 16-byte aligned, free once the queued work is done
+ * The gradient: dout and dstate_out (NULL: zeros) in, saved as the forward call left it; dx, ddt, dz (if z), dB, dC out; dstate (NULL: not
+ * wanted) and dA, dD, ddt_bias float32 (each NULL: not wanted) out. Sums have a fixed order: the same inputs give the same bits. */
+#define MO_MAX_STATES 64
+typedef struct MoScan {
+    int32_t dtype, C, S, G;
+    int64_t T, N;
+    MoRows x, dt, z, Bt, Ct, out;
+    const float *A, *D, *dt_bias;
+    const uint8_t* start;
+    const float* state;
+    float* state_out;
+    void* saved;
+    void* work;
+    MoRows dout, dx, ddt, dz, dB, dC;
+    const float* dstate_out;
+    float *dstate, *dA, *dD, *ddt_bias;
+} MoScan;
+
+int64_t mo_scan_saved(const MoScan* a);
+int64_t mo_scan_work(const MoScan* a, int backward);
+int mo_scan(const MoScan* a, void* stream);
+int mo_scan_backward(const MoScan* a, void* stream);
+
+/* One step of the same: T is not looked at, x, dt, z, out (N, C), Bt, Ct (N, G, S), start (N) or NULL; state_out (N, C, S) is read and
+ * written (state is not used). A starting env's old state is not read. */
+int mo_scan_step(const MoScan* a, void* stream);
+
+/* The norm of many tensors together, norm = sqrt(sum of all values' squares), and with `scale` their values times
+ * min(1, max_norm / (norm + eps)) in place, rounded once. Squares are summed in float64 in a fixed order, so neither large nor tiny
+ * values overflow or vanish.
+ *   t         count >= 0 tensors in host memory (not needed after the call): n values of a type at p, contiguous; none overlaps another
+ *   norm      one float32;   work mo_gradient_work() bytes, 16-byte aligned, free once the queued work is done */
+typedef struct MoTensor { void* p; int64_t n; int32_t dtype, reserved; } MoTensor;
+
+int64_t mo_gradient_work(int64_t count);
+int mo_gradient_norm(const MoTensor* t, int64_t count, int scale, float max_norm, float eps, float* norm, void* work, void* stream);
 
 #ifdef __cplusplus
 #pragma GCC visibility pop
