@@ -1,25 +1,30 @@
 // The selective state space scan over the steps of a rollout.
 #pragma once
+#include <utility>
+
 #include "sums.hpp"
 
 namespace mo {
 
 // A wave has 64 channels of one env, a lane all of a channel's states (or SP of them: then up to four waves share the channels and join their
-// sums in LDS). B and C are the same for all lanes: they lie packed in float32 (k_scan_pack) and come as scalar loads, so a step of a
-// state is one exponential, two products and two fused multiply-adds on registers.
+// sums in LDS). B and C are the same for all lanes: they lie packed in float32 (k_scan_pack) and come as scalar loads a step ahead, so a step of a
+// state is one exponential, two products and two fused multiply-adds on registers. x, dt and z come in 16-byte pieces of whole rows, a
+// chunk of steps ahead, and go to their lanes through LDS; results leave the same way.
 constexpr int SCAN_STEPS = 8;        // steps of a chunk: between two kept states
 constexpr int SCAN_WAVES = 4;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct Scan {
     MoScan a;
-    const float* bc;                 // (T, N, G, 2, SB): B and C padded with zeros to whole slices
+    const float* bc;                 // (whole chunks of steps and a step more, N, G, 2, SB): B and C padded with zeros to whole slices
     float* kept;                     // (chunks, N, SB, C): the states before each chunk, for the gradient; or null
     float *seg_h, *seg_d;            // (segments, N, SB, C), (segments, N, C): see k_scan_enter
-    float *part_bc, *part;           // (gradient) (per, T, N, G, 2, SB), (rows, SB + 2, C)
+    float *part_bc, *part;           // (gradient) (cuts, T, N, G, 2, SB), (rows, SB + 2, C)
     int64_t chunks, each, segments;  // chunks of all steps, and of a segment
     int64_t rows;                    // (gradient) envs' segments that are taken at a time
     int slices, SB, Cg, per;         // waves that share channels, states padded, channels of a group, waves that span them
+    int across, cuts;                // (gradient) waves of channels a workgroup, workgroups of a group's channels
+    int wide;                        // all rows of channels lie on 16 bytes, in whole pieces
 };
 
 typedef const float __attribute__((address_space(4))) * Uniform;   // read by scalar loads: the same for all lanes, not written meanwhile
@@ -42,66 +47,149 @@ __device__ __forceinline__ Size softplus(float r) {
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp2_raw(-z * LOG2E)); }
 
 // B and C of every step in float32, padded.
+__host__ __device__ __forceinline__ int64_t scan_rows(const Scan& k) { return k.chunks * SCAN_STEPS + 1; }
 template <class T> __global__ void __launch_bounds__(256) k_scan_pack(Scan k, float* bc) {
     const MoScan& a = k.a;
     const int64_t id = block_here() * 256 + threadIdx.x, row = id / (2 * k.SB);
-    if (row >= a.T * a.N * a.G) return;
     const int i = (int)(id % (2 * k.SB)), s = i % k.SB, g = (int)(row % a.G);
     const int64_t n = row / a.G % a.N, t = row / a.G / a.N;
+    if (t >= scan_rows(k)) return;
     const MoRows& r = i < k.SB ? a.Bt : a.Ct;
-    bc[id] = s < a.S ? as_f32(((const T*)r.p)[t * r.st + n * r.sn + g * r.sh + s]) : 0.f;
+    bc[id] = t < a.T && s < a.S ? as_f32(((const T*)r.p)[t * r.st + n * r.sn + g * r.sh + s]) : 0.f;
 }
 
 // What a wave works on.
 struct ScanPlace {
     int64_t n, segment;
-    int g, c, lane, s0;              // group, this lane's channel, its first state
+    int g, c0, c, lane, s0, there;   // group, first channel, this lane's, its first state, channels that there are
     bool live;
-    __device__ __forceinline__ ScanPlace(const Scan& k, int64_t wave, int slice, int SP) {
-        const int cbs = k.a.G * k.per, cb = (int)(wave % cbs);
-        const int64_t rest = wave / cbs;
-        n = rest % k.a.N;
-        segment = rest / k.a.N;
+    __device__ __forceinline__ ScanPlace(const Scan& k, int64_t item, int cb, int slice, int SP) {
+        n = item % k.a.N;
+        segment = item / k.a.N;
         g = cb / k.per;
         lane = threadIdx.x % kWave;
-        const int i = cb % k.per * kWave + lane;
-        live = i < k.Cg;
-        c = g * k.Cg + (live ? i : k.Cg - 1);
+        const int i = cb % k.per * kWave;
+        there = min(kWave, k.Cg - i);
+        live = lane < there;
+        c0 = g * k.Cg + i;
+        c = c0 + min(lane, there - 1);
         s0 = slice * SP;
     }
 };
 __device__ __forceinline__ int wave_here() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+// The wave's own LDS: what its lanes wrote is there for its other lanes.
+__device__ __forceinline__ void wave_wrote() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
-template <class T> __device__ __forceinline__ float at_row(const MoRows& r, int64_t t, int64_t n, int c) {
-    return as_f32(((const T*)r.p)[t * r.st + n * r.sn + c]);
-}
-template <class T> __device__ __forceinline__ void to_row(const MoRows& r, int64_t t, int64_t n, int c, float x) {
-    ((T*)r.p)[t * r.st + n * r.sn + c] = as<T>(x);
-}
-// Which of the SCAN_STEPS steps from t0 start an episode, as bits.
-__device__ __forceinline__ unsigned starts_from(const MoScan& a, int64_t t0, int steps, int64_t n, int lane) {
-    if (!a.start) return 0;
-    return (unsigned)__ballot(lane < steps && a.start[(t0 + lane) * a.N + n]);
-}
-template <int SP> __device__ __forceinline__ void load_decays(const MoScan& a, int c, int s0, float (&A)[SP]) {
+// A chunk's rows of 64 channels, zeros where there are none (rows past the last step, channels past the group's). Wide: in 16-byte pieces through
+// registers (ahead of their use); else an element a lane. Where there are none, a place that there is is read and not used: no branches.
+template <class T> struct ChunkIn {
+    static constexpr int EPV = 16 / sizeof(T), PR = kWave / EPV, ROWS = kWave / PR, N = SCAN_STEPS / ROWS;
+    uint4 v[N];
+    static __device__ __forceinline__ T* piece(const MoRows& r, int64_t t0, const ScanPlace& me, int row) {
+        const int p = me.lane % PR * EPV;
+        return (T*)r.p + t0 * r.st + me.n * r.sn + me.c0 + row * r.st + (p < me.there ? p : 0);
+    }
+    __device__ __forceinline__ void ahead(const MoRows& r, int64_t t0, int steps, const ScanPlace& me) {
 #pragma unroll
-    for (int s = 0; s < SP; s++) A[s] = s0 + s < a.S ? a.A[(int64_t)c * a.S + s0 + s] * LOG2E : 0.f;
+        for (int i = 0; i < N; i++) v[i] = *(const uint4*)piece(r, t0, me, min(me.lane / PR + i * ROWS, steps - 1));
+    }
+    __device__ __forceinline__ void arrive(T* to, int steps, const ScanPlace& me, uint32_t none = 0) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const bool there = me.lane / PR + i * ROWS < steps && me.lane % PR * EPV < me.there;
+            *(uint4*)(to + (i * kWave + me.lane) * EPV) = there ? v[i] : uint4{none, none, none, none};
+        }
+    }
+    static __device__ __forceinline__ void narrow(T* to, const MoRows& r, int64_t t0, int steps, const ScanPlace& me, float none = 0.f) {
+        const T* p = (const T*)r.p + t0 * r.st + me.n * r.sn + me.c;
+        T x[SCAN_STEPS];
+#pragma unroll
+        for (int i = 0; i < SCAN_STEPS; i++) {
+            x[i] = *p;
+            if (i + 1 < steps) p += r.st;
+        }
+#pragma unroll
+        for (int i = 0; i < SCAN_STEPS; i++) to[i * kWave + me.lane] = me.live && i < steps ? x[i] : as<T>(none);
+    }
+    // the other way, from LDS to memory
+    static __device__ __forceinline__ void leave(const T* from, const MoRows& r, int64_t t0, int steps, const ScanPlace& me, bool wide) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (me.lane / PR + i * ROWS < steps && me.lane % PR * EPV < me.there)
+                    stream((uint4*)piece(r, t0, me, me.lane / PR + i * ROWS), *(const uint4*)(from + (i * kWave + me.lane) * EPV));
+        } else if (me.live) {
+            T* p = (T*)r.p + t0 * r.st + me.n * r.sn + me.c;
+            for (int i = 0; i < steps; i++, p += r.st) *p = from[i * kWave + me.lane];
+        }
+    }
+};
+// In the place of a dt that is not there: minus infinity, a step of no size, which changes nothing.
+template <class T> constexpr uint32_t NO_SIZE = 0xff800000u;
+template <> inline constexpr uint32_t NO_SIZE<bf16> = 0xff80ff80u;
+// Which of the SCAN_STEPS steps from t0 start an episode: lane i has step i's flag.
+__device__ __forceinline__ uint8_t start_of_lane(const MoScan& a, int64_t t0, int steps, const ScanPlace& me) {
+    return a.start && me.lane < steps ? a.start[(t0 + me.lane) * a.N + me.n] : 0;
 }
+template <int SP> __device__ __forceinline__ void load_decays(const MoScan& a, const ScanPlace& me, float (&A)[SP]) {
+#pragma unroll
+    for (int s = 0; s < SP; s++) A[s] = me.live && me.s0 + s < a.S ? a.A[(int64_t)me.c * a.S + me.s0 + s] * LOG2E : 0.f;
+}
+// A step's B and C, in scalar registers. Loaded a step ahead; nothing moves over the end of a step, or all steps' loads would come first and
+// take more registers than there are.
+template <int SP> struct StepBC { float b[SP], c[SP]; };
+template <int SP, bool WITH_C = true> __device__ __forceinline__ void load_bc(StepBC<SP>& v, Uniform p, int SB) {
+#pragma unroll
+    for (int s = 0; s < SP; s++) {
+        v.b[s] = p[s];
+        if (WITH_C) v.c[s] = p[SB + s];
+    }
+}
+// Where bit I of cuts is set: h = u b, for all states. A branch of the whole wave that the compiler does not see: the steps stay one block.
+template <int I, int SP> __device__ __forceinline__ void if_start_set(unsigned cuts, float (&h)[SP], float u, const float (&b)[SP]) {
+#pragma unroll
+    for (int s = 0; s < SP; s += 4)
+        asm volatile(
+            "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\tv_mul_f32 %0, %[u], %4\n\tv_mul_f32 %1, %[u], %5\n\t"
+            "v_mul_f32 %2, %[u], %6\n\tv_mul_f32 %3, %[u], %7\n.Lstart%=:"
+            : "+v"(h[s]), "+v"(h[s + 1]), "+v"(h[s + 2]), "+v"(h[s + 3])
+            : "s"(b[s]), "s"(b[s + 1]), "s"(b[s + 2]), "s"(b[s + 3]), [u] "v"(u), [m] "s"(cuts), [i] "n"(I)
+            : "scc");
+}
+template <class F, int... I> __device__ __forceinline__ void each_step_of(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <class F> __device__ __forceinline__ void each_step(F f) { each_step_of(f, std::make_integer_sequence<int, SCAN_STEPS>{}); }
+// p + by, known only from here on: the loads behind it come no earlier.
+__device__ __forceinline__ Uniform move_on(Uniform p, int64_t by) {
+    uint64_t q = (uint64_t)(p + by);
+    asm volatile("" : "+s"(q));
+    return (Uniform)q;
+}
+// What a step made is made here, not where it is used.
+__device__ __forceinline__ void made(float& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void end_of_step() { __builtin_amdgcn_sched_barrier(0); }
 
 // Forward. SUMS: only what a segment adds to an entering state: its last states from zero, and the sum of its step sizes (-1 where an episode
 // starts in it: nothing of what enters is left).
 template <class T, int SP, bool SPLIT, bool SUMS>
 __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
     const MoScan& a = k.a;
-    __shared__ float part[SPLIT ? SCAN_WAVES : 1][SCAN_STEPS][kWave];
-    const int w = wave_here(), slice = SPLIT ? w : 0;
+    constexpr int TILE = SCAN_STEPS * kWave;
+    __shared__ __attribute__((aligned(16))) T tiles[SCAN_WAVES][SUMS ? 2 : 3][TILE];
+    __shared__ float part[SPLIT && !SUMS ? SCAN_WAVES : 1][SCAN_STEPS][kWave];
+    const int w = wave_here(), slice = SPLIT ? w : 0, cbs = a.G * k.per;
     const int64_t wave = SPLIT ? block_here() : block_here() * SCAN_WAVES + w;
-    if (wave >= k.segments * a.N * a.G * k.per) return;
-    const ScanPlace me(k, wave, slice, SP);
+    if (wave >= k.segments * a.N * cbs) return;
+    const ScanPlace me(k, wave / cbs, (int)(wave % cbs), slice, SP);
     const int64_t n = me.n, first = me.segment * k.each, last = min(k.chunks, first + k.each);
-    const int c = me.c;
+    const int c = me.c, lane = me.lane;
+    T *lx = tiles[w][0], *ldt = tiles[w][1], *lz = tiles[w][SUMS ? 0 : 2];
+    const bool gate = !SUMS && a.z.p;
     float A[SP], h[SP], total = 0.f;
-    load_decays<SP>(a, c, me.s0, A);
+    load_decays<SP>(a, me, A);
     const int64_t seg0 = ((me.segment * a.N + n) * k.SB + me.s0) * a.C + c;
 #pragma unroll
     for (int s = 0; s < SP; s++) {
@@ -110,53 +198,99 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
         else h[s] = a.state && me.s0 + s < a.S ? a.state[(n * a.C + c) * a.S + me.s0 + s] : 0.f;
     }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, D = a.D ? a.D[c] : 0.f;
-    const auto finish = [&](int64_t t, float y) {
-        y = fmaf(D, a.D ? at_row<T>(a.x, t, n, c) : 0.f, y);
-        if (a.z.p) {
-            const float z = at_row<T>(a.z, t, n, c);
-            y *= z * sigmoid(z);
-        }
-        if (me.live) to_row<T>(a.out, t, n, c, y);
+    ChunkIn<T> ix, idt, iz;
+    uint8_t flag = 0;
+    const auto steps_of = [&](int64_t chunk) { return (int)min((int64_t)SCAN_STEPS, a.T - chunk * SCAN_STEPS); };
+    const auto ahead = [&](int64_t chunk) {
+        const int64_t t0 = chunk * SCAN_STEPS;
+        const int steps = steps_of(chunk);
+        flag = start_of_lane(a, t0, steps, me);
+        if (!k.wide) return;
+        ix.ahead(a.x, t0, steps, me);
+        idt.ahead(a.dt, t0, steps, me);
+        if (gate) iz.ahead(a.z, t0, steps, me);
     };
+    if (first < last) ahead(first);
+    const int64_t bc_step = a.N * a.G * 2 * k.SB;
+    Uniform bc = uniform(k.bc + ((first * SCAN_STEPS * a.N + n) * a.G + me.g) * 2 * k.SB + me.s0);
+    StepBC<SP> now;
+    if (first < last) load_bc<SP, !SUMS>(now, bc, k.SB);
     for (int64_t chunk = first; chunk < last; chunk++) {
         const int64_t t0 = chunk * SCAN_STEPS;
-        const int steps = (int)min((int64_t)SCAN_STEPS, a.T - t0);
-        const unsigned cuts = starts_from(a, t0, steps, n, me.lane);
+        const int steps = steps_of(chunk);
+        const unsigned cuts = (unsigned)__ballot(flag != 0);
+        wave_wrote();                                         // (the last chunk's results have been read)
+        if (k.wide) {
+            ix.arrive(lx, steps, me);
+            idt.arrive(ldt, steps, me, NO_SIZE<T>);
+            if (gate) iz.arrive(lz, steps, me);
+        } else {
+            ChunkIn<T>::narrow(lx, a.x, t0, steps, me);
+            ChunkIn<T>::narrow(ldt, a.dt, t0, steps, me, -INFINITY);
+            if (gate) ChunkIn<T>::narrow(lz, a.z, t0, steps, me);
+        }
+        wave_wrote();
+        if (chunk + 1 < last) ahead(chunk + 1);
         if (!SUMS && k.kept && me.live) {
             float* to = k.kept + ((chunk * a.N + n) * k.SB + me.s0) * a.C + c;
 #pragma unroll
-            for (int s = 0; s < SP; s++) to[(int64_t)s * a.C] = h[s];
+            for (int s = 0; s < SP; s++) __builtin_nontemporal_store(h[s], to + (int64_t)s * a.C);
         }
+        // Nothing but the scalar loads of B and C is waited for between the steps.
+        float d[SCAN_STEPS], u[SCAN_STEPS];
 #pragma unroll
         for (int i = 0; i < SCAN_STEPS; i++) {
-            if (i >= steps) break;
-            const int64_t t = t0 + i;
-            const float x = at_row<T>(a.x, t, n, c), d = softplus(at_row<T>(a.dt, t, n, c) + bias).d, u = d * x;
-            const Uniform B = uniform(k.bc + ((t * a.N + n) * a.G + me.g) * 2 * k.SB + me.s0), C = B + k.SB;
-            if (cuts >> i & 1) {
-#pragma unroll
-                for (int s = 0; s < SP; s++) h[s] = 0.f;
-                total = -1.f;
-            }
-            if (SUMS && total >= 0.f) total += d;
+            d[i] = softplus(as_f32(ldt[i * kWave + lane]) + bias).d;
+            u[i] = d[i] * as_f32(lx[i * kWave + lane]);
+        }
+        end_of_step();
+        each_step([&](auto step) {
+            constexpr int i = decltype(step)::value;
+            StepBC<SP> next;
+            bc = move_on(bc, bc_step);
+            load_bc<SP, !SUMS>(next, bc, k.SB);
             float y = 0.f;
 #pragma unroll
-            for (int s = 0; s < SP; s++) {
-                h[s] = fmaf(exp2_raw(d * A[s]), h[s], u * B[s]);
-                if (!SUMS) y = fmaf(C[s], h[s], y);
-            }
-            if (SUMS) continue;
-            if (SPLIT) part[slice][i][me.lane] = y;
-            else finish(t, y);
+            for (int s = 0; s < SP; s++) h[s] = fmaf(exp2_raw(d[i] * A[s]), h[s], u[i] * now.b[s]);
+            if_start_set<i, SP>(cuts, h, u[i], now.b);
+            if (!SUMS)
+#pragma unroll
+                for (int s = 0; s < SP; s++) y = fmaf(now.c[s], h[s], y);
+            u[i] = y;
+            now = next;
+            made(u[i]);
+            end_of_step();
+        });
+        if (SUMS) {
+#pragma unroll
+            for (int i = 0; i < SCAN_STEPS; i++) total = cuts >> i & 1 || total < 0.f ? -1.f : total + d[i];
+            continue;
         }
-        if (SPLIT && !SUMS) {
+        const auto finish = [&](int i, float y) {
+            y = fmaf(D, as_f32(lx[i * kWave + lane]), y);
+            if (gate) {
+                const float z = as_f32(lz[i * kWave + lane]);
+                y *= z * sigmoid(z);
+            }
+            lx[i * kWave + lane] = as<T>(y);
+        };
+        if (SPLIT) {                                          // (a wave finishes every `slices`th step, in its own tile)
+#pragma unroll
+            for (int i = 0; i < SCAN_STEPS; i++) part[slice][i][lane] = u[i];
             __syncthreads();
             for (int i = slice; i < steps; i += k.slices) {
                 float y = 0.f;
-                for (int s = 0; s < k.slices; s++) y += part[s][i][me.lane];
-                finish(t0 + i, y);
+                for (int s = 0; s < k.slices; s++) y += part[s][i][lane];
+                finish(i, y);
             }
             __syncthreads();
+            if (me.live)
+                for (int i = slice; i < steps; i += k.slices) ((T*)a.out.p)[(t0 + i) * a.out.st + n * a.out.sn + c] = lx[i * kWave + lane];
+        } else {
+#pragma unroll
+            for (int i = 0; i < SCAN_STEPS; i++) finish(i, u[i]);
+            wave_wrote();
+            ChunkIn<T>::leave(lx, a.out, t0, steps, me, k.wide);
         }
     }
     if (!me.live) return;
@@ -198,6 +332,7 @@ inline ScanCut scan_slices(int S) {
     return {SP, slices};
 }
 constexpr int64_t SCAN_FILL = 4096;     // waves that fill the card
+constexpr int SCAN_BACK_WAVES = 8;      // waves a workgroup of the gradient, at most
 inline Scan scan_cut(const MoScan& a, bool backward) {
     Scan k{};
     k.a = a;
@@ -206,21 +341,30 @@ inline Scan scan_cut(const MoScan& a, bool backward) {
     k.SB = c.SP * c.slices;
     k.Cg = a.C / a.G;
     k.per = (k.Cg + kWave - 1) / kWave;
+    const int64_t V = a.dtype == MO_BF16 ? 8 : 4;
+    const auto row = [&](const MoRows& r) { return !r.p || ((uintptr_t)r.p % 16 == 0 && r.st % V == 0 && r.sn % V == 0); };
+    k.wide = k.Cg % V == 0 && row(a.x) && row(a.dt) && row(a.z) && (backward ? row(a.dout) && row(a.dx) && row(a.ddt) && row(a.dz) : row(a.out));
     k.chunks = (a.T + SCAN_STEPS - 1) / SCAN_STEPS;
     // Few sequences are cut over their length: each segment is gone through twice, once for what it adds to the state.
     const int64_t waves = std::max<int64_t>(1, a.N * a.G * k.per * k.slices), most = std::max<int64_t>(1, SCAN_FILL / waves);
     k.segments = most >= 4 ? std::min(most, std::max<int64_t>(1, k.chunks / 4)) : 1;
     k.each = std::max<int64_t>(1, (k.chunks + k.segments - 1) / k.segments);
     k.segments = std::max<int64_t>(1, (k.chunks + k.each - 1) / k.each);
-    k.rows = backward ? std::min(k.segments * a.N, std::max<int64_t>(1, 2 * SCAN_FILL / (a.G * k.per * k.slices))) : 0;
+    k.across = std::min(k.per, SCAN_BACK_WAVES / k.slices);
+    k.cuts = (k.per + k.across - 1) / k.across;
+    if (backward) {   // as many at a time as fill the card, and about the same number of turns for each
+        const int64_t items = k.segments * a.N, fill = std::max<int64_t>(1, SCAN_FILL / (a.G * k.cuts * k.across * k.slices));
+        const int64_t turns = std::max<int64_t>(1, (items + fill - 1) / fill);
+        k.rows = (items + turns - 1) / turns;
+    }
     return k;
 }
 // In floats, each part a multiple of 4 of them.
 inline int64_t whole(int64_t n) { return (n + 3) / 4 * 4; }
-inline int64_t scan_bc(const Scan& k) { return whole(k.a.T * k.a.N * k.a.G * 2 * k.SB); }
+inline int64_t scan_bc(const Scan& k) { return whole(scan_rows(k) * k.a.N * k.a.G * 2 * k.SB); }
 inline int64_t scan_kept(const Scan& k) { return whole(k.chunks * k.a.N * k.SB * k.a.C); }
 inline int64_t scan_segs(const Scan& k) { return k.segments > 1 ? whole(k.segments * k.a.N * (k.SB + 1) * k.a.C) : 0; }
-inline int64_t scan_parts_bc(const Scan& k) { return whole(k.per * k.a.T * k.a.N * k.a.G * 2 * k.SB); }
+inline int64_t scan_parts_bc(const Scan& k) { return k.cuts > 1 ? whole(k.cuts * k.a.T * k.a.N * k.a.G * 2 * k.SB) : 0; }
 inline int64_t scan_parts(const Scan& k) { return whole(k.rows * (k.SB + 2) * k.a.C); }
 inline int64_t scan_work_floats(const Scan& k, bool backward) {
     if (!backward) return (k.a.saved ? 0 : scan_bc(k)) + scan_segs(k);
@@ -251,7 +395,7 @@ template <class T> int scan_forward(const MoScan& a, hipStream_t s) {
     k.seg_h = (float*)a.work + (a.saved ? 0 : scan_bc(k));
     k.seg_d = k.seg_h + k.segments * a.N * k.SB * a.C;
     if (a.T) {
-        const int64_t n = a.T * a.N * a.G * 2 * k.SB;
+        const int64_t n = scan_rows(k) * a.N * a.G * 2 * k.SB;
         hipLaunchKernelGGL((k_scan_pack<T>), grid_of((n + 255) / 256), dim3(256), 0, s, k, bc);
         if (launched("k_scan_pack")) return -1;
     }

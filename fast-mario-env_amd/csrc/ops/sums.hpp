@@ -11,16 +11,16 @@ template <int CTRL> __device__ __forceinline__ float dpp(float x) {
 constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR8 = 0x141, DPP_XOR8 = 0x128;   // (mirrored in eights: l to 7 - l)
 
 // Sums of M values over a wave's 64 lanes, each lane left with one of them: every step sends half of the values to the other half of the
-// lanes, so that M values cost about 2 M instructions and not 12 M. Lane l gets value sum_slot(l) of the M (M a multiple of 8 up to
-// 32; a slot >= M holds nothing), lanes of equal slots the same sum.
+// lanes, so that M values cost about 3 M instructions and not 12 M. Lane l gets value sum_slot(l) of the M (4, 8, 12 or 16; a slot >= M
+// holds nothing), lanes of equal slots the same sum.
 __device__ __forceinline__ int sum_slot(int l, int M) {
-    const int s = ((l >> 5) & 1) | ((l >> 3) & 2) | ((l >> 1) & 4) | ((l << 1) & 8) | ((l << 3) & 16);
-    return M <= 8 ? s & 7 : M <= 16 ? s & 15 : s;
+    const int s = ((l >> 5) & 1) | ((l >> 3) & 2) | ((l >> 1) & 4) | ((l << 1) & 8);
+    return M <= 4 ? s & 3 : M <= 8 ? s & 7 : s;
 }
 template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M]) {
-    static_assert(M % 8 == 0 && M <= 32, "");
+    static_assert(M % 4 == 0 && M <= 16, "");
     const int l = threadIdx.x % kWave;
-    float a[M / 2], b[M / 4], c[M / 8];
+    float a[M / 2], b[M / 4];
     typedef unsigned U2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int i = 0; i < M / 2; i++) {
@@ -32,23 +32,21 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M]) {
         const U2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[2 * i]), __float_as_uint(a[2 * i + 1]), false, false);
         b[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     }
-#pragma unroll
-    for (int i = 0; i < M / 8; i++) c[i] = (l & 8 ? b[2 * i + 1] : b[2 * i]) + dpp<DPP_XOR8>(l & 8 ? b[2 * i] : b[2 * i + 1]);
     float r;
-    if constexpr (M == 8) {
-        r = c[0] + dpp<DPP_MIRROR8>(c[0]);
-        r += dpp<DPP_XOR2>(r);
+    if constexpr (M == 4) {
+        r = b[0] + dpp<DPP_XOR8>(b[0]);
+        r += dpp<DPP_MIRROR8>(r);
     } else {
-        float d[2];
-        d[0] = (l & 4 ? c[1] : c[0]) + dpp<DPP_MIRROR8>(l & 4 ? c[0] : c[1]);
-        if constexpr (M == 16) {
-            r = d[0] + dpp<DPP_XOR2>(d[0]);
+        const float b3 = M == 16 ? b[M / 4 - 1] : 0.f;
+        const float c0 = (l & 8 ? b[1] : b[0]) + dpp<DPP_XOR8>(l & 8 ? b[0] : b[1]);
+        if constexpr (M == 8) {
+            r = c0 + dpp<DPP_MIRROR8>(c0);
         } else {
-            const float c3 = M == 32 ? c[M / 8 - 1] : 0.f;
-            d[1] = (l & 4 ? c3 : c[2]) + dpp<DPP_MIRROR8>(l & 4 ? c[2] : c3);
-            r = (l & 2 ? d[1] : d[0]) + dpp<DPP_XOR2>(l & 2 ? d[0] : d[1]);
+            const float c1 = (l & 8 ? b3 : b[2]) + dpp<DPP_XOR8>(l & 8 ? b[2] : b3);
+            r = (l & 4 ? c1 : c0) + dpp<DPP_MIRROR8>(l & 4 ? c0 : c1);
         }
     }
+    r += dpp<DPP_XOR2>(r);
     return r + dpp<DPP_XOR1>(r);
 }
 
