@@ -62,6 +62,7 @@ template <class T> __global__ void __launch_bounds__(256) k_scan_pack(Scan k, fl
 struct ScanPlace {
     int64_t n, segment;
     int g, c0, c, lane, s0, there;   // group, first channel, this lane's, its first state, channels that there are
+    uint32_t at;                     // this lane's channel, from the first (the last one that there is, where there are fewer)
     bool live;
     __device__ __forceinline__ ScanPlace(const Scan& k, int64_t item, int cb, int slice, int SP) {
         n = item % k.a.N;
@@ -72,8 +73,18 @@ struct ScanPlace {
         there = min(kWave, k.Cg - i);
         live = lane < there;
         c0 = g * k.Cg + i;
-        c = c0 + min(lane, there - 1);
+        at = min(lane, there - 1);
+        c = c0 + (int)at;
         s0 = slice * SP;
+    }
+    // The same, the lane's own values made anew from here on: they would be kept through the steps.
+    __device__ __forceinline__ ScanPlace again() const {
+        ScanPlace p = *this;
+        asm volatile("" : "+v"(p.lane));
+        p.live = p.lane < there;
+        p.at = max(0, min(p.lane, there - 1));
+        p.c = c0 + (int)p.at;
+        return p;
     }
 };
 __device__ __forceinline__ int wave_here() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
@@ -84,18 +95,30 @@ __device__ __forceinline__ void wave_wrote() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The kernel's arguments, read again from here on: kept in registers through the steps they would push the steps' own out.
+__device__ __forceinline__ const Scan& args_again() {
+    typedef const Scan __attribute__((address_space(4))) * Args;
+    uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Scan*)(Args)p;
+}
+// A lane's place behind a pointer that all lanes share: a 32-bit offset, so that the pointer stays in scalar registers.
+template <class P> __device__ __forceinline__ P* lane_at(P* p, uint32_t bytes) {
+    return (P*)((std::conditional_t<std::is_const_v<P>, const char, char>*)p + bytes);
+}
 // A chunk's rows of 64 channels, zeros where there are none (rows past the last step, channels past the group's). Wide: in 16-byte pieces through
 // registers (ahead of their use); else an element a lane. Where there are none, a place that there is is read and not used: no branches.
 template <class T> struct ChunkIn {
     static constexpr int EPV = 16 / sizeof(T), PR = kWave / EPV, ROWS = kWave / PR, N = SCAN_STEPS / ROWS;
     uint4 v[N];
-    static __device__ __forceinline__ T* piece(const MoRows& r, int64_t t0, const ScanPlace& me, int row) {
+    static __device__ __forceinline__ T* base(const MoRows& r, int64_t t0, const ScanPlace& me) { return (T*)r.p + t0 * r.st + me.n * r.sn + me.c0; }
+    static __device__ __forceinline__ uint32_t piece(const MoRows& r, const ScanPlace& me, int row) {   // (a chunk spans less than 2^31 bytes)
         const int p = me.lane % PR * EPV;
-        return (T*)r.p + t0 * r.st + me.n * r.sn + me.c0 + row * r.st + (p < me.there ? p : 0);
+        return ((uint32_t)row * (uint32_t)r.st + (p < me.there ? p : 0)) * (uint32_t)sizeof(T);
     }
     __device__ __forceinline__ void ahead(const MoRows& r, int64_t t0, int steps, const ScanPlace& me) {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = *(const uint4*)piece(r, t0, me, min(me.lane / PR + i * ROWS, steps - 1));
+        for (int i = 0; i < N; i++) v[i] = *(const uint4*)lane_at((const T*)base(r, t0, me), piece(r, me, min(me.lane / PR + i * ROWS, steps - 1)));
     }
     __device__ __forceinline__ void arrive(T* to, int steps, const ScanPlace& me, uint32_t none = 0) const {
 #pragma unroll
@@ -105,11 +128,11 @@ template <class T> struct ChunkIn {
         }
     }
     static __device__ __forceinline__ void narrow(T* to, const MoRows& r, int64_t t0, int steps, const ScanPlace& me, float none = 0.f) {
-        const T* p = (const T*)r.p + t0 * r.st + me.n * r.sn + me.c;
+        const T* p = base(r, t0, me);
         T x[SCAN_STEPS];
 #pragma unroll
         for (int i = 0; i < SCAN_STEPS; i++) {
-            x[i] = *p;
+            x[i] = *lane_at(p, me.at * (uint32_t)sizeof(T));
             if (i + 1 < steps) p += r.st;
         }
 #pragma unroll
@@ -121,10 +144,10 @@ template <class T> struct ChunkIn {
 #pragma unroll
             for (int i = 0; i < N; i++)
                 if (me.lane / PR + i * ROWS < steps && me.lane % PR * EPV < me.there)
-                    stream((uint4*)piece(r, t0, me, me.lane / PR + i * ROWS), *(const uint4*)(from + (i * kWave + me.lane) * EPV));
+                    stream((uint4*)lane_at(base(r, t0, me), piece(r, me, me.lane / PR + i * ROWS)), *(const uint4*)(from + (i * kWave + me.lane) * EPV));
         } else if (me.live) {
-            T* p = (T*)r.p + t0 * r.st + me.n * r.sn + me.c;
-            for (int i = 0; i < steps; i++, p += r.st) *p = from[i * kWave + me.lane];
+            T* p = base(r, t0, me);
+            for (int i = 0; i < steps; i++, p += r.st) *lane_at(p, me.at * (uint32_t)sizeof(T)) = from[i * kWave + me.lane];
         }
     }
 };
@@ -232,9 +255,9 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
         wave_wrote();
         if (chunk + 1 < last) ahead(chunk + 1);
         if (!SUMS && k.kept && me.live) {
-            float* to = k.kept + ((chunk * a.N + n) * k.SB + me.s0) * a.C + c;
+            float* to = k.kept + ((chunk * a.N + n) * k.SB + me.s0) * a.C + me.c0;
 #pragma unroll
-            for (int s = 0; s < SP; s++) __builtin_nontemporal_store(h[s], to + (int64_t)s * a.C);
+            for (int s = 0; s < SP; s++) __builtin_nontemporal_store(h[s], lane_at(to + (int64_t)s * a.C, me.at * 4));
         }
         // Nothing but the scalar loads of B and C is waited for between the steps.
         float d[SCAN_STEPS], u[SCAN_STEPS];
@@ -333,6 +356,7 @@ inline ScanCut scan_slices(int S) {
 }
 constexpr int64_t SCAN_FILL = 4096;     // waves that fill the card
 constexpr int SCAN_BACK_WAVES = 8;      // waves a workgroup of the gradient, at most
+template <class T> constexpr int SCAN_SHARED_LDS = (sizeof(T) == 2 ? 18 : 22) << 10;   // LDS of a wave there that shares its channels
 inline Scan scan_cut(const MoScan& a, bool backward) {
     Scan k{};
     k.a = a;
@@ -342,7 +366,9 @@ inline Scan scan_cut(const MoScan& a, bool backward) {
     k.Cg = a.C / a.G;
     k.per = (k.Cg + kWave - 1) / kWave;
     const int64_t V = a.dtype == MO_BF16 ? 8 : 4;
-    const auto row = [&](const MoRows& r) { return !r.p || ((uintptr_t)r.p % 16 == 0 && r.st % V == 0 && r.sn % V == 0); };
+    const auto row = [&](const MoRows& r) {
+        return !r.p || ((uintptr_t)r.p % 16 == 0 && r.st % V == 0 && r.sn % V == 0 && r.st >= 0 && r.st < ((int64_t)1 << 30) / (SCAN_STEPS * 4));
+    };
     k.wide = k.Cg % V == 0 && row(a.x) && row(a.dt) && row(a.z) && (backward ? row(a.dout) && row(a.dx) && row(a.ddt) && row(a.dz) : row(a.out));
     k.chunks = (a.T + SCAN_STEPS - 1) / SCAN_STEPS;
     // Few sequences are cut over their length: each segment is gone through twice, once for what it adds to the state.
@@ -350,7 +376,8 @@ inline Scan scan_cut(const MoScan& a, bool backward) {
     k.segments = most >= 4 ? std::min(most, std::max<int64_t>(1, k.chunks / 4)) : 1;
     k.each = std::max<int64_t>(1, (k.chunks + k.segments - 1) / k.segments);
     k.segments = std::max<int64_t>(1, (k.chunks + k.each - 1) / k.each);
-    k.across = std::min(k.per, SCAN_BACK_WAVES / k.slices);
+    const int room = k.slices == 1 ? SCAN_BACK_WAVES : (160 << 10) / (a.dtype == MO_BF16 ? SCAN_SHARED_LDS<bf16> : SCAN_SHARED_LDS<float>);
+    k.across = std::min(k.per, std::min(SCAN_BACK_WAVES, room) / k.slices);
     k.cuts = (k.per + k.across - 1) / k.across;
     if (backward) {   // as many at a time as fill the card, and about the same number of turns for each
         const int64_t items = k.segments * a.N, fill = std::max<int64_t>(1, SCAN_FILL / (a.G * k.cuts * k.across * k.slices));

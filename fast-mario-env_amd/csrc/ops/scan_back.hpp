@@ -111,203 +111,125 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan_back_sums(Scan k) {
     if (slice == 0) k.seg_d[(me.segment * a.N + n) * a.C + me.c] = total;
 }
 
-// Workgroups of `wide` waves of channels by `slices`; LDS is a wave's own tiles of x, dt, z and dout (whose places dx, ddt and dz take), its
-// step sizes, and the sums for its workgroup's dB and dC, of two chunks in turn.
-template <class T> constexpr int back_wave_lds() { return 4 * SCAN_STEPS * kWave * (int)sizeof(T) + SCAN_STEPS * kWave * 4 + 2 * SCAN_STEPS * 32 * 4; }
+// Workgroups of `across` waves of channels by `slices`. A wave's own LDS: the tiles of x, dt, z and dout (whose places dx, ddt and dz take); of each step
+// its size d, d's slope by dt, dy and y; the sums for its workgroup's dB and dC, of two chunks in turn; where waves share channels, du and dd.
+template <class T, bool SPLIT> struct BackLds {
+    static constexpr int TILE = SCAN_STEPS * kWave, SUMS = 2 * SCAN_STEPS * 32;
+    static constexpr int BYTES = 4 * TILE * (int)sizeof(T) + (4 * TILE + SUMS + (SPLIT ? 2 * TILE : 0)) * 4;
+    T* t;
+    __device__ __forceinline__ explicit BackLds(char* p) : t((T*)p) {}
+    __device__ __forceinline__ T* x() const { return t; }
+    __device__ __forceinline__ T* dt() const { return t + TILE; }
+    __device__ __forceinline__ T* z() const { return t + 2 * TILE; }
+    __device__ __forceinline__ T* dout() const { return t + 3 * TILE; }
+    __device__ __forceinline__ float* d() const { return (float*)(t + 4 * TILE); }
+    __device__ __forceinline__ float* slope() const { return d() + TILE; }
+    __device__ __forceinline__ float* dy() const { return d() + 2 * TILE; }
+    __device__ __forceinline__ float* y() const { return d() + 3 * TILE; }
+    __device__ __forceinline__ float* sums() const { return d() + 4 * TILE; }        // (2, SCAN_STEPS, 32)
+    __device__ __forceinline__ float* du() const { return sums() + SUMS; }
+    __device__ __forceinline__ float* dd() const { return du() + TILE; }
+};
 
 template <class T, int SP, bool SPLIT>
 __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
     const MoScan& a = k.a;
-    constexpr int TILE = SCAN_STEPS * kWave;
+    typedef BackLds<T, SPLIT> Lds;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ float part[SPLIT ? BACK_WAVES : 1][SPLIT ? SCAN_STEPS : 1][SPLIT ? 3 : 1][kWave];
     const int w = wave_here(), slices = SPLIT ? k.slices : 1, slice = SPLIT ? w % slices : 0, across = w / slices;
     const int64_t items = k.segments * a.N, row = block_here() / (a.G * k.cuts), bg = block_here() % (a.G * k.cuts);
     if (row >= k.rows) return;
     const int g0 = (int)(bg / k.cuts), cut = (int)(bg % k.cuts), in_group = cut * k.across + across;   // (waves past the group's channels join the barriers only)
     const int cb = g0 * k.per + min(in_group, k.per - 1);
-    const bool idle = in_group >= k.per;
-    T* lx = (T*)(lds + w * back_wave_lds<T>());
-    T *ldt = lx + TILE, *lz = lx + 2 * TILE, *ldo = lx + 3 * TILE;
-    float *ld = (float*)(lx + 4 * TILE), *sums = ld + TILE;                // (2, SCAN_STEPS, 32)
+    const Lds l(lds + w * Lds::BYTES);
     const bool gate = a.z.p;
-    ScanPlace me(k, row, cb, slice, SP);
-    if (idle) { me.live = false; me.there = 0; }
-    const int lane = me.lane, c = me.c;
+    ScanPlace place(k, row, cb, slice, SP);
+    if (in_group >= k.per) { place.live = false; place.there = 0; }
     float A[SP], dA[SP], dD = 0.f, dbias = 0.f;
-    load_decays<SP>(a, me, A);
+    const int c = place.c;
+    load_decays<SP>(a, place, A);
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, D = a.D ? a.D[c] : 0.f;
 #pragma unroll
     for (int s = 0; s < SP; s++) dA[s] = 0.f;
-    const auto steps_of = [&](int64_t chunk) { return (int)min((int64_t)SCAN_STEPS, a.T - chunk * SCAN_STEPS); };
-    const int64_t bc_step = a.N * a.G * 2 * k.SB;
     for (int64_t item = row; item < items; item += k.rows) {
-        const int64_t n = me.n = item % a.N;
-        me.segment = item / a.N;
-        const int64_t first = me.segment * k.each, last = min(k.chunks, first + k.each);
-        float Q[SP], before[SP];
+        const int64_t n = place.n = item % a.N;
+        place.segment = item / a.N;
+        const int64_t first = place.segment * k.each, last = min(k.chunks, first + k.each);
+        float Q[SP], before[SP], touch = 0.f;
         ChunkIn<T> ix, idt, iz, ido;
         uint8_t flag = 0;
         const auto ahead = [&](int64_t chunk) {
+            const Scan& k = args_again();
+            const ScanPlace me = place.again();
+            const int lane = me.lane;
             const int64_t t0 = chunk * SCAN_STEPS;
-            const int steps = steps_of(chunk);
-            flag = start_of_lane(a, t0, steps, me);
-            const float* from = k.kept + ((chunk * a.N + n) * k.SB + me.s0) * a.C + c;
-#pragma unroll
-            for (int s = 0; s < SP; s++) before[s] = __builtin_nontemporal_load(from + (int64_t)s * a.C);
+            const int steps = (int)min((int64_t)SCAN_STEPS, k.a.T - t0);
+            flag = start_of_lane(k.a, t0, steps, me);
+            // (a lane for each 64 bytes of the chunk's B and C, which the scalar loads then find in the L2)
+            const int64_t row = ((t0 + lane % SCAN_STEPS) * k.a.N + n) * k.a.G + g0;
+            touch = k.bc[row * 2 * k.SB + min(lane / SCAN_STEPS * 16, 2 * k.SB - 1)];
             if (!k.wide) return;
-            ix.ahead(a.x, t0, steps, me);
-            idt.ahead(a.dt, t0, steps, me);
-            if (gate) iz.ahead(a.z, t0, steps, me);
-            ido.ahead(a.dout, t0, steps, me);
+            ix.ahead(k.a.x, t0, steps, me);
+            idt.ahead(k.a.dt, t0, steps, me);
+            if (gate) iz.ahead(k.a.z, t0, steps, me);
+            ido.ahead(k.a.dout, t0, steps, me);
         };
-        if (first < last) ahead(last - 1);
+        // the states before a chunk: into registers that are free between two chunks
+        const auto states_ahead = [&](int64_t chunk) {
+            const Scan& k = args_again();
+            const ScanPlace me = place.again();
+            const float* from = k.kept + ((chunk * k.a.N + n) * k.SB + me.s0) * k.a.C + me.c0;
+#pragma unroll
+            for (int s = 0; s < SP; s++) before[s] = __builtin_nontemporal_load(lane_at(from + (int64_t)s * k.a.C, me.at * 4));
+        };
+        if (first < last) {
+            ahead(last - 1);
+            states_ahead(last - 1);
+        }
 #pragma unroll
         for (int s = 0; s < SP; s++) {
-            if (!me.live) Q[s] = 0.f;
-            else if (k.segments > 1) Q[s] = k.seg_h[((me.segment * a.N + n) * k.SB + me.s0 + s) * a.C + c];
-            else Q[s] = a.dstate_out && me.s0 + s < a.S ? a.dstate_out[(n * a.C + c) * a.S + me.s0 + s] : 0.f;
+            if (!place.live) Q[s] = 0.f;
+            else if (k.segments > 1) Q[s] = k.seg_h[((place.segment * a.N + n) * k.SB + place.s0 + s) * a.C + c];
+            else Q[s] = a.dstate_out && place.s0 + s < a.S ? a.dstate_out[(n * a.C + c) * a.S + place.s0 + s] : 0.f;
         }
-        for (int64_t chunk = last - 1; chunk >= first; chunk--) {
-            const int64_t t0 = chunk * SCAN_STEPS;
-            const int steps = steps_of(chunk);
-            const unsigned cuts = (unsigned)__ballot(flag != 0);
-            float h[SCAN_STEPS + 1][SP];
-#pragma unroll
-            for (int s = 0; s < SP; s++) h[0][s] = me.live ? before[s] : 0.f;
-            wave_wrote();
-            if (k.wide) {
-                ix.arrive(lx, steps, me);
-                idt.arrive(ldt, steps, me, NO_SIZE<T>);
-                if (gate) iz.arrive(lz, steps, me);
-                ido.arrive(ldo, steps, me);
-            } else {
-                ChunkIn<T>::narrow(lx, a.x, t0, steps, me);
-                ChunkIn<T>::narrow(ldt, a.dt, t0, steps, me, -INFINITY);
-                if (gate) ChunkIn<T>::narrow(lz, a.z, t0, steps, me);
-                ChunkIn<T>::narrow(ldo, a.dout, t0, steps, me);
-            }
-            wave_wrote();
-            Uniform bc = uniform(k.bc + ((t0 * a.N + n) * a.G + g0) * 2 * k.SB + me.s0);
-            {   // the states again
-                float d[SCAN_STEPS], u[SCAN_STEPS];
-#pragma unroll
-                for (int i = 0; i < SCAN_STEPS; i++) {
-                    d[i] = softplus(as_f32(ldt[i * kWave + lane]) + bias).d;
-                    u[i] = d[i] * as_f32(lx[i * kWave + lane]);
-                    ld[i * kWave + lane] = d[i];
-                }
-                StepBC<SP> now;
-                load_bc<SP, false>(now, bc, k.SB);
-                end_of_step();
-                each_step([&](auto step) {
-                    constexpr int i = decltype(step)::value;
-                    StepBC<SP> next;
-                    if constexpr (i + 1 < SCAN_STEPS) {
-                        bc = move_on(bc, bc_step);
-                        load_bc<SP, false>(next, bc, k.SB);
-                    }
-#pragma unroll
-                    for (int s = 0; s < SP; s++) h[i + 1][s] = fmaf(exp2_raw(d[i] * A[s]), h[i][s], u[i] * now.b[s]);
-                    if_start_set<i, SP>(cuts, h[i + 1], u[i], now.b);
-                    if constexpr (i + 1 < SCAN_STEPS) now = next;
-                    end_of_step();
-                });
-            }
-            float* const to_join = sums + (chunk & 1) * SCAN_STEPS * 32;
-            const int slot = sum_slot(lane, 2 * SP);
-            StepBC<SP> now;
-            load_bc<SP>(now, bc, k.SB);
-            each_step([&](auto step) {
-                constexpr int i = SCAN_STEPS - 1 - decltype(step)::value;
-                const int at = i * kWave + lane;
-                const float x = as_f32(lx[at]), dout = as_f32(ldo[at]), d = ld[at], z = gate ? as_f32(lz[at]) : 0.f, raw = as_f32(ldt[at]) + bias;
-                const float sig = sigmoid(z), dy = gate ? dout * (z * sig) : dout, u = d * x;
-                StepBC<SP> next;
-                float y = 0.f, du = 0.f, dd = 0.f, q[SP], v[SP];
-#pragma unroll
-                for (int s = 0; s < SP; s++) {
-                    y = fmaf(now.c[s], h[i + 1][s], y);
-                    v[s] = h[i + 1][s] * dy;
-                }
-                float sum_c = wave_sums<SP>(v);
-                made(y);
-                made(sum_c);
-                end_of_step();
-#pragma unroll
-                for (int s = 0; s < SP; s++) {
-                    Q[s] = fmaf(now.c[s], dy, Q[s]);
-                    du = fmaf(Q[s], now.b[s], du);
-                    v[s] = Q[s] * u;
-                }
-                made(du);
-                if constexpr (i > 0) {
-                    bc = move_on(bc, -bc_step);
-                    load_bc<SP>(next, bc, k.SB);
-                }
-                float sum_b = wave_sums<SP>(v);
-                made(sum_b);
-                end_of_step();
-#pragma unroll
-                for (int s = 0; s < SP; s++) {
-                    Q[s] *= exp2_raw(d * A[s]);
-                    q[s] = Q[s] * h[i][s];
-                }
-                if_start_clear<i, SP>(cuts, Q, q);
-#pragma unroll
-                for (int s = 0; s < SP; s++) {
-                    dd = fmaf(q[s], A[s], dd);
-                    dA[s] = fmaf(q[s], d, dA[s]);
-                }
-                if (slot < SP) to_join[i * 32 + slot + (lane & 1 ? SP : 0)] = lane & 1 ? sum_c : sum_b;
-                if constexpr (SPLIT) {
-                    part[w][i][0][lane] = y;
-                    part[w][i][1][lane] = du;
-                    part[w][i][2][lane] = dd;
-                } else {
-                    const float slope = softplus(raw).slope, ddt = fmaf(du, x, dd * LN2) * slope;
-                    dD = fmaf(dy, x, dD);
-                    dbias += ddt;
-                    lx[at] = as<T>(fmaf(du, d, D * dy));
-                    ldt[at] = as<T>(ddt);
-                    if (gate) lz[at] = as<T>(dout * fmaf(D, x, y) * (sig * fmaf(z, 1.f - sig, 1.f)));
-                }
-                if constexpr (i > 0) now = next;
-                if constexpr (i == SCAN_STEPS / 2) {
-                    if (chunk > first) ahead(chunk - 1);      // (the states that are done with have left their registers)
-                }
-                end_of_step();
-            });
-            __syncthreads();
+        // what a chunk left in LDS goes to memory
+        const auto after_chunk = [&](int64_t chunk, int64_t t0, int steps) {
+            const Scan& k = args_again();
+            const MoScan& a = k.a;
+            const ScanPlace me = place.again();
+            const int lane = me.lane, c = me.c;
             if constexpr (SPLIT) {
                 for (int i = slice; i < steps; i += slices) {
                     const int at = i * kWave + lane;
-                    const float x = as_f32(lx[at]), dout = as_f32(ldo[at]), d = ld[at], z = gate ? as_f32(lz[at]) : 0.f;
-                    const float sig = sigmoid(z), dy = gate ? dout * (z * sig) : dout, slope = softplus(as_f32(ldt[at]) + bias).slope;
-                    float j[3] = {0.f, 0.f, 0.f};
-                    for (int s = 0; s < slices; s++)
-#pragma unroll
-                        for (int m = 0; m < 3; m++) j[m] += part[w - slice + s][i][m][lane];
-                    const float ddt = fmaf(j[1], x, j[2] * LN2) * slope;
+                    float y = 0.f, du = 0.f, dd = 0.f;
+                    for (int s = 0; s < slices; s++) {
+                        const Lds o(lds + (w - slice + s) * Lds::BYTES);
+                        y += o.y()[at];
+                        du += o.du()[at];
+                        dd += o.dd()[at];
+                    }
+                    const float x = as_f32(l.x()[at]), dy = l.dy()[at], ddt = fmaf(du, x, dd * LN2) * l.slope()[at];
                     dD = fmaf(dy, x, dD);
                     dbias += ddt;
                     if (!me.live) continue;
                     const auto row_of = [&](const MoRows& r) { return (T*)r.p + (t0 + i) * r.st + n * r.sn + c; };
-                    *row_of(a.dx) = as<T>(fmaf(j[1], d, D * dy));
+                    *row_of(a.dx) = as<T>(fmaf(du, l.d()[at], D * dy));
                     *row_of(a.ddt) = as<T>(ddt);
-                    if (gate) *row_of(a.dz) = as<T>(dout * fmaf(D, x, j[0]) * (sig * fmaf(z, 1.f - sig, 1.f)));
+                    if (!gate) continue;
+                    const float z = as_f32(l.z()[at]), sig = sigmoid(z);
+                    *row_of(a.dz) = as<T>(as_f32(l.dout()[at]) * fmaf(D, x, y) * (sig * fmaf(z, 1.f - sig, 1.f)));
                 }
             } else {
-                ChunkIn<T>::leave(lx, a.dx, t0, steps, me, k.wide);
-                ChunkIn<T>::leave(ldt, a.ddt, t0, steps, me, k.wide);
-                if (gate) ChunkIn<T>::leave(lz, a.dz, t0, steps, me, k.wide);
+                ChunkIn<T>::leave(l.x(), a.dx, t0, steps, me, k.wide);
+                ChunkIn<T>::leave(l.dt(), a.ddt, t0, steps, me, k.wide);
+                if (gate) ChunkIn<T>::leave(l.z(), a.dz, t0, steps, me, k.wide);
             }
             // dB and dC of the chunk: the workgroup's waves joined (the next chunk's sums go to the other place)
-            for (int i = threadIdx.x; i < steps * 2 * k.SB; i += blockDim.x) {
+            for (int i = w * kWave + lane; i < steps * 2 * k.SB; i += blockDim.x) {
                 const int j = i / (2 * k.SB), m = i % (2 * k.SB), which = m / k.SB, s = m % k.SB, of = s / SP;
                 float x = 0.f;
                 for (int v = of; v < k.across * slices; v += slices)
-                    x += ((float*)(lds + v * back_wave_lds<T>() + 4 * TILE * sizeof(T)) + TILE)[(chunk & 1) * SCAN_STEPS * 32 + j * 32 + which * SP + s % SP];
+                    x += Lds(lds + v * Lds::BYTES).sums()[(chunk & 1) * SCAN_STEPS * 32 + j * 32 + which * SP + s % SP];
                 if (k.cuts > 1) {
                     k.part_bc[((((int64_t)cut * a.T + t0 + j) * a.N + n) * a.G + g0) * 2 * k.SB + m] = x;
                 } else if (s < a.S) {
@@ -316,21 +238,172 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 }
             }
             if constexpr (SPLIT) __syncthreads();             // (their partial sums have been read)
+        };
+        for (int64_t chunk = last - 1; chunk >= first; chunk--) {
+            const Scan& k = args_again();
+            const MoScan& a = k.a;
+            const ScanPlace me = place.again();
+            const int lane = me.lane;
+            const int64_t t0 = chunk * SCAN_STEPS;
+            const int steps = (int)min((int64_t)SCAN_STEPS, a.T - t0);
+            const unsigned cuts = (unsigned)__ballot(flag != 0);
+            asm volatile("" ::"v"(touch));
+            wave_wrote();
+            if (k.wide) {
+                ix.arrive(l.x(), steps, me);
+                idt.arrive(l.dt(), steps, me, NO_SIZE<T>);
+                if (gate) iz.arrive(l.z(), steps, me);
+                ido.arrive(l.dout(), steps, me);
+            } else {
+                ChunkIn<T>::narrow(l.x(), a.x, t0, steps, me);
+                ChunkIn<T>::narrow(l.dt(), a.dt, t0, steps, me, -INFINITY);
+                if (gate) ChunkIn<T>::narrow(l.z(), a.z, t0, steps, me);
+                ChunkIn<T>::narrow(l.dout(), a.dout, t0, steps, me);
+            }
+            wave_wrote();
+#pragma unroll
+            for (int i = 0; i < SCAN_STEPS; i++) {
+                const int at = i * kWave + lane;
+                const Size p = softplus(as_f32(l.dt()[at]) + bias);
+                l.d()[at] = p.d;
+                l.slope()[at] = p.slope;
+                float dy = as_f32(l.dout()[at]);
+                if (gate) {
+                    const float z = as_f32(l.z()[at]);
+                    dy *= z * sigmoid(z);
+                }
+                l.dy()[at] = dy;
+            }
+            end_of_step();
+            float h[SCAN_STEPS][SP];                          // the states before each step
+#pragma unroll
+            for (int s = 0; s < SP; s++) h[0][s] = me.live ? before[s] : 0.f;
+            float* const to_join = l.sums() + (chunk & 1) * SCAN_STEPS * 32;
+            // what a step needs, read a step ahead
+            struct In { float d, dy; T x; };
+            const auto in_of = [&](int i) { return In{l.d()[i * kWave + lane], l.dy()[i * kWave + lane], l.x()[i * kWave + lane]}; };
+            const int64_t bc_step = a.N * a.G * 2 * k.SB;
+            const int SB = k.SB;
+            Uniform bc = uniform(k.bc + ((t0 * a.N + n) * a.G + g0) * 2 * SB + me.s0);
+            StepBC<SP> now;
+            load_bc<SP>(now, bc, SB);
+            In in = in_of(0);
+            // the states again, y and dC
+            each_step([&](auto step) {
+                constexpr int i = decltype(step)::value;
+                StepBC<SP> next;
+                In in_next;
+                if constexpr (i + 1 < SCAN_STEPS) {
+                    bc = move_on(bc, bc_step);
+                    load_bc<SP>(next, bc, SB);
+                    in_next = in_of(i + 1);
+                }
+                const float u = in.d * as_f32(in.x);
+                float v[SP], y = 0.f;
+#pragma unroll
+                for (int s = 0; s < SP; s++) v[s] = fmaf(exp2_raw(in.d * A[s]), h[i][s], u * now.b[s]);
+                if_start_set<i, SP>(cuts, v, u, now.b);
+#pragma unroll
+                for (int s = 0; s < SP; s++) {
+                    if constexpr (i + 1 < SCAN_STEPS) h[i + 1][s] = v[s];
+                    y = fmaf(now.c[s], v[s], y);
+                    v[s] *= in.dy;
+                }
+                l.y()[i * kWave + lane] = y;
+                const float sum = wave_sums<SP>(v);
+                if (sum_slot(lane, SP) < SP) to_join[i * 32 + SP + sum_slot(lane, SP)] = sum;
+                if constexpr (i + 1 < SCAN_STEPS) {
+                    now = next;
+                    in = in_next;
+                }
+                end_of_step();
+            });
+            if constexpr (!SPLIT) {
+                if (gate)
+#pragma unroll
+                    for (int i = 0; i < SCAN_STEPS; i++) {
+                        const int at = i * kWave + lane;
+                        const float z = as_f32(l.z()[at]), sig = sigmoid(z);
+                        l.z()[at] = as<T>(as_f32(l.dout()[at]) * fmaf(D, as_f32(l.x()[at]), l.y()[at]) * (sig * fmaf(z, 1.f - sig, 1.f)));
+                    }
+                end_of_step();
+            }
+            // and back
+            load_bc<SP>(now, bc, SB);
+            in = in_of(SCAN_STEPS - 1);
+            each_step([&](auto step) {
+                constexpr int i = SCAN_STEPS - 1 - decltype(step)::value;
+                const int at = i * kWave + lane;
+                StepBC<SP> next;
+                In in_next;
+                if constexpr (i > 0) {
+                    bc = move_on(bc, -bc_step);
+                    load_bc<SP>(next, bc, SB);
+                    in_next = in_of(i - 1);
+                }
+                const float x = as_f32(in.x), u = in.d * x;
+                float du = 0.f, dd = 0.f, v[SP];
+#pragma unroll
+                for (int s = 0; s < SP; s++) {
+                    Q[s] = fmaf(now.c[s], in.dy, Q[s]);
+                    du = fmaf(Q[s], now.b[s], du);
+                    v[s] = Q[s] * u;
+                }
+                const float sum = wave_sums<SP>(v);
+                if (sum_slot(lane, SP) < SP) to_join[i * 32 + sum_slot(lane, SP)] = sum;
+                made(du);
+                end_of_step();
+#pragma unroll
+                for (int s = 0; s < SP; s++) {
+                    Q[s] *= exp2_raw(in.d * A[s]);
+                    v[s] = Q[s] * h[i][s];
+                }
+                if_start_clear<i, SP>(cuts, Q, v);
+#pragma unroll
+                for (int s = 0; s < SP; s++) {
+                    dd = fmaf(v[s], A[s], dd);
+                    dA[s] = fmaf(v[s], in.d, dA[s]);
+                }
+                if constexpr (SPLIT) {
+                    l.du()[at] = du;
+                    l.dd()[at] = dd;
+                } else {
+                    const float ddt = fmaf(du, x, dd * LN2) * l.slope()[at];
+                    dD = fmaf(in.dy, x, dD);
+                    dbias += ddt;
+                    l.x()[at] = as<T>(fmaf(du, in.d, D * in.dy));
+                    l.dt()[at] = as<T>(ddt);
+                }
+                if constexpr (i > 0) {
+                    now = next;
+                    in = in_next;
+                }
+                if constexpr (i == SCAN_STEPS / 2) {
+                    if (chunk > first) ahead(chunk - 1);      // (the states that are done with have left their registers)
+                }
+                end_of_step();
+            });
+            if (chunk > first) states_ahead(chunk - 1);
+            __syncthreads();
+            after_chunk(chunk, t0, steps);
         }
-        if (first == 0 && a.dstate && me.live)
+        if (first == 0 && a.dstate && place.live)
 #pragma unroll
             for (int s = 0; s < SP; s++)
-                if (me.s0 + s < a.S) a.dstate[(n * a.C + c) * a.S + me.s0 + s] = Q[s];
+                if (place.s0 + s < a.S) a.dstate[(n * a.C + c) * a.S + place.s0 + s] = Q[s];
         __syncthreads();                                      // (one env's last sums are read before the next one's first)
     }
+    const ScanPlace& me = place;
+    const int lane = me.lane;
     if constexpr (SPLIT) {
-        part[w][0][0][lane] = dD;
-        part[w][0][1][lane] = dbias;
+        l.du()[lane] = dD;
+        l.dd()[lane] = dbias;
         __syncthreads();
         dD = dbias = 0.f;
         for (int s = 0; s < slices; s++) {
-            dD += part[w - slice + s][0][0][lane];
-            dbias += part[w - slice + s][0][1][lane];
+            const Lds o(lds + (w - slice + s) * Lds::BYTES);
+            dD += o.du()[lane];
+            dbias += o.dd()[lane];
         }
     }
     if (!me.live) return;
@@ -376,7 +449,8 @@ template <class T> int scan_backward(const MoScan& a, hipStream_t s) {
             hipLaunchKernelGGL((k_scan_enter<true>), grid_of((a.N * k.SB * a.C + 255) / 256), dim3(256), 0, s, k);
         }
         const int waves = k.across * k.slices;
-        hipLaunchKernelGGL((k_scan_back<T, SP, SPLIT>), grid_of(k.rows * a.G * k.cuts), dim3(kWave * waves), waves * back_wave_lds<T>(), s, k);
+        static_assert(BackLds<T, false>::BYTES * SCAN_BACK_WAVES <= 160 << 10 && BackLds<T, true>::BYTES <= SCAN_SHARED_LDS<T>, "");
+        hipLaunchKernelGGL((k_scan_back<T, SP, SPLIT>), grid_of(k.rows * a.G * k.cuts), dim3(kWave * waves), waves * (BackLds<T, SPLIT>::BYTES), s, k);
         if (launched("k_scan_back")) return -1;
         const int64_t n = a.T * a.N * a.G * 2 * k.SB;
         if (n && k.cuts > 1) hipLaunchKernelGGL((k_scan_join<T>), grid_of((n + 255) / 256), dim3(256), 0, s, k);
