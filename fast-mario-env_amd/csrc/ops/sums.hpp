@@ -8,46 +8,69 @@ namespace mo {
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR8 = 0x141, DPP_XOR8 = 0x128;   // (mirrored in eights: l to 7 - l)
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E;
 
-// Sums of M values over a wave's 64 lanes, each lane left with one of them: every step sends half of the values to the other half of the
-// lanes, so that M values cost about 3 M instructions and not 12 M. Lane l gets value sum_slot(l) of the M (4, 8, 12 or 16; a slot >= M
-// holds nothing), lanes of equal slots the same sum.
+// Sums of M values over a wave's 64 lanes, each lane left with one of them: every step keeps half of the values in half of the lanes, so that
+// 16 values cost 35 instructions and not 96. Within rows of 16 lanes a value's sum is written over the other's in the lanes that are its own
+// (DPP's bank mask: two instructions a pair); rows are exchanged by permlane swaps (three). Lane l gets value sum_slot(l) of the M (4, 8,
+// 12 or 16; a slot >= M holds nothing), lanes of equal slots the same sum.
 __device__ __forceinline__ int sum_slot(int l, int M) {
-    const int s = ((l >> 5) & 1) | ((l >> 3) & 2) | ((l >> 1) & 4) | ((l << 1) & 8);
-    return M <= 4 ? s & 3 : M <= 8 ? s & 7 : s;
+    if (M <= 4) return ((l >> 3) & 1) | ((l >> 1) & 2);
+    const int s = ((l >> 3) & 1) | ((l >> 1) & 2) | ((l >> 2) & 4);
+    return M <= 8 ? s : s | ((l >> 2) & 8);
+}
+// x = x + (x of lane l ^ 8), y's likewise in the upper eight lanes of each row; then likewise four and four, the others mirrored. (A DPP operand may
+// not have been written by the two instructions before: the nop, and the order of what follows it.)
+__device__ __forceinline__ void row_sums4(float& x0, float x1, float& x2, float x3) {
+    asm("s_nop 1\n\t"
+        "v_add_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp %1, %1, %1 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %0, %2, %2 row_ror:8 row_mask:0xf bank_mask:0xc\n\tv_add_f32_dpp %1, %3, %3 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "s_nop 1\n\t"
+        "v_add_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %0, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa"
+        : "+v"(x0), "+v"(x2)
+        : "v"(x1), "v"(x3));
+}
+__device__ __forceinline__ void row_sums8(float& x0, float x1, float& x2, float x3, float& x4, float x5, float& x6, float x7) {
+    asm("s_nop 1\n\t"
+        "v_add_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp %1, %1, %1 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %2, %2, %2 row_ror:8 row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp %3, %3, %3 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xc\n\tv_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n\tv_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp %2, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %0, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa\n\tv_add_f32_dpp %2, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa"
+        : "+v"(x0), "+v"(x2), "+v"(x4), "+v"(x6)
+        : "v"(x1), "v"(x3), "v"(x5), "v"(x7));
 }
 template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M]) {
     static_assert(M % 4 == 0 && M <= 16, "");
-    const int l = threadIdx.x % kWave;
-    float a[M / 2], b[M / 4];
     typedef unsigned U2 __attribute__((ext_vector_type(2)));
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < M / 2; i++) {
-        const U2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), false, false);
-        a[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < M / 4; i++) {
-        const U2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[2 * i]), __float_as_uint(a[2 * i + 1]), false, false);
-        b[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-    }
-    float r;
-    if constexpr (M == 4) {
-        r = b[0] + dpp<DPP_XOR8>(b[0]);
-        r += dpp<DPP_MIRROR8>(r);
-    } else {
-        const float b3 = M == 16 ? b[M / 4 - 1] : 0.f;
-        const float c0 = (l & 8 ? b[1] : b[0]) + dpp<DPP_XOR8>(l & 8 ? b[0] : b[1]);
-        if constexpr (M == 8) {
-            r = c0 + dpp<DPP_MIRROR8>(c0);
+    for (int i = 0; i < M / 4; i += 2) {
+        if (i + 1 < M / 4) {
+            row_sums8(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], v[4 * i + 4], v[4 * i + 5], v[4 * i + 6], v[4 * i + 7]);
+            r[i + 1] = v[4 * i + 4];
         } else {
-            const float c1 = (l & 8 ? b3 : b[2]) + dpp<DPP_XOR8>(l & 8 ? b[2] : b3);
-            r = (l & 4 ? c1 : c0) + dpp<DPP_MIRROR8>(l & 4 ? c0 : c1);
+            row_sums4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
+        r[i] = v[4 * i];
     }
-    r += dpp<DPP_XOR2>(r);
-    return r + dpp<DPP_XOR1>(r);
+    if constexpr (M > 4) {                                    // rows 0 and 2 keep the first, rows 1 and 3 the second
+        const auto rows = [](float a, float b) {
+            const U2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+            return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+        };
+        r[0] = rows(r[0], r[1]);
+        if constexpr (M > 8) r[2] = rows(r[2], r[3]);
+    } else {
+        const U2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(r[0]), __float_as_uint(r[0]), false, false);
+        r[0] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    const U2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(r[0]), __float_as_uint(M > 8 ? r[2] : r[0]), false, false);
+    float sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    sum += dpp<DPP_XOR2>(sum);
+    return sum + dpp<DPP_XOR1>(sum);
 }
 
 // Column sums of parameters' gradients: `rows` rows of `lines` x C floats, whose first `S` lines are the columns of `first` (C, S) and the
