@@ -167,15 +167,27 @@ template <int SP, bool WITH_C = true> __device__ __forceinline__ void load_bc(St
     }
 }
 // Where bit I of cuts is set: h = u b, for all states. A branch of the whole wave that the compiler does not see: the steps stay one block.
+template <int I> __device__ __forceinline__ void if_start_set8(unsigned cuts, float* h, float u, const float* b) {
+    asm volatile(
+        "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\t"
+        "v_mul_f32 %0, %[u], %8\n\tv_mul_f32 %1, %[u], %9\n\tv_mul_f32 %2, %[u], %10\n\tv_mul_f32 %3, %[u], %11\n\t"
+        "v_mul_f32 %4, %[u], %12\n\tv_mul_f32 %5, %[u], %13\n\tv_mul_f32 %6, %[u], %14\n\tv_mul_f32 %7, %[u], %15\n.Lstart%=:"
+        : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]), "+v"(h[4]), "+v"(h[5]), "+v"(h[6]), "+v"(h[7])
+        : "s"(b[0]), "s"(b[1]), "s"(b[2]), "s"(b[3]), "s"(b[4]), "s"(b[5]), "s"(b[6]), "s"(b[7]), [u] "v"(u), [m] "s"(cuts), [i] "n"(I)
+        : "scc");
+}
+template <int I> __device__ __forceinline__ void if_start_set4(unsigned cuts, float* h, float u, const float* b) {
+    asm volatile(
+        "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\t"
+        "v_mul_f32 %0, %[u], %4\n\tv_mul_f32 %1, %[u], %5\n\tv_mul_f32 %2, %[u], %6\n\tv_mul_f32 %3, %[u], %7\n.Lstart%=:"
+        : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3])
+        : "s"(b[0]), "s"(b[1]), "s"(b[2]), "s"(b[3]), [u] "v"(u), [m] "s"(cuts), [i] "n"(I)
+        : "scc");
+}
 template <int I, int SP> __device__ __forceinline__ void if_start_set(unsigned cuts, float (&h)[SP], float u, const float (&b)[SP]) {
 #pragma unroll
-    for (int s = 0; s < SP; s += 4)
-        asm volatile(
-            "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\tv_mul_f32 %0, %[u], %4\n\tv_mul_f32 %1, %[u], %5\n\t"
-            "v_mul_f32 %2, %[u], %6\n\tv_mul_f32 %3, %[u], %7\n.Lstart%=:"
-            : "+v"(h[s]), "+v"(h[s + 1]), "+v"(h[s + 2]), "+v"(h[s + 3])
-            : "s"(b[s]), "s"(b[s + 1]), "s"(b[s + 2]), "s"(b[s + 3]), [u] "v"(u), [m] "s"(cuts), [i] "n"(I)
-            : "scc");
+    for (int s = 0; s < SP / 8 * 8; s += 8) if_start_set8<I>(cuts, h + s, u, b + s);
+    if constexpr (SP % 8 == 4) if_start_set4<I>(cuts, h + SP - 4, u, b + SP - 4);
 }
 template <class F, int... I> __device__ __forceinline__ void each_step_of(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 template <class F> __device__ __forceinline__ void each_step(F f) { each_step_of(f, std::make_integer_sequence<int, SCAN_STEPS>{}); }
@@ -200,42 +212,53 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
     const int w = wave_here(), slice = SPLIT ? w : 0, cbs = a.G * k.per;
     const int64_t wave = SPLIT ? block_here() : block_here() * SCAN_WAVES + w;
     if (wave >= k.segments * a.N * cbs) return;
-    const ScanPlace me(k, wave / cbs, (int)(wave % cbs), slice, SP);
-    const int64_t n = me.n, first = me.segment * k.each, last = min(k.chunks, first + k.each);
-    const int c = me.c, lane = me.lane;
+    const ScanPlace place(k, wave / cbs, (int)(wave % cbs), slice, SP);
+    const int64_t n = place.n, first = place.segment * k.each, last = min(k.chunks, first + k.each);
+    const int c = place.c;
     T *lx = tiles[w][0], *ldt = tiles[w][1], *lz = tiles[w][SUMS ? 0 : 2];
     const bool gate = !SUMS && a.z.p;
     float A[SP], h[SP], total = 0.f;
-    load_decays<SP>(a, me, A);
-    const int64_t seg0 = ((me.segment * a.N + n) * k.SB + me.s0) * a.C + c;
+    load_decays<SP>(a, place, A);
+    const int64_t seg0 = ((place.segment * a.N + n) * k.SB + place.s0) * a.C + c;
 #pragma unroll
     for (int s = 0; s < SP; s++) {
         if (SUMS) h[s] = 0.f;
         else if (k.segments > 1) h[s] = k.seg_h[seg0 + (int64_t)s * a.C];
-        else h[s] = a.state && me.s0 + s < a.S ? a.state[(n * a.C + c) * a.S + me.s0 + s] : 0.f;
+        else h[s] = a.state && place.s0 + s < a.S ? a.state[(n * a.C + c) * a.S + place.s0 + s] : 0.f;
     }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, D = a.D ? a.D[c] : 0.f;
     ChunkIn<T> ix, idt, iz;
     uint8_t flag = 0;
-    const auto steps_of = [&](int64_t chunk) { return (int)min((int64_t)SCAN_STEPS, a.T - chunk * SCAN_STEPS); };
+    float touch = 0.f;
     const auto ahead = [&](int64_t chunk) {
+        const Scan& k = args_again();
+        const ScanPlace me = place.again();
         const int64_t t0 = chunk * SCAN_STEPS;
-        const int steps = steps_of(chunk);
-        flag = start_of_lane(a, t0, steps, me);
+        const int steps = (int)min((int64_t)SCAN_STEPS, k.a.T - t0);
+        flag = start_of_lane(k.a, t0, steps, me);
+        // (a lane for each 64 bytes of the chunk's B and C, which the scalar loads then find in the L2)
+        const int64_t row = ((t0 + me.lane % SCAN_STEPS) * k.a.N + n) * k.a.G + me.g;
+        touch = k.bc[row * 2 * k.SB + min(me.lane / SCAN_STEPS * 16, 2 * k.SB - 1)];
         if (!k.wide) return;
-        ix.ahead(a.x, t0, steps, me);
-        idt.ahead(a.dt, t0, steps, me);
-        if (gate) iz.ahead(a.z, t0, steps, me);
+        ix.ahead(k.a.x, t0, steps, me);
+        idt.ahead(k.a.dt, t0, steps, me);
+        if (gate) iz.ahead(k.a.z, t0, steps, me);
     };
     if (first < last) ahead(first);
     const int64_t bc_step = a.N * a.G * 2 * k.SB;
-    Uniform bc = uniform(k.bc + ((first * SCAN_STEPS * a.N + n) * a.G + me.g) * 2 * k.SB + me.s0);
+    const int SB = k.SB;
+    Uniform bc = uniform(k.bc + ((first * SCAN_STEPS * a.N + n) * a.G + place.g) * 2 * SB + place.s0);
     StepBC<SP> now;
-    if (first < last) load_bc<SP, !SUMS>(now, bc, k.SB);
+    if (first < last) load_bc<SP, !SUMS>(now, bc, SB);
     for (int64_t chunk = first; chunk < last; chunk++) {
+        const Scan& k = args_again();
+        const MoScan& a = k.a;
+        const ScanPlace me = place.again();
+        const int lane = me.lane;
         const int64_t t0 = chunk * SCAN_STEPS;
-        const int steps = steps_of(chunk);
+        const int steps = (int)min((int64_t)SCAN_STEPS, a.T - t0);
         const unsigned cuts = (unsigned)__ballot(flag != 0);
+        asm volatile("" ::"v"(touch));
         wave_wrote();                                         // (the last chunk's results have been read)
         if (k.wide) {
             ix.arrive(lx, steps, me);
@@ -265,7 +288,7 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
             constexpr int i = decltype(step)::value;
             StepBC<SP> next;
             bc = move_on(bc, bc_step);
-            load_bc<SP, !SUMS>(next, bc, k.SB);
+            load_bc<SP, !SUMS>(next, bc, SB);
             float y = 0.f;
 #pragma unroll
             for (int s = 0; s < SP; s++) h[s] = fmaf(exp2_raw(d[i] * A[s]), h[s], u[i] * now.b[s]);
@@ -302,14 +325,16 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
             }
             __syncthreads();
             if (me.live)
-                for (int i = slice; i < steps; i += k.slices) ((T*)a.out.p)[(t0 + i) * a.out.st + n * a.out.sn + c] = lx[i * kWave + lane];
+                for (int i = slice; i < steps; i += k.slices) ((T*)a.out.p)[(t0 + i) * a.out.st + n * a.out.sn + me.c] = lx[i * kWave + lane];
         } else {
 #pragma unroll
             for (int i = 0; i < SCAN_STEPS; i++) finish(i, u[i]);
             wave_wrote();
-            ChunkIn<T>::leave(lx, a.out, t0, steps, me, k.wide);
+            const Scan& k = args_again();
+            ChunkIn<T>::leave(lx, k.a.out, t0, steps, place.again(), k.wide);
         }
     }
+    const ScanPlace& me = place;
     if (!me.live) return;
     if (SUMS) {
 #pragma unroll

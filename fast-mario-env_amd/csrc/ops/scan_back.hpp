@@ -12,15 +12,29 @@ namespace mo {
 constexpr int BACK_WAVES = SCAN_BACK_WAVES;
 
 // Where bit I of cuts is set: x = y = 0, for all states.
+template <int I> __device__ __forceinline__ void if_start_clear8(unsigned cuts, float* x, float* y) {
+    asm volatile(
+        "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\t"
+        "v_mov_b32 %0, 0\n\tv_mov_b32 %1, 0\n\tv_mov_b32 %2, 0\n\tv_mov_b32 %3, 0\n\tv_mov_b32 %4, 0\n\tv_mov_b32 %5, 0\n\tv_mov_b32 %6, 0\n\tv_mov_b32 %7, 0\n\t"
+        "v_mov_b32 %8, 0\n\tv_mov_b32 %9, 0\n\tv_mov_b32 %10, 0\n\tv_mov_b32 %11, 0\n\tv_mov_b32 %12, 0\n\tv_mov_b32 %13, 0\n\tv_mov_b32 %14, 0\n\tv_mov_b32 %15, 0\n"
+        ".Lstart%=:"
+        : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]),
+          "+v"(y[0]), "+v"(y[1]), "+v"(y[2]), "+v"(y[3]), "+v"(y[4]), "+v"(y[5]), "+v"(y[6]), "+v"(y[7])
+        : [m] "s"(cuts), [i] "n"(I)
+        : "scc");
+}
+template <int I> __device__ __forceinline__ void if_start_clear4(unsigned cuts, float* x, float* y) {
+    asm volatile(
+        "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\tv_mov_b32 %0, 0\n\tv_mov_b32 %1, 0\n\tv_mov_b32 %2, 0\n\tv_mov_b32 %3, 0\n\t"
+        "v_mov_b32 %4, 0\n\tv_mov_b32 %5, 0\n\tv_mov_b32 %6, 0\n\tv_mov_b32 %7, 0\n.Lstart%=:"
+        : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(y[0]), "+v"(y[1]), "+v"(y[2]), "+v"(y[3])
+        : [m] "s"(cuts), [i] "n"(I)
+        : "scc");
+}
 template <int I, int SP> __device__ __forceinline__ void if_start_clear(unsigned cuts, float (&x)[SP], float (&y)[SP]) {
 #pragma unroll
-    for (int s = 0; s < SP; s += 4)
-        asm volatile(
-            "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\tv_mov_b32 %0, 0\n\tv_mov_b32 %1, 0\n\tv_mov_b32 %2, 0\n\tv_mov_b32 %3, 0\n\t"
-            "v_mov_b32 %4, 0\n\tv_mov_b32 %5, 0\n\tv_mov_b32 %6, 0\n\tv_mov_b32 %7, 0\n.Lstart%=:"
-            : "+v"(x[s]), "+v"(x[s + 1]), "+v"(x[s + 2]), "+v"(x[s + 3]), "+v"(y[s]), "+v"(y[s + 1]), "+v"(y[s + 2]), "+v"(y[s + 3])
-            : [m] "s"(cuts), [i] "n"(I)
-            : "scc");
+    for (int s = 0; s < SP / 8 * 8; s += 8) if_start_clear8<I>(cuts, x + s, y + s);
+    if constexpr (SP % 8 == 4) if_start_clear4<I>(cuts, x + SP - 4, y + SP - 4);
 }
 
 // What a segment adds to the Q that comes out of it, and the sum of its step sizes (-1 where an episode starts in it).
