@@ -8,7 +8,7 @@ namespace mo {
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E;
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140;   // (mirrored: l to 7 - l, l to 15 - l)
 
 // Sums of M values over a wave's 64 lanes, each lane left with one of them: every step keeps half of the values in half of the lanes, so that
 // 16 values cost 35 instructions and not 96. Within rows of 16 lanes a value's sum is written over the other's in the lanes that are its own

@@ -169,7 +169,7 @@ int mo_scan(const MoScan* a, void* stream);
 int mo_scan_backward(const MoScan* a, void* stream);
 
 /* One step of the same: T is not looked at, x, dt, z, out (N, C), Bt, Ct (N, G, S), start (N) or NULL; state_out (N, C, S) is read and
- * written (state is not used). A starting env's old state is not read. */
+ * written (state is not used). Nothing of a starting env's old state is seen. */
 int mo_scan_step(const MoScan* a, void* stream);
 
 /* The norm of many tensors together, norm = sqrt(sum of all values' squares), and with `scale` their values times
