@@ -4,16 +4,17 @@
 
 namespace mo {
 
-// The tensors go into the kernels' arguments, up to TABLE of them a launch. A block takes every gridDim.x-th chunk of the launch's
-// values and leaves one float64 sum of squares; the scaling kernel's blocks each add all blocks' sums, in the same order.
-constexpr int GRADIENT_TABLE = 128, GRADIENT_THREADS = 256, GRADIENT_BLOCKS = 1024;
-constexpr int64_t GRADIENT_CHUNK = 16384;
+// The tensors go into the kernels' arguments, up to GRADIENT_TABLE of them a launch. A workgroup takes every gridDim.x-th chunk of the launch's
+// values and leaves one float64 sum of squares; the scaling kernel's workgroups each add all of these, in the same order, and go through the
+// chunks backwards: what was read last is still in the last-level cache. A chunk is read in 16-byte accesses from the first value that lies on 16 bytes.
+constexpr int GRADIENT_TABLE = 128, GRADIENT_THREADS = 256, GRADIENT_BLOCKS = 2048;
+constexpr int64_t GRADIENT_CHUNK = 4096;    // values of the smallest chunk
 struct Gradients {
     void* p[GRADIENT_TABLE];
     int64_t n[GRADIENT_TABLE];
     uint32_t begin[GRADIENT_TABLE + 1];   // the first chunk of each tensor
     uint8_t bf[GRADIENT_TABLE];
-    int count;
+    int count, chunk;
 };
 static_assert(sizeof(Gradients) < 3500, "");
 
@@ -36,12 +37,35 @@ __device__ __forceinline__ double block_sum(double x, double* s) {
     return x;
 }
 
-template <class T> __device__ __forceinline__ double squares(const T* p, int64_t n) {
-    double x = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += GRADIENT_THREADS) {
-        const double v = as_f32(p[i]);
-        x = fma(v, v, x);
+// f(a value's place, 16 bytes or one value) over the chunk's values; IN_FLIGHT accesses a thread before the first is used.
+constexpr int GRADIENT_IN_FLIGHT = 4;
+template <class T, class Wide, class One> __device__ __forceinline__ void over_chunk(T* p, int n, Wide wide, One one) {
+    constexpr int V = 16 / sizeof(T);
+    const int head = min(n, (int)((-(uintptr_t)p & 15) / sizeof(T))), packs = (n - head) / V, tail = head + packs * V;
+    if ((int)threadIdx.x < head) one(p + threadIdx.x);
+    typedef Pack<std::remove_const_t<T>, V> P;
+    P* at = (P*)(uintptr_t)(p + head);
+    int i = threadIdx.x;
+    for (; i + (GRADIENT_IN_FLIGHT - 1) * GRADIENT_THREADS < packs; i += GRADIENT_IN_FLIGHT * GRADIENT_THREADS) {
+        P x[GRADIENT_IN_FLIGHT];
+#pragma unroll
+        for (int j = 0; j < GRADIENT_IN_FLIGHT; j++) x[j] = at[i + j * GRADIENT_THREADS];
+#pragma unroll
+        for (int j = 0; j < GRADIENT_IN_FLIGHT; j++) wide(at + i + j * GRADIENT_THREADS, x[j]);
     }
+    for (; i < packs; i += GRADIENT_THREADS) wide(at + i, at[i]);
+    if (tail + (int)threadIdx.x < n) one(p + tail + threadIdx.x);
+}
+template <class T> __device__ __forceinline__ double squares(const T* p, int n) {
+    double x = 0.0;
+    const auto add = [&](T y) {
+        const double v = as_f32(y);
+        x = fma(v, v, x);
+    };
+    over_chunk(p, n, [&](const auto*, const auto& y) {
+#pragma unroll
+        for (int v = 0; v < (int)(16 / sizeof(T)); v++) add(y.v[v]);
+    }, [&](const T* y) { add(*y); });
     return x;
 }
 __global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_squares(Gradients g, double* part) {
@@ -49,7 +73,8 @@ __global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_squares(Gradients
     double x = 0.0;
     for (unsigned chunk = blockIdx.x; chunk < g.begin[g.count]; chunk += gridDim.x) {
         const int i = tensor_of(g, chunk);
-        const int64_t at = (int64_t)(chunk - g.begin[i]) * GRADIENT_CHUNK, n = min(GRADIENT_CHUNK, g.n[i] - at);
+        const int64_t at = (int64_t)(chunk - g.begin[i]) * g.chunk;
+        const int n = (int)min((int64_t)g.chunk, g.n[i] - at);
         x += g.bf[i] ? squares((const bf16*)g.p[i] + at, n) : squares((const float*)g.p[i] + at, n);
     }
     x = block_sum(x, s);
@@ -66,8 +91,12 @@ __global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_norm(const double
     const double x = norm_of(part, parts, s);
     if (threadIdx.x == 0) *norm = (float)x;
 }
-template <class T> __device__ __forceinline__ void scale_values(T* p, int64_t n, float by) {
-    for (int64_t i = threadIdx.x; i < n; i += GRADIENT_THREADS) p[i] = as<T>(as_f32(p[i]) * by);
+template <class T> __device__ __forceinline__ void scale_values(T* p, int n, float by) {
+    over_chunk(p, n, [&](auto* to, auto y) {
+#pragma unroll
+        for (int v = 0; v < (int)(16 / sizeof(T)); v++) y.v[v] = as<T>(as_f32(y.v[v]) * by);
+        stream(to, y);
+    }, [&](T* y) { *y = as<T>(as_f32(*y) * by); });
 }
 // (max / (norm + eps) is taken in float64 and the factor rounded once to float32; a norm that is NaN makes everything NaN.)
 __global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_scale(Gradients g, const double* part, int64_t parts, float max_norm, float eps, float* norm) {
@@ -75,9 +104,12 @@ __global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_scale(Gradients g
     const double x = norm_of(part, parts, s), f = (double)max_norm / (x + (double)eps);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)x;
     const float by = f > 1.0 ? 1.f : (float)f;
-    for (unsigned chunk = blockIdx.x; chunk < g.begin[g.count]; chunk += gridDim.x) {
+    const unsigned chunks = g.begin[g.count];
+    for (unsigned back = blockIdx.x; back < chunks; back += gridDim.x) {
+        const unsigned chunk = chunks - 1 - back;
         const int i = tensor_of(g, chunk);
-        const int64_t at = (int64_t)(chunk - g.begin[i]) * GRADIENT_CHUNK, n = min(GRADIENT_CHUNK, g.n[i] - at);
+        const int64_t at = (int64_t)(chunk - g.begin[i]) * g.chunk;
+        const int n = (int)min((int64_t)g.chunk, g.n[i] - at);
         if (g.bf[i]) scale_values((bf16*)g.p[i] + at, n, by);
         else scale_values((float*)g.p[i] + at, n, by);
     }
@@ -88,8 +120,12 @@ inline int64_t gradient_launches(int64_t count) { return std::max<int64_t>(1, (c
 inline int64_t gradient_work(int64_t count) { return 8 * gradient_launches(count) * GRADIENT_BLOCKS; }
 inline int gradient_norm(const MoTensor* t, int64_t count, bool scale, float max_norm, float eps, float* norm, double* part, hipStream_t s) {
     const int64_t launches = gradient_launches(count);
+    int64_t values = 0;
+    for (int64_t i = 0; i < count; i++) values += t[i].n;
+    const int64_t chunk = GRADIENT_CHUNK * std::clamp<int64_t>(values / (GRADIENT_CHUNK * GRADIENT_BLOCKS), 1, 16);
     const auto table = [&](int64_t l, Gradients& g) {
         g = Gradients{};
+        g.chunk = (int)chunk;
         uint64_t chunks = 0;
         for (int64_t i = l * GRADIENT_TABLE; i < std::min(count, (l + 1) * GRADIENT_TABLE); i++) {
             const int k = g.count++;
@@ -97,7 +133,7 @@ inline int gradient_norm(const MoTensor* t, int64_t count, bool scale, float max
             g.n[k] = t[i].n;
             g.bf[k] = t[i].dtype == MO_BF16;
             g.begin[k] = (uint32_t)chunks;
-            chunks += (t[i].n + GRADIENT_CHUNK - 1) / GRADIENT_CHUNK;
+            chunks += (t[i].n + chunk - 1) / chunk;
         }
         g.begin[g.count] = (uint32_t)chunks;
         return (unsigned)std::min<uint64_t>(std::max<uint64_t>(chunks, 1), GRADIENT_BLOCKS);
@@ -114,7 +150,7 @@ inline int gradient_norm(const MoTensor* t, int64_t count, bool scale, float max
         hipLaunchKernelGGL(k_gradient_norm, dim3(1), dim3(GRADIENT_THREADS), 0, s, (const double*)part, parts, norm);
         return launched("k_gradient_norm");
     }
-    for (int64_t l = 0; l < launches; l++) {
+    for (int64_t l = launches - 1; l >= 0; l--) {
         const unsigned blocks = table(l, g);
         hipLaunchKernelGGL(k_gradient_scale, dim3(blocks), dim3(GRADIENT_THREADS), 0, s, g, (const double*)part, parts, max_norm, eps, l ? nullptr : norm);
     }

@@ -8,7 +8,7 @@ namespace mo {
 // is the channel's own is computed by each of its lanes. A workgroup has channels of STEP_ENVS envs, whose states it has in flight together, with the
 // same decays; where an env's rows begin is computed once for all lanes. The states are all there is to move: 8 bytes each, which bound it.
 // FAR: the states are more than the last-level cache holds, and go past it.
-constexpr int STEP_ENVS = 2, STEP_THREADS = 256;
+constexpr int STEP_ENVS = 4, STEP_THREADS = 256;
 struct ScanStep {
     MoScan a;
     int lanes, log_lanes, blocks;    // workgroups of an env
