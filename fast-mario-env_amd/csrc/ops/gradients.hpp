@@ -7,16 +7,15 @@ namespace mo {
 // The tensors go into the kernels' arguments, up to GRADIENT_TABLE of them a launch. A workgroup takes every gridDim.x-th chunk of the launch's
 // values and leaves one float64 sum of squares; the scaling kernel's workgroups each add all of these, in the same order, and go through the
 // chunks backwards: what was read last is still in the last-level cache. A chunk is read in 16-byte accesses from the first value that lies on 16 bytes.
-constexpr int GRADIENT_TABLE = 128, GRADIENT_THREADS = 256, GRADIENT_BLOCKS = 2048;
+constexpr int GRADIENT_TABLE = 240, GRADIENT_THREADS = 256, GRADIENT_BLOCKS = 2048;
 constexpr int64_t GRADIENT_CHUNK = 4096;    // values of the smallest chunk
 struct Gradients {
     void* p[GRADIENT_TABLE];
-    int64_t n[GRADIENT_TABLE];
     uint32_t begin[GRADIENT_TABLE + 1];   // the first chunk of each tensor
-    uint8_t bf[GRADIENT_TABLE];
+    uint32_t last[GRADIENT_TABLE];        // values of its last chunk; the top bit: bf16
     int count, chunk;
 };
-static_assert(sizeof(Gradients) < 3500, "");
+static_assert(sizeof(Gradients) < 3900, "");   // (a launch's arguments are 4 KB)
 
 __device__ __forceinline__ int tensor_of(const Gradients& g, unsigned chunk) {
     int lo = 0, hi = g.count - 1;          // the last tensor that begins at or before the chunk
@@ -37,6 +36,18 @@ __device__ __forceinline__ double block_sum(double x, double* s) {
     return x;
 }
 
+struct GradientChunk {
+    void* p;
+    int n;
+    bool bf;
+    __device__ __forceinline__ GradientChunk(const Gradients& g, unsigned chunk) {
+        const int i = tensor_of(g, chunk);
+        const int64_t at = (int64_t)(chunk - g.begin[i]) * g.chunk;
+        bf = g.last[i] >> 31;
+        n = chunk + 1 < g.begin[i + 1] ? g.chunk : (int)(g.last[i] & 0x7fffffffu);
+        p = bf ? (void*)((bf16*)g.p[i] + at) : (void*)((float*)g.p[i] + at);
+    }
+};
 // f(a value's place, 16 bytes or one value) over the chunk's values; IN_FLIGHT accesses a thread before the first is used.
 constexpr int GRADIENT_IN_FLIGHT = 4;
 template <class T, class Wide, class One> __device__ __forceinline__ void over_chunk(T* p, int n, Wide wide, One one) {
@@ -72,10 +83,8 @@ __global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_squares(Gradients
     __shared__ double s[GRADIENT_THREADS / kWave];
     double x = 0.0;
     for (unsigned chunk = blockIdx.x; chunk < g.begin[g.count]; chunk += gridDim.x) {
-        const int i = tensor_of(g, chunk);
-        const int64_t at = (int64_t)(chunk - g.begin[i]) * g.chunk;
-        const int n = (int)min((int64_t)g.chunk, g.n[i] - at);
-        x += g.bf[i] ? squares((const bf16*)g.p[i] + at, n) : squares((const float*)g.p[i] + at, n);
+        const GradientChunk c(g, chunk);
+        x += c.bf ? squares((const bf16*)c.p, c.n) : squares((const float*)c.p, c.n);
     }
     x = block_sum(x, s);
     if (threadIdx.x == 0) part[blockIdx.x] = x;
@@ -106,12 +115,9 @@ __global__ void __launch_bounds__(GRADIENT_THREADS) k_gradient_scale(Gradients g
     const float by = f > 1.0 ? 1.f : (float)f;
     const unsigned chunks = g.begin[g.count];
     for (unsigned back = blockIdx.x; back < chunks; back += gridDim.x) {
-        const unsigned chunk = chunks - 1 - back;
-        const int i = tensor_of(g, chunk);
-        const int64_t at = (int64_t)(chunk - g.begin[i]) * g.chunk;
-        const int n = (int)min((int64_t)g.chunk, g.n[i] - at);
-        if (g.bf[i]) scale_values((bf16*)g.p[i] + at, n, by);
-        else scale_values((float*)g.p[i] + at, n, by);
+        const GradientChunk c(g, chunks - 1 - back);
+        if (c.bf) scale_values((bf16*)c.p, c.n, by);
+        else scale_values((float*)c.p, c.n, by);
     }
 }
 
@@ -128,12 +134,13 @@ inline int gradient_norm(const MoTensor* t, int64_t count, bool scale, float max
         g.chunk = (int)chunk;
         uint64_t chunks = 0;
         for (int64_t i = l * GRADIENT_TABLE; i < std::min(count, (l + 1) * GRADIENT_TABLE); i++) {
+            if (!t[i].n) continue;
             const int k = g.count++;
+            const int64_t of = (t[i].n + chunk - 1) / chunk;
             g.p[k] = t[i].p;
-            g.n[k] = t[i].n;
-            g.bf[k] = t[i].dtype == MO_BF16;
             g.begin[k] = (uint32_t)chunks;
-            chunks += (t[i].n + chunk - 1) / chunk;
+            g.last[k] = (uint32_t)(t[i].n - (of - 1) * chunk) | (t[i].dtype == MO_BF16 ? 1u << 31 : 0u);
+            chunks += of;
         }
         g.begin[g.count] = (uint32_t)chunks;
         return (unsigned)std::min<uint64_t>(std::max<uint64_t>(chunks, 1), GRADIENT_BLOCKS);
