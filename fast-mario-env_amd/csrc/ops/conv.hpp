@@ -5,6 +5,8 @@
 namespace mo {
 
 constexpr int CONV_THREADS = 256;
+// (Gradient) steps whose loads are in flight: as many as leave two waves a SIMD (128 x 2,048 x 512 bf16, K = 4: 258 us with one, 225 with two).
+template <int V> constexpr int CONV_AHEAD = V > 4 ? 2 : 4;
 
 // A thread holds V neighbouring channels of one env and goes through a segment of the steps with the last K - 1 inputs in registers, cleared where an
 // episode starts; segments begin by reading the K - 1 steps before them.
@@ -79,10 +81,14 @@ __global__ void __launch_bounds__(CONV_THREADS) k_conv(Conv k) {
     float w[K][V], b[V], win[K][V];
     load_taps<V, K>(a, c, w, b);
     load_window<T, V, K>(a, t0, n, c, win);
-    for (int64_t t = t0; t < t1; t++) {
+    const T* from = row_at<T>(a.x, t0, n) + c;               // (moved on from step to step: no products of 64 bits between them)
+    T* to = row_at<T>(a.y, t0, n) + c;
+    const uint8_t* flag = a.start ? a.start + t0 * a.N + n : nullptr;
+    for (int64_t t = t0; t < t1; t++, from += a.x.st, to += a.y.st) {
         float x[V], p[V];
-        load_channels<T, V>(x, row_at<T>(a.x, t, n) + c);
-        const bool cut = a.start && a.start[t * a.N + n];
+        load_channels<T, V>(x, from);
+        const bool cut = flag && *flag;
+        if (flag) flag += a.N;
 #pragma unroll
         for (int v = 0; v < V; v++) {
             p[v] = fmaf(w[K - 1][v], x[v], b[v]);
@@ -96,7 +102,7 @@ __global__ void __launch_bounds__(CONV_THREADS) k_conv(Conv k) {
             for (int j = K - 1; j > 1; j--) win[j - 1][v] = win[j - 2][v];
             if (K > 1) win[0][v] = x[v];
         }
-        store_channels<T, V>(row_at<T>(a.y, t, n) + c, p);
+        store_channels<T, V>(to, p);
     }
     if (t1 != a.T || !a.state_out) return;
 #pragma unroll
@@ -107,8 +113,9 @@ __global__ void __launch_bounds__(CONV_THREADS) k_conv(Conv k) {
 // wait[j]. Where an episode starts, what waits is complete and leaves at once; `age` counts the steps since, so that nothing leaves
 // twice. A segment goes K - 1 steps past its end, for its own last inputs. Inputs before step 0 are the entering state's rows.
 template <class T, int V, int K, int ACT>
-__global__ void __launch_bounds__(CONV_THREADS) k_conv_back(Conv k) {
+__global__ void __launch_bounds__(CONV_THREADS, 2) k_conv_back(Conv k) {
     const MoConv& a = k.a;
+    constexpr int AHEAD = CONV_AHEAD<V>;
     const int lanes = a.C / V;
     const int64_t id = block_here() * CONV_THREADS + threadIdx.x, first = id / lanes;
     const int c = (int)(id % lanes) * V;
@@ -136,11 +143,32 @@ __global__ void __launch_bounds__(CONV_THREADS) k_conv_back(Conv k) {
             else if (a.dstate) store_channels<T, V>((T*)a.dstate + (n * (K - 1) + (K - 1 + t)) * a.C + c, x);
         };
         int age = K - 2;
-        for (int64_t t = t0; t < past; t++) {
+        Pack<T, V> px[AHEAD], pdy[AHEAD];
+        uint8_t pcut[AHEAD];
+        const T *from_x = row_at<T>(a.x, t0, n) + c, *from_dy = row_at<T>(a.dy, t0, n) + c;
+        T* to = row_at<T>(a.dx, t0 - (K - 1), n) + c;
+        const uint8_t* flag = a.start ? a.start + t0 * a.N + n : nullptr;
+        const auto ahead = [&](int i) {
+            px[i] = *(const Pack<T, V>*)from_x;
+            pdy[i] = *(const Pack<T, V>*)from_dy;
+            pcut[i] = flag ? *flag : 0;
+            from_x += a.x.st;
+            from_dy += a.dy.st;
+            if (flag) flag += a.N;
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (t0 + i < past) ahead(i);
+        const auto step = [&](int64_t t, int i) {
             float x[V], dy[V];
-            load_channels<T, V>(x, row_at<T>(a.x, t, n) + c);
-            load_channels<T, V>(dy, row_at<T>(a.dy, t, n) + c);
-            if (a.start && a.start[t * a.N + n]) {
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                x[v] = as_f32(px[i].v[v]);
+                dy[v] = as_f32(pdy[i].v[v]);
+            }
+            const bool cut = pcut[i];
+            if (t + AHEAD < past) ahead(i);
+            if (cut) {
 #pragma unroll
                 for (int j = 1; j < K; j++) {
                     if (j <= age + 1) leave(t - j, wait[j]);
@@ -168,7 +196,11 @@ __global__ void __launch_bounds__(CONV_THREADS) k_conv_back(Conv k) {
                     for (int j = 1; j < K; j++) dw[K - 1 - j][v] = fmaf(dp, win[j - 1][v], dw[K - 1 - j][v]);
                 }
             }
-            if (age >= K - 1) leave(t - (K - 1), wait[K - 1]);
+            if (age >= K - 1) {
+                const int64_t done = t - (K - 1);
+                if (done >= 0 && done >= own) store_channels<T, V>(to, wait[K - 1]);   // (at most t1 - 1)
+                else leave(done, wait[K - 1]);
+            }
 #pragma unroll
             for (int v = 0; v < V; v++) {
 #pragma unroll
@@ -177,7 +209,12 @@ __global__ void __launch_bounds__(CONV_THREADS) k_conv_back(Conv k) {
                 for (int j = K - 1; j > 1; j--) win[j - 1][v] = win[j - 2][v];
                 if (K > 1) win[0][v] = x[v];
             }
-        }
+            to += a.dx.st;
+        };
+        for (int64_t t = t0; t < past; t += AHEAD)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (t + i < past) step(t + i, i);
         if (past == a.T)                                      // the last steps' inputs are what is left, and the state after them
 #pragma unroll
             for (int j = 1; j < K; j++) {
@@ -238,18 +275,24 @@ inline bool conv_wide(const MoConv& a, bool backward, bool step) {
     const auto at = [](const void* p) { return (uintptr_t)p % 16 == 0; };
     return a.C % V == 0 && row(a.x) && at(a.state) && (backward ? row(a.dy) && row(a.dx) && at(a.dstate_out) && at(a.dstate) : row(a.y) && at(a.state_out));
 }
-constexpr int64_t CONV_FILL = 256 * 1024;    // threads that fill the card
+// Threads that fill the card; the gradient's have registers for two waves a SIMD (357 us for forward and gradient of 128 x 2,048 x 512, 368 with twice
+// as many threads).
+constexpr int64_t CONV_FILL = 256 * 1024, CONV_BACK_FILL = 256 * 512;
 inline Conv conv_cut(const MoConv& a, int V, bool backward) {
     Conv k{};
     k.a = a;
-    const int64_t lanes = std::max(1, a.C / V), most = std::max<int64_t>(1, CONV_FILL / std::max<int64_t>(1, lanes * a.N));
+    const int64_t lanes = std::max(1, a.C / V), fill = backward ? CONV_BACK_FILL : CONV_FILL, most = std::max<int64_t>(1, fill / std::max<int64_t>(1, lanes * a.N));
     // long segments where there are enough of them; the K - 1 steps before (and after) each are read again
     k.each = std::max<int64_t>(16, (a.T + most - 1) / most);
     k.segments = std::max<int64_t>(1, (a.T + k.each - 1) / k.each);
-    k.rows = backward ? std::min(k.segments * a.N, std::max<int64_t>(1, CONV_FILL / lanes)) : 0;
+    k.rows = backward ? std::min(k.segments * a.N, std::max<int64_t>(1, fill / lanes)) : 0;
     return k;
 }
-inline int conv_width(const MoConv& a, bool backward, bool step) { return conv_wide(a, backward, step) ? (a.dtype == MO_BF16 ? 8 : 4) : 1; }
+// (The gradient's registers go by K and V: four channels a thread from five taps on.)
+inline int conv_width(const MoConv& a, bool backward, bool step) {
+    if (!conv_wide(a, backward, step)) return 1;
+    return a.dtype == MO_BF16 && !(backward && a.K > 4) ? 8 : 4;
+}
 inline int64_t conv_back_work(const MoConv& a) {
     if (!a.dweight || a.N == 0) return 0;      // (without steps the sums are made all the same: zeros)
     const Conv k = conv_cut(a, conv_width(a, true, false), true);
@@ -277,9 +320,9 @@ template <class T, int V, int K, int ACT, int RUN> int conv_launch(const MoConv&
         }
     }
 }
-template <class T, int V, int RUN, int ACT, int K = 1> int conv_taps(const MoConv& a, hipStream_t s) {
-    if constexpr (K > MO_MAX_TAPS) return fail("taps");
-    else return a.K == K ? conv_launch<T, V, K, ACT, RUN>(a, s) : conv_taps<T, V, RUN, ACT, K + 1>(a, s);
+template <class T, int V, int RUN, int ACT, int K = 1, int LAST = MO_MAX_TAPS> int conv_taps(const MoConv& a, hipStream_t s) {
+    if constexpr (K > LAST) return fail("taps");
+    else return a.K == K ? conv_launch<T, V, K, ACT, RUN>(a, s) : conv_taps<T, V, RUN, ACT, K + 1, LAST>(a, s);
 }
 
 }  // namespace mo

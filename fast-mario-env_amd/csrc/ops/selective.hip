@@ -24,10 +24,17 @@ bool conv_params(const MoConv* a) { return usable(a->weight, "weight", 4) && (!a
 bool maybe(const void* p, const char* name, size_t align) { return !p || usable(p, name, align); }
 
 template <class T, int RUN> int conv_run(const MoConv& a, hipStream_t s) {
-    constexpr int V = 16 / sizeof(T);
     return by_act(a.act, [&](auto act) {
         constexpr int A = decltype(act)::value;
-        return conv_width(a, RUN == 1, RUN == 2) == V ? conv_taps<T, V, RUN, A>(a, s) : conv_taps<T, 1, RUN, A>(a, s);
+        const int V = conv_width(a, RUN == 1, RUN == 2);
+        if constexpr (sizeof(T) == 2) {
+            if (V == 8) return conv_taps<T, 8, RUN, A, 1, RUN == 1 ? 4 : MO_MAX_TAPS>(a, s);
+            if constexpr (RUN == 1)
+                if (V == 4) return conv_taps<T, 4, RUN, A, 5>(a, s);
+        } else {
+            if (V == 4) return conv_taps<T, 4, RUN, A>(a, s);
+        }
+        return conv_taps<T, 1, RUN, A>(a, s);
     });
 }
 
