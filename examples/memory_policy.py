@@ -1,7 +1,7 @@
 """A policy with a memory, trained for a few updates: rollouts of HipVecEnv under `make_memory_net`, then PPO's clipped loss over
 whole sequences of the stored rollout, minibatch by minibatch of envs.
 
-    python examples/memory_policy.py [--rom PATH] [--envs 256] [--steps 64] [--updates 4] [--device cuda]
+    python examples/memory_policy.py [--rom PATH] [--envs 256] [--steps 64] [--updates 4] [--memory attention|scan] [--device cuda]
 """
 import argparse
 import os
@@ -15,7 +15,7 @@ import torch  # noqa: E402
 
 from fast_mario_env_amd import HipVecEnv  # noqa: E402
 from fast_mario_env_amd.memory import make_memory_net  # noqa: E402
-from fast_mario_env_amd.rollout import Rollout  # noqa: E402
+from fast_mario_env_amd.rollout import Rollout, clip_gradients  # noqa: E402
 
 
 def update(net, opt, ro, minibatches=4, clip=0.2):
@@ -30,7 +30,7 @@ def update(net, opt, ro, minibatches=4, clip=0.2):
         loss = -torch.minimum(ratio * a, ratio.clamp(1 - clip, 1 + clip) * a).mean() + 0.5 * (value - ret[:, envs]).square().mean()
         opt.zero_grad(set_to_none=True)
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(net.parameters(), 0.5)
+        clip_gradients(net.parameters(), 0.5)
         opt.step()
         total = total + loss.detach()
     return total / minibatches
@@ -42,12 +42,13 @@ def main():
     ap.add_argument("--envs", type=int, default=256)
     ap.add_argument("--steps", type=int, default=64)
     ap.add_argument("--updates", type=int, default=4)
+    ap.add_argument("--memory", choices=("attention", "scan"), default="attention")
     ap.add_argument("--device", default="cuda")
     args = ap.parse_args()
     with open(args.rom, "rb") as f:
         env = HipVecEnv("1-1", args.envs, seed=0, sticky=0.25, noop_max=30, maxpool=True, rom=f.read(), device=args.device)
     env.reset()
-    net = make_memory_net(device=args.device)
+    net = make_memory_net(device=args.device, memory=args.memory)
     opt = torch.optim.Adam(net.parameters(), 2.5e-4)
     ro = Rollout(env, net, T=args.steps)
     for i in range(args.updates):

@@ -316,48 +316,53 @@ def state_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, start=N
 
 
 # ---------------------------------------------------------------- an actor-critic with a memory
-def make_memory_net(n_actions: int = N_ACTIONS, in_ch: int = 4, heads: int = 8, seed: int = 0, device="cuda"):
+def make_memory_net(n_actions: int = N_ACTIONS, in_ch: int = 4, heads: int = 8, seed: int = 0, device="cuda", memory: str = "attention",
+                    states: int = 16, taps: int = 4):
     """The Nature trunk of `make_net` with a group norm after each convolution, and between its features and the two heads a
-    memory: projection to q, k and v, linear attention with `heads` decaying memories of 512 / heads, group norm a head,
-    projection, added to the features. Random weights. On the GPU the trunk and the memory run in bf16 (the memories
-    themselves and the heads in float32), on the CPU everything in float32."""
+    memory, added to the features:
+
+    - "attention": projection to q, k and v, linear attention with `heads` decaying memories of 512 / heads, group norm a head, projection;
+    - "scan": projection to x and z, causal convolution of x over `taps` steps, projection to step sizes (through 32 values), B and C, a state
+      space scan with `states` states a channel, gated by z, projection.
+
+    Random weights. On the GPU the trunk and the memory run in bf16 (the memories themselves and the heads in float32), on the CPU
+    everything in float32."""
     nn, F = torch.nn, torch.nn.functional
-    width = 512
-    if heads < 1 or width % heads or width // heads > MAX_HEAD:
+    width, rank = 512, 32
+    if memory not in ("attention", "scan"):
+        raise ValueError("make_memory_net: memory must be attention or scan")
+    if memory == "attention" and (heads < 1 or width % heads or width // heads > MAX_HEAD):
         raise ValueError(f"make_memory_net: heads must divide {width} into heads of at most {MAX_HEAD}")
+    if memory == "scan" and not (1 <= states <= MAX_STATES and 1 <= taps <= MAX_TAPS):
+        raise ValueError(f"make_memory_net: 1 .. {MAX_STATES} states and 1 .. {MAX_TAPS} taps")
 
     class MemoryAC(nn.Module):
         def __init__(self):
             super().__init__()
-            self.heads = heads
             self.convs = nn.ModuleList([nn.Conv2d(in_ch, 32, 8, 4), nn.Conv2d(32, 64, 4, 2), nn.Conv2d(64, 64, 3, 1)])
             self.norms = nn.ModuleList([nn.GroupNorm(8, c) for c in (32, 64, 64)])   # (parameters; group_norm_act computes)
             self.fc = nn.Linear(64 * 7 * 7, width)
-            self.qkv = nn.Linear(width, 3 * width, bias=False)
-            self.norm = nn.GroupNorm(heads, width)
+            self._make_memory()
             self.out = nn.Linear(width, width, bias=False)
             self.pi = nn.Linear(width, n_actions)
             self.vf = nn.Linear(width, 1)
-            self.register_buffer("decay", head_decays(heads, "cpu"))
             for m in list(self.convs) + [self.fc]:
                 nn.init.orthogonal_(m.weight, math.sqrt(2.0))
                 nn.init.zeros_(m.bias)
-            for m, gain in ((self.qkv, 1.0), (self.out, 1.0), (self.pi, 0.01), (self.vf, 1.0)):
+            for m, gain in ((self.into, 1.0), (self.out, 1.0), (self.pi, 0.01), (self.vf, 1.0)):
                 nn.init.orthogonal_(m.weight, gain)
             nn.init.zeros_(self.pi.bias)
             nn.init.zeros_(self.vf.bias)
 
-        def initial_state(self, n: int):
-            """The memories of n envs before anything: (n, heads, D, D) float32 zeros."""
-            d = width // heads
-            return torch.zeros(n, heads, d, d, device=self.decay.device)
+        def _device(self):
+            return self.fc.weight.device
 
         def _autocast(self):
-            on = self.decay.is_cuda
+            on = self.fc.weight.is_cuda
             return torch.autocast("cuda" if on else "cpu", dtype=torch.bfloat16, enabled=on)
 
         def _features(self, obs_u8):
-            """uint8 (B, k, 84, 84) -> the projected features and q, k, v of each, (B, 512) and (B, heads, D)."""
+            """uint8 (B, k, 84, 84) -> the projected features and what goes into the memory, (B, 512) and (B, ..)."""
             if obs_u8.is_cuda:
                 x = torch.empty(obs_u8.shape, dtype=torch.bfloat16, device=obs_u8.device, memory_format=torch.channels_last)
                 policy_input(obs_u8.contiguous(), x)
@@ -367,30 +372,28 @@ def make_memory_net(n_actions: int = N_ACTIONS, in_ch: int = 4, heads: int = 8, 
                 for c, g in zip(self.convs, self.norms):
                     x = group_norm_act(c(x), g.num_groups, g.weight, g.bias, eps=g.eps, act="silu")
                 h = F.silu(self.fc(x.flatten(1)))
-                q, k, v = (y.unflatten(-1, (heads, -1)) for y in self.qkv(h).chunk(3, -1))
-            return h, q, k, v
+                return h, self.into(h)
 
-        def _heads(self, h, memory):
+        def _heads(self, h, y):
             with self._autocast():
-                y = group_norm_act(memory.flatten(1), heads, self.norm.weight, self.norm.bias, eps=self.norm.eps, act="silu")
-                h = h + self.out(y)
+                h = h + self.out(self._leave(y))
             h = h.float()
             return self.pi(h), self.vf(h).squeeze(-1)
 
         def forward(self, obs_u8, start=None, state=None):
-            """A rollout: obs_u8 (T, N, k, 84, 84) uint8, start (T, N) bool and state (N, heads, D, D), the memories before it ->
-            logits (T, N, A), values (T, N), the memories after it."""
+            """A rollout: obs_u8 (T, N, k, 84, 84) uint8, start (T, N) bool and state, the memories before it (as `initial_state`
+            makes them) -> logits (T, N, A), values (T, N), the memories after it."""
             T, N = obs_u8.shape[:2]
-            h, q, k, v = self._features(obs_u8.flatten(0, 1))
-            out, state = linear_attention(*(y.unflatten(0, (T, N)) for y in (q, k, v)), self.decay, start, state)
-            logits, value = self._heads(h, out.flatten(0, 1))
+            h, u = self._features(obs_u8.flatten(0, 1))
+            y, state = self._remember(u.unflatten(0, (T, N)), start, state)
+            logits, value = self._heads(h, y.flatten(0, 1))
             return logits.unflatten(0, (T, N)), value.unflatten(0, (T, N)), state
 
         @torch.no_grad()
         def step(self, obs_u8, start, state):
             """One step: obs_u8 (N, k, 84, 84), start (N,) bool or None; state is updated. Logits (N, A), values (N,)."""
-            h, q, k, v = self._features(obs_u8)
-            return self._heads(h, linear_attention_step(q, k, v, self.decay, state, start))
+            h, u = self._features(obs_u8)
+            return self._heads(h, self._remember_step(u, start, state))
 
         @torch.no_grad()
         def act(self, obs_u8, generator=None, start=None, state=None):
@@ -401,8 +404,78 @@ def make_memory_net(n_actions: int = N_ACTIONS, in_ch: int = 4, heads: int = 8, 
             a = (logp - torch.log(-torch.log(u))).argmax(-1)
             return a, logp.gather(-1, a[:, None]).squeeze(-1), value
 
+    class AttentionAC(MemoryAC):
+        def _make_memory(self):
+            self.heads = heads
+            self.qkv = nn.Linear(width, 3 * width, bias=False)
+            self.norm = nn.GroupNorm(heads, width)
+            self.register_buffer("decay", head_decays(heads, "cpu"))
+
+        @property
+        def into(self):
+            return self.qkv
+
+        def initial_state(self, n: int):
+            """The memories of n envs before anything: (n, heads, D, D) float32 zeros."""
+            d = width // heads
+            return torch.zeros(n, heads, d, d, device=self._device())
+
+        def _split(self, u):
+            return (y.unflatten(-1, (heads, -1)) for y in u.chunk(3, -1))
+
+        def _remember(self, u, start, state):
+            out, state = linear_attention(*self._split(u), self.decay, start, state)
+            return out.flatten(2), state
+
+        def _remember_step(self, u, start, state):
+            return linear_attention_step(*self._split(u), self.decay, state, start).flatten(1)
+
+        def _leave(self, y):
+            return group_norm_act(y, heads, self.norm.weight, self.norm.bias, eps=self.norm.eps, act="silu")
+
+    class ScanAC(MemoryAC):
+        def _make_memory(self):
+            self.into = nn.Linear(width, 2 * width, bias=False)
+            self.taps = nn.Parameter(torch.randn(width, taps) / taps ** 0.5)
+            self.taps_bias = nn.Parameter(torch.zeros(width))
+            self.select = nn.Linear(width, rank + 2 * states, bias=False)
+            self.sizes = nn.Linear(rank, width, bias=False)
+            # step sizes from 0.001 to 0.1 and decay rates 1 .. states: memories of a few steps to about a thousand
+            size = torch.exp(torch.rand(width) * math.log(100.0) + math.log(0.001))
+            self.size_bias = nn.Parameter(torch.log(torch.expm1(size)))
+            self.log_rate = nn.Parameter(torch.log(torch.arange(1.0, states + 1.0)).repeat(width, 1))
+            self.skip = nn.Parameter(torch.ones(width))
+
+        def initial_state(self, n: int):
+            """The memories of n envs before anything: zeros, the last inputs (n, taps - 1, 512) and the states (n, 512, states) float32."""
+            dev = self._device()
+            return (torch.zeros(n, taps - 1, width, device=dev, dtype=torch.bfloat16 if dev.type == "cuda" else torch.float32),
+                    torch.zeros(n, width, states, device=dev))
+
+        def _scan_in(self, x):
+            """Of the convolved inputs (.., 512): step sizes, B and C, and what does not go by the step."""
+            with self._autocast():
+                small, B, C = self.select(x).split((rank, states, states), -1)
+                dt = self.sizes(small)
+            return dict(x=x, dt=dt, A=-torch.exp(self.log_rate), B=B.unsqueeze(-2), C=C.unsqueeze(-2), D=self.skip, dt_bias=self.size_bias)
+
+        def _remember(self, u, start, state):
+            x, z = u.chunk(2, -1)
+            window, states_before = (None, None) if state is None else state
+            x, window = causal_conv_act(x, self.taps, self.taps_bias, start, window)
+            y, after = state_scan(**self._scan_in(x), z=z, start=start, state=states_before)
+            return y, (window, after)
+
+        def _remember_step(self, u, start, state):
+            x, z = u.chunk(2, -1)
+            x = causal_conv_act_step(x, self.taps, self.taps_bias, state[0], start)
+            return state_scan_step(**self._scan_in(x), z=z, start=start, state=state[1])
+
+        def _leave(self, y):
+            return y
+
     torch.manual_seed(seed)
-    net = MemoryAC().to(device)
+    net = (AttentionAC if memory == "attention" else ScanAC)().to(device)
     if torch.device(device).type == "cuda":
         net = net.to(memory_format=torch.channels_last)
     return net

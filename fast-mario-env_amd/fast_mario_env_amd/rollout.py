@@ -407,6 +407,13 @@ def _steps_memories(net) -> bool:
     return hasattr(net, "initial_state") and {"start", "state"} <= set(inspect.signature(net.act).parameters)
 
 
+def _each(f, *memories):
+    """f of memories that are one tensor each, or tuples of tensors; None of None."""
+    if memories[0] is None:
+        return None
+    return tuple(map(f, *memories)) if isinstance(memories[0], tuple) else f(*memories)
+
+
 class Rollout:
     """T-step rollouts of `env` (a HipVecEnv) under `net`, stored frame-deduplicated on the env's device."""
 
@@ -428,8 +435,8 @@ class Rollout:
         self.next_val = torch.zeros(n, device=dev)
         self.next_start = torch.zeros(n, dtype=torch.bool, device=dev)
         self._starting = torch.ones(n, dtype=torch.bool, device=dev)   # the current obs is a reset stack
-        self.memory = net.initial_state(n) if _steps_memories(net) else None   # now, and when the rollout began
-        self.memory0 = None if self.memory is None else self.memory.clone()
+        self.memory = net.initial_state(n) if _steps_memories(net) else None   # now, and when the rollout began: a tensor or a tuple of them
+        self.memory0 = _each(lambda m: m.clone(), self.memory)
         self.env_ms = 0.0
 
     def collect(self):
@@ -438,8 +445,7 @@ class Rollout:
         torch, env = self.torch, self.env
         ev = [(torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)) for _ in range(self.T)]
         self.first.copy_(env.obs)
-        if self.memory is not None:
-            self.memory0.copy_(self.memory)
+        _each(lambda m0, m: m0.copy_(m), self.memory0, self.memory)
         for t in range(self.T):
             obs = env.obs                                    # the env's buffer, read in place
             self.frames[t].copy_(obs[:, -1])
@@ -455,7 +461,7 @@ class Rollout:
             if self.bootstrap_timeouts:
                 self._bootstrap(t, term, trunc)
             torch.logical_or(term, trunc, out=self._starting)   # the next obs is a reset stack
-        _, _, v = self._act(env.obs, None if self.memory is None else self.memory.clone())   # (the next rollout steps from here)
+        _, _, v = self._act(env.obs, _each(lambda m: m.clone(), self.memory))   # (the next rollout steps from here)
         self.next_val.copy_(v)
         self.next_start.copy_(self._starting)
         torch.cuda.synchronize(env.dev)
@@ -476,7 +482,7 @@ class Rollout:
         ti = tmask.nonzero().squeeze(-1)
         with torch.no_grad():
             final = self.env.final_obs[ti]
-            _, v = self.net(final) if self.memory is None else self.net.step(final, None, self.memory[ti])
+            _, v = self.net(final) if self.memory is None else self.net.step(final, None, _each(lambda m: m[ti], self.memory))
         self.rew[t, ti] += self.gamma * v
 
     def obs(self, t: int, envs=slice(None)):
@@ -499,7 +505,7 @@ class Rollout:
         episode starts (T, n) and the memories before the first step. `net(*sequence)` computes the rollout again."""
         torch = self.torch
         return (torch.stack([self.obs(t, envs) for t in range(self.T)]), self.start[:, envs].contiguous(),
-                None if self.memory0 is None else self.memory0[envs])
+                _each(lambda m: m[envs], self.memory0))
 
     def advantages(self, gamma: float | None = None, lam: float = 0.95):
         g = self.gamma if gamma is None else gamma
