@@ -358,12 +358,24 @@ template <bool BACK> __global__ void __launch_bounds__(256) k_scan_enter(Scan k)
     const float* from = BACK ? a.dstate_out : a.state;
     const float A = real ? a.A[(int64_t)c * a.S + s] * LOG2E : 0.f;
     float h = from && real ? from[(n * a.C + c) * a.S + s] : 0.f;
-    for (int64_t i = 0; i < k.segments; i++) {
-        const int64_t j = BACK ? k.segments - 1 - i : i;
-        float* at = k.seg_h + ((j * a.N + n) * k.SB + s) * a.C + c;
-        const float d = k.seg_d[(j * a.N + n) * a.C + c], add = *at;
-        *at = h;
-        h = d < 0.f ? add : fmaf(exp2_raw(d * A), h, add);
+    constexpr int IN_FLIGHT = 8;                              // segments whose values are read before they are joined
+    for (int64_t i0 = 0; i0 < k.segments; i0 += IN_FLIGHT) {
+        float add[IN_FLIGHT], d[IN_FLIGHT];
+        const auto of = [&](int i) {
+            const int64_t j = min(i0 + i, k.segments - 1);
+            return BACK ? k.segments - 1 - j : j;
+        };
+#pragma unroll
+        for (int i = 0; i < IN_FLIGHT; i++) {
+            add[i] = k.seg_h[((of(i) * a.N + n) * k.SB + s) * a.C + c];
+            d[i] = k.seg_d[(of(i) * a.N + n) * a.C + c];
+        }
+#pragma unroll
+        for (int i = 0; i < IN_FLIGHT; i++) {
+            if (i0 + i >= k.segments) break;
+            k.seg_h[((of(i) * a.N + n) * k.SB + s) * a.C + c] = h;
+            h = d[i] < 0.f ? add[i] : fmaf(exp2_raw(d[i] * A), h, add[i]);
+        }
     }
 }
 
@@ -375,7 +387,7 @@ inline ScanCut scan_slices(int S) {
 }
 constexpr int64_t SCAN_FILL = 4096;     // waves that fill the card
 constexpr int SCAN_BACK_WAVES = 8;      // waves a workgroup of the gradient, at most
-template <class T> constexpr int SCAN_SHARED_LDS = (sizeof(T) == 2 ? 18 : 22) << 10;   // LDS of a wave there that shares its channels
+template <class T> constexpr int SCAN_SHARED_LDS = (sizeof(T) == 2 ? 18 : 20) << 10;   // LDS of a wave there that shares its channels
 inline Scan scan_cut(const MoScan& a, bool backward) {
     Scan k{};
     k.a = a;
@@ -390,17 +402,21 @@ inline Scan scan_cut(const MoScan& a, bool backward) {
     };
     k.wide = k.Cg % V == 0 && row(a.x) && row(a.dt) && row(a.z) && (backward ? row(a.dout) && row(a.dx) && row(a.ddt) && row(a.dz) : row(a.out));
     k.chunks = (a.T + SCAN_STEPS - 1) / SCAN_STEPS;
-    // Few sequences are cut over their length: each segment is gone through twice, once for what it adds to the state.
-    const int64_t waves = std::max<int64_t>(1, a.N * a.G * k.per * k.slices), most = std::max<int64_t>(1, SCAN_FILL / waves);
-    k.segments = most >= 4 ? std::min(most, std::max<int64_t>(1, k.chunks / 4)) : 1;
-    k.each = std::max<int64_t>(1, (k.chunks + k.segments - 1) / k.segments);
-    k.segments = std::max<int64_t>(1, (k.chunks + k.each - 1) / k.each);
     const int room = k.slices == 1 ? SCAN_BACK_WAVES : (160 << 10) / (a.dtype == MO_BF16 ? SCAN_SHARED_LDS<bf16> : SCAN_SHARED_LDS<float>);
     k.across = std::min(k.per, std::min(SCAN_BACK_WAVES, room) / k.slices);
     k.cuts = (k.per + k.across - 1) / k.across;
-    if (backward) {   // as many at a time as fill the card, and about the same number of turns for each
-        const int64_t items = k.segments * a.N, fill = std::max<int64_t>(1, SCAN_FILL / (a.G * k.cuts * k.across * k.slices));
-        const int64_t turns = std::max<int64_t>(1, (items + fill - 1) / fill);
+    // Few sequences are cut over their length: each segment is gone through twice, once for what it adds to the state. The forward pass has many waves a
+    // compute unit and takes whatever number; the gradient has few, so its segments are as many as run at once (1,999 steps of 8 envs, 512
+    // channels: 32 segments, 160 us; 50, which run in two rounds, 201).
+    const int64_t waves = std::max<int64_t>(1, a.N * a.G * k.per * k.slices), most = std::max<int64_t>(1, SCAN_FILL / waves);
+    const int block = k.across * k.slices, lds = k.slices > 1 ? (a.dtype == MO_BF16 ? 18 : 20) : (a.dtype == MO_BF16 ? 14 : 18);
+    const int64_t at_once = std::max<int64_t>(1, 256 * std::max(1, std::min(160 / (block * lds), (c.SP > 8 ? 8 : 12) / block)) / (a.G * k.cuts));
+    const int64_t want = backward ? at_once / std::max<int64_t>(1, a.N) : most >= 4 ? most : 1;
+    k.segments = std::max<int64_t>(1, std::min(want, k.chunks / 4));
+    k.each = std::max<int64_t>(1, (k.chunks + k.segments - 1) / k.segments);
+    k.segments = std::max<int64_t>(1, (k.chunks + k.each - 1) / k.each);
+    if (backward) {   // as many at a time as run at once, and about the same number of turns for each
+        const int64_t items = k.segments * a.N, turns = std::max<int64_t>(1, (items + at_once - 1) / at_once);
         k.rows = (items + turns - 1) / turns;
     }
     return k;

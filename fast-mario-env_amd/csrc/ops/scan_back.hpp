@@ -129,7 +129,8 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan_back_sums(Scan k) {
 // its size d, d's slope by dt, dy and y; the sums for its workgroup's dB and dC, of two chunks in turn; where waves share channels, du and dd.
 template <class T, bool SPLIT> struct BackLds {
     static constexpr int TILE = SCAN_STEPS * kWave, SUMS = 2 * SCAN_STEPS * 32;
-    static constexpr int BYTES = 4 * TILE * (int)sizeof(T) + (4 * TILE + SUMS + (SPLIT ? 2 * TILE : 0)) * 4;
+    static constexpr bool OVER = sizeof(T) == 4;      // dd takes dt's place, which waves that share channels do not write to
+    static constexpr int BYTES = 4 * TILE * (int)sizeof(T) + (4 * TILE + SUMS + (!SPLIT ? 0 : OVER ? TILE : 2 * TILE)) * 4;
     T* t;
     __device__ __forceinline__ explicit BackLds(char* p) : t((T*)p) {}
     __device__ __forceinline__ T* x() const { return t; }
@@ -142,7 +143,7 @@ template <class T, bool SPLIT> struct BackLds {
     __device__ __forceinline__ float* y() const { return d() + 3 * TILE; }
     __device__ __forceinline__ float* sums() const { return d() + 4 * TILE; }        // (2, SCAN_STEPS, 32)
     __device__ __forceinline__ float* du() const { return sums() + SUMS; }
-    __device__ __forceinline__ float* dd() const { return du() + TILE; }
+    __device__ __forceinline__ float* dd() const { return OVER ? (float*)dt() : du() + TILE; }
 };
 
 template <class T, int SP, bool SPLIT>

@@ -10,6 +10,8 @@
 
 #include <algorithm>
 #include <optional>
+#include <string>
+#include <vector>
 
 #include "../../../include/mario_ops.h"
 
@@ -437,31 +439,38 @@ Tensor scan_step(const Tensor& x, const Tensor& dt, const Tensor& A, const Tenso
 
 // ---------------------------------------------------------------- the gradients' norm
 // Tensors that fill their memory without gaps are taken as they lie; others by a copy, which goes back after scaling. What overlaps in memory is refused.
-Tensor gradient_norm(const std::vector<Tensor>& grads, bool scale, double max_norm, double eps) {
-    const Tensor& first = grads[0];
+Tensor gradient_norm(const std::string& name, const std::vector<Tensor>& given, bool scale, double max_norm, double eps) {
+    const Tensor& first = given[0];
     const c10::DeviceGuard guard(first.device());
+    const at::NoGradGuard no_grad;
     std::vector<Tensor> held;
     std::vector<MoTensor> list;
     std::vector<std::pair<char*, char*>> spans;
-    held.reserve(grads.size());
-    list.reserve(grads.size());
-    for (const Tensor& g : grads) {
-        held.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
-        list.push_back({held.back().data_ptr(), held.back().numel(), dtype_of(g), 0});
-        if (!scale || !g.numel()) continue;
+    held.reserve(given.size());
+    list.reserve(given.size());
+    spans.reserve(given.size());
+    for (const Tensor& g : given) {
+        TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.is_floating_point() && g.device() == first.device(), name, ": gradients must be dense float tensors on one device");
+        TORCH_CHECK_VALUE(g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16, name, ": gradients on the GPU must be float32 or bf16");
+        const bool as_it_lies = g.is_non_overlapping_and_dense() && !g.is_neg();
         int64_t last = 0;
-        for (int64_t d = 0; d < g.dim(); d++) last += (g.size(d) - 1) * g.stride(d);
-        spans.push_back({(char*)g.data_ptr(), (char*)g.data_ptr() + (last + 1) * g.element_size()});
+        for (int64_t d = 0; d < g.dim() && !as_it_lies; d++) {
+            TORCH_CHECK_VALUE(g.stride(d) || g.size(d) < 2, name, ": a gradient shares elements with itself (expanded)");
+            last += (g.size(d) - 1) * g.stride(d);
+        }
+        held.push_back(as_it_lies ? g : g.is_neg() ? g.resolve_neg().contiguous() : g.contiguous());
+        list.push_back({held.back().data_ptr(), g.numel(), dtype_of(g), 0});
+        char* const at = (char*)g.data_ptr();
+        if (scale && g.numel()) spans.push_back({at, at + (as_it_lies ? g.numel() : last + 1) * g.element_size()});
     }
     std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); i++)
-        TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "clip_gradients: two gradients share memory");
+    for (size_t i = 1; i < spans.size(); i++) TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, name, ": two gradients share memory");
     const Tensor norm = at::empty({}, first.options().dtype(at::kFloat)), work = work_of(ok(mo_gradient_work((int64_t)list.size()), "mo_gradient_work"), first);
     ok(mo_gradient_norm(list.data(), (int64_t)list.size(), scale, (float)max_norm, (float)eps, data(norm), data<void>(work), stream_of(first)), "mo_gradient_norm");
     if (scale)
-        for (size_t i = 0; i < grads.size(); i++) {
-            if (held[i].unsafeGetTensorImpl() == grads[i].unsafeGetTensorImpl()) written(grads[i]);
-            else grads[i].copy_(held[i]);
+        for (size_t i = 0; i < given.size(); i++) {
+            if (list[i].p == given[i].data_ptr()) written(given[i]);
+            else given[i].copy_(held[i]);
         }
     return norm;
 }

@@ -337,35 +337,28 @@ def gae(rew, val, start, next_val, next_start, gamma: float = 0.99, lam: float =
     return adv, adv + val
 
 
-def _gradients(parameters, name):
-    """The gradients of tensors (one, or an iterable), each once: float32 or bf16 on one GPU, as the kernels take them, or any on the CPU."""
+def _gradients(parameters):
+    """The gradients of tensors (one, or an iterable), each once."""
     torch = _torch()
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    seen, grads = set(), []
-    for p in parameters:
-        g = p.grad
-        if g is None or id(g) in seen:
-            continue
-        seen.add(id(g))
-        grads.append(g)
-    for g in grads:
-        if g.layout != torch.strided or not g.is_floating_point() or g.device != grads[0].device:
-            raise ValueError(f"{name}: gradients must be dense float tensors on one device")
-        if g.is_cuda and g.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"{name}: gradients on the GPU must be float32 or bf16")
-        if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
-            raise ValueError(f"{name}: a gradient shares elements with itself (expanded)")
-    return grads
+    grads = [g for g in (p.grad for p in parameters) if g is not None]
+    by_id = {id(g): g for g in grads}
+    return grads if len(by_id) == len(grads) else list(by_id.values())
 
 
 def _norm_kernel_takes(grads):
     torch = _torch()
-    return bool(grads) and all(type(g) is torch.Tensor and g.is_cuda and not g.is_neg() for g in grads) and not _transformed(*grads)
+    return bool(grads) and grads[0].is_cuda and all(type(g) is torch.Tensor for g in grads) and not _transformed(*grads)
 
 
-def _norm_plain(grads):
+def _norm_plain(grads, name):
     torch = _torch()
+    for g in grads:
+        if g.layout != torch.strided or not g.is_floating_point() or g.device != grads[0].device:
+            raise ValueError(f"{name}: gradients must be dense float tensors on one device")
+        if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+            raise ValueError(f"{name}: a gradient shares elements with itself (expanded)")
     if not grads:
         return torch.zeros((), dtype=torch.float64)
     return torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt()
@@ -373,28 +366,29 @@ def _norm_plain(grads):
 
 def gradient_norm(parameters):
     """The 2-norm of all gradients of `parameters` (a tensor or an iterable) together, a float32 scalar on their device: squares are summed
-    in float64, so neither large nor tiny values overflow or vanish. Parameters without a gradient count nothing, one that is passed twice
-    counts once. Nothing waits for the GPU; with no gradients at all the result is 0, on the CPU."""
-    grads = _gradients(parameters, "gradient_norm")
+    in float64, so neither large nor tiny values overflow or vanish. Parameters without a gradient count nothing, a gradient that is passed twice
+    counts once. On the GPU gradients are float32 or bf16, of any strides. Nothing waits for the GPU; with no gradients at all the result is 0,
+    on the CPU."""
+    grads = _gradients(parameters)
     if _norm_kernel_takes(grads):
         from ._native import ops
-        return ops().gradient_norm(grads, False, 0.0, 0.0)
-    return _norm_plain(grads).float()
+        return ops().gradient_norm("gradient_norm", grads, False, 0.0, 0.0)
+    return _norm_plain(grads, "gradient_norm").float()
 
 
 def clip_gradients(parameters, max_norm: float, eps: float = 1e-6):
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + eps)), norm that of `gradient_norm`, which is returned: what a
-    training step does between backward and the optimizer. A norm that is NaN or infinite makes
-    gradients NaN or 0 by the same formula; look at the norm. Gradients that share memory are refused."""
+    training step does between backward and the optimizer. A norm that is NaN or infinite makes gradients NaN or 0 by the same formula;
+    look at the norm. Gradients whose places in memory overlap are refused."""
     if not (max_norm >= 0 and eps >= 0):
         raise ValueError("clip_gradients: max_norm and eps must be >= 0")
     torch = _torch()
-    grads = _gradients(parameters, "clip_gradients")
+    grads = _gradients(parameters)
+    if _norm_kernel_takes(grads):
+        from ._native import ops
+        return ops().gradient_norm("clip_gradients", grads, True, float(max_norm), float(eps))
     with torch.no_grad():
-        if _norm_kernel_takes(grads):
-            from ._native import ops
-            return ops().gradient_norm(grads, True, float(max_norm), float(eps))
-        norm = _norm_plain(grads)
+        norm = _norm_plain(grads, "clip_gradients")
         by = (max_norm / (norm + eps)).clamp(max=1.0).float()
         for g in grads:
             g.copy_(g.float() * by if g.dtype != torch.float64 else g * by)
