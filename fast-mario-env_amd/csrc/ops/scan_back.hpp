@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
         const int64_t n = place.n = item % a.N;
         place.segment = item / a.N;
         const int64_t first = place.segment * k.each, last = min(k.chunks, first + k.each);
-        float Q[SP], before[SP], touch = 0.f;
+        float Q[SP], before[SP], touch = 0.f, touch_h = 0.f;
         ChunkIn<T> ix, idt, iz, ido;
         uint8_t flag = 0;
         const auto ahead = [&](int64_t chunk) {
@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
             // (a lane for each 64 bytes of the chunk's B and C, which the scalar loads then find in the L2)
             const int64_t row = ((t0 + lane % SCAN_STEPS) * k.a.N + n) * k.a.G + g0;
             touch = k.bc[row * 2 * k.SB + min(lane / SCAN_STEPS * 16, 2 * k.SB - 1)];
+            // (and one for each 128 bytes of the states before it)
+            touch_h = k.kept[((chunk * k.a.N + n) * k.SB + me.s0 + min(lane / 2, SP - 1)) * k.a.C + me.c0 + min(lane % 2 * 32, max(me.there - 1, 0))];
             if (!k.wide) return;
             ix.ahead(k.a.x, t0, steps, me);
             idt.ahead(k.a.dt, t0, steps, me);
@@ -240,17 +242,17 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 if (gate) ChunkIn<T>::leave(l.z(), a.dz, t0, steps, me, k.wide);
             }
             // dB and dC of the chunk: the workgroup's waves joined (the next chunk's sums go to the other place)
-            for (int i = w * kWave + lane; i < steps * 2 * k.SB; i += blockDim.x) {
-                const int j = i / (2 * k.SB), m = i % (2 * k.SB), which = m / k.SB, s = m % k.SB, of = s / SP;
+            const int SB = SPLIT ? k.SB : SP;
+            float* const part = k.part_bc + ((((int64_t)cut * a.T + t0) * a.N + n) * a.G + g0) * 2 * SB;
+            T* const dB = (T*)a.dB.p + t0 * a.dB.st + n * a.dB.sn + g0 * a.dB.sh;
+            T* const dC = (T*)a.dC.p + t0 * a.dC.st + n * a.dC.sn + g0 * a.dC.sh;
+            for (int i = w * kWave + lane; i < steps * 2 * SB; i += blockDim.x) {
+                const int j = i / (2 * SB), m = i % (2 * SB), which = m / SB, s = m % SB, of = s / SP;
                 float x = 0.f;
                 for (int v = of; v < k.across * slices; v += slices)
                     x += Lds(lds + v * Lds::BYTES).sums()[(chunk & 1) * SCAN_STEPS * 32 + j * 32 + which * SP + s % SP];
-                if (k.cuts > 1) {
-                    k.part_bc[((((int64_t)cut * a.T + t0 + j) * a.N + n) * a.G + g0) * 2 * k.SB + m] = x;
-                } else if (s < a.S) {
-                    const MoRows& r = which ? a.dC : a.dB;
-                    ((T*)r.p)[(t0 + j) * r.st + n * r.sn + g0 * r.sh + s] = as<T>(x);
-                }
+                if (k.cuts > 1) part[j * a.N * a.G * 2 * SB + m] = x;
+                else if (s < a.S) (which ? dC : dB)[j * (which ? a.dC.st : a.dB.st) + s] = as<T>(x);
             }
             if constexpr (SPLIT) __syncthreads();             // (their partial sums have been read)
         };
@@ -398,7 +400,10 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 }
                 end_of_step();
             });
-            if (chunk > first) states_ahead(chunk - 1);
+            if (chunk > first) {
+                asm volatile("" ::"v"(touch_h));
+                states_ahead(chunk - 1);
+            }
             __syncthreads();
             after_chunk(chunk, t0, steps);
         }
