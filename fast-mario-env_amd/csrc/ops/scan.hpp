@@ -42,14 +42,20 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 
 // B and C of every step in float32, padded.
 __host__ __device__ __forceinline__ int64_t scan_rows(const Scan& k) { return k.chunks * SCAN_STEPS + 1; }
-template <class T> __global__ void __launch_bounds__(256) k_scan_pack(Scan k, float* bc) {
+template <class T> __global__ void __launch_bounds__(256) k_scan_pack(Scan k, float* bc) {   // (four values a thread: fewer workgroups to start)
     const MoScan& a = k.a;
-    const int64_t id = block_here() * 256 + threadIdx.x, row = id / (2 * k.SB);
-    const int i = (int)(id % (2 * k.SB)), s = i % k.SB, g = (int)(row % a.G);
+    const int64_t id = block_here() * 256 + threadIdx.x, row = id / (k.SB / 2);
+    const int i = (int)(id % (k.SB / 2)) * 4, s = i % k.SB, g = (int)(row % a.G);
     const int64_t n = row / a.G % a.N, t = row / a.G / a.N;
     if (t >= scan_rows(k)) return;
     const MoRows& r = i < k.SB ? a.Bt : a.Ct;
-    bc[id] = t < a.T && s < a.S ? as_f32(((const T*)r.p)[t * r.st + n * r.sn + g * r.sh + s]) : 0.f;
+    const T* from = (const T*)r.p + t * r.st + n * r.sn + g * r.sh + s;
+    Pack<float, 4> x{};
+    if (t < a.T)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (s + j < a.S) x.v[j] = as_f32(from[j]);
+    *(Pack<float, 4>*)(bc + 4 * id) = x;
 }
 
 // What a wave works on.
@@ -359,23 +365,25 @@ template <bool BACK> __global__ void __launch_bounds__(256) k_scan_enter(Scan k)
     const float A = real ? a.A[(int64_t)c * a.S + s] * LOG2E : 0.f;
     float h = from && real ? from[(n * a.C + c) * a.S + s] : 0.f;
     constexpr int IN_FLIGHT = 8;                              // segments whose values are read before they are joined
-    for (int64_t i0 = 0; i0 < k.segments; i0 += IN_FLIGHT) {
+    const int64_t far = BACK ? k.segments - 1 : 0, to_d = (BACK ? -1 : 1) * a.N * a.C, to_h = to_d * k.SB;
+    float* at = k.seg_h + ((far * a.N + n) * k.SB + s) * a.C + c;
+    const float* size = k.seg_d + (far * a.N + n) * a.C + c;
+    for (int64_t left = k.segments; left > 0; left -= IN_FLIGHT) {
         float add[IN_FLIGHT], d[IN_FLIGHT];
-        const auto of = [&](int i) {
-            const int64_t j = min(i0 + i, k.segments - 1);
-            return BACK ? k.segments - 1 - j : j;
-        };
 #pragma unroll
         for (int i = 0; i < IN_FLIGHT; i++) {
-            add[i] = k.seg_h[((of(i) * a.N + n) * k.SB + s) * a.C + c];
-            d[i] = k.seg_d[(of(i) * a.N + n) * a.C + c];
+            const int64_t j = min((int64_t)i, left - 1);
+            add[i] = at[j * to_h];
+            d[i] = size[j * to_d];
         }
 #pragma unroll
         for (int i = 0; i < IN_FLIGHT; i++) {
-            if (i0 + i >= k.segments) break;
-            k.seg_h[((of(i) * a.N + n) * k.SB + s) * a.C + c] = h;
+            if (i >= left) break;
+            at[i * to_h] = h;
             h = d[i] < 0.f ? add[i] : fmaf(exp2_raw(d[i] * A), h, add[i]);
         }
+        at += IN_FLIGHT * to_h;
+        size += IN_FLIGHT * to_d;
     }
 }
 
@@ -457,7 +465,7 @@ template <class T> int scan_forward(const MoScan& a, hipStream_t s) {
     k.seg_h = (float*)a.work + (a.saved ? 0 : scan_bc(k));
     k.seg_d = k.seg_h + k.segments * a.N * k.SB * a.C;
     if (a.T) {
-        const int64_t n = scan_rows(k) * a.N * a.G * 2 * k.SB;
+        const int64_t n = scan_rows(k) * a.N * a.G * (k.SB / 2);
         hipLaunchKernelGGL((k_scan_pack<T>), grid_of((n + 255) / 256), dim3(256), 0, s, k, bc);
         if (launched("k_scan_pack")) return -1;
     }
