@@ -395,7 +395,11 @@ inline ScanCut scan_slices(int S) {
 }
 constexpr int64_t SCAN_FILL = 4096;     // waves that fill the card
 constexpr int SCAN_BACK_WAVES = 8;      // waves a workgroup of the gradient, at most
-template <class T> constexpr int SCAN_SHARED_LDS = (sizeof(T) == 2 ? 18 : 20) << 10;   // LDS of a wave there that shares its channels
+// LDS of a wave there: four tiles of values, three of float32, sums for dB and dC, dA; more where it shares its channels.
+constexpr int scan_back_lds(int size, int SP, bool split) {
+    constexpr int TILE = SCAN_STEPS * kWave;
+    return 4 * TILE * size + 4 * (3 * TILE + (split ? 1 : 2) * SCAN_STEPS * 32 + SP * kWave + (size == 4 ? 0 : TILE) + (!split ? 0 : size == 4 ? TILE : 2 * TILE));
+}
 inline Scan scan_cut(const MoScan& a, bool backward) {
     Scan k{};
     k.a = a;
@@ -410,15 +414,15 @@ inline Scan scan_cut(const MoScan& a, bool backward) {
     };
     k.wide = k.Cg % V == 0 && row(a.x) && row(a.dt) && row(a.z) && (backward ? row(a.dout) && row(a.dx) && row(a.ddt) && row(a.dz) : row(a.out));
     k.chunks = (a.T + SCAN_STEPS - 1) / SCAN_STEPS;
-    const int room = k.slices == 1 ? SCAN_BACK_WAVES : (160 << 10) / (a.dtype == MO_BF16 ? SCAN_SHARED_LDS<bf16> : SCAN_SHARED_LDS<float>);
+    const int lds = scan_back_lds(a.dtype == MO_BF16 ? 2 : 4, c.SP, k.slices > 1), room = (160 << 10) / lds;
     k.across = std::min(k.per, std::min(SCAN_BACK_WAVES, room) / k.slices);
     k.cuts = (k.per + k.across - 1) / k.across;
     // Few sequences are cut over their length: each segment is gone through twice, once for what it adds to the state. The forward pass has many waves a
     // compute unit and takes whatever number; the gradient has few, so its segments are as many as run at once (1,999 steps of 8 envs, 512
     // channels: 32 segments, 160 us; 50, which run in two rounds, 201).
     const int64_t waves = std::max<int64_t>(1, a.N * a.G * k.per * k.slices), most = std::max<int64_t>(1, SCAN_FILL / waves);
-    const int block = k.across * k.slices, lds = k.slices > 1 ? (a.dtype == MO_BF16 ? 18 : 20) : (a.dtype == MO_BF16 ? 14 : 18);
-    const int64_t at_once = std::max<int64_t>(1, 256 * std::max(1, std::min(160 / (block * lds), (c.SP > 8 ? 8 : 12) / block)) / (a.G * k.cuts));
+    const int block = k.across * k.slices;
+    const int64_t at_once = std::max<int64_t>(1, 256 * std::max(1, std::min((160 << 10) / (block * lds), (c.SP > 8 ? 8 : 12) / block)) / (a.G * k.cuts));
     const int64_t want = backward ? at_once / std::max<int64_t>(1, a.N) : most >= 4 ? most : 1;
     k.segments = std::max<int64_t>(1, std::min(want, k.chunks / 4));
     k.each = std::max<int64_t>(1, (k.chunks + k.segments - 1) / k.segments);

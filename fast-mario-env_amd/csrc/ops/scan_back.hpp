@@ -126,11 +126,12 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan_back_sums(Scan k) {
 }
 
 // Workgroups of `across` waves of channels by `slices`. A wave's own LDS: the tiles of x, dt, z and dout (whose places dx, ddt and dz take); of each step
-// its size d, d's slope by dt, dy and y; the sums for its workgroup's dB and dC, of two chunks in turn; where waves share channels, du and dd.
-template <class T, bool SPLIT> struct BackLds {
-    static constexpr int TILE = SCAN_STEPS * kWave, SUMS = 2 * SCAN_STEPS * 32;
-    static constexpr bool OVER = sizeof(T) == 4;      // dd takes dt's place, which waves that share channels do not write to
-    static constexpr int BYTES = 4 * TILE * (int)sizeof(T) + (4 * TILE + SUMS + (!SPLIT ? 0 : OVER ? TILE : 2 * TILE)) * 4;
+// its size d, d's slope by dt, dy and y; the sums for its workgroup's dB and dC (of two chunks in turn, but where a second barrier follows); dA up to the last chunk; where waves share
+// channels, du and dd. With float32 tiles dy takes dout's place, what dz has of dout and z takes z's, and dd takes dt's.
+template <class T, int SP, bool SPLIT> struct BackLds {
+    static constexpr int TILE = SCAN_STEPS * kWave, TURN = SCAN_STEPS * 32, SUMS = (SPLIT ? 1 : 2) * TURN;
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int BYTES = scan_back_lds(sizeof(T), SP, SPLIT);
     T* t;
     __device__ __forceinline__ explicit BackLds(char* p) : t((T*)p) {}
     __device__ __forceinline__ T* x() const { return t; }
@@ -139,17 +140,26 @@ template <class T, bool SPLIT> struct BackLds {
     __device__ __forceinline__ T* dout() const { return t + 3 * TILE; }
     __device__ __forceinline__ float* d() const { return (float*)(t + 4 * TILE); }
     __device__ __forceinline__ float* slope() const { return d() + TILE; }
-    __device__ __forceinline__ float* dy() const { return d() + 2 * TILE; }
-    __device__ __forceinline__ float* y() const { return d() + 3 * TILE; }
-    __device__ __forceinline__ float* sums() const { return d() + 4 * TILE; }        // (2, SCAN_STEPS, 32)
-    __device__ __forceinline__ float* du() const { return sums() + SUMS; }
-    __device__ __forceinline__ float* dd() const { return OVER ? (float*)dt() : du() + TILE; }
+    __device__ __forceinline__ float* y() const { return d() + 2 * TILE; }
+    __device__ __forceinline__ float* sums(int64_t chunk) const { return d() + 3 * TILE + (SPLIT ? 0 : (chunk & 1) * TURN); }   // (SCAN_STEPS, 32)
+    __device__ __forceinline__ float* dA() const { return d() + 3 * TILE + SUMS; }           // (SP, lanes)
+    __device__ __forceinline__ float* dy() const { return F32 ? (float*)dout() : dA() + SP * kWave; }
+    __device__ __forceinline__ float* du() const { return dA() + SP * kWave + (F32 ? 0 : TILE); }
+    __device__ __forceinline__ float* dd() const { return F32 ? (float*)dt() : du() + TILE; }
 };
+// The part of dz that the step's y does not change.
+__device__ __forceinline__ float gate_slope(float dout, float z, float sig) { return dout * (sig * fmaf(z, 1.f - sig, 1.f)); }
+// sum + x, and what its rounding takes in `rest`, for the next one (compensated summation).
+__device__ __forceinline__ void add_to(float& sum, float& rest, float x) {
+    const float y = x - rest, s = sum + y;
+    rest = (s - sum) - y;
+    sum = s;
+}
 
 template <class T, int SP, bool SPLIT>
 __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
     const MoScan& a = k.a;
-    typedef BackLds<T, SPLIT> Lds;
+    typedef BackLds<T, SP, SPLIT> Lds;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int w = wave_here(), slices = SPLIT ? k.slices : 1, slice = SPLIT ? w % slices : 0, across = w / slices;
     const int64_t items = k.segments * a.N, row = block_here() / (a.G * k.cuts), bg = block_here() % (a.G * k.cuts);
@@ -160,12 +170,12 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
     const bool gate = a.z.p;
     ScanPlace place(k, row, cb, slice, SP);
     if (in_group >= k.per) { place.live = false; place.there = 0; }
-    float A[SP], dA[SP], dD = 0.f, dbias = 0.f;
+    float A[SP], dD = 0.f, dbias = 0.f, dD_rest = 0.f, dbias_rest = 0.f;
     const int c = place.c;
     load_decays<SP>(a, place, A);
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, D = a.D ? a.D[c] : 0.f;
 #pragma unroll
-    for (int s = 0; s < SP; s++) dA[s] = 0.f;
+    for (int s = 0; s < SP; s++) l.dA()[s * kWave + place.lane] = 0.f;
     for (int64_t item = row; item < items; item += k.rows) {
         const int64_t n = place.n = item % a.N;
         place.segment = item / a.N;
@@ -226,15 +236,15 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                         dd += o.dd()[at];
                     }
                     const float x = as_f32(l.x()[at]), dy = l.dy()[at], ddt = fmaf(du, x, dd * LN2) * l.slope()[at];
-                    dD = fmaf(dy, x, dD);
-                    dbias += ddt;
+                    add_to(dD, dD_rest, dy * x);
+                    add_to(dbias, dbias_rest, ddt);
                     if (!me.live) continue;
                     const auto row_of = [&](const MoRows& r) { return (T*)r.p + (t0 + i) * r.st + n * r.sn + c; };
                     *row_of(a.dx) = as<T>(fmaf(du, l.d()[at], D * dy));
                     *row_of(a.ddt) = as<T>(ddt);
                     if (!gate) continue;
-                    const float z = as_f32(l.z()[at]), sig = sigmoid(z);
-                    *row_of(a.dz) = as<T>(as_f32(l.dout()[at]) * fmaf(D, x, y) * (sig * fmaf(z, 1.f - sig, 1.f)));
+                    const float z = as_f32(l.z()[at]);
+                    *row_of(a.dz) = as<T>(fmaf(D, x, y) * (Lds::F32 ? z : gate_slope(as_f32(l.dout()[at]), z, sigmoid(z))));
                 }
             } else {
                 ChunkIn<T>::leave(l.x(), a.dx, t0, steps, me, k.wide);
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 const int j = i / (2 * SB), m = i % (2 * SB), which = m / SB, s = m % SB, of = s / SP;
                 float x = 0.f;
                 for (int v = of; v < k.across * slices; v += slices)
-                    x += Lds(lds + v * Lds::BYTES).sums()[(chunk & 1) * SCAN_STEPS * 32 + j * 32 + which * SP + s % SP];
+                    x += Lds(lds + v * Lds::BYTES).sums(chunk)[j * 32 + which * SP + s % SP];
                 if (k.cuts > 1) part[j * a.N * a.G * 2 * SB + m] = x;
                 else if (s < a.S) (which ? dC : dB)[j * (which ? a.dC.st : a.dB.st) + s] = as<T>(x);
             }
@@ -284,18 +294,20 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 const Size p = softplus(as_f32(l.dt()[at]) + bias);
                 l.d()[at] = p.d;
                 l.slope()[at] = p.slope;
-                float dy = as_f32(l.dout()[at]);
+                const float dout = as_f32(l.dout()[at]);
                 if (gate) {
-                    const float z = as_f32(l.z()[at]);
-                    dy *= z * sigmoid(z);
+                    const float z = as_f32(l.z()[at]), sig = sigmoid(z);
+                    if constexpr (Lds::F32) l.z()[at] = gate_slope(dout, z, sig);
+                    l.dy()[at] = dout * (z * sig);
+                } else if constexpr (!Lds::F32) {
+                    l.dy()[at] = dout;
                 }
-                l.dy()[at] = dy;
             }
             end_of_step();
             float h[SCAN_STEPS][SP];                          // the states before each step
 #pragma unroll
             for (int s = 0; s < SP; s++) h[0][s] = me.live ? before[s] : 0.f;
-            float* const to_join = l.sums() + (chunk & 1) * SCAN_STEPS * 32;
+            float* const to_join = l.sums(chunk);
             // what a step needs, read a step ahead
             struct In { float d, dy; T x; };
             const auto in_of = [&](int i) { return In{l.d()[i * kWave + lane], l.dy()[i * kWave + lane], l.x()[i * kWave + lane]}; };
@@ -340,12 +352,15 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
 #pragma unroll
                     for (int i = 0; i < SCAN_STEPS; i++) {
                         const int at = i * kWave + lane;
-                        const float z = as_f32(l.z()[at]), sig = sigmoid(z);
-                        l.z()[at] = as<T>(as_f32(l.dout()[at]) * fmaf(D, as_f32(l.x()[at]), l.y()[at]) * (sig * fmaf(z, 1.f - sig, 1.f)));
+                        const float z = as_f32(l.z()[at]);
+                        l.z()[at] = as<T>(fmaf(D, as_f32(l.x()[at]), l.y()[at]) * (Lds::F32 ? z : gate_slope(as_f32(l.dout()[at]), z, sigmoid(z))));
                     }
                 end_of_step();
             }
             // and back
+            float dA[SP], dD_here = 0.f, dbias_here = 0.f;    // the chunk's own (the sum of all of them goes on in LDS)
+#pragma unroll
+            for (int s = 0; s < SP; s++) dA[s] = 0.f;
             load_bc<SP>(now, bc, SB);
             in = in_of(SCAN_STEPS - 1);
             each_step([&](auto step) {
@@ -386,8 +401,8 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                     l.dd()[at] = dd;
                 } else {
                     const float ddt = fmaf(du, x, dd * LN2) * l.slope()[at];
-                    dD = fmaf(in.dy, x, dD);
-                    dbias += ddt;
+                    dD_here = fmaf(in.dy, x, dD_here);
+                    dbias_here += ddt;
                     l.x()[at] = as<T>(fmaf(du, in.d, D * in.dy));
                     l.dt()[at] = as<T>(ddt);
                 }
@@ -400,6 +415,12 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 }
                 end_of_step();
             });
+#pragma unroll
+            for (int s = 0; s < SP; s++) l.dA()[s * kWave + lane] += dA[s];
+            if constexpr (!SPLIT) {
+                add_to(dD, dD_rest, dD_here);
+                add_to(dbias, dbias_rest, dbias_here);
+            }
             if (chunk > first) {
                 asm volatile("" ::"v"(touch_h));
                 states_ahead(chunk - 1);
@@ -429,7 +450,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
     if (!me.live) return;
     float* to = k.part + row * (k.SB + 2) * a.C + c;
 #pragma unroll
-    for (int s = 0; s < SP; s++) to[(int64_t)(me.s0 + s) * a.C] = dA[s];
+    for (int s = 0; s < SP; s++) to[(int64_t)(me.s0 + s) * a.C] = l.dA()[s * kWave + lane];
     if (slice == 0) {
         to[(int64_t)k.SB * a.C] = dD;
         to[(int64_t)(k.SB + 1) * a.C] = dbias;
@@ -469,8 +490,8 @@ template <class T> int scan_backward(const MoScan& a, hipStream_t s) {
             hipLaunchKernelGGL((k_scan_enter<true>), grid_of((a.N * k.SB * a.C + 255) / 256), dim3(256), 0, s, k);
         }
         const int waves = k.across * k.slices;
-        static_assert(BackLds<T, false>::BYTES * SCAN_BACK_WAVES <= 160 << 10 && BackLds<T, true>::BYTES <= SCAN_SHARED_LDS<T>, "");
-        hipLaunchKernelGGL((k_scan_back<T, SP, SPLIT>), grid_of(k.rows * a.G * k.cuts), dim3(kWave * waves), waves * (BackLds<T, SPLIT>::BYTES), s, k);
+        static_assert(scan_back_lds(sizeof(T), 16, false) * SCAN_BACK_WAVES <= 160 << 10, "");
+        hipLaunchKernelGGL((k_scan_back<T, SP, SPLIT>), grid_of(k.rows * a.G * k.cuts), dim3(kWave * waves), waves * (BackLds<T, SP, SPLIT>::BYTES), s, k);
         if (launched("k_scan_back")) return -1;
         const int64_t n = a.T * a.N * a.G * 2 * k.SB;
         if (n && k.cuts > 1) hipLaunchKernelGGL((k_scan_join<T>), grid_of((n + 255) / 256), dim3(256), 0, s, k);
