@@ -162,6 +162,31 @@ template <int SP> __device__ __forceinline__ void load_decays(const MoScan& a, c
 #pragma unroll
     for (int s = 0; s < SP; s++) A[s] = me.live && me.s0 + s < a.S ? a.A[(int64_t)me.c * a.S + me.s0 + s] * LOG2E : 0.f;
 }
+// A channel's states as they lie, zeros past the last (or of none); in 16-byte accesses where they allow it (a lane's states lie 4 S
+// bytes from its neighbour's).
+__device__ __forceinline__ bool in_fours(const MoScan& a, const float* p) { return a.S % 4 == 0 && (uintptr_t)p % 16 == 0; }
+template <int SP> __device__ __forceinline__ void load_states(const MoScan& a, const float* p, int64_t n, int c, int s0, float (&h)[SP]) {
+    const float* from = p + (n * a.C + c) * a.S + s0;
+    if (p && in_fours(a, p)) {
+#pragma unroll
+        for (int s = 0; s < SP; s += 4) *(Pack<float, 4>*)(h + s) = s0 + s < a.S ? *(const Pack<float, 4>*)(from + s) : Pack<float, 4>{};
+    } else {
+#pragma unroll
+        for (int s = 0; s < SP; s++) h[s] = p && s0 + s < a.S ? from[s] : 0.f;
+    }
+}
+template <int SP> __device__ __forceinline__ void store_states(const MoScan& a, float* p, int64_t n, int c, int s0, const float (&h)[SP]) {
+    float* to = p + (n * a.C + c) * a.S + s0;
+    if (in_fours(a, p)) {
+#pragma unroll
+        for (int s = 0; s < SP; s += 4)
+            if (s0 + s < a.S) *(Pack<float, 4>*)(to + s) = *(const Pack<float, 4>*)(h + s);
+    } else {
+#pragma unroll
+        for (int s = 0; s < SP; s++)
+            if (s0 + s < a.S) to[s] = h[s];
+    }
+}
 // A step's B and C, in scalar registers. Loaded a step ahead; nothing moves over the end of a step, or all steps' loads would come first and
 // take more registers than there are.
 template <int SP> struct StepBC { float b[SP], c[SP]; };
@@ -226,12 +251,10 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
     float A[SP], h[SP], total = 0.f;
     load_decays<SP>(a, place, A);
     const int64_t seg0 = ((place.segment * a.N + n) * k.SB + place.s0) * a.C + c;
+    if (!SUMS && k.segments == 1) load_states<SP>(a, a.state, n, c, place.s0, h);
+    else
 #pragma unroll
-    for (int s = 0; s < SP; s++) {
-        if (SUMS) h[s] = 0.f;
-        else if (k.segments > 1) h[s] = k.seg_h[seg0 + (int64_t)s * a.C];
-        else h[s] = a.state && place.s0 + s < a.S ? a.state[(n * a.C + c) * a.S + place.s0 + s] : 0.f;
-    }
+        for (int s = 0; s < SP; s++) h[s] = SUMS ? 0.f : k.seg_h[seg0 + (int64_t)s * a.C];
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, D = a.D ? a.D[c] : 0.f;
     ChunkIn<T> ix, idt, iz;
     uint8_t flag = 0;
@@ -347,9 +370,7 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
         for (int s = 0; s < SP; s++) k.seg_h[seg0 + (int64_t)s * a.C] = h[s];
         if (slice == 0) k.seg_d[(me.segment * a.N + n) * a.C + c] = total;
     } else if (last == k.chunks) {
-#pragma unroll
-        for (int s = 0; s < SP; s++)
-            if (me.s0 + s < a.S) a.state_out[(n * a.C + c) * a.S + me.s0 + s] = h[s];
+        store_states<SP>(a, a.state_out, n, c, me.s0, h);
     }
 }
 

@@ -213,12 +213,12 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
             ahead(last - 1);
             states_ahead(last - 1);
         }
+        if (k.segments == 1) load_states<SP>(a, a.dstate_out, n, c, place.s0, Q);
+        else
 #pragma unroll
-        for (int s = 0; s < SP; s++) {
-            if (!place.live) Q[s] = 0.f;
-            else if (k.segments > 1) Q[s] = k.seg_h[((place.segment * a.N + n) * k.SB + place.s0 + s) * a.C + c];
-            else Q[s] = a.dstate_out && place.s0 + s < a.S ? a.dstate_out[(n * a.C + c) * a.S + place.s0 + s] : 0.f;
-        }
+            for (int s = 0; s < SP; s++) Q[s] = k.seg_h[((place.segment * a.N + n) * k.SB + place.s0 + s) * a.C + c];
+#pragma unroll
+        for (int s = 0; s < SP; s++) Q[s] = place.live ? Q[s] : 0.f;
         // what a chunk left in LDS goes to memory
         const auto after_chunk = [&](int64_t chunk, int64_t t0, int steps) {
             const Scan& k = args_again();
@@ -428,10 +428,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
             __syncthreads();
             after_chunk(chunk, t0, steps);
         }
-        if (first == 0 && a.dstate && place.live)
-#pragma unroll
-            for (int s = 0; s < SP; s++)
-                if (place.s0 + s < a.S) a.dstate[(n * a.C + c) * a.S + place.s0 + s] = Q[s];
+        if (first == 0 && a.dstate && place.live) store_states<SP>(a, a.dstate, n, c, place.s0, Q);
         __syncthreads();                                      // (one env's last sums are read before the next one's first)
     }
     const ScanPlace& me = place;
