@@ -583,6 +583,47 @@ def test_scan_what_is_not_finite_stays_in_its_episode(bad, T, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N,C,S,G", [(20, 3, 1100, 16, 1), (17, 3, 300, 64, 1), (9, 2, 1300, 40, 2), (40, 300, 520, 4, 1), (3, 2, 9000, 16, 1)])
+def test_scan_more_channels_than_a_workgroup_has(T, N, C, S, G, dtype):
+    """Sums over a group's channels that several workgroups leave, and more envs than are taken at a time."""
+    check_scan(*scan_inputs(T, N, C, S, G, dtype))
+
+
+@pytest.mark.gpu
+def test_two_graphs_and_two_streams_at_once():
+    """Two captured passes, replayed in turn and on two streams at once, each against its eager result."""
+    def make(seed):
+        a, dout, ds = scan_inputs(200, 3, 64, 16, 1, torch.bfloat16, seed=seed)
+        leaves = [a[n].requires_grad_() for n in _NAMES]
+
+        def work():
+            y, last = state_scan(**a)
+            return [y.detach(), last.detach(), *torch.autograd.grad((y, last), leaves, (dout, ds))]
+        return work
+
+    works, graphs, held = [make(s) for s in (1, 2)], [], []
+    want = [[t.clone() for t in w()] for w in works]
+    torch.cuda.synchronize()
+    for w in works:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(w())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in works]
+    for i in range(4):
+        for g, s in zip(graphs, streams):
+            if i % 2:
+                g.replay()
+            else:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for h, e in zip(held, want):
+            assert all(torch.equal(x, y) for x, y in zip(h, e)), i
+
+
+@pytest.mark.gpu
 def test_scan_empty():
     for T, N in ((0, 3), (4, 0), (0, 0)):
         a, dout, ds = scan_inputs(T, N, 8, 4, 1, torch.bfloat16)
