@@ -9,7 +9,8 @@ constexpr int CONV_THREADS = 256;
 template <int V> constexpr int CONV_AHEAD = V > 4 ? 2 : 4;
 
 // A thread holds V neighbouring channels of one env and goes through a segment of the steps with the last K - 1 inputs in registers, cleared where an
-// episode starts; segments begin by reading the K - 1 steps before them.
+// episode starts; segments begin by reading the K - 1 steps before them. The forward pass is bound by memory (128 x 2,048 x 512 bf16: 107 us, 5.0
+// TB/s), the gradient by the vector units (195 to 215 us, 91 % busy: 40 instructions a value, the argument made again among them).
 struct Conv {
     MoConv a;
     int64_t each, segments;    // steps of a segment
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(CONV_THREADS, 2) k_conv_back(Conv k) {
     store_channels<float, V>(to + (int64_t)K * a.C, db);
 }
 
-// One step: the window is the state, which moves on by one.
+// One step: the window is the state, which moves on by one. Bound by memory: 32,768 envs, 512 channels, four taps, bf16 76 us, 3.5 TB/s.
 template <class T, int V, int K, int ACT>
 __global__ void __launch_bounds__(CONV_THREADS) k_conv_step(MoConv a) {
     const int lanes = a.C / V;

@@ -9,6 +9,11 @@ namespace mo {
 //   R = C dy + Q,  dC = sum_c h dy,  dB = sum_c R u,  du = sum_s R B,  Q = R a,  q = Q h_{t-1},  dA += q d,  dd = du x + sum_s q A
 // (u = d x, a = exp(d A); Q and q are 0 where the episode starts). The sums over channels are joined in the wave (wave_sums), then in LDS over the
 // workgroup's waves, which have neighbouring channels of one env and segment.
+// The 8 x 16 states of a chunk take half of a wave's 256 registers, so two waves share a SIMD; the other way round, states kept for every step would be
+// 64 bytes a channel to write and read where all else is 22. Bound by the vector units and by two waves' waits: 128 steps x 2,048 envs x
+// 512 channels of 16 states in bf16 2,210 us, the units busy 72 % of them with 400 instructions a step (half of it the states again and the sums over
+// lanes). One wave a SIMD with spills in the steps took 6,400; steps that wait for their own inputs 4,240; sums over lanes by swaps
+// alone 2,570.
 constexpr int BACK_WAVES = SCAN_BACK_WAVES;
 
 // Where bit I of cuts is set: x = y = 0, for all states.

@@ -11,7 +11,7 @@ template <int CTRL> __device__ __forceinline__ float dpp(float x) {
 constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140;   // (mirrored: l to 7 - l, l to 15 - l)
 
 // Sums of M values over a wave's 64 lanes, each lane left with one of them: every step keeps half of the values in half of the lanes, so that
-// 16 values cost 35 instructions and not 96. Within rows of 16 lanes a value's sum is written over the other's in the lanes that are its own
+// 16 values cost 35 instructions and not 96 (47 with swaps alone). Within rows of 16 lanes a value's sum is written over the other's in the lanes that are its own
 // (DPP's bank mask: two instructions a pair); rows are exchanged by permlane swaps (three). Lane l gets value sum_slot(l) of the M (4, 8,
 // 12 or 16; a slot >= M holds nothing), lanes of equal slots the same sum.
 __device__ __forceinline__ int sum_slot(int l, int M) {
