@@ -445,7 +445,7 @@ def test_convolution_what_is_not_finite_stays_in_its_episode(bad, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("N,C,K", [(1, 1, 1), (3, 64, 4), (700, 40, 4), (5, 33, 2), (2, 16, 8), (4, 7, 3)])
+@pytest.mark.parametrize("N,C,K", [(1, 1, 1), (3, 64, 4), (700, 40, 4), (5, 33, 2), (2, 16, 8), (4, 7, 3), (66003, 64, 4), (66001, 32, 7)])
 def test_convolution_step_is_the_convolution(N, C, K, dtype):
     T = 6
     x, w, b, start, state, _, _ = conv_inputs(T, N, C, K, dtype, starts=0.4)
