@@ -19,12 +19,12 @@ struct Conv {
 };
 
 template <int ACT> __device__ __forceinline__ float act_of(float p) {
-    if (ACT == MO_ACT_RELU) return fmaxf(p, 0.f);
+    if (ACT == MO_ACT_RELU) return p <= 0.f ? 0.f : p;   // (a NaN stays one, and its gradient goes on)
     if (ACT == MO_ACT_SILU) return p * __builtin_amdgcn_rcpf(1.f + __expf(-p));
     return p;
 }
 template <int ACT> __device__ __forceinline__ float act_slope(float p) {
-    if (ACT == MO_ACT_RELU) return p > 0.f ? 1.f : 0.f;
+    if (ACT == MO_ACT_RELU) return p <= 0.f ? 0.f : 1.f;
     if (ACT == MO_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.f + __expf(-p));
         return s * fmaf(p, 1.f - s, 1.f);

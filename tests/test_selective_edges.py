@@ -1,0 +1,55 @@
+"""The operators of a memory that selects and of the gradients' norm where a value, a layout or a state is out of the ordinary: values that are not
+finite, states that go on from a sequence to single steps, gradients that share memory or only lie between one another. Definitions and
+bounds are those of test_selective.py."""
+import pytest
+import torch
+
+from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step
+from test_selective import DTYPES, conv_inputs
+
+
+def same_kind(got, want, what):
+    """NaN where the definition has NaN, an infinity where it has that infinity, finite elsewhere."""
+    assert got.shape == want.shape, what
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    for inf in (float("inf"), -float("inf")):
+        assert torch.equal(got == inf, want == inf), (what, inf)
+
+
+# ---------------------------------------------------------------- convolution
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+@pytest.mark.parametrize("C,K", [(16, 4), (5, 4), (64, 8), (8, 1)])
+def test_convolution_keeps_a_nan(C, K, act, dtype):
+    """A NaN among the inputs, the weights, the biases or in the state shows in every step that sees it and in its weights' gradient, and nowhere else."""
+    T, N, c = 24, 2, 3
+    x, w, b, _, state, dy, _ = conv_inputs(T, N, C, K, dtype, starts=None)
+
+    def run(x, w, b, state):
+        leaves = [t.detach().requires_grad_() for t in (x, w)]
+        y, _ = causal_conv_act(*leaves, b, None, state, act)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    clean = run(x, w, b, state)
+    for name in ("x", "w", "b", "state"):
+        if name == "state" and K == 1:
+            continue
+        a = dict(x=x.clone(), w=w.clone(), b=b.clone(), state=state.clone())
+        hit = torch.zeros(T, N, C, dtype=torch.bool, device="cuda")
+        if name == "x":
+            a["x"][9, 1, c], hit[9:9 + K, 1, c] = float("nan"), True
+        elif name == "state":
+            a["state"][1, -1, c], hit[:K - 1, 1, c] = float("nan"), True
+        else:
+            a[name][c], hit[:, :, c] = float("nan"), True
+        y, dx, dw = run(**a)
+        assert torch.isnan(y[hit]).all() and torch.equal(y[~hit], clean[0][~hit]), name
+        others = [i for i in range(C) if i != c]
+        assert torch.equal(dx[..., others], clean[1][..., others]) and torch.equal(dw[others], clean[2][others]), name
+        if name == "x":
+            assert torch.isnan(dw[c]).all()
+        if name != "state":
+            s = state.clone()
+            step = causal_conv_act_step(a["x"][9], a["w"], a["b"], s, act=act)
+            assert torch.equal(torch.isnan(step), hit[9])
