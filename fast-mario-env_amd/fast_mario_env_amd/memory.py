@@ -191,7 +191,7 @@ def _conv_plain(x, weight, bias, start, state, act):
         every = torch.cat([window, x[t][:, None]], 1)
         p = (every.float() * w).sum(1)
         p = p if bias is None else p + bias.float()
-        out.append(p.clamp(min=0.0) if act == "relu" else p * torch.sigmoid(p) if act == "silu" else p)
+        out.append(torch.relu(p) if act == "relu" else p * torch.sigmoid(p) if act == "silu" else p)
         window = every[:, 1:]
     out = torch.stack(out).to(x.dtype) if out else x.new_empty(x.shape)
     return out, window.clone() if window is state else window

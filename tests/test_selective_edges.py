@@ -53,3 +53,16 @@ def test_convolution_keeps_a_nan(C, K, act, dtype):
             s = state.clone()
             step = causal_conv_act_step(a["x"][9], a["w"], a["b"], s, act=act)
             assert torch.equal(torch.isnan(step), hit[9])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_convolution_relu_at_zero(device):
+    """relu's slope is 0 where its argument is 0 (nothing but zeros, no bias), 1 where it is a NaN: on either device."""
+    x, w, _, _, _, dy, _ = conv_inputs(9, 2, 8, 4, torch.float32, starts=None, device=device)
+    for value, slope in ((0.0, 0.0), (float("nan"), 1.0)):
+        leaf = torch.full_like(x, value).requires_grad_()
+        b = torch.zeros(8, device=device, requires_grad=True)
+        y, _ = causal_conv_act(leaf, w, b, act="relu")
+        dx, db = torch.autograd.grad(y, (leaf, b), dy)
+        assert torch.equal(y.detach().nan_to_num(5.0), torch.full_like(y, 0.0 if value == 0.0 else 5.0))
+        assert torch.allclose(db, slope * dy.sum((0, 1)), atol=18 * 2.0 ** -24 * 18) and torch.isfinite(dx).all() and (dx == 0).all() == (slope == 0)
