@@ -266,10 +266,9 @@ def _scan_plain(x, dt, A, B, C, D, z, dt_bias, start, state):
     for t in range(T):
         xt, raw = x[t].float(), dt[t].float() if dt_bias is None else dt[t].float() + dt_bias.float()
         d = torch.logaddexp(raw, torch.zeros_like(raw))
-        a = torch.exp(d[..., None] * A) * h
         if start is not None:
-            a = torch.where(start[t][:, None, None], torch.zeros_like(a), a)
-        h = a + (d * xt)[..., None] * B[t].float().repeat_interleave(rep, 1)
+            h = torch.where(start[t][:, None, None], torch.zeros_like(h), h)   # (before the product, whose gradient reads it)
+        h = torch.exp(d[..., None] * A) * h + (d * xt)[..., None] * B[t].float().repeat_interleave(rep, 1)
         y = (C[t].float().repeat_interleave(rep, 1) * h).sum(-1)
         y = y if D is None else y + D.float() * xt
         if z is not None:

@@ -4,8 +4,8 @@ bounds are those of test_selective.py."""
 import pytest
 import torch
 
-from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step
-from test_selective import DTYPES, conv_inputs
+from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, state_scan
+from test_selective import DTYPES, conv_inputs, scan_inputs
 
 
 def same_kind(got, want, what):
@@ -66,3 +66,48 @@ def test_convolution_relu_at_zero(device):
         dx, db = torch.autograd.grad(y, (leaf, b), dy)
         assert torch.equal(y.detach().nan_to_num(5.0), torch.full_like(y, 0.0 if value == 0.0 else 5.0))
         assert torch.allclose(db, slope * dy.sum((0, 1)), atol=18 * 2.0 ** -24 * 18) and torch.isfinite(dx).all() and (dx == 0).all() == (slope == 0)
+
+
+# ---------------------------------------------------------------- scan
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_cpu_what_is_not_finite_stays_in_its_episode(bad):
+    """On the CPU too: a value that is not finite shows in no step and no gradient of a step of another episode, and in no
+    gradient at all where no step sees it."""
+    T, N, C, S = 12, 2, 6, 3
+    a, dout, ds = scan_inputs(T, N, C, S, 1, torch.float32, device="cpu")
+    x, w, b, _, window, dy, dw = conv_inputs(T, N, C, 4, torch.float32, device="cpu")
+    start = a["start"] = torch.zeros(T, N, dtype=torch.bool)
+    start[4], start[8] = True, True
+
+    def run(a, dout, x, window):
+        leaves = {n: a[n].detach().requires_grad_() for n in ("x", "dt", "B", "C", "z")}
+        y, end = state_scan(**{**a, **leaves})
+        leaf = x.detach().requires_grad_()
+        y2, last = causal_conv_act(leaf, w, b, start, window)
+        return [y.detach(), y2.detach(), *torch.autograd.grad((y, end), list(leaves.values()), (dout, ds)), *torch.autograd.grad((y2, last), leaf, (dy, dw))]
+
+    clean = run(a, dout, x, window)
+    for where in (0, 3, 4, 7, 8, T - 1):
+        hit = slice(where // 4 * 4, where // 4 * 4 + 4)
+        for name in ("x", "dt", "B", "C", "z", "dout", "state"):
+            b2, do, x2, st2 = dict(a), dout.clone(), x.clone(), window
+            if name == "dout":
+                do[where] = bad
+            elif name == "state":
+                if where:
+                    continue
+                b2["state"], st2 = torch.full_like(a["state"], bad), torch.full_like(window, bad)
+            else:
+                b2[name] = a[name].clone()
+                b2[name][where] = x2[where] = bad
+            for got, want in zip(run(b2, do, x2, st2), clean):
+                for part in (slice(0, hit.start), slice(hit.stop, T)):
+                    assert torch.equal(got[part], want[part]), (where, name)
+    start[0] = True                                          # a state that nothing looks at: no gradient knows it
+    names = ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "state")
+    leaves = {n: a[n].detach().requires_grad_() for n in names}
+    dirty = {**leaves, "state": torch.full_like(a["state"], bad).requires_grad_()}
+    for v in (leaves, dirty):
+        y, end = state_scan(**{**a, **v})
+        v["grads"] = torch.autograd.grad((y, end), [v[n] for n in names], (dout, ds))
+    assert all(torch.equal(p, q) for p, q in zip(leaves["grads"], dirty["grads"]))
