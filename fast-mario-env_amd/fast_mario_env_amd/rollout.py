@@ -364,6 +364,59 @@ def _norm_plain(grads, name):
     return torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt()
 
 
+def _share_elements(a, b):
+    """Whether two strided tensors share an element; where their strides are no common grid, whether they might. Both are boxes of the grid that all
+    their strides span (the bytes of an element its last direction): if the place of one in the other's coordinates has room enough
+    that no two points of the grid between them have one address, they share an element where the boxes meet in every direction."""
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    sides = []
+    for t in (a, b):
+        size = t.element_size()
+        side = [(s * size, n) for s, n in zip(t.stride(), t.shape) if n > 1] + [(1, size)]
+        if len({s for s, _ in side}) < len(side):
+            return True
+        sides.append(dict(side))
+    steps = sorted({*sides[0], *sides[1]}, reverse=True)
+
+    def places(k, rest):
+        if k == len(steps):
+            if rest == 0:
+                yield ()
+            return
+        q = rest // steps[k]
+        for c in (q, q + 1):
+            for more in places(k + 1, rest - c * steps[k]):
+                yield (c, *more)
+
+    for place in places(0, b.data_ptr() - a.data_ptr()):
+        room, apart = 0, False               # room: from the first to the last address of the directions so far
+        for s, c in zip(reversed(steps), reversed(place)):
+            na, nb = sides[0].get(s, 1), sides[1].get(s, 1)
+            if room >= s:
+                break
+            room += s * (max(na, c + nb) - 1 - min(0, c))
+            apart = apart or c >= na or c + nb <= 0
+        else:
+            return not apart
+    return True
+
+
+def _check_apart(grads, name):
+    """Refuses gradients that share memory with one another."""
+    torch = _torch()
+    if any(type(g) not in (torch.Tensor, torch.nn.Parameter) or g.is_meta for g in grads) or _transformed(*grads):
+        return                               # (they have no addresses)
+    spans = [(g.data_ptr(), g.data_ptr() + g.element_size() * (1 + sum((n - 1) * s for n, s in zip(g.shape, g.stride()))), g) for g in grads if g.numel()]
+    spans.sort(key=lambda s: s[0])
+    for i, (_, end, g) in enumerate(spans):
+        for begin, _, other in spans[i + 1:]:
+            if begin >= end:
+                break
+            if _share_elements(g, other):
+                raise ValueError(f"{name}: two gradients share memory")
+
+
 def gradient_norm(parameters):
     """The 2-norm of all gradients of `parameters` (a tensor or an iterable) together, a float32 scalar on their device: squares are summed
     in float64, so neither large nor tiny values overflow or vanish. Parameters without a gradient count nothing, a gradient that is passed twice
@@ -389,6 +442,7 @@ def clip_gradients(parameters, max_norm: float, eps: float = 1e-6):
         return ops().gradient_norm("clip_gradients", grads, True, float(max_norm), float(eps))
     with torch.no_grad():
         norm = _norm_plain(grads, "clip_gradients")
+        _check_apart(grads, "clip_gradients")
         by = (max_norm / (norm + eps)).clamp(max=1.0).float()
         for g in grads:
             g.copy_(g.float() * by if g.dtype != torch.float64 else g * by)

@@ -1,10 +1,13 @@
 """The operators of a memory that selects and of the gradients' norm where a value, a layout or a state is out of the ordinary: values that are not
 finite, states that go on from a sequence to single steps, gradients that share memory or only lie between one another. Definitions and
 bounds are those of test_selective.py."""
+import random
+
 import pytest
 import torch
 
 from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, state_scan
+from fast_mario_env_amd.rollout import _share_elements, clip_gradients, gradient_norm
 from test_selective import DTYPES, conv_inputs, scan_inputs
 
 
@@ -111,3 +114,53 @@ def test_cpu_what_is_not_finite_stays_in_its_episode(bad):
         y, end = state_scan(**{**a, **v})
         v["grads"] = torch.autograd.grad((y, end), [v[n] for n in names], (dout, ds))
     assert all(torch.equal(p, q) for p, q in zip(leaves["grads"], dirty["grads"]))
+
+# ---------------------------------------------------------------- the gradients' norm
+def parameters_of(*grads):
+    ps = [torch.zeros_like(g, requires_grad=True) for g in grads]
+    for p, g in zip(ps, grads):
+        p.grad = g
+    return ps
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_clipping_refuses_shared_elements(device):
+    """Gradients that share an element are refused before anything is scaled, on either device."""
+    n = lambda *s: torch.randn(s, generator=torch.Generator().manual_seed(0)).to(device)   # noqa: E731
+    flat, wide, cube = n(64), n(6, 40), n(5, 6, 8)
+    for buf, parts in ((flat, (flat[:40], flat[30:])), (wide, (wide[:, :6], wide[:, 5:])), (wide, (wide, wide[2:3, 7])), (wide, (wide[:4], wide[3])),
+                       (flat, (flat[::2], flat[10:20])), (flat, (flat[::2], flat[::3])), (cube, (cube[:, :3, 2:5], cube[:, 2:, 4:])), (wide, (wide.t(), wide[1:3, 39:])),
+                       (flat, (flat[:1], flat[1:], flat[5]))):
+        before = buf.clone()
+        with pytest.raises(ValueError, match="share"):
+            clip_gradients(parameters_of(*parts), 0.1)
+        assert torch.equal(buf, before)
+        want = torch.cat([p.flatten() for p in parts]).double().norm()      # (the norm alone changes nothing: whatever it is given)
+        assert abs(gradient_norm(parameters_of(*parts)).double() - want) <= 2.0 ** -23 * want
+
+
+def test_elements_shared_or_not_by_enumeration():
+    """Random views of one buffer: boxes of its own grid are told exactly; where one takes every second row, what is said not to share never does."""
+    rng, base = random.Random(1), torch.zeros(4, 5, 6, 7)
+    for _ in range(3000):
+        views, boxes = [], True
+        for _ in range(2):
+            v = base
+            for d in range(4):
+                lo = rng.randrange(v.shape[d])
+                v = v.narrow(d, lo, rng.randint(1, v.shape[d] - lo))
+            if rng.random() < 0.3:
+                v, boxes = v[:, :, ::2], False
+            if rng.random() < 0.3:
+                v = v.select(rng.randrange(4), 0)
+            if rng.random() < 0.3:
+                v = v.transpose(0, -1)
+            views.append(v)
+        at = [torch.zeros(base.numel(), dtype=torch.bool) for _ in views]
+        for a, v in zip(at, views):
+            a.as_strided(v.shape, v.stride(), v.storage_offset()).fill_(True)
+        shared, said = bool((at[0] & at[1]).any()), _share_elements(*views)
+        assert said == shared or said and not boxes
