@@ -438,33 +438,38 @@ Tensor scan_step(const Tensor& x, const Tensor& dt, const Tensor& A, const Tenso
 }
 
 // ---------------------------------------------------------------- the gradients' norm
-// Tensors that fill their memory without gaps are taken as they lie; others by a copy, which goes back after scaling. What overlaps in memory is refused.
-Tensor gradient_norm(const std::string& name, const std::vector<Tensor>& given, bool scale, double max_norm, double eps) {
+// Tensors that fill their memory without gaps are taken as they lie; others by a copy, which goes back after scaling. None where they are to be
+// scaled and the spans of two cross, unless the caller knows them `apart`: whether they share elements takes longer to find out.
+Maybe gradient_norm(const std::string& name, const std::vector<Tensor>& given, bool scale, double max_norm, double eps, bool apart) {
     const Tensor& first = given[0];
     const c10::DeviceGuard guard(first.device());
     const at::NoGradGuard no_grad;
-    std::vector<Tensor> held;
-    std::vector<MoTensor> list;
+    const auto lies = [](const Tensor& g) { return g.is_non_overlapping_and_dense() && !g.is_neg(); };
     std::vector<std::pair<char*, char*>> spans;
-    held.reserve(given.size());
-    list.reserve(given.size());
     spans.reserve(given.size());
     for (const Tensor& g : given) {
         TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.is_floating_point() && g.device() == first.device(), name, ": gradients must be dense float tensors on one device");
         TORCH_CHECK_VALUE(g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16, name, ": gradients on the GPU must be float32 or bf16");
-        const bool as_it_lies = g.is_non_overlapping_and_dense() && !g.is_neg();
+        const bool as_it_lies = lies(g);
         int64_t last = 0;
         for (int64_t d = 0; d < g.dim() && !as_it_lies; d++) {
             TORCH_CHECK_VALUE(g.stride(d) || g.size(d) < 2, name, ": a gradient shares elements with itself (expanded)");
             last += (g.size(d) - 1) * g.stride(d);
         }
-        held.push_back(as_it_lies ? g : g.is_neg() ? g.resolve_neg().contiguous() : g.contiguous());
-        list.push_back({held.back().data_ptr(), g.numel(), dtype_of(g), 0});
         char* const at = (char*)g.data_ptr();
-        if (scale && g.numel()) spans.push_back({at, at + (as_it_lies ? g.numel() : last + 1) * g.element_size()});
+        if (scale && !apart && g.numel()) spans.push_back({at, at + (as_it_lies ? g.numel() : last + 1) * g.element_size()});
     }
     std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); i++) TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, name, ": two gradients share memory");
+    for (size_t i = 1; i < spans.size(); i++)
+        if (spans[i].first < spans[i - 1].second) return std::nullopt;
+    std::vector<Tensor> held;
+    std::vector<MoTensor> list;
+    held.reserve(given.size());
+    list.reserve(given.size());
+    for (const Tensor& g : given) {
+        held.push_back(lies(g) ? g : g.is_neg() ? g.resolve_neg().contiguous() : g.contiguous());
+        list.push_back({held.back().data_ptr(), g.numel(), dtype_of(g), 0});
+    }
     const Tensor norm = at::empty({}, first.options().dtype(at::kFloat)), work = work_of(ok(mo_gradient_work((int64_t)list.size()), "mo_gradient_work"), first);
     ok(mo_gradient_norm(list.data(), (int64_t)list.size(), scale, (float)max_norm, (float)eps, data(norm), data<void>(work), stream_of(first)), "mo_gradient_norm");
     if (scale)

@@ -425,21 +425,26 @@ def gradient_norm(parameters):
     grads = _gradients(parameters)
     if _norm_kernel_takes(grads):
         from ._native import ops
-        return ops().gradient_norm("gradient_norm", grads, False, 0.0, 0.0)
+        return ops().gradient_norm("gradient_norm", grads, False, 0.0, 0.0, True)
     return _norm_plain(grads, "gradient_norm").float()
 
 
 def clip_gradients(parameters, max_norm: float, eps: float = 1e-6):
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + eps)), norm that of `gradient_norm`, which is returned: what a
     training step does between backward and the optimizer. A norm that is NaN or infinite makes gradients NaN or 0 by the same formula;
-    look at the norm. Gradients whose places in memory overlap are refused."""
+    look at the norm. Gradients that share elements with one another are refused; views that only lie between one another, such as columns of one
+    matrix, are taken (where their strides are those of one buffer's: others whose places cross are refused too)."""
     if not (max_norm >= 0 and eps >= 0):
         raise ValueError("clip_gradients: max_norm and eps must be >= 0")
     torch = _torch()
     grads = _gradients(parameters)
     if _norm_kernel_takes(grads):
         from ._native import ops
-        return ops().gradient_norm("clip_gradients", grads, True, float(max_norm), float(eps))
+        norm = ops().gradient_norm("clip_gradients", grads, True, float(max_norm), float(eps), False)
+        if norm is not None:
+            return norm
+        _check_apart(grads, "clip_gradients")    # (some lie between one another, or share memory)
+        return ops().gradient_norm("clip_gradients", grads, True, float(max_norm), float(eps), True)
     with torch.no_grad():
         norm = _norm_plain(grads, "clip_gradients")
         _check_apart(grads, "clip_gradients")

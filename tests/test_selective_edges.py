@@ -164,3 +164,30 @@ def test_elements_shared_or_not_by_enumeration():
             a.as_strided(v.shape, v.stride(), v.storage_offset()).fill_(True)
         shared, said = bool((at[0] & at[1]).any()), _share_elements(*views)
         assert said == shared or said and not boxes
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_clipping_takes_views_that_lie_between_one_another(device):
+    """Views of one buffer that share no element, wherever they lie: their values are scaled once, the rest of the buffer is left."""
+    n = lambda *s: torch.randn(s, generator=torch.Generator().manual_seed(0)).to(device)   # noqa: E731
+    def parts_of(k):
+        if k < 4:
+            w = n(30, 40)
+            return w, ((w[:, :5], w[:, 5:]), (w[:, 20:], w[1:, :10], w[0, :4]), (w[::2], w[1::2], w[0:0]), (w.t()[3], w[:, 4:30:5], w[2:9, :3]))[k]
+        if k < 6:
+            c = n(4, 6, 8)
+            return c, ((c[:, :3, 2:5], c[:, 3:, 4:], c[1:3, 0:2, :2]), (c[..., 0], c[..., 1:].transpose(0, 2), ))[k - 4]
+        f = n(64)
+        return f, ((f[::2], f[1::2]), (f[::3], f[1::3], f[2::3], f[:0]), (f[0], f[1:30], f[30:31], f[40:]))[k - 6]
+
+    for k in range(9):
+        buf, parts = parts_of(k)
+        mine = torch.zeros_like(buf)
+        for p in parts:                                      # (which elements of the buffer are in a part)
+            mine.as_strided(p.shape, p.stride(), p.storage_offset()).add_(1.0)
+        assert mine.max() == 1.0 and len(parts) > 1
+        before, want = buf.double(), torch.cat([p.flatten() for p in parts]).double().norm()
+        norm = clip_gradients(parameters_of(*parts), 0.5, eps=0.0)
+        assert abs(norm.double() - want) <= 2.0 ** -23 * want
+        after = torch.where(mine > 0, before * (0.5 / want), before)
+        assert ((buf.double() - after).abs() <= 2.0 ** -22 * after.abs()).all(), k
