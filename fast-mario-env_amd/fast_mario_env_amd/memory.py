@@ -40,6 +40,11 @@ def _kernel_takes(*ts):
     return not _transformed(*ts)
 
 
+def _own(last, state):
+    """A state as it is returned: one that the steps take, and not the caller's."""
+    return last.clone(memory_format=torch.contiguous_format) if last is state else last.contiguous()
+
+
 def head_decays(heads: int, device="cuda"):
     """Factors (heads,) whose memories last from about 22 steps (half-life) to about 1,400: 1 - 2^-5 .. 1 - 2^-11."""
     return (1.0 - 2.0 ** -torch.linspace(5.0, 11.0, heads, dtype=torch.float64)).float().to(device)
@@ -76,7 +81,7 @@ def _attend_plain(q, k, v, decay, start, state, scale):
         S = S + k[t].float()[..., :, None] * v[t].float()[..., None, :]
         out.append((q[t].float()[..., :, None] * S).sum(-2) * scale)
     out = torch.stack(out).to(q.dtype) if out else v.new_empty(v.shape)
-    return out, S.clone() if S is state else S
+    return out, _own(S, state)
 
 
 def linear_attention(q, k, v, decay, start=None, state=None, scale=None):
@@ -194,7 +199,7 @@ def _conv_plain(x, weight, bias, start, state, act):
         out.append(torch.relu(p) if act == "relu" else p * torch.sigmoid(p) if act == "silu" else p)
         window = every[:, 1:]
     out = torch.stack(out).to(x.dtype) if out else x.new_empty(x.shape)
-    return out, window.clone() if window is state else window
+    return out, _own(window, state)
 
 
 def causal_conv_act(x, weight, bias=None, start=None, state=None, act="silu"):
@@ -276,7 +281,7 @@ def _scan_plain(x, dt, A, B, C, D, z, dt_bias, start, state):
             y = y * (zt * torch.sigmoid(zt))
         out.append(y)
     out = torch.stack(out).to(x.dtype) if out else x.new_empty(x.shape)
-    return out, h.clone() if h is state else h
+    return out, _own(h, state)
 
 
 def state_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, start=None, state=None):

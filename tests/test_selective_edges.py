@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, state_scan
+from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, linear_attention, make_memory_net, state_scan, state_scan_step
 from fast_mario_env_amd.rollout import _share_elements, clip_gradients, gradient_norm
 from test_selective import DTYPES, conv_inputs, scan_inputs
 
@@ -69,6 +69,41 @@ def test_convolution_relu_at_zero(device):
         dx, db = torch.autograd.grad(y, (leaf, b), dy)
         assert torch.equal(y.detach().nan_to_num(5.0), torch.full_like(y, 0.0 if value == 0.0 else 5.0))
         assert torch.allclose(db, slope * dy.sum((0, 1)), atol=18 * 2.0 ** -24 * 18) and torch.isfinite(dx).all() and (dx == 0).all() == (slope == 0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("T", [1, 2, 7])
+def test_steps_go_on_from_a_sequence(T, device):
+    """The state that a sequence returns is one that the steps take and update, without copies of it elsewhere; so are the network's memories."""
+    x, w, b, start, state, _, _ = conv_inputs(T + 4, 3, 8, 4, torch.float32, device=device)
+    a, _, _ = scan_inputs(T + 4, 3, 8, 4, 1, torch.float32, device=device)
+    timed = lambda part: {n: v[part] if n in ("x", "dt", "B", "C", "z", "start") else v for n, v in a.items()}   # noqa: E731
+    for given in (None, state):
+        y, _ = causal_conv_act(x, w, b, start, given)
+        _, s = causal_conv_act(x[:T], w, b, start[:T], given)
+        for t in range(T, T + 4):
+            assert torch.allclose(causal_conv_act_step(x[t], w, b, s, start[t]), y[t], atol=1e-5)
+    y, _ = state_scan(**a)
+    _, h = state_scan(**timed(slice(0, T)))
+    for t in range(T, T + 4):
+        assert torch.allclose(state_scan_step(**{**timed(t), "state": h}), y[t], atol=1e-4)
+    back = lambda t: t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim())))   # noqa: E731
+    for n in (0, 1, T):                                      # inputs of another order in memory
+        for given in (None, back):
+            c = {k: back(v[:n] if k in ("x", "dt", "B", "C", "z", "start") else v) for k, v in a.items()}
+            c["state"] = given and c["state"]
+            q, d, m = back(torch.randn(n, 3, 2, 4, device=device)), torch.ones(2, device=device), torch.zeros(3, 2, 4, 4, device=device)
+            for last in (causal_conv_act(back(x[:n]), back(w), b, None, given and given(state))[1], state_scan(**c)[1],
+                         linear_attention(q, q, q, d, None, given and given(m))[1]):
+                assert last.is_contiguous()
+    if device == "cpu":
+        net = make_memory_net(device="cpu", memory="scan")
+        obs = torch.randint(0, 256, (T + 2, 3, 4, 84, 84), dtype=torch.uint8, generator=torch.Generator().manual_seed(0))
+        with torch.no_grad():
+            logits, _, _ = net(obs)
+            _, _, memories = net(obs[:T])
+            for t in range(T, T + 2):
+                assert torch.allclose(net.step(obs[t], None, memories)[0], logits[t], atol=1e-5)
 
 
 # ---------------------------------------------------------------- scan
