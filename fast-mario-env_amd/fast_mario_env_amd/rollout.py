@@ -448,9 +448,9 @@ def clip_gradients(parameters, max_norm: float, eps: float = 1e-6):
     with torch.no_grad():
         norm = _norm_plain(grads, "clip_gradients")
         _check_apart(grads, "clip_gradients")
-        by = (max_norm / (norm + eps)).clamp(max=1.0).float()
+        by = (max_norm / (norm + eps)).clamp(max=1.0)
         for g in grads:
-            g.copy_(g.float() * by if g.dtype != torch.float64 else g * by)
+            g.copy_(g.float() * by.float() if g.dtype != torch.float64 else g * by)
         return norm.float()
 
 

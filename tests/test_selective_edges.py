@@ -226,3 +226,15 @@ def test_clipping_takes_views_that_lie_between_one_another(device):
         assert abs(norm.double() - want) <= 2.0 ** -23 * want
         after = torch.where(mine > 0, before * (0.5 / want), before)
         assert ((buf.double() - after).abs() <= 2.0 ** -22 * after.abs()).all(), k
+
+
+def test_clipping_float64_on_cpu():
+    """Gradients in float64 are scaled by a factor in float64: a division, a sum and a product, 2^-53 each, and the norm's own 2^-52."""
+    g = torch.randn(1000, generator=torch.Generator().manual_seed(2), dtype=torch.float64)
+    half = torch.randn(50, generator=torch.Generator().manual_seed(3))
+    ps = parameters_of(g.clone(), half.clone())
+    norm = torch.cat([g, half.double()]).norm()
+    assert torch.allclose(clip_gradients(ps, 0.5).double(), norm, rtol=2.0 ** -24)
+    by = 0.5 / (norm + 1e-6)
+    assert ((ps[0].grad - g * by).abs() <= 2.0 ** -50 * (g * by).abs()).all()
+    assert ((ps[1].grad.double() - half.double() * by).abs() <= 2.0 ** -22 * half.double().abs() * by).all()
