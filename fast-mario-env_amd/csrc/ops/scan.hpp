@@ -61,6 +61,15 @@ template <class T> __global__ void __launch_bounds__(256) k_scan_pack(Scan k, fl
     *(Pack<float, 4>*)(bc + 4 * id) = x;
 }
 
+// All ones or none, in a scalar register; and x, or 0 whatever x is (0 times an infinity is none). One instruction with a scalar operand: the compiler would
+// make a select of it, whose masks take two registers each.
+__device__ __forceinline__ uint32_t mask_of(bool there) {
+    uint32_t m = __builtin_amdgcn_readfirstlane(there ? -1 : 0);
+    asm("" : "+s"(m));
+    return m;
+}
+__device__ __forceinline__ float masked(float x, uint32_t m) { return __uint_as_float(__float_as_uint(x) & m); }
+
 // What a wave works on.
 struct ScanPlace {
     int64_t n, segment;
@@ -338,8 +347,9 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
             for (int i = 0; i < SCAN_STEPS; i++) total = cuts >> i & 1 || total < 0.f ? -1.f : total + d[i];
             continue;
         }
+        const uint32_t with_D = mask_of(a.D);
         const auto finish = [&](int i, float y) {
-            y = fmaf(D, as_f32(lx[i * kWave + lane]), y);
+            y = fmaf(D, masked(as_f32(lx[i * kWave + lane]), with_D), y);
             if (gate) {
                 const float z = as_f32(lz[i * kWave + lane]);
                 y *= z * sigmoid(z);

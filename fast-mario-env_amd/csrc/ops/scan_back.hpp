@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
             const ScanPlace me = place.again();
             const int lane = me.lane, c = me.c;
             if constexpr (SPLIT) {
+                const uint32_t with_D = mask_of(a.D);
                 for (int i = slice; i < steps; i += slices) {
                     const int at = i * kWave + lane;
                     float y = 0.f, du = 0.f, dd = 0.f;
@@ -245,11 +246,11 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                     add_to(dbias, dbias_rest, ddt);
                     if (!me.live) continue;
                     const auto row_of = [&](const MoRows& r) { return (T*)r.p + (t0 + i) * r.st + n * r.sn + c; };
-                    *row_of(a.dx) = as<T>(fmaf(du, l.d()[at], D * dy));
+                    *row_of(a.dx) = as<T>(fmaf(du, l.d()[at], D * masked(dy, with_D)));
                     *row_of(a.ddt) = as<T>(ddt);
                     if (!gate) continue;
                     const float z = as_f32(l.z()[at]);
-                    *row_of(a.dz) = as<T>(fmaf(D, x, y) * (Lds::F32 ? z : gate_slope(as_f32(l.dout()[at]), z, sigmoid(z))));
+                    *row_of(a.dz) = as<T>(fmaf(D, masked(x, with_D), y) * (Lds::F32 ? z : gate_slope(as_f32(l.dout()[at]), z, sigmoid(z))));
                 }
             } else {
                 ChunkIn<T>::leave(l.x(), a.dx, t0, steps, me, k.wide);
@@ -313,6 +314,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
 #pragma unroll
             for (int s = 0; s < SP; s++) h[0][s] = me.live ? before[s] : 0.f;
             float* const to_join = l.sums(chunk);
+            const uint32_t with_D = mask_of(a.D);
             // what a step needs, read a step ahead
             struct In { float d, dy; T x; };
             const auto in_of = [&](int i) { return In{l.d()[i * kWave + lane], l.dy()[i * kWave + lane], l.x()[i * kWave + lane]}; };
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                     for (int i = 0; i < SCAN_STEPS; i++) {
                         const int at = i * kWave + lane;
                         const float z = as_f32(l.z()[at]);
-                        l.z()[at] = as<T>(fmaf(D, as_f32(l.x()[at]), l.y()[at]) * (Lds::F32 ? z : gate_slope(as_f32(l.dout()[at]), z, sigmoid(z))));
+                        l.z()[at] = as<T>(fmaf(D, masked(as_f32(l.x()[at]), with_D), l.y()[at]) * (Lds::F32 ? z : gate_slope(as_f32(l.dout()[at]), z, sigmoid(z))));
                     }
                 end_of_step();
             }
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                     const float ddt = fmaf(du, x, dd * LN2) * l.slope()[at];
                     dD_here = fmaf(in.dy, x, dD_here);
                     dbias_here += ddt;
-                    l.x()[at] = as<T>(fmaf(du, in.d, D * in.dy));
+                    l.x()[at] = as<T>(fmaf(du, in.d, D * masked(in.dy, with_D)));
                     l.dt()[at] = as<T>(ddt);
                 }
                 if constexpr (i > 0) {

@@ -8,7 +8,7 @@ import torch
 
 from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, linear_attention, make_memory_net, state_scan, state_scan_step
 from fast_mario_env_amd.rollout import _share_elements, clip_gradients, gradient_norm
-from test_selective import DTYPES, conv_inputs, scan_inputs
+from test_selective import DTYPES, conv_inputs, scan64, scan_inputs
 
 
 def same_kind(got, want, what):
@@ -149,6 +149,56 @@ def test_cpu_what_is_not_finite_stays_in_its_episode(bad):
         y, end = state_scan(**{**a, **v})
         v["grads"] = torch.autograd.grad((y, end), [v[n] for n in names], (dout, ds))
     assert all(torch.equal(p, q) for p, q in zip(leaves["grads"], dirty["grads"]))
+
+
+def rising(T, N, C, S, G, dtype, D, z):
+    """Inputs whose products are all positive but for z's, and decays that do not vanish: an infinity keeps its sign."""
+    a, dout, ds = scan_inputs(T, N, C, S, G, dtype, starts=None, D=D, z=z)
+    for n in ("x", "B", "C", "state"):
+        a[n] = a[n].abs() + 0.25
+    a["A"] = a["A"].clamp(min=-1.0)
+    if D:
+        a["D"] = a["D"].abs()
+    a["start"] = torch.zeros(T, N, dtype=torch.bool, device="cuda")
+    a["start"][T // 2, 0] = True
+    return a, dout.abs() + 0.25, ds.abs()
+
+
+def check_infinite(a, dout, ds):
+    """y, the state and the gradients that do not add infinities of both signs, against the definition."""
+    names = ("x", "B", "C", "z", "state")
+    leaves = {n: a[n].detach().requires_grad_() for n in names if a[n] is not None}
+    y, last = state_scan(**{**a, **leaves})
+    got = dict(zip(leaves, torch.autograd.grad((y, last), list(leaves.values()), (dout, ds))))
+    with torch.no_grad():
+        again = state_scan(**a)
+    want = scan64(*(a[n] for n in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "start", "state")), dout, ds)
+    for v, u in zip((y.detach(), last.detach()), again):
+        assert torch.equal(v.nan_to_num(7.0), u.nan_to_num(7.0))
+    same_kind(y.detach(), want[0], "y")
+    same_kind(last.detach(), want[1], "state")
+    for n, g in got.items():
+        same_kind(g, want[2]["d" + n], "d" + n)
+    h = a["state"].clone()
+    for t in range(3):
+        one = {n: v[t] if v is not None and n in ("x", "dt", "B", "C", "z", "start") else v for n, v in a.items()}
+        same_kind(state_scan_step(**{**one, "state": h}), want[0][t], "step")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("z", [False, True])
+@pytest.mark.parametrize("T,C,S,G", [(20, 64, 16, 1), (20, 40, 4, 2), (20, 48, 64, 1), (600, 24, 8, 1), (600, 70, 24, 2)])
+def test_scan_without_D_keeps_an_infinity(T, C, S, G, z, dtype):
+    """An infinite x, an infinite gradient of y: what is not there adds no 0 times infinity."""
+    for D in (False, True):
+        for what in ("x", "dout"):
+            a, dout, ds = rising(T, 2, C, S, G, dtype, D, z)
+            if a["z"] is not None:
+                a["z"] = a["z"].abs() + 0.25
+            (a["x"] if what == "x" else dout)[2, 1, 5] = float("inf")
+            check_infinite(a, dout, ds)
+
 
 # ---------------------------------------------------------------- the gradients' norm
 def parameters_of(*grads):
