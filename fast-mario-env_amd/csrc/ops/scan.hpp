@@ -70,6 +70,20 @@ __device__ __forceinline__ uint32_t mask_of(bool there) {
 }
 __device__ __forceinline__ float masked(float x, uint32_t m) { return __uint_as_float(__float_as_uint(x) & m); }
 
+// Where a lane has registers for more states than there are (PAD), the rest stay 0: a product of 0 and an infinite d x would not be, and so
+// reach y and the gradients of step sizes. Without slices at most three of a lane's states are not there, in the last slice most may not be. Kernels of
+// their own, for the masks take an instruction for each such state and step (128 x 512 x 512, bf16, forward and gradient, without and with them: 13
+// states 748 and 801 us, 20 states 1,255 and 1,331, 49 states 3,771 and 4,029).
+template <int SP, bool SPLIT, bool PAD> struct Real {
+    static constexpr int FROM = !PAD ? SP : SPLIT ? 0 : SP - 3;   // those before are there
+    uint32_t m[PAD ? SP - FROM : 1];
+    __device__ __forceinline__ explicit Real(int there) {
+#pragma unroll
+        for (int s = FROM; s < SP; s++) m[s - FROM] = mask_of(s < there);
+    }
+    __device__ __forceinline__ float operator()(float x, int s) const { return s < FROM ? x : masked(x, m[s < FROM ? 0 : s - FROM]); }
+};
+
 // What a wave works on.
 struct ScanPlace {
     int64_t n, segment;
@@ -172,7 +186,7 @@ __device__ __forceinline__ uint8_t start_of_lane(const MoScan& a, int64_t t0, in
 }
 template <int SP> __device__ __forceinline__ void load_decays(const MoScan& a, const ScanPlace& me, float (&A)[SP]) {
 #pragma unroll
-    for (int s = 0; s < SP; s++) A[s] = me.live && me.s0 + s < a.S ? a.A[(int64_t)me.c * a.S + me.s0 + s] * LOG2E : 0.f;
+    for (int s = 0; s < SP; s++) A[s] = !me.live ? 0.f : me.s0 + s < a.S ? a.A[(int64_t)me.c * a.S + me.s0 + s] * LOG2E : -1.f;   // (0 times an infinite d is none)
 }
 // A channel's states as they lie, zeros past the last (or of none); in 16-byte accesses where they allow it (a lane's states lie 4 S
 // bytes from its neighbour's).
@@ -246,7 +260,7 @@ __device__ __forceinline__ void end_of_step() { __builtin_amdgcn_sched_barrier(0
 
 // Forward. SUMS: only what a segment adds to an entering state: its last states from zero, and the sum of its step sizes (-1 where an episode
 // starts in it: nothing of what enters is left).
-template <class T, int SP, bool SPLIT, bool SUMS>
+template <class T, int SP, bool SPLIT, bool SUMS, bool PAD>
 __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
     const MoScan& a = k.a;
     constexpr int TILE = SCAN_STEPS * kWave;
@@ -260,13 +274,14 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
     const int c = place.c;
     T *lx = tiles[w][0], *ldt = tiles[w][1], *lz = tiles[w][SUMS ? 0 : 2];
     const bool gate = !SUMS && a.z.p;
+    const Real<SP, SPLIT, PAD> real(a.S - place.s0);
     float A[SP], h[SP], total = 0.f;
     load_decays<SP>(a, place, A);
     const int64_t seg0 = ((place.segment * a.N + n) * k.SB + place.s0) * a.C + c;
     if (!SUMS && k.segments == 1) load_states<SP>(a, a.state, n, c, place.s0, h);
     else
 #pragma unroll
-        for (int s = 0; s < SP; s++) h[s] = SUMS ? 0.f : k.seg_h[seg0 + (int64_t)s * a.C];
+        for (int s = 0; s < SP; s++) h[s] = SUMS ? 0.f : real(k.seg_h[seg0 + (int64_t)s * a.C], s);
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, D = a.D ? a.D[c] : 0.f;
     ChunkIn<T> ix, idt, iz;
     uint8_t flag = 0;
@@ -334,6 +349,9 @@ __global__ void __launch_bounds__(SCAN_WAVES* kWave) k_scan(Scan k) {
 #pragma unroll
             for (int s = 0; s < SP; s++) h[s] = fmaf(exp2_raw(d[i] * A[s]), h[s], u[i] * now.b[s]);
             if_start_set<i, SP>(cuts, h, u[i], now.b);
+            if (PAD)
+#pragma unroll
+                for (int s = 0; s < SP; s++) h[s] = real(h[s], s);
             if (!SUMS)
 #pragma unroll
                 for (int s = 0; s < SP; s++) y = fmaf(now.c[s], h[s], y);
@@ -480,16 +498,18 @@ inline int64_t scan_work_floats(const Scan& k, bool backward) {
     return scan_segs(k) + scan_parts_bc(k) + scan_parts(k) + column_sums_work(k.rows, k.SB + 2, k.a.C);
 }
 
+// f(states a lane, whether waves share channels, whether some of the states are not there)
 template <class F> int by_states(const Scan& k, F f) {
     const int SP = k.SB / k.slices;
+    const auto padded = [&](auto sp, auto split) { return k.SB == k.a.S ? f(sp, split, std::false_type{}) : f(sp, split, std::true_type{}); };
     if (k.slices == 1) {
-        if (SP == 4) return f(std::integral_constant<int, 4>{}, std::false_type{});
-        if (SP == 8) return f(std::integral_constant<int, 8>{}, std::false_type{});
-        if (SP == 12) return f(std::integral_constant<int, 12>{}, std::false_type{});
-        return f(std::integral_constant<int, 16>{}, std::false_type{});
+        if (SP == 4) return padded(std::integral_constant<int, 4>{}, std::false_type{});
+        if (SP == 8) return padded(std::integral_constant<int, 8>{}, std::false_type{});
+        if (SP == 12) return padded(std::integral_constant<int, 12>{}, std::false_type{});
+        return padded(std::integral_constant<int, 16>{}, std::false_type{});
     }
-    if (SP == 12) return f(std::integral_constant<int, 12>{}, std::true_type{});
-    return f(std::integral_constant<int, 16>{}, std::true_type{});
+    if (SP == 12) return padded(std::integral_constant<int, 12>{}, std::true_type{});
+    return padded(std::integral_constant<int, 16>{}, std::true_type{});
 }
 inline void scan_launch_shape(const Scan& k, int64_t waves, dim3& grid, dim3& block) {
     grid = grid_of(k.slices > 1 ? waves : (waves + SCAN_WAVES - 1) / SCAN_WAVES);
@@ -508,16 +528,16 @@ template <class T> int scan_forward(const MoScan& a, hipStream_t s) {
         hipLaunchKernelGGL((k_scan_pack<T>), grid_of((n + 255) / 256), dim3(256), 0, s, k, bc);
         if (launched("k_scan_pack")) return -1;
     }
-    return by_states(k, [&](auto sp, auto split) {
+    return by_states(k, [&](auto sp, auto split, auto pad) {
         constexpr int SP = decltype(sp)::value;
-        constexpr bool SPLIT = decltype(split)::value;
+        constexpr bool SPLIT = decltype(split)::value, PAD = decltype(pad)::value;
         dim3 grid, block;
         scan_launch_shape(k, k.segments * a.N * a.G * k.per, grid, block);
         if (k.segments > 1) {
-            hipLaunchKernelGGL((k_scan<T, SP, SPLIT, true>), grid, block, 0, s, k);
+            hipLaunchKernelGGL((k_scan<T, SP, SPLIT, true, false>), grid, block, 0, s, k);
             hipLaunchKernelGGL((k_scan_enter<false>), grid_of((a.N * k.SB * a.C + 255) / 256), dim3(256), 0, s, k);
         }
-        hipLaunchKernelGGL((k_scan<T, SP, SPLIT, false>), grid, block, 0, s, k);
+        hipLaunchKernelGGL((k_scan<T, SP, SPLIT, false, PAD>), grid, block, 0, s, k);
         return launched("k_scan");
     });
 }

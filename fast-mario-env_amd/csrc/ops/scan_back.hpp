@@ -161,7 +161,7 @@ __device__ __forceinline__ void add_to(float& sum, float& rest, float x) {
     sum = s;
 }
 
-template <class T, int SP, bool SPLIT>
+template <class T, int SP, bool SPLIT, bool PAD>
 __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
     const MoScan& a = k.a;
     typedef BackLds<T, SP, SPLIT> Lds;
@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
     const bool gate = a.z.p;
     ScanPlace place(k, row, cb, slice, SP);
     if (in_group >= k.per) { place.live = false; place.there = 0; }
+    const Real<SP, SPLIT, PAD> real(a.S - place.s0);
     float A[SP], dD = 0.f, dbias = 0.f, dD_rest = 0.f, dbias_rest = 0.f;
     const int c = place.c;
     load_decays<SP>(a, place, A);
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
 #pragma unroll
             for (int s = 0; s < SP; s++) Q[s] = k.seg_h[((place.segment * a.N + n) * k.SB + place.s0 + s) * a.C + c];
 #pragma unroll
-        for (int s = 0; s < SP; s++) Q[s] = place.live ? Q[s] : 0.f;
+        for (int s = 0; s < SP; s++) Q[s] = place.live ? real(Q[s], s) : 0.f;
         // what a chunk left in LDS goes to memory
         const auto after_chunk = [&](int64_t chunk, int64_t t0, int steps) {
             const Scan& k = args_again();
@@ -341,6 +342,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 if_start_set<i, SP>(cuts, v, u, now.b);
 #pragma unroll
                 for (int s = 0; s < SP; s++) {
+                    v[s] = real(v[s], s);
                     if constexpr (i + 1 < SCAN_STEPS) h[i + 1][s] = v[s];
                     y = fmaf(now.c[s], v[s], y);
                     v[s] *= in.dy;
@@ -384,7 +386,7 @@ __global__ void __launch_bounds__(BACK_WAVES* kWave, 2) k_scan_back(Scan k) {
                 float du = 0.f, dd = 0.f, v[SP];
 #pragma unroll
                 for (int s = 0; s < SP; s++) {
-                    Q[s] = fmaf(now.c[s], in.dy, Q[s]);
+                    Q[s] = real(fmaf(now.c[s], in.dy, Q[s]), s);
                     du = fmaf(Q[s], now.b[s], du);
                     v[s] = Q[s] * u;
                 }
@@ -484,9 +486,9 @@ template <class T> int scan_backward(const MoScan& a, hipStream_t s) {
     k.part_bc = (float*)a.work + scan_segs(k);
     k.part = k.part_bc + scan_parts_bc(k);
     float* more = k.part + scan_parts(k);
-    return by_states(k, [&](auto sp, auto split) {
+    return by_states(k, [&](auto sp, auto split, auto pad) {
         constexpr int SP = decltype(sp)::value;
-        constexpr bool SPLIT = decltype(split)::value;
+        constexpr bool SPLIT = decltype(split)::value, PAD = decltype(pad)::value;
         if (k.segments > 1) {
             dim3 grid, block;
             scan_launch_shape(k, k.segments * a.N * a.G * k.per, grid, block);
@@ -495,7 +497,7 @@ template <class T> int scan_backward(const MoScan& a, hipStream_t s) {
         }
         const int waves = k.across * k.slices;
         static_assert(scan_back_lds(sizeof(T), 16, false) * SCAN_BACK_WAVES <= 160 << 10, "");
-        hipLaunchKernelGGL((k_scan_back<T, SP, SPLIT>), grid_of(k.rows * a.G * k.cuts), dim3(kWave * waves), waves * (BackLds<T, SP, SPLIT>::BYTES), s, k);
+        hipLaunchKernelGGL((k_scan_back<T, SP, SPLIT, PAD>), grid_of(k.rows * a.G * k.cuts), dim3(kWave * waves), waves * (BackLds<T, SP, SPLIT>::BYTES), s, k);
         if (launched("k_scan_back")) return -1;
         const int64_t n = a.T * a.N * a.G * 2 * k.SB;
         if (n && k.cuts > 1) hipLaunchKernelGGL((k_scan_join<T>), grid_of((n + 255) / 256), dim3(256), 0, s, k);

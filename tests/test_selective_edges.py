@@ -200,6 +200,22 @@ def test_scan_without_D_keeps_an_infinity(T, C, S, G, z, dtype):
             check_infinite(a, dout, ds)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [20, 600])
+@pytest.mark.parametrize("C,S,G", [(64, 1, 1), (40, 3, 2), (65, 13, 1), (48, 20, 1), (30, 33, 3), (24, 49, 1), (8, 2, 1)])
+def test_scan_of_any_number_of_states_keeps_an_infinity(C, S, G, T, dtype):
+    """Numbers of states that fill no whole registers: the rest of them take no part."""
+    for what in ("x", "dout", "state", "dt"):
+        a, dout, ds = rising(T, 2, C, S, G, dtype, True, True)
+        a["z"] = a["z"].abs() + 0.25
+        if what == "state":
+            a["state"][1, 5] = float("inf")
+        else:
+            (dout if what == "dout" else a[what])[2, 1, 5] = float("inf")
+        check_infinite(a, dout, ds)
+
+
 # ---------------------------------------------------------------- the gradients' norm
 def parameters_of(*grads):
     ps = [torch.zeros_like(g, requires_grad=True) for g in grads]
