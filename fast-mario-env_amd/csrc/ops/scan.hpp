@@ -229,7 +229,7 @@ template <int I> __device__ __forceinline__ void if_start_set8(unsigned cuts, fl
         "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\t"
         "v_mul_f32 %0, %[u], %8\n\tv_mul_f32 %1, %[u], %9\n\tv_mul_f32 %2, %[u], %10\n\tv_mul_f32 %3, %[u], %11\n\t"
         "v_mul_f32 %4, %[u], %12\n\tv_mul_f32 %5, %[u], %13\n\tv_mul_f32 %6, %[u], %14\n\tv_mul_f32 %7, %[u], %15\n.Lstart%=:"
-        : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]), "+v"(h[4]), "+v"(h[5]), "+v"(h[6]), "+v"(h[7])
+        : "+&v"(h[0]), "+&v"(h[1]), "+&v"(h[2]), "+&v"(h[3]), "+&v"(h[4]), "+&v"(h[5]), "+&v"(h[6]), "+&v"(h[7])
         : "s"(b[0]), "s"(b[1]), "s"(b[2]), "s"(b[3]), "s"(b[4]), "s"(b[5]), "s"(b[6]), "s"(b[7]), [u] "v"(u), [m] "s"(cuts), [i] "n"(I)
         : "scc");
 }
@@ -237,7 +237,7 @@ template <int I> __device__ __forceinline__ void if_start_set4(unsigned cuts, fl
     asm volatile(
         "s_bitcmp1_b32 %[m], %[i]\n\ts_cbranch_scc0 .Lstart%=\n\t"
         "v_mul_f32 %0, %[u], %4\n\tv_mul_f32 %1, %[u], %5\n\tv_mul_f32 %2, %[u], %6\n\tv_mul_f32 %3, %[u], %7\n.Lstart%=:"
-        : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3])
+        : "+&v"(h[0]), "+&v"(h[1]), "+&v"(h[2]), "+&v"(h[3])
         : "s"(b[0]), "s"(b[1]), "s"(b[2]), "s"(b[3]), [u] "v"(u), [m] "s"(cuts), [i] "n"(I)
         : "scc");
 }

@@ -20,7 +20,8 @@ __device__ __forceinline__ int sum_slot(int l, int M) {
     return M <= 8 ? s : s | ((l >> 2) & 8);
 }
 // x = x + (x of lane l ^ 8), y's likewise in the upper eight lanes of each row; then likewise four and four, the others mirrored. (An operand of DPP or a
-// permlane swap may not have been written by the two instructions before: the nops at both ends, and the order between them.)
+// permlane swap may not have been written by the two instructions before: the nops at both ends, and the order between them. What is written before the
+// last input is read shares no register with an input, equal or not: the `&`.)
 __device__ __forceinline__ void row_sums4(float& x0, float x1, float& x2, float x3) {
     asm("s_nop 1\n\t"
         "v_add_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp %1, %1, %1 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
@@ -28,7 +29,7 @@ __device__ __forceinline__ void row_sums4(float& x0, float x1, float& x2, float 
         "s_nop 1\n\t"
         "v_add_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
         "v_add_f32_dpp %0, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa\n\ts_nop 1"
-        : "+v"(x0), "+v"(x2)
+        : "+&v"(x0), "+&v"(x2)
         : "v"(x1), "v"(x3));
 }
 __device__ __forceinline__ void row_sums8(float& x0, float x1, float& x2, float x3, float& x4, float x5, float& x6, float x7) {
@@ -39,7 +40,7 @@ __device__ __forceinline__ void row_sums8(float& x0, float x1, float& x2, float 
         "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n\tv_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
         "v_add_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp %2, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
         "v_add_f32_dpp %0, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa\n\tv_add_f32_dpp %2, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa\n\ts_nop 1"
-        : "+v"(x0), "+v"(x2), "+v"(x4), "+v"(x6)
+        : "+&v"(x0), "+&v"(x2), "+&v"(x4), "+&v"(x6)
         : "v"(x1), "v"(x3), "v"(x5), "v"(x7));
 }
 template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M]) {
