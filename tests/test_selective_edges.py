@@ -8,7 +8,7 @@ import torch
 
 from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, linear_attention, make_memory_net, state_scan, state_scan_step
 from fast_mario_env_amd.rollout import _share_elements, clip_gradients, gradient_norm
-from test_selective import DTYPES, conv_inputs, scan64, scan_inputs
+from test_selective import DTYPES, check_scan, conv_inputs, scan64, scan_inputs
 
 
 def same_kind(got, want, what):
@@ -214,6 +214,24 @@ def test_scan_of_any_number_of_states_keeps_an_infinity(C, S, G, T, dtype):
         else:
             (dout if what == "dout" else a[what])[2, 1, 5] = float("inf")
         check_infinite(a, dout, ds)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("past", [-8, 0, 8, 1])
+def test_scan_of_steps_far_apart(past, dtype):
+    """Steps as far apart as a chunk's places fit 32 bits, and farther: the same bits as from tensors without gaps, and within the bounds."""
+    T, N, C, S = 9, 2, 64, 16
+    a, dout, ds = scan_inputs(T, N, C, S, 1, dtype)
+    step = 2 ** 28 // dtype.itemsize + past
+    buf = torch.zeros((T - 1) * step + N * (3 * C + 2 * S), dtype=dtype, device="cuda")
+    view = buf.as_strided((T, N, 3 * C + 2 * S), (step, 3 * C + 2 * S, 1))
+    view.normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    x, dt, z, B, Ct = view.split((C, C, C, S, S), -1)
+    far = {**a, "x": x, "dt": dt, "z": z, "B": B.unsqueeze(2), "C": Ct.unsqueeze(2)}
+    y, last, got = check_scan(far, dout, ds)
+    y2, last2, got2 = check_scan({n: v.contiguous() for n, v in far.items()}, dout, ds)
+    assert torch.equal(y, y2) and torch.equal(last, last2) and all(torch.equal(g, got2[n]) for n, g in got.items())
 
 
 # ---------------------------------------------------------------- the gradients' norm
