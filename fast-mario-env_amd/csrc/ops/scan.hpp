@@ -472,7 +472,10 @@ inline Scan scan_cut(const MoScan& a, bool backward) {
     k.cuts = (k.per + k.across - 1) / k.across;
     // Few sequences are cut over their length: each segment is gone through twice, once for what it adds to the state. The forward pass has many waves a
     // compute unit and takes whatever number; the gradient has few, so its segments are as many as run at once (1,999 steps of 8 envs, 512
-    // channels: 32 segments, 160 us; 50, which run in two rounds, 201).
+    // channels: 32 segments, 160 us; 50, which run in two rounds, 201). The forward pass is cut where four times its waves or more fill the card (512
+    // channels of 16 states in bf16, cut and in one piece: 512 steps x 80 envs, six times, 194 us and 250; 128 envs, four times, 512 steps 271 and 253,
+    // 1,999 steps 946 and 958; 170 envs, three times, 351 and 335), and a segment has four chunks at least (with two, four or eight: forward 128 x 8
+    // 31, 43 and 68 us, 128 x 64 67, 62 and 74; forward and gradient by the gradient's segments, 300 x 8 145, 176 and 272, 1,999 x 8 329, 330 and 340).
     const int64_t waves = std::max<int64_t>(1, a.N * a.G * k.per * k.slices), most = std::max<int64_t>(1, SCAN_FILL / waves);
     const int block = k.across * k.slices;
     const int64_t at_once = std::max<int64_t>(1, 256 * std::max(1, std::min((160 << 10) / (block * lds), (c.SP > 8 ? 8 : 12) / block)) / (a.G * k.cuts));
