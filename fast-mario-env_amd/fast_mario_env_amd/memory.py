@@ -267,14 +267,15 @@ def _scan_plain(x, dt, A, B, C, D, z, dt_bias, start, state):
     """The recurrence step by step in torch operations, in float32."""
     T, N, ch = x.shape
     h = x.new_zeros((N,) + A.shape, dtype=torch.float32) if state is None else state
-    A, rep, out = A.float(), ch // B.shape[2], []
+    A, out = A.float(), []
+    every = lambda v: v.float().unsqueeze(2).expand(N, v.shape[1], ch // v.shape[1], v.shape[2]).reshape(N, ch, v.shape[2])   # noqa: E731 (a group's channels)
     for t in range(T):
         xt, raw = x[t].float(), dt[t].float() if dt_bias is None else dt[t].float() + dt_bias.float()
         d = torch.logaddexp(raw, torch.zeros_like(raw))
         if start is not None:
             h = torch.where(start[t][:, None, None], torch.zeros_like(h), h)   # (before the product, whose gradient reads it)
-        h = torch.exp(d[..., None] * A) * h + (d * xt)[..., None] * B[t].float().repeat_interleave(rep, 1)
-        y = (C[t].float().repeat_interleave(rep, 1) * h).sum(-1)
+        h = torch.exp(d[..., None] * A) * h + (d * xt)[..., None] * every(B[t])
+        y = (every(C[t]) * h).sum(-1)
         y = y if D is None else y + D.float() * xt
         if z is not None:
             zt = z[t].float()

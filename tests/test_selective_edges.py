@@ -322,3 +322,45 @@ def test_clipping_float64_on_cpu():
     by = 0.5 / (norm + 1e-6)
     assert ((ps[0].grad - g * by).abs() <= 2.0 ** -50 * (g * by).abs()).all()
     assert ((ps[1].grad.double() - half.double() * by).abs() <= 2.0 ** -22 * half.double().abs() * by).all()
+
+
+# ---------------------------------------------------------------- what follows a call
+@pytest.mark.gpu
+def test_what_torch_transforms_takes_torch_operations():
+    """Forward-mode tangents, vmap, functional gradients, a dispatch mode and tracing see the operations (a kernel called by address would pass them by);
+    the results are the kernels'. Float32 on both sides: a few hundred roundings of 2^-24 a value."""
+    import torch.autograd.forward_ad as fwd
+    from torch.utils.flop_counter import FlopCounterMode
+    a, dout, _ = scan_inputs(6, 3, 8, 4, 2, torch.float32)
+    x, w, b, start, state, dy, _ = conv_inputs(6, 3, 8, 4, torch.float32)
+    scan = lambda v: state_scan(**{**a, "x": v})[0]          # noqa: E731
+    conv = lambda v: causal_conv_act(v, w, b, start, state)[0]   # noqa: E731
+    step = {n: v[0] if n in ("x", "dt", "B", "C", "z", "start") else v for n, v in a.items()}
+    near = lambda p, q: torch.allclose(p, q, rtol=1e-4, atol=1e-4)   # noqa: E731
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for f, at, back in ((scan, a["x"], dout), (conv, x, dy)):
+        y, u = f(at), torch.randn(at.shape, generator=g, device="cuda")
+        leaf = at.clone().requires_grad_()
+        (grad,) = torch.autograd.grad(f(leaf), leaf, back)
+        with fwd.dual_level():
+            primal, tangent = fwd.unpack_dual(f(fwd.make_dual(at, u)))
+        assert near(primal, y) and tangent is not None
+        assert near((tangent * back).sum() / 100, (grad * u).sum() / 100)      # (one sum of 144 products of size 1 to 10, either way)
+        many = torch.stack([at, 0.5 * at, -at])
+        assert near(torch.func.vmap(f)(many), torch.stack([f(v) for v in many]))
+        assert near(torch.func.grad(lambda v: (f(v) * back).sum())(at), grad)
+        with FlopCounterMode(display=False):
+            assert near(f(at), y)
+        assert near(torch.jit.trace(f, at, check_trace=False)(0.5 * at), f(0.5 * at))
+    states = torch.stack([a["state"], 2 * a["state"]])
+    windows = torch.stack([state, 2 * state])
+    want = [[t.clone() for t in ts] for ts in (states, windows)]
+    ys = [[state_scan_step(**{**step, "state": s}) for s in want[0]], [causal_conv_act_step(x[0], w, b, s, start[0]) for s in want[1]]]
+    got = torch.func.vmap(lambda s: state_scan_step(**{**step, "state": s}))(states), torch.func.vmap(lambda s: causal_conv_act_step(x[0], w, b, s, start[0]))(windows)
+    for y, e, s, m in zip(got, ys, (states, windows), want):
+        assert near(y, torch.stack(e)) and near(s, torch.stack(m))
+    old = [torch.randn(40, generator=g, device="cuda") for _ in range(3)]
+    ps = parameters_of(*(o.clone() for o in old))
+    with FlopCounterMode(display=False):
+        norm = clip_gradients(ps, 0.5)
+    assert near(norm, torch.cat(old).norm()) and all(near(p.grad, o * (0.5 / norm)) for p, o in zip(ps, old))
