@@ -109,7 +109,7 @@ int mo_group_norm_backward(const MoNorm* a, void* stream);
  *   state_out the same after the last step, 0 where its episode holds no input; must not overlap state; NULL: not wanted
  * The gradient: dy (T, N, C) and dstate_out (N, K - 1, C; NULL: zeros) in; dx (T, N, C), dstate (N, K - 1, C; NULL: not wanted), dweight (C, K)
  * and dbias (C) (both NULL: not wanted) out; work mo_conv_work() bytes, 16-byte aligned, free once the queued work is done. Sums are
- * float32 in a fixed order. */
+ * float32 in a fixed order. With N = 0 nothing is written. */
 #define MO_MAX_TAPS 8
 typedef struct MoConv {
     int32_t dtype, act, C, K;
@@ -141,12 +141,14 @@ int mo_conv_step(const MoConv* a, void* stream);
  *   C >= 1, 1 <= S <= MO_MAX_STATES, G >= 1 a divisor of C, T >= 0, N >= 0
  *   x, dt, z, out  (T, N, C), channels contiguous, MoRows.sh not used; z.p NULL: no factor of z
  *   Bt, Ct    (T, N, G, S), states contiguous, MoRows.sh the groups' stride
- *   A         (C, S) float32, none above 0 (a memory that grows may overflow earlier than step by step);   D, dt_bias (C) float32 or NULL (0)
+ *   A         (C, S) float32, none above 0 (a memory that grows may overflow earlier than step by step; an infinite one whose decay over
+ *             many steps rounds to 0 becomes NaN);   D, dt_bias (C) float32 or NULL (not there)
  *   start, state, state_out  as for linear attention, states (N, C, S) float32 contiguous
  *   saved     mo_scan_saved() bytes, 16-byte aligned, for mo_scan_backward to take up, or NULL: no gradient is wanted
  *   work      mo_scan_work() bytes, 16-byte aligned, free once the queued work is done
  * The gradient: dout and dstate_out (NULL: zeros) in, saved as the forward call left it; dx, ddt, dz (if z), dB, dC out; dstate (NULL: not
- * wanted) and dA, dD, ddt_bias float32 (each NULL: not wanted) out. Sums have a fixed order: the same inputs give the same bits. */
+ * wanted) and dA, dD, ddt_bias float32 (each NULL: not wanted) out. Sums have a fixed order: the same inputs give the same bits. With N = 0
+ * nothing is written. */
 #define MO_MAX_STATES 64
 typedef struct MoScan {
     int32_t dtype, C, S, G;
