@@ -134,7 +134,7 @@ def _norm_plain(x, groups, weight, bias, eps, act):
     if weight is not None:
         one = (1, -1) + (1,) * (x.dim() - 2)
         z = z * weight.float().view(one) + bias.float().view(one)
-    z = z.clamp(min=0.0) if act == "relu" else z * torch.sigmoid(z) if act == "silu" else z
+    z = torch.relu(z) if act == "relu" else z * torch.sigmoid(z) if act == "silu" else z
     return z.to(x.dtype)
 
 

@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, linear_attention, make_memory_net, state_scan, state_scan_step
+from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, group_norm_act, linear_attention, make_memory_net, state_scan, state_scan_step
 from fast_mario_env_amd.rollout import _share_elements, clip_gradients, gradient_norm
 from test_selective import DTYPES, check_scan, conv_inputs, scan64, scan_inputs
 
@@ -364,3 +364,12 @@ def test_what_torch_transforms_takes_torch_operations():
     with FlopCounterMode(display=False):
         norm = clip_gradients(ps, 0.5)
     assert near(norm, torch.cat(old).norm()) and all(near(p.grad, o * (0.5 / norm)) for p, o in zip(ps, old))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_group_norm_relu_at_zero(device):
+    """Where relu's argument is 0 (a group without spread, no bias), its slope is 0 on either device."""
+    x = torch.ones(3, 8, device=device)
+    w, b = torch.ones(8, device=device, requires_grad=True), torch.zeros(8, device=device, requires_grad=True)
+    y = group_norm_act(x, 2, w, b, act="relu")
+    assert (y == 0).all() and all((g == 0).all() for g in torch.autograd.grad(y, (w, b), torch.ones_like(y)))
