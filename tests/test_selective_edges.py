@@ -6,7 +6,8 @@ import random
 import pytest
 import torch
 
-from fast_mario_env_amd.memory import causal_conv_act, causal_conv_act_step, group_norm_act, linear_attention, make_memory_net, state_scan, state_scan_step
+from fast_mario_env_amd.memory import (causal_conv_act, causal_conv_act_step, group_norm_act, linear_attention, linear_attention_step, make_memory_net,
+                                       state_scan, state_scan_step)
 from fast_mario_env_amd.rollout import _share_elements, clip_gradients, gradient_norm
 from test_selective import DTYPES, check_scan, conv_inputs, scan64, scan_inputs
 
@@ -373,3 +374,34 @@ def test_group_norm_relu_at_zero(device):
     w, b = torch.ones(8, device=device, requires_grad=True), torch.zeros(8, device=device, requires_grad=True)
     y = group_norm_act(x, 2, w, b, act="relu")
     assert (y == 0).all() and all((g == 0).all() for g in torch.autograd.grad(y, (w, b), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_what_torch_transforms_of_attention_and_group_norm(device):
+    """The same for the operators of the memory that decays by constants, and their step."""
+    import torch.autograd.forward_ad as fwd
+    g = torch.Generator().manual_seed(4)
+    n = lambda *s: torch.randn(s, generator=g).to(device)    # noqa: E731
+    q, k, v, state = n(6, 3, 2, 8), n(6, 3, 2, 8), n(6, 3, 2, 5), n(3, 2, 8, 5)
+    decay, start = torch.tensor([0.9, 0.99], device=device), torch.zeros(6, 3, dtype=torch.bool, device=device)
+    start[2, 1] = True
+    w, b = n(8), n(8)
+    attend = lambda t: linear_attention(t, k, v, decay, start, state)[0]    # noqa: E731
+    norm = lambda t: group_norm_act(t, 2, w, b, act="silu")  # noqa: E731
+    near = lambda p, r: torch.allclose(p, r, rtol=1e-4, atol=1e-4)   # noqa: E731
+    for f, at in ((attend, q), (norm, n(4, 8, 3))):
+        y, u = f(at), n(*at.shape)
+        back, leaf = n(*y.shape), at.clone().requires_grad_()
+        (grad,) = torch.autograd.grad(f(leaf), leaf, back)
+        with fwd.dual_level():
+            primal, tangent = fwd.unpack_dual(f(fwd.make_dual(at, u)))
+        assert near(primal, y) and near((tangent * back).sum() / 100, (grad * u).sum() / 100)
+        many = torch.stack([at, 0.5 * at, -at])
+        assert near(torch.func.vmap(f)(many), torch.stack([f(t) for t in many]))
+        assert near(torch.func.grad(lambda t: (f(t) * back).sum())(at), grad)
+        assert near(torch.jit.trace(f, at, check_trace=False)(0.5 * at), f(0.5 * at))
+    states = torch.stack([state, 2 * state])
+    want = [s.clone() for s in states]
+    ys = [linear_attention_step(q[0], k[0], v[0], decay, s, start[0]) for s in want]
+    got = torch.func.vmap(lambda s: linear_attention_step(q[0], k[0], v[0], decay, s, start[0]))(states)
+    assert near(got, torch.stack(ys)) and near(states, torch.stack(want))
